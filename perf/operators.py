@@ -1,0 +1,412 @@
+"""The operators of the 8-bit paged KV cache, and what each costs: a step's block tables and
+slot maps built on the GPU from request lengths, the append that quantises new K/V rows into
+the cache, and the attention over it (chunks of new tokens, and single tokens).
+
+A cached row of one (token, KV head) is `head_dim` e4m3 codes and one power-of-two scale (an
+exponent byte, e8m0): value = code * 2^(byte - 127), the least scale that holds the row's
+largest magnitude in e4m3's 448. A block is one slab: the codes [block_size, kv_heads,
+head_dim], then the scale bytes [kv_heads, block_size], padded to 128 bytes.
+
+Lengths are fixed by the case (so the work is); values, block placement and free lists come
+from the seed.
+"""
+
+from __future__ import annotations
+
+import math
+import os
+import sys
+from pathlib import Path
+from types import SimpleNamespace
+
+import numpy as np
+import torch
+
+own = False
+
+DTYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+DEVICE = "cuda"
+
+GPT2 = {"heads": 12, "kv_heads": 12, "head_dim": 64, "block_size": 16}
+GQA = {"heads": 32, "kv_heads": 8, "head_dim": 128, "block_size": 16}
+
+
+# ---------------------------------------------------------------------- cases
+def _attend(name, dtype, shape, seqs, new, cached):
+    return {"name": name, "op": "attend", "dtype": dtype, **shape, "seqs": seqs, "new_min": new[0],
+            "new_max": new[1], "cached_min": cached[0], "cached_max": cached[1]}
+
+
+def _append(name, dtype, shape, tokens):
+    return {"name": name, "op": "append", "dtype": dtype, "kv_heads": shape["kv_heads"],
+            "head_dim": shape["head_dim"], "block_size": shape["block_size"], "tokens": tokens}
+
+
+def _layout(name, seqs, block_size, new, cached):
+    return {"name": name, "op": "layout", "seqs": seqs, "block_size": block_size, "new_min": new[0],
+            "new_max": new[1], "cached_min": cached[0], "cached_max": cached[1]}
+
+
+def listed():
+    return [
+        # The tables and slots of a GPT-2 decode step at low concurrency: the smallest call.
+        _layout("layout decode x8", 8, 16, (1, 1), (17, 700)),
+        # A step that admits chunks of many prompts: thousands of slots, many new blocks.
+        _layout("layout chunks x256", 256, 16, (1, 512), (0, 8192)),
+        # One layer's append of a GPT-2 decode step.
+        _append("append gpt2 fp16 x32", "fp16", GPT2, 32),
+        # One layer's append of a prefill step of long chunks.
+        _append("append gqa bf16 x8192", "bf16", GQA, 8192),
+        # A decode call of a GPT-2 serving batch.
+        _attend("decode gpt2 fp16 x32", "fp16", GPT2, 32, (1, 1), (16, 1000)),
+        # The same at the framework's default dtype.
+        _attend("decode gpt2 fp32 x32", "fp32", GPT2, 32, (1, 1), (16, 1000)),
+        # Decode of a full batch of long conversations, and of a lone very long one.
+        _attend("decode gqa bf16 x64", "bf16", GQA, 64, (1, 1), (1024, 16384)),
+        _attend("decode gqa bf16 x1 long", "bf16", GQA, 1, (1, 1), (100000, 100000)),
+        # Chunked prefill of long prompts.
+        _attend("chunks gqa bf16 x16", "bf16", GQA, 16, (512, 512), (0, 4096)),
+        # Short tails of new tokens behind cached prefixes.
+        _attend("tails gqa bf16 x12", "bf16", GQA, 12, (1, 64), (512, 8192)),
+        # A mixed step off the beaten path: another head dim, block size and dtype.
+        _attend("mixed odd fp16 x12", "fp16", {"heads": 32, "kv_heads": 32, "head_dim": 80, "block_size": 32}, 12,
+                (1, 200), (0, 1500)),
+        # Fresh prompts at the default dtype.
+        _attend("prompts gpt2 fp32 x8", "fp32", GPT2, 8, (16, 256), (0, 0)),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _shape(rng):
+    """Head layouts: the two usual ones, or any of the others that caches come in."""
+    if rng.random() < 0.5:
+        return dict(rng.choice([GPT2, GQA]))
+    kv = rng.choice([1, 2, 3, 4, 5, 8, 12])
+    return {"heads": kv * rng.choice([1, 2, 3, 4, 6, 8]), "kv_heads": kv,
+            "head_dim": rng.choice([32, 48, 64, 80, 96, 112, 128]), "block_size": rng.choice([8, 16, 32, 64])}
+
+
+def draw(rng):
+    kind = rng.choice(["layout", "append", "decode", "decode", "decode long", "chunks", "tails", "prompts"])
+    if kind == "layout":
+        seqs = _log(rng, 1, 1024)
+        new = _log(rng, 1, max(2, min(1024, 65536 // seqs)))
+        cached = _log(rng, 1, 16384)
+        c = _layout("", seqs, rng.choice([8, 16, 32, 64]), (rng.randint(0, 1), new), (rng.randint(0, cached), cached))
+    elif kind == "append":
+        c = _append("", rng.choice(["fp16", "bf16", "fp32"]), _shape(rng), _log(rng, 1, 8192))
+    else:
+        shape, dtype = _shape(rng), rng.choice(["fp16", "bf16", "bf16", "fp32"])
+        per_token = shape["kv_heads"] * shape["head_dim"]
+        if kind == "decode":
+            lo = _log(rng, 1, 1024)
+            new, cached = (1, 1), (lo, _log(rng, lo, 8192))
+            seqs = _log(rng, 1, max(1, min(64, 400_000_000 // (per_token * cached[1]))))
+        elif kind == "decode long":
+            n = _log(rng, 8192, 100000)
+            new, cached, seqs = (1, 1), (n // 2, n), rng.randint(1, 4)
+        elif kind == "chunks":
+            n = _log(rng, 64, 512)
+            new, cached, seqs = (rng.randint(1, n), n), (0, _log(rng, 64, 3584)), _log(rng, 1, 2048 // n)
+            shape, dtype = dict(rng.choice([shape, GQA])), rng.choice(["fp16", "bf16"])
+        elif kind == "tails":
+            lo = _log(rng, 64, 2048)
+            new, cached, seqs = (1, _log(rng, 2, 96)), (lo, _log(rng, lo, 6000)), _log(rng, 1, 12)
+        else:
+            new, cached, seqs = (rng.randint(1, 16), _log(rng, 17, 400)), (0, rng.choice([0, 64, 300])), _log(rng, 1, 8)
+        c = _attend("", dtype, shape, seqs, new, cached)
+    c.pop("name", None)
+    return c
+
+
+# ---------------------------------------------------------------------- inputs
+def _lengths(c):
+    """(contexts after the pass, new tokens) per sequence, the same for every seed."""
+    rng = np.random.default_rng(1337)
+    new = rng.integers(c["new_min"], c["new_max"] + 1, c["seqs"])
+    cached = rng.integers(c["cached_min"], c["cached_max"] + 1, c["seqs"])
+    if c["op"] == "attend":
+        new = np.maximum(new, 1)
+    return (new + cached).astype(np.int64), new.astype(np.int64)
+
+
+def _blocks_before(c, ctx, new):
+    """Blocks that each sequence holds before a layout call: those of its cached tokens."""
+    return -(-(ctx - new) // c["block_size"])
+
+
+def _cache(num_blocks, block_size, kv_heads, head_dim):
+    """(codes [blocks, block_size, kv_heads, head_dim], scales [blocks, block_size, kv_heads]),
+    both uint8 views of one slab a block."""
+    rows = block_size * kv_heads
+    block = -(-rows * (head_dim + 1) // 128) * 128
+    slab = torch.zeros(num_blocks, block, dtype=torch.uint8, device=DEVICE)
+    codes = slab.as_strided((num_blocks, block_size, kv_heads, head_dim), (block, kv_heads * head_dim, head_dim, 1))
+    scales = slab.as_strided((num_blocks, block_size, kv_heads), (block, 1, block_size), rows * head_dim)
+    return codes, scales
+
+
+def _fill(cache, g):
+    """Cached rows of unit-normal tokens whose size varies by row, as keys and values do."""
+    codes, scales = cache
+    for at in range(0, codes.shape[0], 4096):                 # bounded scratch
+        c, s = codes[at:at + 4096], scales[at:at + 4096]
+        x = torch.empty(c.shape, device=DEVICE).normal_(generator=g)
+        x *= torch.empty(s.shape, device=DEVICE).normal_(0.0, 0.5, generator=g).exp_()[..., None]
+        b = torch.empty(s.shape, dtype=torch.uint8, device=DEVICE)
+        c.copy_(_quantize(x, b))
+        s.copy_(b)
+
+
+def prepare(case, seed):
+    c = case
+    g = torch.Generator(device=DEVICE).manual_seed(seed)
+    host = np.random.default_rng(seed)
+    s = SimpleNamespace(case=c)
+    if c["op"] == "append":
+        dt, bs, t = DTYPES[c["dtype"]], c["block_size"], c["tokens"]
+        num_blocks = -(-t // bs) * 5 // 4 + 1
+        s.k_cache, s.v_cache = (_cache(num_blocks, bs, c["kv_heads"], c["head_dim"]) for _ in range(2))
+        _fill(s.k_cache, g)
+        _fill(s.v_cache, g)
+        # The projection writes Q, K and V of a token side by side: K and V are strided views.
+        qkv = torch.empty(t, 3, c["kv_heads"], c["head_dim"], device=DEVICE).normal_(generator=g).to(dt)
+        s.k, s.v = qkv[:, 1], qkv[:, 2]
+        s.slots_host = torch.from_numpy(host.permutation(num_blocks * bs)[:t])
+        s.slots = s.slots_host.to(DEVICE)
+        return s
+    ctx, new = _lengths(c)
+    bs = c["block_size"]
+    need = -(-ctx // bs)
+    num_blocks = int(need.sum()) * 5 // 4 + 1
+    ids = host.permutation(num_blocks)
+    tables = np.zeros((len(need), max(1, int(need.max()))), dtype=np.int64)
+    held = _blocks_before(c, ctx, new) if c["op"] == "layout" else need
+    at = 0
+    for i, n in enumerate(held):
+        tables[i, :n] = ids[at:at + n]
+        at += n
+    s.tokens = int(new.sum())
+    s.ctx_host, s.new_host = torch.from_numpy(ctx), torch.from_numpy(new)
+    s.ctx, s.new, s.tables = s.ctx_host.to(DEVICE), s.new_host.to(DEVICE), torch.from_numpy(tables).to(DEVICE)
+    if c["op"] == "layout":
+        s.held = torch.from_numpy(held).to(DEVICE)
+        s.free = torch.from_numpy(ids[at:]).to(DEVICE)
+        return s
+    kv, d = c["kv_heads"], c["head_dim"]
+    s.k_cache, s.v_cache = (_cache(num_blocks, bs, kv, d) for _ in range(2))
+    _fill(s.k_cache, g)
+    _fill(s.v_cache, g)
+    # Queries a little larger than unit: scores spread over several units, as in trained heads.
+    s.q = torch.empty(s.tokens, c["heads"], d, device=DEVICE).normal_(0.0, 1.5, generator=g).to(DTYPES[c["dtype"]])
+    s.scale = d ** -0.5
+    return s
+
+
+def _typed(cache):
+    """A cache's codes and scales as the 8-bit floats that they are."""
+    return cache[0].view(torch.float8_e4m3fn), cache[1].view(torch.float8_e8m0fnu)
+
+
+# ---------------------------------------------------------------------- run
+def run(state):
+    s, c = state, state.case
+    if c["op"] == "layout":
+        if own:
+            got = _framework().step_layout(s.tables, s.held, s.ctx, s.new, s.free, c["block_size"], s.tokens)
+            return {"tables": got.block_tables, "held": got.held, "slots": got.slots, "positions": got.positions,
+                    "starts": got.query_start, "counts": got.counts}
+        return _plain_layout(s.tables, s.held, s.ctx, s.new, s.free, c["block_size"], s.tokens)
+    k_cache, v_cache = _typed(s.k_cache), _typed(s.v_cache)
+    if c["op"] == "append":
+        if own:
+            _framework().kv8_append(k_cache, v_cache, s.k, s.v, s.slots, host_slots=s.slots_host)
+        else:
+            _plain_append(s.k_cache, s.k, s.slots)
+            _plain_append(s.v_cache, s.v, s.slots)
+        return {"k": k_cache[0], "k_scales": k_cache[1], "v": v_cache[0], "v_scales": v_cache[1]}
+    if own:
+        f = _framework()
+        ctx, new = f.attach_host(s.ctx, s.ctx_host), f.attach_host(s.new, s.new_host)
+        return {"out": f.paged_attention_kv8(s.q, k_cache, v_cache, s.tables, ctx, new, s.scale)}
+    return {"out": _plain_attention(s.q, s.k_cache, s.v_cache, s.tables, s.ctx, s.new, s.scale, int(s.ctx_host.max()),
+                                    int(s.new_host.max()))}
+
+
+_imported = None
+
+
+def _framework():
+    """The entry points that a user calls, on the library's kernels."""
+    global _imported
+    if _imported is None:
+        os.environ["ATTENTION"] = "hip"
+        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "llm-inference-server_amd"))
+        from inference_server.core.attention_hip import attach_host
+        from inference_server.core.kv8 import kv8_append, paged_attention_kv8
+        from inference_server.core.step_layout import step_layout
+
+        _imported = SimpleNamespace(attach_host=attach_host, kv8_append=kv8_append,
+                                    paged_attention_kv8=paged_attention_kv8, step_layout=step_layout)
+    return _imported
+
+
+# ---------------------------------------------------------------------- plain forms
+def _quantize(x, scales):
+    """Codes (uint8) of fp32 rows x [..., dim]; their scale bytes go to `scales` [...]. A row
+    with a value that is not finite is the NaN scale over zero codes."""
+    m, e = torch.frexp(x.abs().amax(-1))                     # amax = m 2^e, m in [1/2, 1)
+    b = (e + (127 - 9) + (m > 0.875)).clamp(min=0)           # 448 = 0.875 * 2^9
+    b = torch.where(m == 0, 0, b)
+    ok = torch.isfinite(x).all(-1)
+    y = torch.where(ok[..., None], x * torch.exp2((127 - b).float())[..., None], 0.0)
+    scales.copy_(torch.where(ok, b, 255))
+    return y.to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+def _plain_append(cache, rows, slots):
+    codes, scales = cache
+    bs = codes.shape[1]
+    b = torch.empty(rows.shape[:2], dtype=torch.uint8, device=rows.device)
+    codes[slots // bs, slots % bs] = _quantize(rows.float(), b)
+    scales[slots // bs, slots % bs] = b
+
+
+def _values(cache, blocks):
+    """fp32 values [..., block_size, kv_heads, dim] of some blocks."""
+    return cache[0][blocks].view(torch.float8_e4m3fn).float() * torch.exp2(cache[1][blocks].float() - 127)[..., None]
+
+
+def _plain_attention(q, k_cache, v_cache, tables, ctx, new, scale, max_ctx, max_new):
+    tokens, heads, dim = q.shape
+    bs, kv = k_cache[0].shape[1:3]
+    seqs = ctx.shape[0]
+    wide = tables[:, :-(-max_ctx // bs)]
+    keys = _values(k_cache, wide).flatten(1, 2).transpose(1, 2)               # [seqs, kv, keys, dim]
+    vals = _values(v_cache, wide).flatten(1, 2).transpose(1, 2)
+    start = new.cumsum(0) - new
+    t = torch.arange(max_new, device=q.device)
+    rows = (start[:, None] + t).clamp(max=tokens - 1)
+    qs = q[rows].float().view(seqs, max_new, kv, heads // kv, dim).permute(0, 2, 3, 1, 4)
+    score = torch.matmul(qs.reshape(seqs, kv, -1, dim), keys.transpose(-1, -2)) * scale
+    last = (ctx - new)[:, None] + t                                           # position of each query
+    seen = torch.arange(score.shape[-1], device=q.device) <= last[..., None]  # [seqs, new, keys]
+    score = score.view(seqs, kv, heads // kv, max_new, -1).masked_fill(~seen[:, None, None], -math.inf)
+    w = torch.exp(score - score.amax(-1, keepdim=True))
+    total = w.sum(-1, keepdim=True)
+    out = torch.matmul(w.flatten(2, 3), vals).view(seqs, kv, heads // kv, max_new, dim) / total
+    out = out.permute(0, 3, 1, 2, 4).reshape(seqs, max_new, heads, dim)
+    seq = torch.repeat_interleave(torch.arange(seqs, device=q.device), new, output_size=tokens)
+    at = torch.arange(tokens, device=q.device) - start[seq]
+    return out[seq, at].to(q.dtype)
+
+
+def _plain_layout(tables, held, ctx, new, free, bs, tokens):
+    width = tables.shape[1]
+    need = (ctx + bs - 1) // bs
+    fresh = (need - held).clamp(min=0)
+    first = fresh.cumsum(0) - fresh
+    start = torch.cat([new.new_zeros(1), new.cumsum(0)])
+    bad = (((new < 0) | (new > ctx) | (held < 0) | (held > width) | (need > width)).sum()
+           + (start[-1] > tokens))
+    wanted = fresh.sum()
+    ok = (bad == 0) & (wanted <= free.shape[0])
+    col = torch.arange(width, device=ctx.device)
+    take = (col >= held[:, None]) & (col < need[:, None]) & ok
+    pick = (first[:, None] + col - held[:, None]).clamp(0, max(0, free.shape[0] - 1))
+    tables = torch.where(take, free[pick], tables) if free.shape[0] else tables
+    t = torch.arange(tokens, device=ctx.device)
+    seq = torch.searchsorted(start[1:], t, right=True).clamp(max=ctx.shape[0] - 1)
+    real = ok & (t < start[-1])
+    pos = torch.where(real, ctx[seq] - new[seq] + t - start[seq], 0)
+    slots = torch.where(real, tables[seq, pos // bs] * bs + pos % bs, -1)
+    return {"tables": tables, "held": torch.where(ok, torch.maximum(held, need), held), "slots": slots,
+            "positions": pos, "starts": start, "counts": torch.stack([torch.where(ok, wanted, 0), wanted, bad])}
+
+
+# ---------------------------------------------------------------------- work
+def work(case):
+    c = case
+    if c["op"] == "append":
+        rows = 2 * c["tokens"] * c["kv_heads"]
+        size = 4 if c["dtype"] == "fp32" else 2
+        return {"bytes": rows * (c["head_dim"] * (size + 1) + 1) + 8 * c["tokens"], "flops": 0}
+    ctx, new = _lengths(c)
+    bs = c["block_size"]
+    if c["op"] == "layout":
+        held = _blocks_before(c, ctx, new)
+        fresh = int((-(-ctx // bs) - held).sum())
+        touched = int(np.where(new > 0, held - (ctx - new) // bs, 0).sum())    # held blocks that take new tokens
+        return {"bytes": 8 * (5 * c["seqs"] + 1 + touched + 2 * fresh + 2 * int(new.sum())), "flops": 0}
+    row, size = c["heads"] * c["head_dim"], 4 if c["dtype"] == "fp32" else 2
+    keys = new * (ctx - new) + new * (new + 1) // 2                             # keys seen by the new tokens
+    return {"bytes": 2 * int(ctx.sum()) * c["kv_heads"] * (c["head_dim"] + 1) + 2 * int(new.sum()) * row * size,
+            "flops": 4 * int(keys.sum()) * row}
+
+
+# ---------------------------------------------------------------------- exact
+def exact(case, seed):
+    """The definitions in 64 bits: tables of the 8-bit values, sequences one by one."""
+    s, c = prepare(case, seed), case
+    if c["op"] == "layout":
+        return _exact_layout(s, c)
+    # e4m3: bias 7, 3 bits of mantissa, no infinity, subnormals below 2^-6.
+    byte = np.arange(128)
+    mag = np.where(byte < 8, byte * 2.0 ** -9, (8 + byte % 8) * 2.0 ** (byte // 8 - 10))
+    mag[127] = np.nan
+    e4m3 = np.concatenate([mag, -mag])
+    if c["op"] == "append":
+        out = {}
+        for name, cache, rows in (("k", s.k_cache, s.k), ("v", s.v_cache, s.v)):
+            codes = e4m3[cache[0].cpu().numpy()]
+            scales = np.exp2(cache[1].cpu().numpy().astype(np.float64) - 127)
+            x = rows.double().cpu().numpy()
+            size = np.abs(x).max(-1)
+            scale = np.exp2(np.ceil(np.log2(np.maximum(size, 2.0 ** -130) / 448)))
+            scale = np.where(scale * 224 >= size, scale / 2, scale)            # log2 may be off at a power of two
+            scale = np.where(scale * 448 < size, scale * 2, scale).clip(2.0 ** -127)
+            y = np.abs(x / scale[..., None])
+            step = np.exp2(np.maximum(np.floor(np.log2(np.maximum(y, 2.0 ** -20))), -6) - 3)
+            y = np.copysign(np.round(y / step) * step, x)                      # ties to even
+            at = s.slots_host.numpy()
+            codes[at // c["block_size"], at % c["block_size"]] = y
+            scales[at // c["block_size"], at % c["block_size"]] = scale
+            out |= {name: torch.from_numpy(codes), name + "_scales": torch.from_numpy(scales)}
+        return out
+    value = torch.from_numpy(e4m3).to(DEVICE)
+    group, bs = c["heads"] // c["kv_heads"], c["block_size"]
+    out = torch.empty(s.q.shape, dtype=torch.float64, device=DEVICE)
+    at = 0
+    for i in range(c["seqs"]):
+        n, m = int(s.ctx_host[i]), int(s.new_host[i])
+        ids = s.tables[i, :-(-n // bs)]
+        k, v = (value[x[ids].long()] * torch.exp2(e[ids].double() - 127)[..., None]
+                for x, e in (s.k_cache, s.v_cache))
+        k, v = (x.reshape(-1, c["kv_heads"], c["head_dim"])[:n].transpose(0, 1).contiguous() for x in (k, v))
+        hidden = torch.arange(n, device=DEVICE)[None] > torch.arange(n - m, n, device=DEVICE)[:, None]
+        for h in range(c["heads"]):
+            score = s.q[at:at + m, h].double() @ k[h // group].t().contiguous() * s.scale
+            out[at:at + m, h] = score.masked_fill(hidden, -math.inf).softmax(-1) @ v[h // group]
+        at += m
+    return {"out": out}
+
+
+def _exact_layout(s, c):
+    ctx, new, held = s.ctx_host.tolist(), s.new_host.tolist(), s.held.tolist()
+    tables, free, bs = s.tables.cpu(), s.free.tolist(), c["block_size"]
+    slots, positions, starts, taken = [], [], [0], 0
+    for i, (n, m) in enumerate(zip(ctx, new)):
+        while held[i] * bs < n:
+            tables[i, held[i]] = free[taken]
+            held[i] += 1
+            taken += 1
+        row = tables[i].tolist()
+        positions += range(n - m, n)
+        slots += [row[p // bs] * bs + p % bs for p in range(n - m, n)]
+        starts.append(len(slots))
+    long = lambda v: torch.tensor(v, dtype=torch.long)  # noqa: E731
+    return {"tables": tables, "held": long(held), "slots": long(slots), "positions": long(positions),
+            "starts": long(starts), "counts": long([taken, taken, 0])}
