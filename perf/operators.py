@@ -324,7 +324,7 @@ def _plain_layout(tables, held, ctx, new, free, bs, tokens):
     pos = torch.where(real, ctx[seq] - new[seq] + t - start[seq], 0)
     slots = torch.where(real, tables[seq, pos // bs] * bs + pos % bs, -1)
     return {"tables": tables, "held": torch.where(ok, torch.maximum(held, need), held), "slots": slots,
-            "positions": pos, "starts": start, "counts": torch.stack([torch.where(ok, wanted, 0), wanted, bad])}
+            "positions": pos, "starts": torch.where(ok, start, 0), "counts": torch.stack([torch.where(ok, wanted, 0), wanted, bad])}
 
 
 # ---------------------------------------------------------------------- work
