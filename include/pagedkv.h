@@ -436,6 +436,99 @@ int pkv_lm_head_argmax(
     int64_t* out_ids, void* workspace, int64_t workspace_bytes,
     hipStream_t stream);
 
+/* ------------------------------------------------------------------ 8-bit cache
+ * A paged cache of 8-bit K/V, without counterpart in the reference: half the bytes of a
+ * 16-bit pool a token, so twice the tokens in a budget and half the traffic of a decode step.
+ *
+ * A row of one (token, KV head) is head_dim e4m3 codes (OCP: bias 7, largest magnitude 448,
+ * no infinity) and one scale byte b (e8m0): value = code * 2^(b - 127), b the least with which
+ * the row's largest magnitude is at most 448 (0 for a row of zeros). A row with a value that
+ * is not finite is the NaN row: b = 255 and codes 0. Codes are finite (a code of NaN under
+ * another scale is not a row that the append writes, and may reach rows that do not see it).
+ *
+ *   codes   [num_blocks, block_size, num_kv_heads, head_dim], strides (code_stride_block,
+ *           code_stride_slot, code_stride_head, 1)
+ *   scales  [num_blocks, block_size, num_kv_heads], strides (scale_stride_block,
+ *           scale_stride_slot, scale_stride_head)
+ *
+ * uint8, identical strides for K and V; `dtype` is that of the queries, the output and the
+ * appended rows. head_dim at most 512. */
+
+/* Quantise row t of k_new / v_new ([num_tokens, num_kv_heads, head_dim], element strides
+ * new_stride_t / new_stride_h, unit innermost stride) into flat slot slots[t] of the cache.
+ * x * 2^(127 - b) is rounded once, to the nearest code, ties to even. Slots must be distinct;
+ * those outside [0, num_blocks * block_size) are skipped. */
+int pkv_kv8_append(
+    void* k_codes, void* v_codes,
+    int64_t code_stride_block, int64_t code_stride_slot, int64_t code_stride_head,
+    void* k_scales, void* v_scales,
+    int64_t scale_stride_block, int64_t scale_stride_slot, int64_t scale_stride_head,
+    int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+    const void* k_new, const void* v_new, int64_t new_stride_t, int64_t new_stride_h,
+    const int64_t* slots, int64_t num_tokens, int dtype,
+    hipStream_t stream);
+
+/* Attention over the 8-bit cache: pkv_paged_attention_prefill's contract (chunks of new
+ * tokens, prompts, mixes with decode), or pkv_paged_attention_decode's where query_start_loc
+ * is NULL (one token per sequence). Scores, softmax and sums are in float32, the output is
+ * rounded once; a key that a row does not see never reaches it, whatever it holds (NaN rows
+ * included), and a row that sees no key (a context of 0) is zero. max_query_len bounds the
+ * query lengths (0: num_tokens) and max_context_len the contexts: they size the grid.
+ * Block ids outside the pool are never dereferenced.
+ *
+ * host_context_lens / host_query_lens (HOST memory, int64 [num_seqs], or NULL) decide whether
+ * and how contexts are cut into runs of separate workgroups, as in
+ * pkv_paged_attention_prefill_split, and so does workspace: at least
+ * pkv_kv8_attention_workspace_bytes() bytes for the same sizes and lengths, its first 256 KiB
+ * zero when a call starts (every completed call leaves them zero; it can be the decode calls'
+ * workspace). With a smaller one, or NULL, no context is cut. */
+int64_t pkv_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                                          int64_t head_dim, int64_t num_tokens, int64_t max_query_len,
+                                          int64_t max_context_len, const int64_t* host_context_lens,
+                                          const int64_t* host_query_lens);
+int pkv_kv8_attention(
+    void* out, int64_t out_stride_t, int64_t out_stride_h,
+    const void* query, int64_t q_stride_t, int64_t q_stride_h,
+    const void* k_codes, const void* v_codes,
+    int64_t code_stride_block, int64_t code_stride_slot, int64_t code_stride_head,
+    const void* k_scales, const void* v_scales,
+    int64_t scale_stride_block, int64_t scale_stride_slot, int64_t scale_stride_head,
+    int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+    const int64_t* block_tables, int64_t table_stride, int64_t table_width,
+    const int64_t* context_lens, const int64_t* query_start_loc,
+    int64_t num_seqs, int64_t num_heads, int64_t num_tokens, int64_t max_query_len, int64_t max_context_len,
+    const int64_t* host_context_lens, const int64_t* host_query_lens,
+    float scale, int dtype,
+    void* workspace, int64_t workspace_bytes,
+    hipStream_t stream);
+
+/* ------------------------------------------------------------------ step layout
+ * The block tables and slot maps of a step, on the GPU, from request lengths: what
+ * BlockTable.ensure_capacity and slot_range (inference_server/core/block_table.py:70-108,
+ * 137-159) and the packing of PagedExecutor._pack (core/paged_executor.py:211-263) do on the
+ * host, one launch for the batch. For sequence i: context_lens[i] tokens cached after the step,
+ * query_lens[i] of them new, held[i] blocks in row i of block_tables
+ * (int64 [num_seqs, table_width], row stride table_stride). The blocks that it lacks
+ * (ceil(context / block_size) - held) come from the front of free_blocks [num_free], in
+ * sequence order, and are written behind its held ones, in place.
+ *
+ * Out, int64: held_out [num_seqs] blocks held now (not `held` itself); slots and positions
+ * [num_tokens] of the packed new tokens (the context's last query_lens[i] positions), -1 and 0
+ * for rows past the last one; query_start_loc [num_seqs + 1]; counts [3] = blocks taken, blocks
+ * needed, impossible lengths (a query length below 0 or above its context, a context beyond
+ * the table's width, held outside it, more new tokens than num_tokens).
+ *
+ * All or nothing: if blocks needed > num_free, or any length is impossible, no table changes,
+ * held_out = held, every slot is -1 and query_start_loc is all 0, so that the appends and
+ * attention calls queued behind it do nothing. A call repeated on the same inputs gives the
+ * same result (held is not advanced in place). */
+int pkv_step_layout(
+    int64_t* block_tables, int64_t table_stride, int64_t table_width,
+    const int64_t* held, const int64_t* context_lens, const int64_t* query_lens, int64_t num_seqs,
+    const int64_t* free_blocks, int64_t num_free, int64_t block_size, int64_t num_tokens,
+    int64_t* held_out, int64_t* slots, int64_t* positions, int64_t* query_start_loc, int64_t* counts,
+    hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,187 @@
+// Attention over the 8-bit paged cache: the generic kernel and the extern "C" entry points.
+//
+// Generic kernel: any block size, head_dim <= 512, GQA group, stride and softmax scale. One
+// wave per (token, query head), lanes split head_dim, one key a step, online softmax in fp32.
+// It takes the shapes that the matrix kernels decline.
+#include "kv8.h"
+
+namespace pkv {
+namespace {
+
+// Elements [lane * EPL, +EPL) would need aligned rows; lane, lane + 64, ... needs nothing.
+template <typename T, int EPL>
+__global__ __launch_bounds__(256) void kv8_generic_kernel(const Kv8Params p) {
+    const int lane = lane_id();
+    const int64_t tok = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int head = (int)blockIdx.y;
+    if (tok >= p.num_tokens) return;
+    int seq = (int)tok;
+    int64_t q_start = tok, q_len = 1;
+    if (p.qsl) {
+        // The last sequence with query_start_loc <= tok owns it; tokens past the last one
+        // belong to no sequence.
+        if (tok >= p.qsl[p.num_seqs]) return;
+        int lo = 0, hi = p.num_seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.qsl[mid] <= tok) lo = mid; else hi = mid;
+        }
+        seq = lo;
+        q_start = p.qsl[seq];
+        q_len = p.qsl[seq + 1] - q_start;
+    }
+    const int64_t cap = p.table_width * p.block_size;
+    int64_t n_keys = p.ctx_lens[seq] - q_len + (tok - q_start) + 1;
+    n_keys = n_keys < cap ? n_keys : cap;
+    const int kvh = head / p.group;
+    const T* qrow = reinterpret_cast<const T*>(p.q) + tok * p.q_st + (int64_t)head * p.q_sh;
+    float q[EPL], acc[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        const int d = lane + 64 * e;
+        q[e] = d < p.head_dim ? to_f32(qrow[d]) : 0.f;
+        acc[e] = 0.f;
+    }
+    const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.k) + kvh * p.sh;
+    const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.v) + kvh * p.sh;
+    const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
+    float m = kNegInf, l = 0.f;
+    for (int64_t j = 0; j < n_keys; ++j) {
+        int64_t blk = table[j / p.block_size];
+        const bool ok = (uint64_t)blk < (uint64_t)p.num_blocks;   // a bad id reads as zeros
+        blk = ok ? blk : 0;
+        const int64_t at = j % p.block_size;
+        const int64_t row = blk * p.sb + at * p.ss, sc = blk * p.ssb + at * p.sss + kvh * p.ssh;
+        const float ks = ok ? scale_of(p.ks[sc]) : 0.f, vs = ok ? scale_of(p.vs[sc]) : 0.f;
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int d = lane + 64 * e;
+            if (d < p.head_dim && ok) s += q[e] * __builtin_amdgcn_cvt_f32_fp8(kc[row + d], 0);
+        }
+        s = wave_sum(s) * ks * p.scale_log2;
+        const float m_new = fmaxf(m, s);
+        const float m_off = m_new == kNegInf ? 0.f : m_new;
+        const float alpha = fast_exp2(m - m_off);   // 0 on the first key (m = -inf)
+        const float pj = fast_exp2(s - m_off), w = pj * vs;
+        l = l * alpha + pj;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+            const int d = lane + 64 * e;
+            const float vd = d < p.head_dim && ok ? __builtin_amdgcn_cvt_f32_fp8(vc[row + d], 0) : 0.f;
+            acc[e] = acc[e] * alpha + w * vd;
+        }
+        m = m_new;
+    }
+    T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)head * p.out_sh;
+    const float inv = n_keys > 0 ? 1.f / l : 0.f;   // a row without keys is zero
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+        const int d = lane + 64 * e;
+        if (d < p.head_dim) orow[d] = from_f32<T>(acc[e] * inv);
+    }
+}
+
+template <typename T>
+int launch_generic_t(const Kv8Params& p, hipStream_t stream) {
+    const int64_t gx = ceil_div(p.num_tokens, 4);
+    if (gx > 0x7fffffff) return fail(PKV_EUNSUPPORTED, "kv8_attention: grid too large");
+    const dim3 grid((unsigned)gx, (unsigned)p.num_heads);
+    if (p.head_dim <= 64) kv8_generic_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
+    else if (p.head_dim <= 128) kv8_generic_kernel<T, 2><<<grid, 256, 0, stream>>>(p);
+    else if (p.head_dim <= 256) kv8_generic_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
+    else if (p.head_dim <= 512) kv8_generic_kernel<T, 8><<<grid, 256, 0, stream>>>(p);
+    else return fail(PKV_EUNSUPPORTED, "kv8_attention: head_dim %d > 512", p.head_dim);
+    return check_launch("kv8 generic attention");
+}
+
+}  // namespace
+
+int launch_kv8_generic(const Kv8Params& p, int dtype, hipStream_t stream) {
+    switch (dtype) {
+        case PKV_FLOAT32: return launch_generic_t<float>(p, stream);
+        case PKV_FLOAT16: return launch_generic_t<_Float16>(p, stream);
+        default: return launch_generic_t<bf16_t>(p, stream);
+    }
+}
+
+}  // namespace pkv
+
+using namespace pkv;
+
+extern "C" int64_t pkv_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                                                     int64_t head_dim, int64_t num_tokens, int64_t max_query_len,
+                                                     int64_t max_context_len, const int64_t* host_context_lens,
+                                                     const int64_t* host_query_lens) {
+    return 0;
+}
+
+extern "C" int pkv_kv8_attention(
+    void* out, int64_t out_stride_t, int64_t out_stride_h, const void* query, int64_t q_stride_t, int64_t q_stride_h,
+    const void* k_codes, const void* v_codes, int64_t code_stride_block, int64_t code_stride_slot,
+    int64_t code_stride_head, const void* k_scales, const void* v_scales, int64_t scale_stride_block,
+    int64_t scale_stride_slot, int64_t scale_stride_head, int64_t num_blocks, int64_t block_size,
+    int64_t num_kv_heads, int64_t head_dim, const int64_t* block_tables, int64_t table_stride, int64_t table_width,
+    const int64_t* context_lens, const int64_t* query_start_loc, int64_t num_seqs, int64_t num_heads,
+    int64_t num_tokens, int64_t max_query_len, int64_t max_context_len, const int64_t* host_context_lens,
+    const int64_t* host_query_lens, float scale, int dtype, void* workspace, int64_t workspace_bytes,
+    hipStream_t stream) {
+    clear_error();
+    if (dtype != PKV_FLOAT32 && dtype != PKV_FLOAT16 && dtype != PKV_BFLOAT16)
+        return fail(PKV_EINVAL, "kv8_attention: unknown dtype %d", dtype);
+    if (num_seqs < 0 || num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 ||
+        num_blocks < 0 || table_width < 0 || max_query_len < 0 || max_context_len < 0)
+        return fail(PKV_EINVAL, "kv8_attention: bad sizes");
+    if (num_heads % num_kv_heads)
+        return fail(PKV_EINVAL, "kv8_attention: %lld query heads not divisible by %lld kv heads", (long long)num_heads,
+                    (long long)num_kv_heads);
+    if (num_seqs > 0x7fffffff || num_tokens > 0x7fffffff || num_heads > 65535 || head_dim > 512 ||
+        block_size > 0x7fffffff || table_width > 0x7fffffff / block_size)
+        return fail(PKV_EUNSUPPORTED, "kv8_attention: sizes beyond what the kernels index");
+    if (!query_start_loc && num_tokens != num_seqs)
+        return fail(PKV_EINVAL, "kv8_attention: %lld tokens of %lld sequences need query_start_loc",
+                    (long long)num_tokens, (long long)num_seqs);
+    if (num_tokens == 0 || num_seqs == 0) return PKV_OK;
+    if (!out || !query || !k_codes || !v_codes || !k_scales || !v_scales || !context_lens ||
+        (!block_tables && table_width > 0))
+        return fail(PKV_EINVAL, "kv8_attention: null pointer");
+    Kv8Params p = {};
+    p.out = out;
+    p.out_st = out_stride_t;
+    p.out_sh = out_stride_h;
+    p.q = query;
+    p.q_st = q_stride_t;
+    p.q_sh = q_stride_h;
+    p.k = k_codes;
+    p.v = v_codes;
+    p.sb = code_stride_block;
+    p.ss = code_stride_slot;
+    p.sh = code_stride_head;
+    p.ks = (const uint8_t*)k_scales;
+    p.vs = (const uint8_t*)v_scales;
+    p.ssb = scale_stride_block;
+    p.sss = scale_stride_slot;
+    p.ssh = scale_stride_head;
+    p.num_blocks = num_blocks;
+    p.block_size = (int)block_size;
+    p.block_shift = block_size & (block_size - 1) ? -1 : 63 - __builtin_clzll((unsigned long long)block_size);
+    p.num_kv_heads = (int)num_kv_heads;
+    p.head_dim = (int)head_dim;
+    p.tables = block_tables;
+    p.table_stride = table_stride;
+    p.table_width = table_width;
+    p.ctx_lens = context_lens;
+    p.qsl = query_start_loc;
+    p.num_seqs = (int)num_seqs;
+    p.num_heads = (int)num_heads;
+    p.group = (int)(num_heads / num_kv_heads);
+    p.num_tokens = num_tokens;
+    p.max_query_len = (int)(!query_start_loc ? 1 : max_query_len && max_query_len < num_tokens ? max_query_len
+                                                                                              : num_tokens);
+    p.max_context_len = max_context_len;
+    p.scale = scale;
+    p.scale_log2 = scale * kLog2e;
+    p.splits = 1;
+    p.split_tiles = 0x7fffffff;
+    return launch_kv8_generic(p, dtype, stream);
+}

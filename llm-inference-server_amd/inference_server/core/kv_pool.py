@@ -124,12 +124,20 @@ class PagedKVPool:
         self.num_blocks = num_blocks
         self.block_size = block_size
         self.device = device
-        shape = (num_blocks, block_size, dims.num_kv_heads, dims.head_dim)
-        self.k = [torch.zeros(shape, dtype=dims.dtype, device=device) for _ in range(dims.num_layers)]
-        self.v = [torch.zeros(shape, dtype=dims.dtype, device=device) for _ in range(dims.num_layers)]
+        self.k = self._allocate()
+        self.v = self._allocate()
         self._ptr_table: torch.Tensor | None = None
         # Side stream for the PCIe halves of a swap (default priority, made on first use).
         self._copy: torch.cuda.Stream | None = None
+
+    def _allocate(self) -> list[torch.Tensor]:
+        shape = (self.num_blocks, self.block_size, self.dims.num_kv_heads, self.dims.head_dim)
+        return [torch.zeros(shape, dtype=self.dims.dtype, device=self.device) for _ in range(self.dims.num_layers)]
+
+    def _host_shape(self, n: int) -> tuple[tuple[int, ...], torch.dtype]:
+        """Shape and dtype of a swap's one host buffer for n blocks: 2L layers first."""
+        shape = (2 * self.dims.num_layers, n, self.block_size, self.dims.num_kv_heads, self.dims.head_dim)
+        return shape, self.dims.dtype
 
     @classmethod
     def from_model(cls, model, **kwargs) -> "PagedKVPool":
@@ -285,12 +293,12 @@ class PagedKVPool:
             return HostBlocks(k=[to_host(t) for t in self.k], v=[to_host(t) for t in self.v])
 
         L, n = self.dims.num_layers, len(blocks)
-        shape = (2 * L, n, self.block_size, self.dims.num_kv_heads, self.dims.head_dim)
-        packed = torch.empty(shape, dtype=self.dims.dtype, pin_memory=True)
+        shape, dtype = self._host_shape(n)
+        packed = torch.empty(shape, dtype=dtype, pin_memory=True)
         if n == 0:
             return HostBlocks(k=list(packed[:L]), v=list(packed[L:]), packed=packed)
         idx = self._index(blocks)
-        staging = torch.empty(shape, dtype=self.dims.dtype, device=self.device)
+        staging = torch.empty(shape, dtype=dtype, device=self.device)
         rc = native.lib().pkv_gather_blocks(
             self.pointer_table().data_ptr(), 2 * L, self.num_blocks, self.block_bytes,
             idx.data_ptr(), n, staging.data_ptr(), self._stream(),
@@ -331,8 +339,8 @@ class PagedKVPool:
         packed = host.packed
         if packed is None or not packed.is_pinned() or not packed.is_contiguous():
             packed = torch.stack(host.k + host.v).contiguous().pin_memory()
-        expect = (2 * self.dims.num_layers, n, self.block_size, self.dims.num_kv_heads, self.dims.head_dim)
-        if tuple(packed.shape) != expect or packed.dtype != self.dims.dtype:
+        expect, dtype = self._host_shape(n)
+        if tuple(packed.shape) != expect or packed.dtype != dtype:
             raise ValueError(f"swap_in: host blocks {tuple(packed.shape)} {packed.dtype} do not fit pool {expect}")
         idx = self._index(blocks)
         # Allocated on the current stream: the copy stream first catches up with it, so

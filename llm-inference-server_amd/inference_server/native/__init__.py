@@ -7,6 +7,7 @@ missing or its ABI version differs: the HIP path never falls back to anything el
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -147,6 +148,39 @@ SIGNATURES: dict[str, tuple] = {
     "pkv_scatter_blocks": (_int, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr]),
     "pkv_swap_out": (_int, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr]),
     "pkv_swap_in": (_int, [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr]),
+    "pkv_kv8_append": (
+        _int,
+        [_ptr, _ptr, _i64, _i64, _i64,     # k_codes, v_codes, code strides
+         _ptr, _ptr, _i64, _i64, _i64,     # k_scales, v_scales, scale strides
+         _i64, _i64, _i64, _i64,           # num_blocks, block_size, num_kv_heads, head_dim
+         _ptr, _ptr, _i64, _i64,           # k_new, v_new, new strides (t, h)
+         _ptr, _i64, _int,                 # slots, num_tokens, dtype
+         _ptr],
+    ),
+    "pkv_kv8_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr]),
+    "pkv_kv8_attention": (
+        _int,
+        [_ptr, _i64, _i64,                 # out, strides
+         _ptr, _i64, _i64,                 # query, strides
+         _ptr, _ptr, _i64, _i64, _i64,     # k_codes, v_codes, code strides
+         _ptr, _ptr, _i64, _i64, _i64,     # k_scales, v_scales, scale strides
+         _i64, _i64, _i64, _i64,           # num_blocks, block_size, num_kv_heads, head_dim
+         _ptr, _i64, _i64,                 # block_tables, table_stride, table_width
+         _ptr, _ptr,                       # context_lens, query_start_loc (or None)
+         _i64, _i64, _i64, _i64, _i64,     # num_seqs, num_heads, num_tokens, max_query_len, max_context_len
+         _ptr, _ptr,                       # host context_lens, host query_lens
+         _f32, _int,
+         _ptr, _i64,                       # workspace, workspace_bytes
+         _ptr],
+    ),
+    "pkv_step_layout": (
+        _int,
+        [_ptr, _i64, _i64,                 # block_tables, table_stride, table_width
+         _ptr, _ptr, _ptr, _i64,           # held, context_lens, query_lens, num_seqs
+         _ptr, _i64, _i64, _i64,           # free_blocks, num_free, block_size, num_tokens
+         _ptr, _ptr, _ptr, _ptr, _ptr,     # held_out, slots, positions, query_start_loc, counts
+         _ptr],
+    ),
     "pkv_lm_head_argmax_workspace_bytes": (_i64, [_i64, _i64]),
     "pkv_lm_head_argmax": (
         _int,
@@ -221,6 +255,17 @@ def stream_capture_id(stream: int) -> int:
     out = ctypes.c_uint64()
     check(lib().pkv_stream_capture_id(stream, ctypes.byref(out)), "pkv_stream_capture_id")
     return out.value
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one: a stream takes launches and
+    allocations of its own device only."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:
