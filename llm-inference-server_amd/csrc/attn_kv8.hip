@@ -105,6 +105,68 @@ int launch_kv8_generic(const Kv8Params& p, int dtype, hipStream_t stream) {
     }
 }
 
+// ------------------------------------------------------------------ decode
+bool kv8_decode_applies(const Kv8Params& p, int dtype) {
+    if (p.head_dim % 16 || p.head_dim < 32 || p.head_dim > 128 || p.block_shift < 2) return false;
+    if (p.num_seqs > kKv8DecodeMaxSeqs || p.num_blocks < 1) return false;
+    if ((int64_t)p.max_query_len * p.group > kKv8DecodeRows) return false;
+    // Keys and units in 32 bits; so are the offsets of a lane inside 16 slots.
+    const int64_t cap = p.table_width * p.block_size;
+    if (cap > (1 << 30) || (cap / 32 + 1) * p.num_seqs > (1 << 30)) return false;
+    if (p.ss < 0 || p.ss > (1 << 26) || p.sss < 0 || p.sss > (1 << 26)) return false;
+    const int64_t isz = dtype == PKV_FLOAT32 ? 4 : 2;
+    const uint64_t rows = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * isz) |
+                          (uint64_t)(p.q_sh * isz) | (uint64_t)(p.out_st * isz) | (uint64_t)(p.out_sh * isz);
+    const uint64_t codes = (uint64_t)(uintptr_t)p.k | (uint64_t)(uintptr_t)p.v | (uint64_t)p.sb | (uint64_t)p.ss |
+                           (uint64_t)p.sh;
+    return rows % 8 == 0 && codes % 4 == 0;
+}
+
+// Runs for every CU to hold kPerCu workgroups. A run is a workgroup's unless sequences are short
+// and (sequence, KV head) pairs fill the GPU's waves by themselves.
+int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* host_qlen) {
+    constexpr int kCus = 256, kPerCu = 3;
+    int64_t units = 0;
+    for (int i = 0; i < p.num_seqs; ++i) {
+        const int64_t c = host_ctx ? host_ctx[i] : p.max_context_len;
+        if (!host_qlen || host_qlen[i] > 0) units += c > 32 ? ceil_div(c, 32) : 1;
+    }
+    const int64_t pairs = (int64_t)p.num_seqs * p.num_kv_heads;
+    p.decode_coop = pairs < 4 * kCus * kPerCu || units >= 8 * (int64_t)p.num_seqs;
+    p.decode_min_units = p.decode_coop ? 8 : 2;
+    p.decode_rows = (int)((int64_t)p.max_query_len * p.group);
+    int64_t most = kCus * kPerCu * (p.decode_coop ? 1 : 4) / p.num_kv_heads;
+    const int64_t bound = units / p.decode_min_units;
+    most = most < bound ? most : bound;
+    p.slots = (int)(most < 1 ? 1 : most);
+    if (pairs * 4 > kMergeCounterBytes) return 0;
+    return (int64_t)p.slots * 2 * p.num_kv_heads * p.decode_rows * (p.head_dim + 2) * 4;
+}
+
+namespace {
+
+// Whether the decode kernel takes a batch of these sizes, strides and addresses aside.
+Kv8Params sizes_of(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_tokens,
+                   int64_t max_query_len, int64_t max_context_len) {
+    Kv8Params p = {};
+    p.num_seqs = (int)num_seqs;
+    p.num_heads = (int)num_heads;
+    p.num_kv_heads = (int)num_kv_heads;
+    p.group = (int)(num_heads / num_kv_heads);
+    p.head_dim = (int)head_dim;
+    p.num_tokens = num_tokens;
+    p.max_query_len = (int)(max_query_len && max_query_len < num_tokens ? max_query_len : num_tokens);
+    p.max_context_len = max_context_len;
+    p.splits = 1;
+    p.split_tiles = 0x7fffffff;
+    return p;
+}
+
+bool few_rows(const Kv8Params& p) {
+    return p.num_seqs <= kKv8DecodeMaxSeqs && (int64_t)p.max_query_len * p.group <= kKv8DecodeRows;
+}
+
+}  // namespace
 }  // namespace pkv
 
 using namespace pkv;
@@ -113,7 +175,13 @@ extern "C" int64_t pkv_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t n
                                                      int64_t head_dim, int64_t num_tokens, int64_t max_query_len,
                                                      int64_t max_context_len, const int64_t* host_context_lens,
                                                      const int64_t* host_query_lens) {
-    return 0;
+    if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_tokens <= 0 ||
+        num_seqs > 0x7fffffff || num_tokens > 0x7fffffff || num_heads % num_kv_heads)
+        return 0;
+    Kv8Params p = sizes_of(num_seqs, num_heads, num_kv_heads, head_dim, num_tokens, max_query_len, max_context_len);
+    if (!few_rows(p)) return 0;
+    const int64_t parts = kv8_decode_plan(p, host_context_lens, host_query_lens);
+    return parts ? kMergeCounterBytes + parts : 0;
 }
 
 extern "C" int pkv_kv8_attention(
@@ -145,7 +213,8 @@ extern "C" int pkv_kv8_attention(
     if (!out || !query || !k_codes || !v_codes || !k_scales || !v_scales || !context_lens ||
         (!block_tables && table_width > 0))
         return fail(PKV_EINVAL, "kv8_attention: null pointer");
-    Kv8Params p = {};
+    Kv8Params p = sizes_of(num_seqs, num_heads, num_kv_heads, head_dim, num_tokens,
+                           query_start_loc ? max_query_len : 1, max_context_len);
     p.out = out;
     p.out_st = out_stride_t;
     p.out_sh = out_stride_h;
@@ -165,23 +234,29 @@ extern "C" int pkv_kv8_attention(
     p.num_blocks = num_blocks;
     p.block_size = (int)block_size;
     p.block_shift = block_size & (block_size - 1) ? -1 : 63 - __builtin_clzll((unsigned long long)block_size);
-    p.num_kv_heads = (int)num_kv_heads;
-    p.head_dim = (int)head_dim;
     p.tables = block_tables;
     p.table_stride = table_stride;
     p.table_width = table_width;
     p.ctx_lens = context_lens;
     p.qsl = query_start_loc;
-    p.num_seqs = (int)num_seqs;
-    p.num_heads = (int)num_heads;
-    p.group = (int)(num_heads / num_kv_heads);
-    p.num_tokens = num_tokens;
-    p.max_query_len = (int)(!query_start_loc ? 1 : max_query_len && max_query_len < num_tokens ? max_query_len
-                                                                                              : num_tokens);
-    p.max_context_len = max_context_len;
     p.scale = scale;
     p.scale_log2 = scale * kLog2e;
-    p.splits = 1;
-    p.split_tiles = 0x7fffffff;
+    const uint64_t scales = (uint64_t)(uintptr_t)k_scales | (uint64_t)(uintptr_t)v_scales |
+                            (uint64_t)scale_stride_block | (uint64_t)scale_stride_head;
+    p.scales4 = scales % 4 == 0;
+    if (kv8_decode_applies(p, dtype)) {
+        const int64_t parts = kv8_decode_plan(p, host_context_lens, host_query_lens);
+        if (parts && workspace && workspace_bytes >= kMergeCounterBytes + parts) {
+            char* ws = reinterpret_cast<char*>(workspace);
+            p.ws_cnt = reinterpret_cast<uint32_t*>(ws);
+            p.ws_o = reinterpret_cast<float*>(ws + kMergeCounterBytes);
+            p.ws_ml = p.ws_o + parts / (4 * (head_dim + 2)) * head_dim;
+        }
+        switch (dtype) {
+            case PKV_FLOAT32: return launch_kv8_decode<float>(p, stream);
+            case PKV_FLOAT16: return launch_kv8_decode<_Float16>(p, stream);
+            default: return launch_kv8_decode<bf16_t>(p, stream);
+        }
+    }
     return launch_kv8_generic(p, dtype, stream);
 }

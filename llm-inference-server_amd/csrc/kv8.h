@@ -25,7 +25,11 @@ struct Kv8Params : AttnParams {
     const uint8_t* vs;
     int64_t ssb, sss, ssh;           // scale strides (bytes): block, slot, head
     int64_t max_context_len;
-    int slots;                       // decode: runs that the batch's keys are cut into, per KV head
+    bool scales4;                    // scale bytes of 4 slots (4-aligned) can be one load, if sss = 1
+    // Decode: the most runs that the batch's keys are cut into, per KV head, the units of 32
+    // keys that a run has at least, whether a run is a workgroup's (else a wave's), and the
+    // rows of a partial (ws_o, ws_ml by [slot][side][KV head][row]; null: sequences stay whole).
+    int slots, decode_min_units, decode_coop, decode_rows;
 };
 
 // 2^(b - 127), NaN for 255.
@@ -41,9 +45,16 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
     return b < 0 ? 0u : (uint32_t)b;
 }
 
-// Decode (attn_kv8_decode.hip): rows of at most 16 (token, query head) pairs per (sequence,
-// KV head). Chunks (attn_kv8_chunk.hip): 128 rows a workgroup. Both return PKV_EUNSUPPORTED
-// without an error for what they do not take; the generic kernel takes the rest.
+// Decode (kv8_decode.h): at most 16 (token, query head) pairs per (sequence, KV head). What it
+// asks of the shape, strides and addresses; its plan; its launch, by type.
+constexpr int kKv8DecodeRows = 16, kKv8DecodeMaxSeqs = 2048;
+bool kv8_decode_applies(const Kv8Params& p, int dtype);
+// Sets p's decode fields but the pointers; returns the bytes of partials that cutting takes.
+int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* host_qlen);
+template <typename T>
+int launch_kv8_decode(const Kv8Params& p, hipStream_t stream);
+
+// The rest: any shape.
 int launch_kv8_generic(const Kv8Params& p, int dtype, hipStream_t stream);
 
 }  // namespace pkv
