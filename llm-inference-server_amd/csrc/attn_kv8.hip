@@ -143,6 +143,18 @@ int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* ho
     return (int64_t)p.slots * 2 * p.num_kv_heads * p.decode_rows * (p.head_dim + 2) * 4;
 }
 
+// ------------------------------------------------------------------ chunks
+bool kv8_chunk_applies(const Kv8Params& p, int dtype) {
+    if (p.head_dim % 16 || p.head_dim < 32 || p.head_dim > 128 || p.block_shift < 0 || p.num_blocks < 1) return false;
+    if (!(p.scale > 0.f) || p.table_width * p.block_size > (1 << 30)) return false;
+    const int64_t isz = dtype == PKV_FLOAT32 ? 4 : 2;
+    const uint64_t probe = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * isz) |
+                           (uint64_t)(p.q_sh * isz) | (uint64_t)(p.out_st * isz) | (uint64_t)(p.out_sh * isz) |
+                           (uint64_t)(uintptr_t)p.k | (uint64_t)(uintptr_t)p.v | (uint64_t)p.sb | (uint64_t)p.ss |
+                           (uint64_t)p.sh;
+    return probe % 16 == 0;
+}
+
 namespace {
 
 // Whether the decode kernel takes a batch of these sizes, strides and addresses aside.
@@ -162,6 +174,14 @@ Kv8Params sizes_of(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, in
     return p;
 }
 
+// One token per sequence: the merge then finds its splits from the contexts, so the grid has to
+// hold them for any contexts up to the bound.
+SplitPlan chunk_plan(const Kv8Params& p, const int64_t* host_ctx, const int64_t* host_qlen) {
+    const bool single = p.max_query_len == 1 && p.num_tokens == p.num_seqs;
+    return prefill_split_plan(p.num_seqs, p.num_heads, p.num_kv_heads, p.head_dim, p.num_tokens,
+                              single ? nullptr : host_ctx, single ? nullptr : host_qlen, p.max_context_len);
+}
+
 bool few_rows(const Kv8Params& p) {
     return p.num_seqs <= kKv8DecodeMaxSeqs && (int64_t)p.max_query_len * p.group <= kKv8DecodeRows;
 }
@@ -179,9 +199,12 @@ extern "C" int64_t pkv_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t n
         num_seqs > 0x7fffffff || num_tokens > 0x7fffffff || num_heads % num_kv_heads)
         return 0;
     Kv8Params p = sizes_of(num_seqs, num_heads, num_kv_heads, head_dim, num_tokens, max_query_len, max_context_len);
-    if (!few_rows(p)) return 0;
-    const int64_t parts = kv8_decode_plan(p, host_context_lens, host_query_lens);
-    return parts ? kMergeCounterBytes + parts : 0;
+    if (few_rows(p)) {
+        const int64_t parts = kv8_decode_plan(p, host_context_lens, host_query_lens);
+        if (parts) return kMergeCounterBytes + parts;
+    }
+    const SplitPlan plan = chunk_plan(p, host_context_lens, host_query_lens);
+    return plan.splits > 1 ? kMergeCounterBytes + plan.total() : 0;
 }
 
 extern "C" int pkv_kv8_attention(
@@ -257,6 +280,26 @@ extern "C" int pkv_kv8_attention(
             case PKV_FLOAT16: return launch_kv8_decode<_Float16>(p, stream);
             default: return launch_kv8_decode<bf16_t>(p, stream);
         }
+    }
+    if (kv8_chunk_applies(p, dtype)) {
+        const SplitPlan plan = chunk_plan(p, host_context_lens, host_query_lens);
+        if (plan.splits > 1 && workspace && workspace_bytes >= kMergeCounterBytes + plan.total()) {
+            // Behind the counters' room, which stays zero.
+            char* ws = reinterpret_cast<char*>(workspace) + kMergeCounterBytes;
+            p.splits = plan.splits;
+            p.split_tiles = plan.split_tiles;
+            p.split_items = plan.items;
+            p.ws_rows = reinterpret_cast<int*>(ws);
+            p.ws_ml = reinterpret_cast<float*>(ws + plan.rows_bytes);
+            p.ws_o = reinterpret_cast<float*>(ws + plan.rows_bytes + plan.ml_bytes);
+        }
+        int rc;
+        switch (dtype) {
+            case PKV_FLOAT32: rc = launch_kv8_chunk<float>(p, stream); break;
+            case PKV_FLOAT16: rc = launch_kv8_chunk<_Float16>(p, stream); break;
+            default: rc = launch_kv8_chunk<bf16_t>(p, stream);
+        }
+        if (rc != PKV_EUNSUPPORTED) return rc;
     }
     return launch_kv8_generic(p, dtype, stream);
 }

@@ -1,0 +1,4 @@
+// Attention of chunks over the 8-bit cache, fp32 queries (kv8_chunk.h).
+#include "kv8_chunk.h"
+
+template int pkv::launch_kv8_chunk<float>(const pkv::Kv8Params& p, hipStream_t stream);

@@ -54,6 +54,13 @@ int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* ho
 template <typename T>
 int launch_kv8_decode(const Kv8Params& p, hipStream_t stream);
 
+// Chunks (kv8_chunk.h): 128 rows a workgroup. What it asks likewise; contexts are cut by
+// prefill_split_plan. Its launch returns PKV_EUNSUPPORTED, without an error, for grids that
+// are too large.
+bool kv8_chunk_applies(const Kv8Params& p, int dtype);
+template <typename T>
+int launch_kv8_chunk(const Kv8Params& p, hipStream_t stream);
+
 // The rest: any shape.
 int launch_kv8_generic(const Kv8Params& p, int dtype, hipStream_t stream);
 

@@ -1,0 +1,418 @@
+// Attention of chunks of new tokens over the 8-bit paged cache on MFMA (gfx950): the kernel,
+// instantiated by type in attn_kv8_chunk_*.hip. Head_dim a multiple of 16 from 32 to 128, any
+// GQA group, block sizes that are powers of two, codes in 16-byte steps, softmax scale > 0.
+//
+// Bound: MFMA and VALU for long chunks. The formulation is the 16-bit prefill kernel's
+// (attn_prefill.hip): 128 (token, query head) rows a workgroup, 32 a wave; S^T = K Q^T and
+// O^T += V^T P^T on 32x32x16, so that a lane owns one query row, its softmax is lane-local but
+// for one swap, and P^T feeds the second product from the accumulator; contexts of few rows cut
+// into runs (prefill_split_plan) and merged. What differs is the staging:
+//
+//  * 64 keys of K and V a tile are loaded as codes (16 bytes, 16 dims, a piece; a thread has
+//    head_dim / 64 pieces of each), converted to the cached values - code * 2^(b - 127) in one
+//    v_cvt_scalef32_pk a pair, exact - and written to LDS as 16-bit rows. Converting once for the
+//    workgroup instead of in each of its four waves costs a quarter of the VALU time, of which
+//    the softmax leaves little; a tile's LDS traffic is the 16-bit kernel's.
+//  * Loads of the next tile are in flight under the current one's products, its block ids and
+//    scale bytes one tile further ahead.
+//  * NaN: a row whose scale is NaN (its codes are 0) makes its key's scores NaN, also if it is
+//    V's, whose row is staged as zeros: the causal mask then hides it from rows that do not see
+//    it, which a weight of 0 times NaN would not.
+//
+// Values are bf16 for bf16 and fp32 queries (exact), fp16 for fp16 queries, halved: a row's
+// largest value may round up past fp16's. fp32 queries and weights enter as three bf16 pieces
+// each (24 bits); 16-bit types' weights are rounded to the type, as the 16-bit kernel does.
+#pragma once
+
+#include "kv8.h"
+#include "prefill_common.h"
+
+namespace pkv {
+namespace {
+
+// The 16-bit type that values take in LDS, and what they are multiplied by; and the power of two
+// that weights are multiplied by. fp16 weights below 2^-14 would lose digits: with the running
+// maximum at 2^7, and raised past 2^8 only, they reach 2^15 and keep all of them down to 2^-21.
+template <typename T>
+struct Stage {
+    typedef bf16_t E;
+    static constexpr float kFactor = 1.f;
+    static constexpr float kLift = 0.f;
+    static constexpr uint32_t kNan2 = 0x7fc07fc0u;
+    template <bool HI>
+    __device__ __forceinline__ static uint32_t cvt(uint32_t w, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+    }
+};
+template <>
+struct Stage<_Float16> {
+    typedef _Float16 E;
+    static constexpr float kFactor = 0.5f;
+    static constexpr float kLift = 7.f;
+    static constexpr uint32_t kNan2 = 0x7e007e00u;
+    template <bool HI>
+    __device__ __forceinline__ static uint32_t cvt(uint32_t w, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+    }
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void kv8_chunk_kernel(
+    const Kv8Params p) {
+    typedef typename Stage<T>::E E;
+    constexpr int DSTEPS = D / 16;            // S^T contraction steps
+    constexpr int DTILES = (D + 31) / 32;     // O^T tiles of 32 dims (the last may be half a tile)
+    constexpr int ROWB = D * 2;               // bytes of a staged row
+    constexpr int CPR = ROWB / 16;            // its 16-byte chunks
+    constexpr int PPR = D / 16;               // its pieces of 16 codes
+    constexpr int PIECES = (kKT * PPR + 255) / 256;   // per thread and tile, of K and of V
+    constexpr bool kWhole = kKT * PPR % 256 == 0;
+    constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+
+    __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kKT * D];
+    __shared__ __attribute__((aligned(1024))) uint16_t s_v0[kKT * D];
+    __shared__ __attribute__((aligned(1024))) uint16_t s_k1[kKT * D];
+    __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kKT * D];
+
+    PrefillItem it;
+    if (!prefill_item<kRows, kKT>(p, p.block_size, it)) return;
+    const uint32_t G = (uint32_t)p.group;
+    const int kvh = it.kvh, split = it.split, seq = it.seq;
+    const int64_t q_first = it.q_first;
+    const int q_len = it.q_len;
+    const int ctx = it.ctx < 0 ? 0 : it.ctx;
+    const int n_rows = q_len * (int)G;
+    const int row0 = it.row_tile * kRows;
+    const int pos0 = ctx - q_len;             // position of the sequence's first query
+    const int rows = n_rows - row0 < kRows ? n_rows - row0 : kRows;
+    const int q0 = (int)((uint32_t)row0 / G);
+    const int q_last = (int)((uint32_t)(row0 + rows - 1) / G);
+    const int kmax = pos0 + q_last + 1 < 0 ? 0 : pos0 + q_last + 1;   // keys that the workgroup sees
+    const int first_pos = pos0 + q0;
+    const int n_tiles = (kmax + kKT - 1) / kKT;
+    int t_begin = 0, t_end = n_tiles, run = n_tiles;
+    if (it.splits > 1 && n_tiles > 0) {
+        run = split_run(n_tiles, it.splits, p.split_tiles);
+        t_begin = split * run;
+        t_end = n_tiles - t_begin < run ? n_tiles : t_begin + run;
+    }
+    // A later split of a sequence whose tile ends before it; without keys the first one writes zeros.
+    if (t_begin >= n_tiles && split > 0) return;
+
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int tid = (int)threadIdx.x;
+    const int h = lane >> 5, col = lane & 31;
+    const int wrow = wave * kQT + col;
+    const bool my_live = wrow < rows;         // rows past the last one repeat it, not stored
+    const uint32_t my_row = (uint32_t)(row0 + (my_live ? wrow : rows - 1));
+    const int my_q = (int)(my_row / G);
+    const int my_head = kvh * (int)G + (int)(my_row - (uint32_t)my_q * G);
+    const int my_pos = pos0 + my_q;
+    const int wave_rows = rows - wave * kQT < kQT ? rows - wave * kQT : kQT;
+    const int wave_kmax = wave_rows > 0 ? pos0 + (int)((uint32_t)(row0 + wave * kQT + wave_rows - 1) / G) + 1 : 0;
+
+    f32x16 o[DTILES];
+#pragma unroll
+    for (int t = 0; t < DTILES; ++t) o[t] = f32x16{};
+    float m_run = kNegInf, l_run = 0.f;
+    const float scale_log2 = p.scale_log2 * (1.f / Stage<T>::kFactor);
+
+    // ---- staging: piece j of a thread is codes 16 c .. 16 c + 15 of key row r of the tile.
+    const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.k) + kvh * p.sh;
+    const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.v) + kvh * p.sh;
+    const uint8_t* ksb = p.ks + kvh * p.ssh;
+    const uint8_t* vsb = p.vs + kvh * p.ssh;
+    const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
+    int piece_row[PIECES], piece_at[PIECES];
+    uint32_t lds0[PIECES], lds1[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        const int i = 256 * j + tid;
+        const int r = i / PPR < kKT ? i / PPR : kKT - 1, c = i % PPR;
+        piece_row[j] = r;
+        piece_at[j] = 16 * c;
+        lds0[j] = (uint32_t)(r * ROWB + (((2 * c) ^ lds_swizzle<D>(r)) << 4));
+        lds1[j] = (uint32_t)(r * ROWB + (((2 * c + 1) ^ lds_swizzle<D>(r)) << 4));
+    }
+    const int in_block = p.block_size - 1;
+    struct Raw {
+        Vec16 k[PIECES], v[PIECES];
+    };
+    // Bytes of a piece's scales: K's, V's in bits 8 to 15.
+    int64_t id[PIECES];
+    uint32_t sc[PIECES];
+    Raw raw;
+    // Keys past the last one of the workgroup repeat it: masked in S, finite in V.
+    auto key_of = [&](int kt, int j) {
+        const int key = kt * kKT + piece_row[j];
+        return key < kmax ? key : kmax - 1;
+    };
+    auto load_ids = [&](int kt) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) id[j] = table[key_of(kt, j) >> p.block_shift];
+    };
+    auto load_tile = [&](int kt) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const int64_t b = (uint64_t)id[j] < (uint64_t)p.num_blocks ? id[j] : 0;   // never out of the cache
+            const int at = key_of(kt, j) & in_block;
+            const int64_t off = b * p.sb + at * p.ss + piece_at[j], so = b * p.ssb + at * p.sss;
+            raw.k[j] = load16(kc + off);
+            raw.v[j] = load16(vc + off);
+            sc[j] = (uint32_t)ksb[so] | (uint32_t)vsb[so] << 8;
+        }
+    };
+    auto store_tile = [&](uint16_t* sk, uint16_t* sv) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            if (!kWhole && 256 * j + tid >= kKT * PPR) continue;
+            const uint32_t kb = sc[j] & 255u, vb = sc[j] >> 8;
+            const bool bad = kb == (uint32_t)kScaleNan || vb == (uint32_t)kScaleNan;
+            const float ks = (bad ? 1.f : scale_of(kb)) * Stage<T>::kFactor;
+            const float vs = (bad ? 1.f : scale_of(vb)) * Stage<T>::kFactor;
+            uint32_t a[8], b[8];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                a[2 * w] = Stage<T>::template cvt<false>(raw.k[j].w[w], ks);
+                a[2 * w + 1] = Stage<T>::template cvt<true>(raw.k[j].w[w], ks);
+                b[2 * w] = Stage<T>::template cvt<false>(raw.v[j].w[w], vs);
+                b[2 * w + 1] = Stage<T>::template cvt<true>(raw.v[j].w[w], vs);
+            }
+            if (bad) {
+#pragma unroll
+                for (int w = 0; w < 8; ++w) {
+                    a[w] = Stage<T>::kNan2;
+                    b[w] = 0u;
+                }
+            }
+            store16((char*)sk + lds0[j], Vec16{{a[0], a[1], a[2], a[3]}});
+            store16((char*)sk + lds1[j], Vec16{{a[4], a[5], a[6], a[7]}});
+            store16((char*)sv + lds0[j], Vec16{{b[0], b[1], b[2], b[3]}});
+            store16((char*)sv + lds1[j], Vec16{{b[4], b[5], b[6], b[7]}});
+        }
+    };
+
+    // ---- LDS operands of this lane (as in the 16-bit kernel).
+    const int grp = lane >> 4;
+    const int tr_key = (lane & 15) >> 2;
+    const int tr_col = 16 * (grp & 1) + 4 * (lane & 3);
+    const int k_swz = lds_swizzle<D>(col);
+    const int v_cb = tr_col >> 3;
+    const int v_lo_swz = lds_swizzle<D>(4 * (grp >> 1) + tr_key);
+    const int v_hi_swz = lds_swizzle<D>(4 * (grp >> 1) + tr_key + 8);
+    const int v_byte = 8 * (lane & 1);
+    uint32_t koff[DSTEPS], voff_lo[DTILES], voff_hi[DTILES];
+#pragma unroll
+    for (int s = 0; s < DSTEPS; ++s) {
+        koff[s] = (uint32_t)(col * ROWB + (((2 * s + h) ^ k_swz) << 4));
+        asm volatile("" : "+v"(koff[s]));
+    }
+#pragma unroll
+    for (int t = 0; t < DTILES; ++t) {
+        // Columns past head_dim re-read the tile's first chunks: output rows never stored.
+        const int c = 4 * t + v_cb < CPR ? 4 * t + v_cb : 4 * t + (v_cb & 1);
+        voff_lo[t] = (uint32_t)((4 * (grp >> 1) + tr_key) * ROWB + v_byte + ((c ^ v_lo_swz) << 4));
+        voff_hi[t] = (uint32_t)((4 * (grp >> 1) + tr_key + 8) * ROWB + v_byte + ((c ^ v_hi_swz) << 4));
+        asm volatile("" : "+v"(voff_lo[t]), "+v"(voff_hi[t]));
+    }
+
+    if (t_begin < t_end) load_ids(t_begin);
+    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7], in NP pieces.
+    u32x4 qf[NP][DSTEPS];
+    {
+        const T* q = reinterpret_cast<const T*>(p.q) + (q_first + my_q) * p.q_st + (int64_t)my_head * p.q_sh;
+#pragma unroll
+        for (int s = 0; s < DSTEPS; ++s) {
+            if constexpr (sizeof(T) == 2) {
+                const Vec16 v = load16(q + s * 16 + h * 8);
+                qf[0][s] = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+            } else {
+                const Vec16 a = load16(q + s * 16 + h * 8), b = load16(q + s * 16 + h * 8 + 4);
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = __builtin_bit_cast(float, a.w[i]);
+                    x[4 + i] = __builtin_bit_cast(float, b.w[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    qf[i][s] = u32x4{Mfma<E>::pack(x[0], x[1]), Mfma<E>::pack(x[2], x[3]), Mfma<E>::pack(x[4], x[5]),
+                                     Mfma<E>::pack(x[6], x[7])};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] -= (float)(__bf16)x[e];
+                }
+            }
+        }
+    }
+
+    auto tile = [&](int kt, const uint16_t* tile_k, const uint16_t* tile_v, uint16_t* nk, uint16_t* nv) {
+        lds_barrier();                        // tile kt is staged, tile kt - 1 is done with
+        const bool more = kt + 1 < t_end;
+        if (more) load_tile(kt + 1);
+        if (kt + 2 < t_end) load_ids(kt + 2);
+        const bool sees = kt * kKT < wave_kmax;
+        if (sees) {
+            __builtin_amdgcn_s_setprio(1);
+            f32x16 st[2];
+            st[0] = f32x16{};
+            st[1] = f32x16{};
+#pragma unroll
+            for (int s = 0; s < DSTEPS; ++s)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tile_k) +
+                                                                    half * 32 * ROWB + koff[s]);
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) st[half] = Mfma<E>::run(u32x4{a.x, a.y, a.z, a.w}, qf[i][s], st[half]);
+                }
+            __builtin_amdgcn_s_setprio(0);
+            if (kt * kKT + kKT - 1 > first_pos) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = kt * kKT + half * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+                        if (key > my_pos) st[half][r] = kNegInf;
+                    }
+            }
+            float mt = kNegInf;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[half][r]);
+            mt = max_across32(mt) * scale_log2;   // scale > 0: max commutes with it
+            asm("" : "+v"(mt));
+            const bool raise = mt > m_run + kRescaleThreshold;
+            const float m_new = raise ? mt : m_run;
+            const float alpha = raise ? fast_exp2(m_run - mt) : 1.f;
+            if (__builtin_amdgcn_ballot_w64(raise)) {
+#pragma unroll
+                for (int t = 0; t < DTILES; ++t) o[t] *= alpha;
+            }
+            m_run = m_new;
+            const float m_off = m_new == kNegInf ? 0.f : m_new - Stage<T>::kLift;
+            float psum = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float e = fast_exp2(fmaf(st[half][r], scale_log2, -m_off));
+                    st[half][r] = e;
+                    psum += e;
+                }
+            psum = sum_across32(psum);
+            l_run = l_run * alpha + psum;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                f32x16& sv = st[s >> 1];
+                const int r0 = 8 * (s & 1);
+                u32x4 pb[NP];
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    pb[i] = u32x4{Mfma<E>::pack(sv[r0 + 0], sv[r0 + 1]), Mfma<E>::pack(sv[r0 + 2], sv[r0 + 3]),
+                                  Mfma<E>::pack(sv[r0 + 4], sv[r0 + 5]), Mfma<E>::pack(sv[r0 + 6], sv[r0 + 7])};
+                    if (i + 1 < NP)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sv[r0 + e] -= (float)(__bf16)sv[r0 + e];
+                }
+                const char* vgrp = reinterpret_cast<const char*>(tile_v) + ((s >> 1) * 32 + 16 * (s & 1)) * ROWB;
+#pragma unroll
+                for (int t = 0; t < DTILES; ++t) {
+                    const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_lo[t]));
+                    const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_hi[t]));
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) o[t] = Mfma<E>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
+                }
+            }
+        }
+        if (more) store_tile(nk, nv);
+    };
+    if (t_begin < t_end) {
+        load_tile(t_begin);
+        if (t_begin + 1 < t_end) load_ids(t_begin + 1);
+        store_tile(s_k0, s_v0);
+    }
+    for (int kt = t_begin; kt < t_end; kt += 2) {
+        tile(kt, s_k0, s_v0, s_k1, s_v1);
+        if (kt + 1 < t_end) tile(kt + 1, s_k1, s_v1, s_k0, s_v0);
+    }
+
+    // ---- store: the lane holds dims 32 t + 8 (r / 4) + 4 h + r % 4 of its row.
+    if (!my_live) return;
+    const int64_t tok = q_first + my_q;
+    constexpr float kBack = 1.f / Stage<T>::kFactor;
+    if (run < n_tiles && my_pos >= 0) {
+        const int64_t row = tok * p.num_heads + my_head;
+        const int64_t slot = row * p.splits + split;
+        float* po = p.ws_o + slot * D + 4 * h;
+#pragma unroll
+        for (int t = 0; t < DTILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (32 * t + 8 * i < D)
+                    *reinterpret_cast<float4*>(po + 32 * t + 8 * i) =
+                        make_float4(o[t][4 * i] * kBack, o[t][4 * i + 1] * kBack, o[t][4 * i + 2] * kBack,
+                                    o[t][4 * i + 3] * kBack);
+        // The merge skips a part whose maximum is -inf; one whose scores were all NaN has to count.
+        if (h == 0)
+            *reinterpret_cast<float2*>(p.ws_ml + slot * 2) =
+                make_float2(m_run == kNegInf && l_run != 0.f ? 0.f : m_run, l_run);
+        if (p.ws_rows && h == 0 && split == 0) p.ws_rows[row] = my_pos / (run * kKT) + 1;
+        return;
+    }
+    if (split > 0) return;
+    if (p.ws_rows && h == 0) p.ws_rows[tok * p.num_heads + my_head] = 0;   // finished here
+    const float inv = l_run == 0.f ? 0.f : kBack / l_run;                  // no key: zero
+    T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)my_head * p.out_sh;
+#pragma unroll
+    for (int t = 0; t < DTILES; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (32 * t + 8 * i >= D) continue;
+            T* to = orow + 32 * t + 8 * i + 4 * h;
+            const float4 v = make_float4(o[t][4 * i] * inv, o[t][4 * i + 1] * inv, o[t][4 * i + 2] * inv,
+                                         o[t][4 * i + 3] * inv);
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to) = v;
+            else *reinterpret_cast<uint2*>(to) = make_uint2(Mfma<T>::pack(v.x, v.y), Mfma<T>::pack(v.z, v.w));
+        }
+}
+
+// Workgroups of the flat grid, as the 16-bit kernel's.
+inline int64_t kv8_chunk_workgroups(const Kv8Params& p) {
+    const int64_t grid = ceil_div((int64_t)p.max_query_len * p.group, kRows) * p.num_seqs;
+    const int64_t fill = p.num_tokens * p.group / kRows + p.num_seqs;
+    int64_t items = (grid < fill || p.num_seqs > kPrefillSortSeqs ? grid : fill) * p.num_kv_heads;
+    if (p.splits > 1 && p.split_items > items) items = p.split_items;
+    return ceil_div(items, 8) * 8;
+}
+
+template <typename T, int D>
+int launch_kv8_chunk_d(const Kv8Params& p, hipStream_t stream) {
+    kv8_chunk_kernel<T, D><<<dim3((unsigned)kv8_chunk_workgroups(p)), 256, 0, stream>>>(p);
+    const int rc = check_launch("kv8 chunk attention");
+    if (rc || p.splits == 1) return rc;
+    const int64_t rows = p.num_tokens * p.num_heads;
+    prefill_merge_kernel<T, D><<<dim3((unsigned)ceil_div(rows, kMergeRows<D>)), 256, 0, stream>>>(p);
+    return check_launch("kv8 chunk merge");
+}
+
+}  // namespace
+
+template <typename T>
+int launch_kv8_chunk(const Kv8Params& p, hipStream_t stream) {
+    // One grid dimension; rows of a sequence in 32 bits.
+    if (kv8_chunk_workgroups(p) > 0x7fffffff) return PKV_EUNSUPPORTED;
+    if (((int64_t)p.max_query_len + kRows) * p.group > 0x7fffffff) return PKV_EUNSUPPORTED;
+    switch (p.head_dim) {
+        case 32: return launch_kv8_chunk_d<T, 32>(p, stream);
+        case 48: return launch_kv8_chunk_d<T, 48>(p, stream);
+        case 64: return launch_kv8_chunk_d<T, 64>(p, stream);
+        case 80: return launch_kv8_chunk_d<T, 80>(p, stream);
+        case 96: return launch_kv8_chunk_d<T, 96>(p, stream);
+        case 112: return launch_kv8_chunk_d<T, 112>(p, stream);
+        default: return launch_kv8_chunk_d<T, 128>(p, stream);
+    }
+}
+
+}  // namespace pkv

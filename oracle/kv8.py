@@ -41,12 +41,12 @@ def quantize(x: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
 
 def attention(q, k, v, tables, ctx, qlens, scale):
     """q [T, H, D] float64, k / v = (codes, scales) uint8 arrays [NB, bs, Hkv(, D)]. Returns
-    (out, size, slack) [T, H, D]: the exact output; sum of p |v|; and the relative error that
-    fp32 dot products of any order, exponentials and sums may put on the weights."""
+    (out, size, slack, flat): the exact output; sum of p |v|; the relative error that fp32 dot
+    products of any order, exponentials and sums may put on the weights; and sum of |v|."""
     heads, dim = q.shape[1:]
     bs, kv = k[0].shape[1:3]
     out = np.zeros(q.shape)
-    size = np.zeros(q.shape)
+    size, flat = np.zeros(q.shape), np.zeros(q.shape)
     slack = np.zeros(q.shape[:2] + (1,))
     at = 0
     for i, (n, m) in enumerate(zip(ctx, qlens)):
@@ -64,9 +64,10 @@ def attention(q, k, v, tables, ctx, qlens, scale):
                 p = w / w.sum()
                 out[at + t, h] = p @ vv
                 size[at + t, h] = p @ np.abs(vv)
+                flat[at + t, h] = np.abs(vv).sum(0)
                 # |error of a score| <= (dim + 8) half steps of the sum of its terms' sizes; it
                 # enters a weight and the sum of weights.
                 reach = (np.abs(kk) @ np.abs(q[at + t, h])).max() * abs(scale)
                 slack[at + t, h] = 2.0 ** -24 * (2 * (dim + 8) * reach + seen + 8)
         at += m
-    return out, size, slack
+    return out, size, slack, flat

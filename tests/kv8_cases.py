@@ -66,12 +66,14 @@ def batch(lens, *, heads, kv, d, bs, dtype, seed=0, device="cpu", layout=slab, w
 
 def check(s, out, scale=None, rows=slice(None), raws=None):
     """out against the exact attention: an output rounding; a rounding of each weight to the
-    type (16 bits), on the sum of their parts; and what fp32 leaves."""
+    type (16 bits), on the sum of their parts; and what fp32 leaves. fp16 weights, the largest
+    of them 2^7 at least, are off by up to half a subnormal step, 2^-25, where they are small:
+    2^-32 of each value, as the weights' sum is no less than the largest."""
     k_raw, v_raw = raws or (s.k_raw, s.v_raw)
-    want, size, slack = oracle.attention(s.q.double().cpu().numpy(), k_raw, v_raw, s.tables, s.ctx, s.new,
+    want, size, slack, flat = oracle.attention(s.q.double().cpu().numpy(), k_raw, v_raw, s.tables, s.ctx, s.new,
                                          s.scale if scale is None else scale)
     u = HALF_STEP[s.dtype]
-    tol = u * np.abs(want) + (u + slack) * size + LEAST[s.dtype]
+    tol = u * np.abs(want) + (u + slack) * size + LEAST[s.dtype] + (2.0 ** -32 * flat if s.dtype is torch.float16 else 0)
     got = out.double().cpu().numpy()
     assert got.shape == want.shape
     nan = np.isnan(want)
