@@ -122,25 +122,39 @@ bool kv8_decode_applies(const Kv8Params& p, int dtype) {
     return rows % 8 == 0 && codes % 4 == 0;
 }
 
-// Runs for every CU to hold kPerCu workgroups. A run is a workgroup's unless sequences are short
-// and (sequence, KV head) pairs fill the GPU's waves by themselves.
+// How a decode batch is cut; the bytes of partials that it takes (0: none are wanted, or there are
+// more (sequence, KV head) pairs than merge counters).
 int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* host_qlen) {
-    constexpr int kCus = 256, kPerCu = 3;
-    int64_t units = 0;
-    for (int i = 0; i < p.num_seqs; ++i) {
-        const int64_t c = host_ctx ? host_ctx[i] : p.max_context_len;
-        if (!host_qlen || host_qlen[i] > 0) units += c > 32 ? ceil_div(c, 32) : 1;
-    }
-    const int64_t pairs = (int64_t)p.num_seqs * p.num_kv_heads;
-    p.decode_coop = pairs < 4 * kCus * kPerCu || units >= 8 * (int64_t)p.num_seqs;
-    p.decode_min_units = p.decode_coop ? 8 : 2;
+    constexpr int64_t kWorkgroups = 256 * 3;    // that the GPU holds
+    constexpr int64_t kEvenUnits = 24;          // per workgroup of even runs
+    const int64_t heads = p.num_kv_heads, seqs = p.num_seqs, pairs = seqs * heads;
+    int64_t units = 0, runs = 0;
+    auto each = [&](auto f) {
+        for (int64_t i = 0; i < seqs; ++i) {
+            if (host_qlen && host_qlen[i] <= 0) continue;
+            const int64_t c = host_ctx ? host_ctx[i] : p.max_context_len;
+            f(c > 32 ? ceil_div(c, 32) : 1);
+        }
+    };
+    each([&](int64_t u) { units += u; });
     p.decode_rows = (int)((int64_t)p.max_query_len * p.group);
-    int64_t most = kCus * kPerCu * (p.decode_coop ? 1 : 4) / p.num_kv_heads;
-    const int64_t bound = units / p.decode_min_units;
-    most = most < bound ? most : bound;
-    p.slots = (int)(most < 1 ? 1 : most);
-    if (pairs * 4 > kMergeCounterBytes) return 0;
-    return (int64_t)p.slots * 2 * p.num_kv_heads * p.decode_rows * (p.head_dim + 2) * 4;
+    const bool cuts = pairs * 4 <= kMergeCounterBytes;
+    auto bytes = [&](int64_t numbers) { return numbers * heads * p.decode_rows * (p.head_dim + 2) * 4; };
+    if (cuts && units * heads >= kWorkgroups * kEvenUnits) {
+        p.decode_mode = kKv8Even;
+        p.decode_min_units = 8;
+        const int64_t most = kWorkgroups / heads;
+        p.decode_slots = p.decode_grid = (int)(most < 1 ? 1 : most);
+        return bytes(2 * p.decode_slots);
+    }
+    p.decode_mode = pairs >= kWorkgroups ? kKv8WaveRuns : kKv8Runs;
+    p.decode_min_units = p.decode_mode == kKv8Runs ? 8 : 4;
+    const int64_t most = kWorkgroups * (p.decode_mode == kKv8Runs ? 1 : 4) / heads;
+    p.decode_slots = (int)(most < 1 ? 1 : most);
+    each([&](int64_t u) { runs += ceil_div(u, p.decode_min_units); });
+    const int64_t room = p.decode_slots > 2 * seqs ? p.decode_slots : 2 * seqs;
+    p.decode_grid = (int)(runs < room ? runs > seqs ? runs : seqs : room);
+    return cuts && runs > seqs ? bytes(p.decode_grid) : 0;
 }
 
 // ------------------------------------------------------------------ chunks
@@ -274,6 +288,10 @@ extern "C" int pkv_kv8_attention(
             p.ws_cnt = reinterpret_cast<uint32_t*>(ws);
             p.ws_o = reinterpret_cast<float*>(ws + kMergeCounterBytes);
             p.ws_ml = p.ws_o + parts / (4 * (head_dim + 2)) * head_dim;
+        } else if (p.decode_mode == kKv8Even) {
+            // No room for partials: a workgroup a sequence.
+            p.decode_mode = kKv8Runs;
+            p.decode_grid = p.num_seqs;
         }
         switch (dtype) {
             case PKV_FLOAT32: return launch_kv8_decode<float>(p, stream);

@@ -26,10 +26,10 @@ struct Kv8Params : AttnParams {
     int64_t ssb, sss, ssh;           // scale strides (bytes): block, slot, head
     int64_t max_context_len;
     bool scales4;                    // scale bytes of 4 slots (4-aligned) can be one load, if sss = 1
-    // Decode: the most runs that the batch's keys are cut into, per KV head, the units of 32
-    // keys that a run has at least, whether a run is a workgroup's (else a wave's), and the
-    // rows of a partial (ws_o, ws_ml by [slot][side][KV head][row]; null: sequences stay whole).
-    int slots, decode_min_units, decode_coop, decode_rows;
+    // Decode: how the batch's keys are cut (kKv8Even ...), into how many runs per KV head at most,
+    // the grid's room for them, the units of 32 keys that a run has at least, and the rows of a
+    // partial (ws_o, ws_ml by [number][KV head][row]; null: sequences stay whole).
+    int decode_mode, decode_slots, decode_grid, decode_min_units, decode_rows;
 };
 
 // 2^(b - 127), NaN for 255.
@@ -47,6 +47,7 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
 
 // Decode (kv8_decode.h): at most 16 (token, query head) pairs per (sequence, KV head). What it
 // asks of the shape, strides and addresses; its plan; its launch, by type.
+enum { kKv8Even, kKv8Runs, kKv8WaveRuns };
 constexpr int kKv8DecodeRows = 16, kKv8DecodeMaxSeqs = 2048;
 bool kv8_decode_applies(const Kv8Params& p, int dtype);
 // Sets p's decode fields but the pointers; returns the bytes of partials that cutting takes.

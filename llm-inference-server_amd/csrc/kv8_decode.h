@@ -188,93 +188,60 @@ struct Part {
     }
 };
 
+// LDS of a workgroup: the waves' parts of a segment.
+template <int D>
+struct DecodeLds {
+    __attribute__((aligned(16))) float o[4][kDecodeRows * D];
+    float2 ml[4][kDecodeRows];
+    uint32_t arrived[4];
+};
+
+__device__ __forceinline__ int decode_ctx(const Kv8Params& p, int seq) {
+    const int64_t cap = p.table_width * (int64_t)p.block_size, c = p.ctx_lens[seq];
+    return (int)(c < 0 ? 0 : c < cap ? c : cap);
+}
+// Units of a sequence; one that has queries has one at least.
+__device__ __forceinline__ int decode_units(const Kv8Params& p, int seq) {
+    const int u = (int)(((uint32_t)decode_ctx(p, seq) + kUnit - 1) / kUnit);
+    if (p.qsl && p.qsl[seq + 1] <= p.qsl[seq]) return 0;
+    return u > 0 ? u : 1;
+}
+
+// The threads of a run: its workgroup's, or its wave's.
+template <bool COOP>
+__device__ __forceinline__ void run_sync() {
+    if constexpr (COOP) lds_barrier(); else wave_lds_sync();
+}
+
+// Units [a, b) of sequence `seq` (all of them: `whole`) for KV head kvh. Else this is one of the
+// `parts` that the sequence is cut into: its partial is number own(), the k-th one part(k).
 // BIG: block sizes from 16 up, where 16 keys share a block and addresses are uniform.
-template <typename T, int D, bool BIG>
-__global__ __launch_bounds__(256) void kv8_decode_kernel(const Kv8Params p) {
+template <typename T, int D, bool BIG, bool COOP, typename Own, typename PartOf>
+__device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>& lds, int seq, int kvh, int a, int b,
+                                               bool whole, int parts, Own own, PartOf part_of) {
     constexpr int KD = D / 16;                  // dwords of K a lane holds of each row
     constexpr int KS = (D + 31) / 32;           // contraction steps of S^T
     // Neighbouring dims of V that a lane holds: 8 at head_dim 128, else 4 of each 64.
     constexpr int VD = D == 128 ? 2 : (D + 63) / 64;   // dwords
     constexpr int NQ = Qk<T>::kPieces, NP = sizeof(T) == 4 ? 3 : 2;
+    constexpr int NI = BIG ? 1 : 4;
 
-    __shared__ int s_before[kDecodeMaxSeqs + 1];
-    __shared__ int s_wave[4];
-    __shared__ __attribute__((aligned(16))) float s_o[4][kDecodeRows * D];
-    __shared__ float2 s_ml[4][kDecodeRows];
-    __shared__ uint32_t s_arrived[4];
-
-    const int tid = (int)threadIdx.x, lane = lane_id();
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int n = lane & 15, kb = lane >> 4;
-    const int G = p.group;
-    const int64_t cap = p.table_width * (int64_t)p.block_size;
+    const int G = p.group, heads = p.num_kv_heads;
+    const int step = COOP ? 4 : 1;
+    int x = a + (COOP ? wave : 0);
 
-    // ---- units before each sequence. A sequence with queries has one unit at least.
-    auto ctx_of = [&](int i) {
-        const int64_t c = p.ctx_lens[i];
-        return (int)(c < 0 ? 0 : c < cap ? c : cap);
-    };
-    auto units_of = [&](int i) {
-        if (p.qsl && p.qsl[i + 1] <= p.qsl[i]) return 0;
-        const int u = (int)(((uint32_t)ctx_of(i) + kUnit - 1) / kUnit);
-        return u > 0 ? u : 1;
-    };
-    const int per = (p.num_seqs + 255) / 256, first = tid * per;
-    {
-        int own = 0, u[8];                      // 2048 sequences over 256 threads
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            u[j] = j < per && first + j < p.num_seqs ? units_of(first + j) : 0;
-            own += u[j];
-        }
-        int run = own;
-#pragma unroll
-        for (int by = 1; by < 64; by *= 2) {
-            const int up = __shfl_up(run, by);
-            if (lane >= by) run += up;
-        }
-        if (lane == 63) s_wave[wave] = run;
-        __syncthreads();
-        run -= own;
-        for (int w = 0; w < wave; ++w) run += s_wave[w];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < per && first + j < p.num_seqs) {
-                s_before[first + j] = run;
-                run += u[j];
-            }
-        if (tid == 0) s_before[p.num_seqs] = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
-        __syncthreads();
-    }
-    const int total = __builtin_amdgcn_readfirstlane(s_before[p.num_seqs]);
-
-    // ---- this run: KV head, slot, units [u0, u1).
-    const bool coop = p.decode_coop != 0;
-    const int heads = p.num_kv_heads;
-    int slots = total / p.decode_min_units;
-    slots = slots < 1 ? 1 : slots < p.slots ? slots : p.slots;
-    int kvh, slot;
-    {
-        // Workgroup L is on XCD L % 8: the heads of 8 slots take 8 * heads workgroups, one
-        // slot an XCD.
-        const int id = coop ? (int)blockIdx.x : ((int)blockIdx.x >> 3) * 32 + (int)(blockIdx.x & 7) + 8 * wave;
-        const int set = id / (8 * heads), in = id % (8 * heads);
-        slot = set * 8 + (in & 7);
-        kvh = in >> 3;
-    }
-    if (slot >= slots) return;                  // uniform in the workgroup where it cooperates
-    const int u0 = (int)((int64_t)slot * total / slots), u1 = (int)((int64_t)(slot + 1) * total / slots);
-    int seq = 0;
-    {
-        int lo = 0, hi = p.num_seqs;            // the last sequence with s_before <= u0
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (s_before[mid] <= u0) lo = mid; else hi = mid;
-        }
-        seq = __builtin_amdgcn_readfirstlane(lo);
-        // Sequences whole (no room for partials): those that begin in this run.
-        if (!p.ws_o && s_before[seq] < u0) ++seq;
-    }
+    const int ctx = __builtin_amdgcn_readfirstlane(decode_ctx(p, seq));
+    const int64_t q_first = p.qsl ? p.qsl[seq] : seq;
+    const int q_len = __builtin_amdgcn_readfirstlane(p.qsl ? (int)(p.qsl[seq + 1] - q_first) : 1);
+    const int rows = q_len * G < kDecodeRows ? q_len * G : kDecodeRows;
+    const int pos0 = ctx - q_len;               // of the first token
+    const int row = n < rows ? n : rows - 1;
+    const int limit = pos0 + row / G;           // last key that the row sees
+    auto row_token = [&](int r) { return q_first + r / G; };
+    auto row_head = [&](int r) { return (int64_t)kvh * G + r % G; };
 
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.k) + kvh * p.sh;
     const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.v) + kvh * p.sh;
@@ -291,370 +258,528 @@ __global__ __launch_bounds__(256) void kv8_decode_kernel(const Kv8Params p) {
         v_off[c] = (uint32_t)(d < D ? d : 0) + (BIG ? (uint32_t)(4 * kb * p.ss) : 0u);
     }
     const uint32_t s_off = BIG ? (uint32_t)(4 * kb * p.sss) : 0u;
-    const int step = coop ? 4 : 1, turn = coop ? wave : 0;
-    // Among the threads of a run: its workgroup, or its wave.
-    auto sync = [&]() {
-        if (coop) lds_barrier(); else wave_lds_sync();
-    };
 
     struct Unit {
         uint32_t k[2][KD], v[2][4][VD], ks[2], vs[2];
     };
+    // ---- block ids of a unit. BIG: lane l holds that of 16-key tile l % 2. Else each lane
+    // those of its K rows and V row groups. Indexes stop at the context's last block.
+    const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
+    const int last = (ctx - 1) >> p.block_shift;
+    auto load_ids = [&](int u, int64_t (&ids)[NI]) {
+        auto id = [&](int key) {
+            const int at = key >> p.block_shift;
+            return table[at < last ? at : last];
+        };
+        if constexpr (BIG) {
+            ids[0] = id(kUnit * u + 16 * (lane & 1));
+        } else {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                ids[t] = id(kUnit * u + 16 * t + n);
+                ids[2 + t] = id(kUnit * u + 16 * t + 4 * kb);
+            }
+        }
+    };
+    const int in_block = p.block_size - 1;
+    auto load_unit = [&](int u, const int64_t (&ids)[NI], Unit& f) {
+        auto inside = [&](int64_t id) { return (uint64_t)id < (uint64_t)p.num_blocks ? id : 0; };   // never out of the cache
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int64_t k_id = inside(BIG ? readlane64(ids[0], t) : ids[BIG ? 0 : t]);
+            const int64_t v_id = BIG ? k_id : inside(ids[BIG ? 0 : 2 + t]);
+            const int k_at = (kUnit * u + 16 * t + (BIG ? 0 : n)) & in_block;
+            const int v_at = (kUnit * u + 16 * t + (BIG ? 0 : 4 * kb)) & in_block;
+            const uint8_t* k = kc + (k_id * p.sb + k_at * p.ss);
+            const uint8_t* v = vc + (v_id * p.sb + v_at * p.ss);
+            load_dwords<KD>(k + k_off, f.k[t]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint8_t* vr = v + r * p.ss;
+                if constexpr (D == 128) {
+                    load_dwords<2>(vr + v_off[0], f.v[t][r]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < VD; ++c)
+                        f.v[t][r][c] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vr + v_off[c]));
+                }
+            }
+            const int64_t so = v_id * p.ssb + v_at * p.sss;
+            const uint8_t* ks = ksb + so + s_off;
+            const uint8_t* vs = vsb + so + s_off;
+            if (scales_together) {
+                f.ks[t] = *reinterpret_cast<const uint32_t*>(ks);
+                f.vs[t] = *reinterpret_cast<const uint32_t*>(vs);
+            } else {
+                f.ks[t] = f.vs[t] = 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    f.ks[t] |= (uint32_t)ks[r * p.sss] << (8 * r);
+                    f.vs[t] |= (uint32_t)vs[r * p.sss] << (8 * r);
+                }
+            }
+        }
+    };
 
+    // The first unit's ids, the queries, then its rows: in this order no load waits for one that it
+    // does not need.
+    Unit f, g;
+    int64_t ids[NI];
+    const bool any = ctx > 0 && x < b;
+    if (any) load_ids(x, ids);
+    // Q^T: elements [kb D / 4, + D / 4) of the lane's row, 8 a step.
+    constexpr int QW = D / 4 * (int)sizeof(T) / 8;
+    uint2 qraw[QW];
+    {
+        const T* q = reinterpret_cast<const T*>(p.q) + row_token(row) * p.q_st + row_head(row) * p.q_sh + kb * (D / 4);
+#pragma unroll
+        for (int i = 0; i < QW; ++i) qraw[i] = reinterpret_cast<const uint2*>(q)[i];
+    }
+    if (any) {
+        load_unit(x, ids, f);
+        load_ids(x + step, ids);
+    }
+    u32x4 qf[NQ][KS];
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+        uint32_t w[NQ][4] = {};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if (8 * j + 4 * half >= D / 4) continue;
+            if constexpr (sizeof(T) == 2) {
+                w[0][2 * half] = qraw[2 * j + half].x;
+                w[0][2 * half + 1] = qraw[2 * j + half].y;
+            } else {
+                const uint2 u = qraw[4 * j + 2 * half], v = qraw[4 * j + 2 * half + 1];
+                float r[4] = {__builtin_bit_cast(float, u.x), __builtin_bit_cast(float, u.y),
+                              __builtin_bit_cast(float, v.x), __builtin_bit_cast(float, v.y)};
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    w[i][2 * half] = pack_bf16(r[0], r[1]);
+                    w[i][2 * half + 1] = pack_bf16(r[2], r[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[e] -= (float)(__bf16)r[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) qf[i][j] = u32x4{w[i][0], w[i][1], w[i][2], w[i][3]};
+    }
+
+    f32x4 o[4 * VD];
+#pragma unroll
+    for (int i = 0; i < 4 * VD; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = kNegInf, l_run = 0.f;         // l: this lane's keys only, until the end
+
+    auto compute = [&](int u, Unit& f) {
+        const int key0 = kUnit * u;
+        const bool masked = key0 + kUnit - 1 > pos0;         // some row does not see some key
+        float s[8], vs[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+                const u32x4 kf = Qk<T>::keys(f.k[t][2 * j], 2 * j + 1 < KD ? f.k[t][2 * j + 1 < KD ? 2 * j + 1 : 0] : 0u);
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) st = Qk<T>::run(kf, qf[i][j], st);
+            }
+            float ks4[4], vs4[4];
+            scales4(f.ks[t], ks4);
+            scales4(f.vs[t], vs4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[4 * t + r] = st[r] * ks4[r] * p.scale_log2;
+                vs[4 * t + r] = vs4[r];
+            }
+        }
+        if (masked) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int key = key0 + 16 * (e >> 2) + 4 * kb + (e & 3);
+                if (key > limit) s[e] = kNegInf;
+                // Slots behind the context hold anything: 0 times a NaN would be NaN.
+                if (key >= ctx)
+#pragma unroll
+                    for (int c = 0; c < VD; ++c) f.v[e >> 2][e & 3][c] = 0;
+            }
+        }
+        float mt = s[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mt = fmaxf(mt, s[e]);
+        mt = max_across32(max_across16(mt));
+        const bool raise = mt > m_run + kLazy;
+        const float m_new = raise ? mt : m_run;
+        if (__builtin_amdgcn_ballot_w64(raise)) {
+            const float alpha = raise ? fast_exp2(m_run - m_new) : 1.f;
+#pragma unroll
+            for (int i = 0; i < 4 * VD; ++i) o[i] *= alpha;
+            l_run *= alpha;
+            m_run = m_new;
+        }
+        const float m_off = m_run == kNegInf ? 0.f : m_run;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float pe = fast_exp2(s[e] - m_off);
+            l_run += pe;
+            w[e] = pe * vs[e];
+        }
+        if (masked) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (key0 + 16 * (e >> 2) + 4 * kb + (e & 3) > limit) w[e] = 0.f;
+        }
+        u32x4 pf[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            pf[i] = u32x4{pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3]), pack_bf16(w[4], w[5]), pack_bf16(w[6], w[7])};
+            if (i + 1 < NP)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] -= (float)(__bf16)w[e];
+        }
+#pragma unroll
+        for (int c = 0; c < VD; ++c) {
+            uint32_t d0[4], d1[4];
+            const uint32_t r0[4] = {f.v[0][0][c], f.v[0][1][c], f.v[0][2][c], f.v[0][3][c]};
+            const uint32_t r1[4] = {f.v[1][0][c], f.v[1][1][c], f.v[1][2][c], f.v[1][3][c]};
+            transpose4(r0, d0);
+            transpose4(r1, d1);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const u32x4 vf = u32x4{codes_bf16<false>(d0[j]), codes_bf16<true>(d0[j]), codes_bf16<false>(d1[j]),
+                                       codes_bf16<true>(d1[j])};
+#pragma unroll
+                for (int i = 0; i < NP; ++i) o[4 * c + j] = mfma_bf16(vf, pf[i], o[4 * c + j]);
+            }
+        }
+    };
+
+    if (any)
+        while (true) {
+            if (x + step < b) {
+                load_unit(x + step, ids, g);
+                load_ids(x + 2 * step, ids);
+            }
+            compute(x, f);
+            x += step;
+            if (x >= b) break;
+            if (x + step < b) {
+                load_unit(x + step, ids, f);
+                load_ids(x + 2 * step, ids);
+            }
+            compute(x, g);
+            x += step;
+            if (x >= b) break;
+        }
+
+    // ---- the waves' parts meet in LDS, row by row.
+    l_run = sum_across32(sum_across16(l_run));
+    if (n < rows) {
+#pragma unroll
+        for (int c = 0; c < VD; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = D == 128 ? 8 * (4 * kb + r) + 4 * c : 64 * c + 4 * (4 * kb + r);
+                if (d < D)
+                    *reinterpret_cast<float4*>(&lds.o[wave][n * D + d]) =
+                        make_float4(o[4 * c][r], o[4 * c + 1][r], o[4 * c + 2][r], o[4 * c + 3][r]);
+            }
+        if (kb == 0) lds.ml[wave][n] = make_float2(m_run, l_run);
+    }
+    run_sync<COOP>();
+    constexpr int nthr = COOP ? 256 : 64;
+    const int thr = COOP ? (int)threadIdx.x : lane, wave0 = COOP ? 0 : wave;
+    const int items = rows * (D / 4);           // 4 elements of a row each
+    auto out4 = [&](int e, const Part& x4) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4;
+        store4<T>(reinterpret_cast<T*>(p.out) + row_token(r) * p.out_st + row_head(r) * p.out_sh + d, x4.result());
+    };
+    auto partial = [&](int64_t number, int r) { return (number * heads + kvh) * p.decode_rows + r; };
+    for (int e = thr; e < items; e += nthr) {
+        const int r = e / (D / 4);
+        Part acc = {kNegInf, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+        for (int w = 0; w < (COOP ? 4 : 1); ++w) {
+            const float2 ml = lds.ml[wave0 + w][r];
+            acc.add(ml.x, ml.y, *reinterpret_cast<const float4*>(&lds.o[wave0 + w][e * 4]));
+        }
+        if (whole) {
+            out4(e, acc);
+        } else {
+            const int64_t at = partial(own(), r);
+            uint64_t* po = reinterpret_cast<uint64_t*>(p.ws_o + at * D + e % (D / 4) * 4);
+            agent_store(po, pair_bits(acc.o.x, acc.o.y));
+            agent_store(po + 1, pair_bits(acc.o.z, acc.o.w));
+            if (e % (D / 4) == 0) agent_store(reinterpret_cast<uint64_t*>(p.ws_ml + at * 2), pair_bits(acc.m, acc.l));
+        }
+    }
+    if (!whole) {
+        // The stores have reached the agent's coherence point before the counter moves (a
+        // release fence would write back the XCD's whole L2 instead).
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        run_sync<COOP>();
+        uint32_t* cnt = p.ws_cnt + ((int64_t)seq * heads + kvh);
+        if (thr == 0) lds.arrived[wave0] = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        run_sync<COOP>();
+        if (__builtin_amdgcn_readfirstlane(lds.arrived[wave0]) == (uint32_t)(parts - 1)) {
+            if (thr == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            // Threads beyond the items share the parts: group g takes g, g + groups, ...; group 0
+            // then adds the groups up, in order.
+            int groups = 1;
+            while (groups * 2 * items <= nthr) groups *= 2;
+            const int g = groups > 1 ? thr / items : 0;
+            float* so = lds.o[wave0];           // the parts are out: free (8 floats a thread)
+            constexpr int CH = 4;               // partials whose loads are in flight together
+            for (int e0 = 0; e0 < items; e0 += nthr) {
+                const int e = e0 + thr - g * items, r = e / (D / 4);
+                const bool mine = g < groups && e < items;
+                Part acc = {kNegInf, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+                for (int s = g; mine && s < parts; s += CH * groups) {
+                    uint64_t ml[CH], oa[CH], ob[CH];
+#pragma unroll
+                    for (int j = 0; j < CH; ++j) {
+                        const int64_t at = partial(part_of(s + j * groups < parts ? s + j * groups : parts - 1), r);
+                        const uint64_t* po = reinterpret_cast<const uint64_t*>(p.ws_o + at * D + e % (D / 4) * 4);
+                        ml[j] = agent_load(reinterpret_cast<const uint64_t*>(p.ws_ml + at * 2));
+                        oa[j] = agent_load(po);
+                        ob[j] = agent_load(po + 1);
+                    }
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (s + j * groups < parts)
+                            acc.add(lo_of(ml[j]), hi_of(ml[j]),
+                                    make_float4(lo_of(oa[j]), hi_of(oa[j]), lo_of(ob[j]), hi_of(ob[j])));
+                }
+                if (groups > 1) {
+                    if (mine && g > 0) {
+                        float* to = so + ((g - 1) * items + e) * 8;
+                        *reinterpret_cast<float4*>(to) = acc.o;
+                        *reinterpret_cast<float2*>(to + 4) = make_float2(acc.m, acc.l);
+                    }
+                    run_sync<COOP>();
+                    for (int k = 0; mine && g == 0 && k < groups - 1; ++k) {
+                        const float* from = so + (k * items + e) * 8;
+                        const float2 ml = *reinterpret_cast<const float2*>(from + 4);
+                        acc.add(ml.x, ml.y, *reinterpret_cast<const float4*>(from));
+                    }
+                }
+                if (mine && g == 0) out4(e, acc);
+            }
+        }
+    }
+}
+
+// (Slot, KV head) of a workgroup or wave: the heads of 8 slots take 8 * heads of them, one slot an
+// XCD (workgroup L runs on XCD L % 8).
+template <bool COOP>
+__device__ __forceinline__ void decode_place(const Kv8Params& p, int wave, int& slot, int& kvh) {
+    const int id = COOP ? (int)blockIdx.x : ((int)blockIdx.x >> 3) * 32 + (int)(blockIdx.x & 7) + 8 * wave;
+    const int set = id / (8 * p.num_kv_heads), in = id - set * (8 * p.num_kv_heads);
+    slot = set * 8 + (in & 7);
+    kvh = in >> 3;
+}
+
+// Exclusive running sums of v over the workgroup's 256 threads, and their total.
+__device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
+    const int lane = lane_id(), wave = (int)(threadIdx.x >> 6);
+    int run = v;
+#pragma unroll
+    for (int by = 1; by < 64; by *= 2) {
+        const int up = __shfl_up(run, by);
+        if (lane >= by) run += up;
+    }
+    lds_barrier();                              // s_wave's last readers are done
+    if (lane == 63) s_wave[wave] = run;
+    lds_barrier();
+    total = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    run -= v;
+    for (int w = 0; w < wave; ++w) run += s_wave[w];
+    return run;
+}
+constexpr int kDecodePer = kDecodeMaxSeqs / 256;    // sequences per thread, at most
+
+// Even runs: slot s of S takes units [s U / S, (s + 1) U / S) of all the batch's U, sequence after
+// sequence.
+template <typename T, int D, bool BIG>
+__global__ __launch_bounds__(256) void kv8_decode_even_kernel(const Kv8Params p) {
+    __shared__ int s_before[kDecodeMaxSeqs + 1];
+    __shared__ int s_wave[4];
+    __shared__ DecodeLds<D> lds;
+    const int per = (p.num_seqs + 255) / 256, first = (int)threadIdx.x * per;
+    int total;
+    {
+        int own = 0, u[kDecodePer];
+#pragma unroll
+        for (int j = 0; j < kDecodePer; ++j) {
+            u[j] = j < per && first + j < p.num_seqs ? decode_units(p, first + j) : 0;
+            own += u[j];
+        }
+        int run = block_scan(own, s_wave, total);
+#pragma unroll
+        for (int j = 0; j < kDecodePer; ++j)
+            if (j < per && first + j < p.num_seqs) {
+                s_before[first + j] = run;
+                run += u[j];
+            }
+        if (threadIdx.x == 0) s_before[p.num_seqs] = total;
+        lds_barrier();
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    int slots = total / p.decode_min_units, slot, kvh;
+    slots = slots < 1 ? 1 : slots < p.decode_slots ? slots : p.decode_slots;
+    decode_place<true>(p, 0, slot, kvh);
+    if (slot >= slots) return;
+    const int u0 = (int)((int64_t)slot * total / slots), u1 = (int)((int64_t)(slot + 1) * total / slots);
+    int seq = 0;
+    for (int hi = p.num_seqs; hi - seq > 1;) {      // the last sequence with s_before <= u0
+        const int mid = (seq + hi) >> 1;
+        if (s_before[mid] <= u0) seq = mid; else hi = mid;
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
     for (; seq < p.num_seqs; ++seq) {
         const int before = __builtin_amdgcn_readfirstlane(s_before[seq]);
         const int after = __builtin_amdgcn_readfirstlane(s_before[seq + 1]);
         if (before >= u1) break;
         if (after == before) continue;
-        const int a = p.ws_o && before < u0 ? u0 - before : 0;
-        const int b = p.ws_o && after > u1 ? u1 - before : after - before;
+        const int a = before < u0 ? u0 - before : 0, b = after > u1 ? u1 - before : after - before;
         const bool whole = a == 0 && b == after - before;
-
-        const int ctx = __builtin_amdgcn_readfirstlane(ctx_of(seq));
-        const int64_t q_first = p.qsl ? p.qsl[seq] : seq;
-        const int q_len = __builtin_amdgcn_readfirstlane(p.qsl ? (int)(p.qsl[seq + 1] - q_first) : 1);
-        const int rows = q_len * G < kDecodeRows ? q_len * G : kDecodeRows;
-        const int pos0 = ctx - q_len;           // of the first token
-        const int row = n < rows ? n : rows - 1;
-        const int limit = pos0 + row / G;       // last key that the row sees
-        auto row_token = [&](int r) { return q_first + r / G; };
-        auto row_head = [&](int r) { return (int64_t)kvh * G + r % G; };
-
-        // ---- Q^T: elements [kb D / 4, + D / 4) of the lane's row, 8 a step.
-        u32x4 qf[NQ][KS];
-        {
-            const T* q = reinterpret_cast<const T*>(p.q) + row_token(row) * p.q_st + row_head(row) * p.q_sh + kb * (D / 4);
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                uint32_t w[NQ][4] = {};
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (8 * j + 4 * half >= D / 4) continue;
-                    if constexpr (sizeof(T) == 2) {
-                        const u32x2 v = *reinterpret_cast<const u32x2*>(q + 8 * j + 4 * half);
-                        w[0][2 * half] = v.x;
-                        w[0][2 * half + 1] = v.y;
-                    } else {
-                        const float2 x = *reinterpret_cast<const float2*>(q + 8 * j + 4 * half);
-                        const float2 y = *reinterpret_cast<const float2*>(q + 8 * j + 4 * half + 2);
-                        float r[4] = {x.x, x.y, y.x, y.y};
-#pragma unroll
-                        for (int i = 0; i < NQ; ++i) {
-                            w[i][2 * half] = pack_bf16(r[0], r[1]);
-                            w[i][2 * half + 1] = pack_bf16(r[2], r[3]);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) r[e] -= (float)(__bf16)r[e];
-                        }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) qf[i][j] = u32x4{w[i][0], w[i][1], w[i][2], w[i][3]};
-            }
-        }
-
-        f32x4 o[4 * VD];
-#pragma unroll
-        for (int i = 0; i < 4 * VD; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m_run = kNegInf, l_run = 0.f;     // l: this lane's keys only, until the end
-
-        // ---- block ids of a unit. BIG: lane l holds that of 16-key tile l % 2. Else each lane
-        // those of its K rows and V row groups. Indexes stop at the context's last block.
-        const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
-        const int last = (ctx - 1) >> p.block_shift;
-        constexpr int NI = BIG ? 1 : 4;
-        auto load_ids = [&](int x, int64_t (&ids)[NI]) {
-            auto id = [&](int key) {
-                const int at = key >> p.block_shift;
-                const int64_t b = table[at < last ? at : last];
-                return (uint64_t)b < (uint64_t)p.num_blocks ? b : 0;   // never followed out of the cache
-            };
-            if constexpr (BIG) {
-                ids[0] = id(kUnit * x + 16 * (lane & 1));
-            } else {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    ids[t] = id(kUnit * x + 16 * t + n);
-                    ids[2 + t] = id(kUnit * x + 16 * t + 4 * kb);
-                }
-            }
-        };
-        const int in_block = p.block_size - 1;
-        auto load_unit = [&](int x, const int64_t (&ids)[NI], Unit& f) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int64_t k_id = BIG ? readlane64(ids[0], t) : ids[BIG ? 0 : t];
-                const int64_t v_id = BIG ? k_id : ids[BIG ? 0 : 2 + t];
-                const int k_at = (kUnit * x + 16 * t + (BIG ? 0 : n)) & in_block;
-                const int v_at = (kUnit * x + 16 * t + (BIG ? 0 : 4 * kb)) & in_block;
-                const uint8_t* k = kc + (k_id * p.sb + k_at * p.ss);
-                const uint8_t* v = vc + (v_id * p.sb + v_at * p.ss);
-                load_dwords<KD>(k + k_off, f.k[t]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint8_t* vr = v + r * p.ss;
-                    if constexpr (D == 128) {
-                        load_dwords<2>(vr + v_off[0], f.v[t][r]);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < VD; ++c)
-                            f.v[t][r][c] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vr + v_off[c]));
-                    }
-                }
-                const int64_t so = v_id * p.ssb + v_at * p.sss;
-                const uint8_t* ks = ksb + so + s_off;
-                const uint8_t* vs = vsb + so + s_off;
-                if (scales_together) {
-                    f.ks[t] = *reinterpret_cast<const uint32_t*>(ks);
-                    f.vs[t] = *reinterpret_cast<const uint32_t*>(vs);
-                } else {
-                    f.ks[t] = f.vs[t] = 0;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        f.ks[t] |= (uint32_t)ks[r * p.sss] << (8 * r);
-                        f.vs[t] |= (uint32_t)vs[r * p.sss] << (8 * r);
-                    }
-                }
-            }
-        };
-
-        auto compute = [&](int x, Unit& f) {
-            const int key0 = kUnit * x;
-            const bool masked = key0 + kUnit - 1 > pos0;     // some row does not see some key
-            float s[8], vs[8];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    const u32x4 kf = Qk<T>::keys(f.k[t][2 * j], 2 * j + 1 < KD ? f.k[t][2 * j + 1 < KD ? 2 * j + 1 : 0] : 0u);
-#pragma unroll
-                    for (int i = 0; i < NQ; ++i) st = Qk<T>::run(kf, qf[i][j], st);
-                }
-                float ks4[4], vs4[4];
-                scales4(f.ks[t], ks4);
-                scales4(f.vs[t], vs4);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[4 * t + r] = st[r] * ks4[r] * p.scale_log2;
-                    vs[4 * t + r] = vs4[r];
-                }
-            }
-            if (masked) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int key = key0 + 16 * (e >> 2) + 4 * kb + (e & 3);
-                    if (key > limit) s[e] = kNegInf;
-                    // Slots behind the context hold anything: 0 times a NaN would be NaN.
-                    if (key >= ctx)
-#pragma unroll
-                        for (int c = 0; c < VD; ++c) f.v[e >> 2][e & 3][c] = 0;
-                }
-            }
-            float mt = s[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) mt = fmaxf(mt, s[e]);
-            mt = max_across32(max_across16(mt));
-            const bool raise = mt > m_run + kLazy;
-            const float m_new = raise ? mt : m_run;
-            if (__builtin_amdgcn_ballot_w64(raise)) {
-                const float alpha = raise ? fast_exp2(m_run - m_new) : 1.f;
-#pragma unroll
-                for (int i = 0; i < 4 * VD; ++i) o[i] *= alpha;
-                l_run *= alpha;
-                m_run = m_new;
-            }
-            const float m_off = m_run == kNegInf ? 0.f : m_run;
-            float w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float pe = fast_exp2(s[e] - m_off);
-                l_run += pe;
-                w[e] = pe * vs[e];
-            }
-            if (masked) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (key0 + 16 * (e >> 2) + 4 * kb + (e & 3) > limit) w[e] = 0.f;
-            }
-            u32x4 pf[NP];
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                pf[i] = u32x4{pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3]), pack_bf16(w[4], w[5]), pack_bf16(w[6], w[7])};
-                if (i + 1 < NP)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] -= (float)(__bf16)w[e];
-            }
-#pragma unroll
-            for (int c = 0; c < VD; ++c) {
-                uint32_t d0[4], d1[4];
-                const uint32_t r0[4] = {f.v[0][0][c], f.v[0][1][c], f.v[0][2][c], f.v[0][3][c]};
-                const uint32_t r1[4] = {f.v[1][0][c], f.v[1][1][c], f.v[1][2][c], f.v[1][3][c]};
-                transpose4(r0, d0);
-                transpose4(r1, d1);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const u32x4 vf = u32x4{codes_bf16<false>(d0[j]), codes_bf16<true>(d0[j]), codes_bf16<false>(d1[j]),
-                                           codes_bf16<true>(d1[j])};
-#pragma unroll
-                    for (int i = 0; i < NP; ++i) o[4 * c + j] = mfma_bf16(vf, pf[i], o[4 * c + j]);
-                }
-            }
-        };
-
-        int x = a + turn;
-        if (ctx > 0 && x < b) {
-            Unit f, g;
-            int64_t ids[NI];
-            load_ids(x, ids);
-            load_unit(x, ids, f);
-            load_ids(x + step, ids);
-            while (true) {
-                if (x + step < b) {
-                    load_unit(x + step, ids, g);
-                    load_ids(x + 2 * step, ids);
-                }
-                compute(x, f);
-                x += step;
-                if (x >= b) break;
-                if (x + step < b) {
-                    load_unit(x + step, ids, f);
-                    load_ids(x + 2 * step, ids);
-                }
-                compute(x, g);
-                x += step;
-                if (x >= b) break;
-            }
-        }
-
-        // ---- the waves' parts meet in LDS, row by row.
-        l_run = sum_across32(sum_across16(l_run));
-        if (n < rows) {
-#pragma unroll
-            for (int c = 0; c < VD; ++c)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = D == 128 ? 8 * (4 * kb + r) + 4 * c : 64 * c + 4 * (4 * kb + r);
-                    if (d < D)
-                        *reinterpret_cast<float4*>(&s_o[wave][n * D + d]) =
-                            make_float4(o[4 * c][r], o[4 * c + 1][r], o[4 * c + 2][r], o[4 * c + 3][r]);
-                }
-            if (kb == 0) s_ml[wave][n] = make_float2(m_run, l_run);
-        }
-        sync();
-        const int nthr = coop ? 256 : 64, thr = coop ? tid : lane;
-        const int parts = coop ? 4 : 1, part0 = coop ? 0 : wave;
-        const int items = rows * (D / 4);       // 4 elements of a row each
-        auto out4 = [&](int e, const Part& x4) {
-            const int r = e / (D / 4), d = e % (D / 4) * 4;
-            T* to = reinterpret_cast<T*>(p.out) + row_token(r) * p.out_st + row_head(r) * p.out_sh + d;
-            store4<T>(to, x4.result());
-        };
-        // Partials of slot s: side 0 of the sequence that it begins in, side 1 of one that it ends in.
-        auto partial = [&](int s, int side) { return ((int64_t)(s * 2 + side) * heads + kvh) * p.decode_rows; };
-        for (int e = thr; e < items; e += nthr) {
-            const int r = e / (D / 4);
-            Part acc = {kNegInf, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-            for (int w = part0; w < part0 + parts; ++w) {
-                const float2 ml = s_ml[w][r];
-                acc.add(ml.x, ml.y, *reinterpret_cast<const float4*>(&s_o[w][e * 4]));
-            }
-            if (whole) {
-                out4(e, acc);
-            } else {
-                const int64_t at = partial(slot, before <= u0 ? 0 : 1) + r;
-                uint64_t* po = reinterpret_cast<uint64_t*>(p.ws_o + at * D + e % (D / 4) * 4);
-                agent_store(po, pair_bits(acc.o.x, acc.o.y));
-                agent_store(po + 1, pair_bits(acc.o.z, acc.o.w));
-                if (e % (D / 4) == 0) agent_store(reinterpret_cast<uint64_t*>(p.ws_ml + at * 2), pair_bits(acc.m, acc.l));
-            }
-        }
-        if (!whole) {
-            // The stores have reached the agent's coherence point before the counter moves
-            // (a release fence would write back the XCD's whole L2 instead).
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            sync();
-            // Slots that hold a unit of this sequence.
-            auto slot_of = [&](int64_t u) { return (int)(((u + 1) * slots - 1) / total); };
-            const int s0 = slot_of(before), s1 = slot_of(after - 1);
-            uint32_t* cnt = p.ws_cnt + ((int64_t)seq * heads + kvh);
-            if (thr == 0) s_arrived[wave] = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            sync();
-            const bool merge = __builtin_amdgcn_readfirstlane(s_arrived[coop ? 0 : wave]) == (uint32_t)(s1 - s0);
-            if (merge) {
-                if (thr == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                // Threads beyond the items share the partials: group g takes s0 + g, s0 + g + groups,
-                // ...; group 0 then adds the groups up, in order.
-                int groups = 1;
-                while (groups * 2 * items <= nthr) groups *= 2;
-                const int g = groups > 1 ? thr / items : 0;
-                float* so = s_o[part0];         // the parts are out: free (8 floats a thread)
-                constexpr int CH = 4;           // partials whose loads are in flight together
-                for (int e0 = 0; e0 < items; e0 += nthr) {
-                    const int e = e0 + thr - g * items, r = e / (D / 4);
-                    const bool mine = g < groups && e < items;
-                    Part acc = {kNegInf, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-                    for (int s = s0 + g; mine && s <= s1; s += CH * groups) {
-                        uint64_t ml[CH], oa[CH], ob[CH];
-#pragma unroll
-                        for (int j = 0; j < CH; ++j) {
-                            const int sj = s + j * groups <= s1 ? s + j * groups : s1;
-                            // Side 1 where the slot began before this sequence: the first one only.
-                            const int64_t at = partial(sj, (int64_t)sj * total / slots < before ? 1 : 0) + r;
-                            const uint64_t* po = reinterpret_cast<const uint64_t*>(p.ws_o + at * D + e % (D / 4) * 4);
-                            ml[j] = agent_load(reinterpret_cast<const uint64_t*>(p.ws_ml + at * 2));
-                            oa[j] = agent_load(po);
-                            ob[j] = agent_load(po + 1);
-                        }
-#pragma unroll
-                        for (int j = 0; j < CH; ++j)
-                            if (s + j * groups <= s1)
-                                acc.add(lo_of(ml[j]), hi_of(ml[j]),
-                                        make_float4(lo_of(oa[j]), hi_of(oa[j]), lo_of(ob[j]), hi_of(ob[j])));
-                    }
-                    if (groups > 1) {
-                        if (mine && g > 0) {
-                            float* to = so + ((g - 1) * items + e) * 8;
-                            *reinterpret_cast<float4*>(to) = acc.o;
-                            *reinterpret_cast<float2*>(to + 4) = make_float2(acc.m, acc.l);
-                        }
-                        sync();
-                        for (int k = 0; mine && g == 0 && k < groups - 1; ++k) {
-                            const float* from = so + (k * items + e) * 8;
-                            const float2 ml = *reinterpret_cast<const float2*>(from + 4);
-                            acc.add(ml.x, ml.y, *reinterpret_cast<const float4*>(from));
-                        }
-                    }
-                    if (mine && g == 0) out4(e, acc);
-                }
-            }
-        }
-        sync();                                 // s_o, s_ml are free again
+        // The slot that holds a unit. A slot's partials: number 2 s of the sequence that it begins
+        // in, 2 s + 1 of the one that it ends in.
+        auto slot_of = [&](int64_t u) { return (int)(((u + 1) * slots - 1) / total); };
+        const int s0 = slot_of(before), s1 = slot_of(after - 1);
+        decode_segment<T, D, BIG, true>(
+            p, lds, seq, kvh, a, b, whole, s1 - s0 + 1, [&]() { return 2 * slot + (before <= u0 ? 0 : 1); },
+            [&](int k) { return 2 * (s0 + k) + ((int64_t)(s0 + k) * total / slots < before ? 1 : 0); });
+        lds_barrier();                              // lds is free again
     }
 }
 
-template <typename T, int D>
+// Runs that stay inside a sequence: the shortest runs, no less than decode_min_units, with which
+// all of them are at most decode_slots (twice the sequences if that is more); a sequence's are of
+// even lengths. A workgroup (COOP) or wave has one.
+template <typename T, int D, bool BIG, bool COOP>
+__global__ __launch_bounds__(256) void kv8_decode_runs_kernel(const Kv8Params p) {
+    __shared__ int s_wave[4];
+    __shared__ int s_found[4][5];                   // by run slot of the workgroup
+    __shared__ DecodeLds<D> lds;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    int slot, kvh;
+    decode_place<COOP>(p, wave, slot, kvh);
+    constexpr int kWhole = 1 << 30;                 // units: no sequence has more
+    int seq, runs, number, units;                   // a sequence, its runs, this one's number, its units
+    auto run_length = [&](int total) {
+        int len = p.ws_o ? p.decode_min_units : kWhole;     // no room for partials: sequences stay whole
+        const int room = p.decode_slots > 2 * p.num_seqs ? p.decode_slots - p.num_seqs : p.num_seqs;
+        const int even = (total + room - 1) / room;
+        return len > even ? len : even;
+    };
+    if (p.num_seqs <= 64) {
+        // Every wave for itself: lane i has sequence i.
+        const int lane = lane_id();
+        const int u = lane < p.num_seqs ? decode_units(p, lane) : 0;
+        int run = u;
+#pragma unroll
+        for (int by = 1; by < 64; by *= 2) {
+            const int up = __shfl_up(run, by);
+            if (lane >= by) run += up;
+        }
+        int len = run_length(__builtin_amdgcn_readlane(run, 63)), mine;
+        while (true) {
+            run = mine = (u + len - 1) / len;
+#pragma unroll
+            for (int by = 1; by < 64; by *= 2) {
+                const int up = __shfl_up(run, by);
+                if (lane >= by) run += up;
+            }
+            if (__builtin_amdgcn_readlane(run, 63) <= p.decode_grid || len == kWhole) break;
+            len = kWhole;                           // longer contexts than the grid was sized for
+        }
+        const uint64_t after = __builtin_amdgcn_ballot_w64(run > slot);
+        if (!after) return;
+        seq = __builtin_ctzll(after);
+        runs = __builtin_amdgcn_readlane(mine, seq);
+        number = slot - (__builtin_amdgcn_readlane(run, seq) - runs);
+        units = __builtin_amdgcn_readlane(u, seq);
+    } else {
+        const int per = (p.num_seqs + 255) / 256, first = (int)threadIdx.x * per;
+        int own = 0, u[kDecodePer], total;
+#pragma unroll
+        for (int j = 0; j < kDecodePer; ++j) {
+            u[j] = j < per && first + j < p.num_seqs ? decode_units(p, first + j) : 0;
+            own += u[j];
+        }
+        block_scan(own, s_wave, total);
+        int len = run_length(total), run;
+        while (true) {
+            own = 0;
+#pragma unroll
+            for (int j = 0; j < kDecodePer; ++j) own += (u[j] + len - 1) / len;
+            run = block_scan(own, s_wave, total);
+            if (total <= p.decode_grid || len == kWhole) break;
+            len = kWhole;
+        }
+        // The thread that has a run's sequence says so; a workgroup of wave runs has 4.
+        if (threadIdx.x < 4) s_found[threadIdx.x][0] = -1;
+        lds_barrier();
+#pragma unroll
+        for (int j = 0; j < kDecodePer; ++j) {
+            const int mine = (u[j] + len - 1) / len;
+            for (int w = 0; w < (COOP ? 1 : 4); ++w) {
+                int ws, head;
+                decode_place<COOP>(p, w, ws, head);
+                if (mine && ws >= run && ws < run + mine) {
+                    s_found[w][0] = first + j;
+                    s_found[w][1] = mine;
+                    s_found[w][2] = ws - run;
+                    s_found[w][3] = u[j];
+                }
+            }
+            run += mine;
+        }
+        lds_barrier();
+        const int w = COOP ? 0 : wave;
+        seq = __builtin_amdgcn_readfirstlane(s_found[w][0]);
+        if (seq < 0) return;
+        runs = __builtin_amdgcn_readfirstlane(s_found[w][1]);
+        number = __builtin_amdgcn_readfirstlane(s_found[w][2]);
+        units = __builtin_amdgcn_readfirstlane(s_found[w][3]);
+    }
+    const int a = (int)((int64_t)units * number / runs), b = (int)((int64_t)units * (number + 1) / runs);
+    decode_segment<T, D, BIG, COOP>(p, lds, seq, kvh, a, b, runs == 1, runs, [&]() { return slot; },
+                                    [&](int k) { return slot - number + k; });
+}
+
+template <typename T, int D, bool BIG>
 int launch_kv8_decode_d(const Kv8Params& p, hipStream_t stream) {
-    const int64_t sets = ceil_div(p.slots, 8) * 8 * p.num_kv_heads;   // (slot, head) pairs
-    const int64_t wgs = p.decode_coop ? sets : ceil_div(sets, 32) * 8;
+    const int64_t places = ceil_div(p.decode_grid, 8) * 8 * p.num_kv_heads;   // of (slot, KV head)
+    const int64_t wgs = p.decode_mode == kKv8WaveRuns ? ceil_div(places, 32) * 8 : places;
     if (wgs > 0x7fffffff) return fail(PKV_EUNSUPPORTED, "kv8 decode attention: grid too large");
-    if (p.block_size >= 16) kv8_decode_kernel<T, D, true><<<dim3((unsigned)wgs), 256, 0, stream>>>(p);
-    else kv8_decode_kernel<T, D, false><<<dim3((unsigned)wgs), 256, 0, stream>>>(p);
+    const dim3 grid((unsigned)wgs);
+    if (p.decode_mode == kKv8Even) kv8_decode_even_kernel<T, D, BIG><<<grid, 256, 0, stream>>>(p);
+    else if (p.decode_mode == kKv8Runs) kv8_decode_runs_kernel<T, D, BIG, true><<<grid, 256, 0, stream>>>(p);
+    else kv8_decode_runs_kernel<T, D, BIG, false><<<grid, 256, 0, stream>>>(p);
     return check_launch("kv8 decode attention");
+}
+
+template <typename T, bool BIG>
+int launch_kv8_decode_b(const Kv8Params& p, hipStream_t stream) {
+    switch (p.head_dim) {
+        case 32: return launch_kv8_decode_d<T, 32, BIG>(p, stream);
+        case 48: return launch_kv8_decode_d<T, 48, BIG>(p, stream);
+        case 64: return launch_kv8_decode_d<T, 64, BIG>(p, stream);
+        case 80: return launch_kv8_decode_d<T, 80, BIG>(p, stream);
+        case 96: return launch_kv8_decode_d<T, 96, BIG>(p, stream);
+        case 112: return launch_kv8_decode_d<T, 112, BIG>(p, stream);
+        default: return launch_kv8_decode_d<T, 128, BIG>(p, stream);
+    }
 }
 
 }  // namespace
 
 template <typename T>
 int launch_kv8_decode(const Kv8Params& p, hipStream_t stream) {
-    switch (p.head_dim) {
-        case 32: return launch_kv8_decode_d<T, 32>(p, stream);
-        case 48: return launch_kv8_decode_d<T, 48>(p, stream);
-        case 64: return launch_kv8_decode_d<T, 64>(p, stream);
-        case 80: return launch_kv8_decode_d<T, 80>(p, stream);
-        case 96: return launch_kv8_decode_d<T, 96>(p, stream);
-        case 112: return launch_kv8_decode_d<T, 112>(p, stream);
-        default: return launch_kv8_decode_d<T, 128>(p, stream);
-    }
+    return p.block_size >= 16 ? launch_kv8_decode_b<T, true>(p, stream) : launch_kv8_decode_b<T, false>(p, stream);
 }
 
 }  // namespace pkv
