@@ -27,6 +27,8 @@
 //    several heads.
 #pragma once
 
+#include <type_traits>
+
 #include "kv8.h"
 
 namespace pkv {
@@ -116,6 +118,17 @@ __device__ __forceinline__ void scales4(uint32_t w, float (&s)[4]) {
     for (int i = 0; i < 4; ++i) {
         const uint32_t b = e[i] & 0x7f800000u;
         s[i] = __builtin_bit_cast(float, b > 0x00400000u ? b : 0x00400000u);
+    }
+}
+
+__device__ __forceinline__ void scales8(const uint32_t (&w)[2], float (&s)[8]) {
+    float a[4], b[4];
+    scales4(w[0], a);
+    scales4(w[1], b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        s[i] = a[i];
+        s[4 + i] = b[i];
     }
 }
 
@@ -259,14 +272,12 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
     }
     const uint32_t s_off = BIG ? (uint32_t)(4 * kb * p.sss) : 0u;
 
-    struct Unit {
-        uint32_t k[2][KD], v[2][4][VD], ks[2], vs[2];
-    };
     // ---- block ids of a unit. BIG: lane l holds that of 16-key tile l % 2. Else each lane
     // those of its K rows and V row groups. Indexes stop at the context's last block.
     const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
-    const int last = (ctx - 1) >> p.block_shift;
-    auto load_ids = [&](int u, int64_t (&ids)[NI]) {
+    const int last = (ctx - 1) >> p.block_shift, in_block = p.block_size - 1;
+    int64_t ids[NI];
+    auto load_ids = [&](int u) {
         auto id = [&](int key) {
             const int at = key >> p.block_shift;
             return table[at < last ? at : last];
@@ -281,52 +292,53 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
             }
         }
     };
-    const int in_block = p.block_size - 1;
-    auto load_unit = [&](int u, const int64_t (&ids)[NI], Unit& f) {
-        auto inside = [&](int64_t id) { return (uint64_t)id < (uint64_t)p.num_blocks ? id : 0; };   // never out of the cache
+    auto inside = [&](int64_t id) { return (uint64_t)id < (uint64_t)p.num_blocks ? id : 0; };   // never out of the cache
+    auto load_scales = [&](const uint8_t* at) {
+        if (scales_together) return *reinterpret_cast<const uint32_t*>(at);
+        uint32_t w = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w |= (uint32_t)at[r * p.sss] << (8 * r);
+        return w;
+    };
+    // K of a unit: rows 16 t + n; its scales, and V: rows 16 t + 4 kb + r.
+    uint32_t kw[2][KD], vw[2][4][VD], ksw[2], vsw[2];
+    int64_t v_row[2], s_row[2];
+    auto load_k = [&](int u) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int64_t k_id = inside(BIG ? readlane64(ids[0], t) : ids[BIG ? 0 : t]);
             const int64_t v_id = BIG ? k_id : inside(ids[BIG ? 0 : 2 + t]);
             const int k_at = (kUnit * u + 16 * t + (BIG ? 0 : n)) & in_block;
             const int v_at = (kUnit * u + 16 * t + (BIG ? 0 : 4 * kb)) & in_block;
-            const uint8_t* k = kc + (k_id * p.sb + k_at * p.ss);
-            const uint8_t* v = vc + (v_id * p.sb + v_at * p.ss);
-            load_dwords<KD>(k + k_off, f.k[t]);
+            const int64_t k_row = k_id * p.sb + k_at * p.ss;
+            v_row[t] = BIG ? k_row : v_id * p.sb + v_at * p.ss;
+            s_row[t] = v_id * p.ssb + v_at * p.sss;
+            load_dwords<KD>(kc + k_row + k_off, kw[t]);
+            ksw[t] = load_scales(ksb + s_row[t] + s_off);
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint8_t* vr = v + r * p.ss;
+                const uint8_t* vr = vc + v_row[t] + r * p.ss;
                 if constexpr (D == 128) {
-                    load_dwords<2>(vr + v_off[0], f.v[t][r]);
+                    load_dwords<2>(vr + v_off[0], vw[t][r]);
                 } else {
 #pragma unroll
                     for (int c = 0; c < VD; ++c)
-                        f.v[t][r][c] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vr + v_off[c]));
+                        vw[t][r][c] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vr + v_off[c]));
                 }
             }
-            const int64_t so = v_id * p.ssb + v_at * p.sss;
-            const uint8_t* ks = ksb + so + s_off;
-            const uint8_t* vs = vsb + so + s_off;
-            if (scales_together) {
-                f.ks[t] = *reinterpret_cast<const uint32_t*>(ks);
-                f.vs[t] = *reinterpret_cast<const uint32_t*>(vs);
-            } else {
-                f.ks[t] = f.vs[t] = 0;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    f.ks[t] |= (uint32_t)ks[r * p.sss] << (8 * r);
-                    f.vs[t] |= (uint32_t)vs[r * p.sss] << (8 * r);
-                }
-            }
+            vsw[t] = load_scales(vsb + s_row[t] + s_off);
         }
     };
 
     // The first unit's ids, the queries, then its rows: in this order no load waits for one that it
     // does not need.
-    Unit f, g;
-    int64_t ids[NI];
     const bool any = ctx > 0 && x < b;
-    if (any) load_ids(x, ids);
+    if (any) load_ids(x);
     // Q^T: elements [kb D / 4, + D / 4) of the lane's row, 8 a step.
     constexpr int QW = D / 4 * (int)sizeof(T) / 8;
     uint2 qraw[QW];
@@ -336,8 +348,9 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
         for (int i = 0; i < QW; ++i) qraw[i] = reinterpret_cast<const uint2*>(q)[i];
     }
     if (any) {
-        load_unit(x, ids, f);
-        load_ids(x + step, ids);
+        load_k(x);
+        load_v();
+        load_ids(x + step);
     }
     u32x4 qf[NQ][KS];
 #pragma unroll
@@ -371,29 +384,30 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
     for (int i = 0; i < 4 * VD; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = kNegInf, l_run = 0.f;         // l: this lane's keys only, until the end
 
-    auto compute = [&](int u, Unit& f) {
-        const int key0 = kUnit * u;
+    while (any) {
+        const int key0 = kUnit * x;
         const bool masked = key0 + kUnit - 1 > pos0;         // some row does not see some key
+        const bool more = x + step < b;
         float s[8], vs[8];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
-                const u32x4 kf = Qk<T>::keys(f.k[t][2 * j], 2 * j + 1 < KD ? f.k[t][2 * j + 1 < KD ? 2 * j + 1 : 0] : 0u);
+                const u32x4 kf = Qk<T>::keys(kw[t][2 * j], 2 * j + 1 < KD ? kw[t][2 * j + 1 < KD ? 2 * j + 1 : 0] : 0u);
 #pragma unroll
                 for (int i = 0; i < NQ; ++i) st = Qk<T>::run(kf, qf[i][j], st);
             }
-            float ks4[4], vs4[4];
-            scales4(f.ks[t], ks4);
-            scales4(f.vs[t], vs4);
+            float ks4[4];
+            scales4(ksw[t], ks4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[4 * t + r] = st[r] * ks4[r] * p.scale_log2;
-                vs[4 * t + r] = vs4[r];
-            }
+            for (int r = 0; r < 4; ++r) s[4 * t + r] = st[r] * ks4[r] * p.scale_log2;
         }
+        // K's registers are free: the next unit's, under this one's softmax and second product. V's
+        // follow below, under the next one's first product.
+        if (more) load_k(x + step);
         if (masked) {
+            asm volatile("");                   // a branch, not selects in every unit
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int key = key0 + 16 * (e >> 2) + 4 * kb + (e & 3);
@@ -401,7 +415,7 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
                 // Slots behind the context hold anything: 0 times a NaN would be NaN.
                 if (key >= ctx)
 #pragma unroll
-                    for (int c = 0; c < VD; ++c) f.v[e >> 2][e & 3][c] = 0;
+                    for (int c = 0; c < VD; ++c) vw[e >> 2][e & 3][c] = 0;
             }
         }
         float mt = s[0];
@@ -409,15 +423,15 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
         for (int e = 1; e < 8; ++e) mt = fmaxf(mt, s[e]);
         mt = max_across32(max_across16(mt));
         const bool raise = mt > m_run + kLazy;
-        const float m_new = raise ? mt : m_run;
         if (__builtin_amdgcn_ballot_w64(raise)) {
-            const float alpha = raise ? fast_exp2(m_run - m_new) : 1.f;
+            const float alpha = raise ? fast_exp2(m_run - mt) : 1.f;
 #pragma unroll
             for (int i = 0; i < 4 * VD; ++i) o[i] *= alpha;
             l_run *= alpha;
-            m_run = m_new;
+            m_run = raise ? mt : m_run;
         }
         const float m_off = m_run == kNegInf ? 0.f : m_run;
+        scales8(vsw, vs);
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -426,6 +440,7 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
             w[e] = pe * vs[e];
         }
         if (masked) {
+            asm volatile("");
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (key0 + 16 * (e >> 2) + 4 * kb + (e & 3) > limit) w[e] = 0.f;
@@ -441,8 +456,8 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
 #pragma unroll
         for (int c = 0; c < VD; ++c) {
             uint32_t d0[4], d1[4];
-            const uint32_t r0[4] = {f.v[0][0][c], f.v[0][1][c], f.v[0][2][c], f.v[0][3][c]};
-            const uint32_t r1[4] = {f.v[1][0][c], f.v[1][1][c], f.v[1][2][c], f.v[1][3][c]};
+            const uint32_t r0[4] = {vw[0][0][c], vw[0][1][c], vw[0][2][c], vw[0][3][c]};
+            const uint32_t r1[4] = {vw[1][0][c], vw[1][1][c], vw[1][2][c], vw[1][3][c]};
             transpose4(r0, d0);
             transpose4(r1, d1);
 #pragma unroll
@@ -453,25 +468,11 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
                 for (int i = 0; i < NP; ++i) o[4 * c + j] = mfma_bf16(vf, pf[i], o[4 * c + j]);
             }
         }
-    };
-
-    if (any)
-        while (true) {
-            if (x + step < b) {
-                load_unit(x + step, ids, g);
-                load_ids(x + 2 * step, ids);
-            }
-            compute(x, f);
-            x += step;
-            if (x >= b) break;
-            if (x + step < b) {
-                load_unit(x + step, ids, f);
-                load_ids(x + 2 * step, ids);
-            }
-            compute(x, g);
-            x += step;
-            if (x >= b) break;
-        }
+        if (!more) break;
+        load_v();
+        x += step;
+        load_ids(x + step);
+    }
 
     // ---- the waves' parts meet in LDS, row by row.
     l_run = sum_across32(sum_across16(l_run));
@@ -580,15 +581,25 @@ __device__ __forceinline__ void decode_place(const Kv8Params& p, int wave, int& 
     kvh = in >> 3;
 }
 
+// Inclusive running sums over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+    auto add = [&](auto ctrl, auto rows) {
+        v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    using std::integral_constant;
+    add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());    // row_shr 1, 2, 4, 8
+    add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+    add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+    add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+    add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());    // row_bcast 15, to rows 1 and 3
+    add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());    // row_bcast 31, to rows 2 and 3
+    return v;
+}
+
 // Exclusive running sums of v over the workgroup's 256 threads, and their total.
 __device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
     const int lane = lane_id(), wave = (int)(threadIdx.x >> 6);
-    int run = v;
-#pragma unroll
-    for (int by = 1; by < 64; by *= 2) {
-        const int up = __shfl_up(run, by);
-        if (lane >= by) run += up;
-    }
+    int run = wave_scan(v);
     lds_barrier();                              // s_wave's last readers are done
     if (lane == 63) s_wave[wave] = run;
     lds_barrier();
@@ -597,12 +608,14 @@ __device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
     for (int w = 0; w < wave; ++w) run += s_wave[w];
     return run;
 }
+// Waves a SIMD that registers are held to (128, 168 or 256 a lane): what fits without spills.
+template <typename T, int D>
+constexpr int kDecodeWaves = sizeof(T) == 2 ? (D <= 64 ? 4 : 3) : (D <= 80 ? 3 : 2);
 constexpr int kDecodePer = kDecodeMaxSeqs / 256;    // sequences per thread, at most
 
-// Even runs: slot s of S takes units [s U / S, (s + 1) U / S) of all the batch's U, sequence after
-// sequence.
+// Even runs: the batch's units, sequence after sequence, cut into equal slots.
 template <typename T, int D, bool BIG>
-__global__ __launch_bounds__(256) void kv8_decode_even_kernel(const Kv8Params p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWaves<T, D>))) void kv8_decode_even_kernel(const Kv8Params p) {
     __shared__ int s_before[kDecodeMaxSeqs + 1];
     __shared__ int s_wave[4];
     __shared__ DecodeLds<D> lds;
@@ -630,7 +643,11 @@ __global__ __launch_bounds__(256) void kv8_decode_even_kernel(const Kv8Params p)
     slots = slots < 1 ? 1 : slots < p.decode_slots ? slots : p.decode_slots;
     decode_place<true>(p, 0, slot, kvh);
     if (slot >= slots) return;
-    const int u0 = (int)((int64_t)slot * total / slots), u1 = (int)((int64_t)(slot + 1) * total / slots);
+    // Slots [0, more) have len + 1 units, the others len.
+    const int len = total / slots, more = total - len * slots;
+    auto start_of = [&](int s) { return s * len + (s < more ? s : more); };
+    auto slot_of = [&](int u) { return u < more * (len + 1) ? u / (len + 1) : (u - more) / len; };
+    const int u0 = start_of(slot), u1 = start_of(slot + 1);
     int seq = 0;
     for (int hi = p.num_seqs; hi - seq > 1;) {      // the last sequence with s_before <= u0
         const int mid = (seq + hi) >> 1;
@@ -644,13 +661,12 @@ __global__ __launch_bounds__(256) void kv8_decode_even_kernel(const Kv8Params p)
         if (after == before) continue;
         const int a = before < u0 ? u0 - before : 0, b = after > u1 ? u1 - before : after - before;
         const bool whole = a == 0 && b == after - before;
-        // The slot that holds a unit. A slot's partials: number 2 s of the sequence that it begins
-        // in, 2 s + 1 of the one that it ends in.
-        auto slot_of = [&](int64_t u) { return (int)(((u + 1) * slots - 1) / total); };
+        // A slot's partials: number 2 s of the sequence that it begins in, 2 s + 1 of the one that
+        // it ends in.
         const int s0 = slot_of(before), s1 = slot_of(after - 1);
         decode_segment<T, D, BIG, true>(
             p, lds, seq, kvh, a, b, whole, s1 - s0 + 1, [&]() { return 2 * slot + (before <= u0 ? 0 : 1); },
-            [&](int k) { return 2 * (s0 + k) + ((int64_t)(s0 + k) * total / slots < before ? 1 : 0); });
+            [&](int k) { return 2 * (s0 + k) + (start_of(s0 + k) < before ? 1 : 0); });
         lds_barrier();                              // lds is free again
     }
 }
@@ -659,7 +675,7 @@ __global__ __launch_bounds__(256) void kv8_decode_even_kernel(const Kv8Params p)
 // all of them are at most decode_slots (twice the sequences if that is more); a sequence's are of
 // even lengths. A workgroup (COOP) or wave has one.
 template <typename T, int D, bool BIG, bool COOP>
-__global__ __launch_bounds__(256) void kv8_decode_runs_kernel(const Kv8Params p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWaves<T, D>))) void kv8_decode_runs_kernel(const Kv8Params p) {
     __shared__ int s_wave[4];
     __shared__ int s_found[4][5];                   // by run slot of the workgroup
     __shared__ DecodeLds<D> lds;
@@ -678,20 +694,11 @@ __global__ __launch_bounds__(256) void kv8_decode_runs_kernel(const Kv8Params p)
         // Every wave for itself: lane i has sequence i.
         const int lane = lane_id();
         const int u = lane < p.num_seqs ? decode_units(p, lane) : 0;
-        int run = u;
-#pragma unroll
-        for (int by = 1; by < 64; by *= 2) {
-            const int up = __shfl_up(run, by);
-            if (lane >= by) run += up;
-        }
+        int run = wave_scan(u);
         int len = run_length(__builtin_amdgcn_readlane(run, 63)), mine;
         while (true) {
-            run = mine = (u + len - 1) / len;
-#pragma unroll
-            for (int by = 1; by < 64; by *= 2) {
-                const int up = __shfl_up(run, by);
-                if (lane >= by) run += up;
-            }
+            mine = (u + len - 1) / len;
+            run = wave_scan(mine);
             if (__builtin_amdgcn_readlane(run, 63) <= p.decode_grid || len == kWhole) break;
             len = kWhole;                           // longer contexts than the grid was sized for
         }
@@ -745,7 +752,8 @@ __global__ __launch_bounds__(256) void kv8_decode_runs_kernel(const Kv8Params p)
         number = __builtin_amdgcn_readfirstlane(s_found[w][2]);
         units = __builtin_amdgcn_readfirstlane(s_found[w][3]);
     }
-    const int a = (int)((int64_t)units * number / runs), b = (int)((int64_t)units * (number + 1) / runs);
+    const int each = units / runs, more = units - each * runs;      // runs [0, more) have one more
+    const int a = number * each + (number < more ? number : more), b = a + each + (number < more ? 1 : 0);
     decode_segment<T, D, BIG, COOP>(p, lds, seq, kvh, a, b, runs == 1, runs, [&]() { return slot; },
                                     [&](int k) { return slot - number + k; });
 }
