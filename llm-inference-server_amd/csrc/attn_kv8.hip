@@ -113,7 +113,11 @@ bool kv8_decode_applies(const Kv8Params& p, int dtype) {
     // Keys and units in 32 bits; so are the offsets of a lane inside 16 slots.
     const int64_t cap = p.table_width * p.block_size;
     if (cap > (1 << 30) || (cap / 32 + 1) * p.num_seqs > (1 << 30)) return false;
-    if (p.ss < 0 || p.ss > (1 << 26) || p.sss < 0 || p.sss > (1 << 26)) return false;
+    if (p.ss < 0 || p.ss > (1 << 26) || p.ss * p.block_size > (1 << 30)) return false;
+    if (p.sb < 0 || p.sb > 0x7fffffff || p.ssb < 0 || p.ssb > 0x7fffffff || p.num_blocks > 0x7fffffff) return false;
+    // 4 scale bytes are one load.
+    const uint64_t scales = (uint64_t)(uintptr_t)p.ks | (uint64_t)(uintptr_t)p.vs | (uint64_t)p.ssb | (uint64_t)p.ssh;
+    if (p.sss != 1 || scales % 4) return false;
     const int64_t isz = dtype == PKV_FLOAT32 ? 4 : 2;
     const uint64_t rows = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * isz) |
                           (uint64_t)(p.q_sh * isz) | (uint64_t)(p.out_st * isz) | (uint64_t)(p.out_sh * isz);
@@ -126,23 +130,24 @@ bool kv8_decode_applies(const Kv8Params& p, int dtype) {
 // more (sequence, KV head) pairs than merge counters).
 int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* host_qlen) {
     constexpr int64_t kWorkgroups = 256 * 3;    // that the GPU holds
-    constexpr int64_t kEvenUnits = 24;          // per workgroup of even runs
+    const int64_t keys = p.head_dim <= 64 ? 64 : 32;    // of a unit
+    constexpr int64_t kEvenKeys = 768;          // per workgroup of even runs, at least
     const int64_t heads = p.num_kv_heads, seqs = p.num_seqs, pairs = seqs * heads;
     int64_t units = 0, runs = 0;
     auto each = [&](auto f) {
         for (int64_t i = 0; i < seqs; ++i) {
             if (host_qlen && host_qlen[i] <= 0) continue;
             const int64_t c = host_ctx ? host_ctx[i] : p.max_context_len;
-            f(c > 32 ? ceil_div(c, 32) : 1);
+            f(c > keys ? ceil_div(c, keys) : 1);
         }
     };
     each([&](int64_t u) { units += u; });
     p.decode_rows = (int)((int64_t)p.max_query_len * p.group);
     const bool cuts = pairs * 4 <= kMergeCounterBytes;
     auto bytes = [&](int64_t numbers) { return numbers * heads * p.decode_rows * (p.head_dim + 2) * 4; };
-    if (cuts && units * heads >= kWorkgroups * kEvenUnits) {
+    if (cuts && units * keys * heads >= kWorkgroups * kEvenKeys) {
         p.decode_mode = kKv8Even;
-        p.decode_min_units = 8;
+        p.decode_min_units = (int)(256 / keys);
         const int64_t most = kWorkgroups / heads;
         p.decode_slots = p.decode_grid = (int)(most < 1 ? 1 : most);
         return bytes(2 * p.decode_slots);
@@ -153,8 +158,9 @@ int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* ho
     p.decode_slots = (int)(most < 1 ? 1 : most);
     each([&](int64_t u) { runs += ceil_div(u, p.decode_min_units); });
     const int64_t room = p.decode_slots > 2 * seqs ? p.decode_slots : 2 * seqs;
-    p.decode_grid = (int)(runs < room ? runs > seqs ? runs : seqs : room);
-    return cuts && runs > seqs ? bytes(p.decode_grid) : 0;
+    p.decode_whole = !cuts || runs <= seqs;
+    p.decode_grid = (int)(p.decode_whole ? seqs : runs < room ? runs : room);
+    return p.decode_whole ? 0 : bytes(p.decode_grid);
 }
 
 // ------------------------------------------------------------------ chunks
@@ -278,9 +284,6 @@ extern "C" int pkv_kv8_attention(
     p.qsl = query_start_loc;
     p.scale = scale;
     p.scale_log2 = scale * kLog2e;
-    const uint64_t scales = (uint64_t)(uintptr_t)k_scales | (uint64_t)(uintptr_t)v_scales |
-                            (uint64_t)scale_stride_block | (uint64_t)scale_stride_head;
-    p.scales4 = scales % 4 == 0;
     if (kv8_decode_applies(p, dtype)) {
         const int64_t parts = kv8_decode_plan(p, host_context_lens, host_query_lens);
         if (parts && workspace && workspace_bytes >= kMergeCounterBytes + parts) {
@@ -288,9 +291,10 @@ extern "C" int pkv_kv8_attention(
             p.ws_cnt = reinterpret_cast<uint32_t*>(ws);
             p.ws_o = reinterpret_cast<float*>(ws + kMergeCounterBytes);
             p.ws_ml = p.ws_o + parts / (4 * (head_dim + 2)) * head_dim;
-        } else if (p.decode_mode == kKv8Even) {
-            // No room for partials: a workgroup a sequence.
-            p.decode_mode = kKv8Runs;
+        } else {
+            // No room for partials, or no need: a workgroup or wave a sequence.
+            if (p.decode_mode == kKv8Even) p.decode_mode = kKv8Runs;
+            p.decode_whole = 1;
             p.decode_grid = p.num_seqs;
         }
         switch (dtype) {

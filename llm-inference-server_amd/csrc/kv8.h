@@ -25,11 +25,10 @@ struct Kv8Params : AttnParams {
     const uint8_t* vs;
     int64_t ssb, sss, ssh;           // scale strides (bytes): block, slot, head
     int64_t max_context_len;
-    bool scales4;                    // scale bytes of 4 slots (4-aligned) can be one load, if sss = 1
     // Decode: how the batch's keys are cut (kKv8Even ...), into how many runs per KV head at most,
-    // the grid's room for them, the units of 32 keys that a run has at least, and the rows of a
-    // partial (ws_o, ws_ml by [number][KV head][row]; null: sequences stay whole).
-    int decode_mode, decode_slots, decode_grid, decode_min_units, decode_rows;
+    // the grid's room for them, the units that a run has at least, whether no sequence is cut,
+    // and the rows of a partial (ws_o, ws_ml by [number][KV head][row]).
+    int decode_mode, decode_slots, decode_grid, decode_min_units, decode_whole, decode_rows;
 };
 
 // 2^(b - 127), NaN for 255.

@@ -1,11 +1,12 @@
 // Decode attention over the 8-bit paged cache on MFMA (gfx950): the kernel, instantiated by
 // type in attn_kv8_decode_*.hip. Head_dim a multiple of 16 from 32 to 128, at most 16 rows
 // ((token, query head) pairs) per (sequence, KV head), block sizes that are powers of two from
-// 4 up, codes in 4-byte steps, queries and output in 8-byte ones.
+// 4 up, scale bytes of a block together (slot stride 1) and 4-byte aligned, codes in 4-byte
+// steps, queries and output in 8-byte ones.
 //
 // Bound: HBM for batches of tens of MB (head_dim + 1 bytes a cached row), latency below that.
 //
-//  * Split: the batch's keys, in units of 32, sequence after sequence, are cut into `slots` even
+//  * Split: the batch's keys, in units of 32 (64 up to head_dim 64), sequence after sequence, are cut into `slots` even
 //    runs per KV head, whatever the lengths: a prefix sum over the sequences, which every
 //    workgroup takes by itself, tells it its own. A run is a workgroup's (its four waves take
 //    turns at the units) or, where sequences are short and many, a single wave's. A sequence
@@ -34,7 +35,8 @@
 namespace pkv {
 namespace {
 
-constexpr int kUnit = 32;                       // keys
+// Keys a wave takes at a time: 8 KiB of K and V at most.
+constexpr int unit_keys(int head_dim) { return head_dim <= 64 ? 64 : 32; }
 constexpr int kDecodeRows = kKv8DecodeRows;
 constexpr int kDecodeMaxSeqs = kKv8DecodeMaxSeqs;   // prefix sums in LDS
 constexpr float kLazy = 8.f;                    // base 2: maxima are raised past 2^8 only
@@ -47,12 +49,13 @@ typedef uint32_t u32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// N dwords at a 4-byte aligned address.
+// N dwords at a 4-byte aligned address that the lane has, or at a lane's offset from a uniform one
+// (a buffer load: no address arithmetic on the vector unit, where the compiler spends 64-bit
+// adds and register pairs on every load of the plain form). Nontemporal.
 template <int N>
 __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t (&w)[N]) {
-    int i = 0;
 #pragma unroll
-    for (; i + 4 <= N; i += 4) {
+    for (int i = 0; i + 4 <= N; i += 4) {
         const u32x4_a4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_a4*>(p + 4 * i));
         w[i] = v.x;
         w[i + 1] = v.y;
@@ -65,6 +68,33 @@ __device__ __forceinline__ void load_dwords(const uint8_t* p, uint32_t (&w)[N]) 
         w[(N & ~3) + 1] = v.y;
     }
     if constexpr (N % 2) w[N - 1] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p + 4 * (N - 1)));
+}
+struct Uniform {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ explicit Uniform(const uint8_t* p)
+        : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, -1, 0x00027000)) {}
+};
+// The nontemporal bit of a buffer load, for rows of whole 128-byte lines: shorter ones share lines
+// with other heads' rows, which other workgroups of the XCD are to find in its L2 (32 GPT-2
+// sequences 16.2 us with it, 14.8 without; 64 of 1-16k at head_dim 128 197 us, 205 without).
+template <int D>
+constexpr int kNt = D == 128 ? 2 : 0;
+template <int NT, int N>
+__device__ __forceinline__ void load_dwords(const Uniform& base, uint32_t lane_off, int off, uint32_t (&w)[N]) {
+#pragma unroll
+    for (int i = 0; i + 4 <= N; i += 4) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(base.r, (int)lane_off + 4 * i, off, NT);
+        w[i] = v.x;
+        w[i + 1] = v.y;
+        w[i + 2] = v.z;
+        w[i + 3] = v.w;
+    }
+    if constexpr (N % 4 >= 2) {
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(base.r, (int)lane_off + 4 * (N & ~3), off, NT);
+        w[N & ~3] = v.x;
+        w[(N & ~3) + 1] = v.y;
+    }
+    if constexpr (N % 2) w[N - 1] = __builtin_amdgcn_raw_buffer_load_b32(base.r, (int)lane_off + 4 * (N - 1), off, NT);
 }
 
 __device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
@@ -118,17 +148,6 @@ __device__ __forceinline__ void scales4(uint32_t w, float (&s)[4]) {
     for (int i = 0; i < 4; ++i) {
         const uint32_t b = e[i] & 0x7f800000u;
         s[i] = __builtin_bit_cast(float, b > 0x00400000u ? b : 0x00400000u);
-    }
-}
-
-__device__ __forceinline__ void scales8(const uint32_t (&w)[2], float (&s)[8]) {
-    float a[4], b[4];
-    scales4(w[0], a);
-    scales4(w[1], b);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        s[i] = a[i];
-        s[4 + i] = b[i];
     }
 }
 
@@ -201,12 +220,12 @@ struct Part {
     }
 };
 
-// LDS of a workgroup: the waves' parts of a segment.
-template <int D>
+// LDS of a workgroup of W waves: the waves' parts of a segment.
+template <int D, int W>
 struct DecodeLds {
-    __attribute__((aligned(16))) float o[4][kDecodeRows * D];
-    float2 ml[4][kDecodeRows];
-    uint32_t arrived[4];
+    __attribute__((aligned(16))) float o[W][kDecodeRows * D];
+    float2 ml[W][kDecodeRows];
+    uint32_t arrived[W];
 };
 
 __device__ __forceinline__ int decode_ctx(const Kv8Params& p, int seq) {
@@ -214,37 +233,64 @@ __device__ __forceinline__ int decode_ctx(const Kv8Params& p, int seq) {
     return (int)(c < 0 ? 0 : c < cap ? c : cap);
 }
 // Units of a sequence; one that has queries has one at least.
+template <int D>
 __device__ __forceinline__ int decode_units(const Kv8Params& p, int seq) {
-    const int u = (int)(((uint32_t)decode_ctx(p, seq) + kUnit - 1) / kUnit);
+    const int u = (int)(((uint32_t)decode_ctx(p, seq) + unit_keys(D) - 1) / unit_keys(D));
     if (p.qsl && p.qsl[seq + 1] <= p.qsl[seq]) return 0;
     return u > 0 ? u : 1;
 }
 
-// The threads of a run: its workgroup's, or its wave's.
-template <bool COOP>
+// The threads of a run of NW waves: its workgroup's, or its wave's.
+template <int NW>
 __device__ __forceinline__ void run_sync() {
-    if constexpr (COOP) lds_barrier(); else wave_lds_sync();
+    if constexpr (NW > 1) lds_barrier(); else wave_lds_sync();
 }
 
-// Units [a, b) of sequence `seq` (all of them: `whole`) for KV head kvh. Else this is one of the
-// `parts` that the sequence is cut into: its partial is number own(), the k-th one part(k).
+// Units [a, b) of sequence `seq` for KV head kvh by NW waves. parts = 1: all of the sequence (b
+// is not looked at). Else the sequence is cut into so many parts, of which this is one: its
+// partial is number own(), the k-th one part_of(k).
 // BIG: block sizes from 16 up, where 16 keys share a block and addresses are uniform.
-template <typename T, int D, bool BIG, bool COOP, typename Own, typename PartOf>
-__device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>& lds, int seq, int kvh, int a, int b,
-                                               bool whole, int parts, Own own, PartOf part_of) {
+template <typename T, int D, bool BIG, int NW, typename Lds, typename Own, typename PartOf>
+__device__ __forceinline__ void decode_segment(const Kv8Params& p, Lds& lds, int seq, int kvh, int a, int b, int parts,
+                                               Own own, PartOf part_of) {
+    const bool whole = parts == 1;
     constexpr int KD = D / 16;                  // dwords of K a lane holds of each row
     constexpr int KS = (D + 31) / 32;           // contraction steps of S^T
     // Neighbouring dims of V that a lane holds: 8 at head_dim 128, else 4 of each 64.
     constexpr int VD = D == 128 ? 2 : (D + 63) / 64;   // dwords
     constexpr int NQ = Qk<T>::kPieces, NP = sizeof(T) == 4 ? 3 : 2;
-    constexpr int NI = BIG ? 1 : 4;
+    constexpr int kUnit = unit_keys(D), NT = kUnit / 16;    // tiles of 16 keys
+    constexpr int NI = BIG ? 1 : 2 * NT;
 
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int n = lane & 15, kb = lane >> 4;
     const int G = p.group, heads = p.num_kv_heads;
-    const int step = COOP ? 4 : 1;
-    int x = a + (COOP ? wave : 0);
+    int x = a + (NW > 1 ? wave : 0);            // this wave's unit, in steps of NW
+
+    // ---- block ids of a unit. BIG: lane l holds that of 16-key tile l % NT. Else each lane
+    // those of its K rows and V row groups. Indexes stop at the row's end: what stands behind a
+    // context's last block is never used.
+    const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
+    const int last = (int)p.table_width - 1, in_block = p.block_size - 1;
+    int64_t raw_ids[NI];
+    auto load_ids = [&](int u) {
+        auto id = [&](int key) {
+            const int at = key >> p.block_shift;
+            return table[at < last ? at : last];
+        };
+        if constexpr (BIG) {
+            raw_ids[0] = id(kUnit * u + 16 * (lane & (NT - 1)));
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                raw_ids[t] = id(kUnit * u + 16 * t + n);
+                raw_ids[NT + t] = id(kUnit * u + 16 * t + 4 * kb);
+            }
+        }
+    };
+    // The first unit's ids go out before the context's length is known.
+    if (last >= 0) load_ids(x);
 
     const int ctx = __builtin_amdgcn_readfirstlane(decode_ctx(p, seq));
     const int64_t q_first = p.qsl ? p.qsl[seq] : seq;
@@ -256,101 +302,89 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
     auto row_token = [&](int r) { return q_first + r / G; };
     auto row_head = [&](int r) { return (int64_t)kvh * G + r % G; };
 
+    if (whole) b = (int)(((uint32_t)ctx + kUnit - 1) / kUnit);
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.k) + kvh * p.sh;
     const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.v) + kvh * p.sh;
     const uint8_t* ksb = p.ks + kvh * p.ssh;
     const uint8_t* vsb = p.vs + kvh * p.ssh;
-    const bool scales_together = p.sss == 1 && p.scales4;
     // Lane offsets: K row n of a tile, a quarter of it; V rows 4 kb .. 4 kb + 3, dims from n (past
     // head_dim: some others, never stored).
-    const uint32_t k_off = (uint32_t)(kb * (D / 4)) + (BIG ? (uint32_t)(n * p.ss) : 0u);
+    // K: dims [kb D / 4, + D / 4); at head_dim 128 two pieces of 16, so that a load takes 64
+    // neighbouring bytes of each row.
+    constexpr int KP = D == 128 ? 2 : 1, KW = KD / KP;      // pieces, dwords of one
+    const uint32_t k_off = (uint32_t)(kb * 4 * KW) + (BIG ? (uint32_t)(n * p.ss) : 0u);
     uint32_t v_off[VD];
 #pragma unroll
     for (int c = 0; c < VD; ++c) {
         const int d = D == 128 ? 8 * n : 64 * c + 4 * n;
         v_off[c] = (uint32_t)(d < D ? d : 0) + (BIG ? (uint32_t)(4 * kb * p.ss) : 0u);
     }
-    const uint32_t s_off = BIG ? (uint32_t)(4 * kb * p.sss) : 0u;
+    const uint32_t s_off = BIG ? (uint32_t)(4 * kb) : 0u;
 
-    // ---- block ids of a unit. BIG: lane l holds that of 16-key tile l % 2. Else each lane
-    // those of its K rows and V row groups. Indexes stop at the context's last block.
-    const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
-    const int last = (ctx - 1) >> p.block_shift, in_block = p.block_size - 1;
-    int64_t ids[NI];
-    auto load_ids = [&](int u) {
-        auto id = [&](int key) {
-            const int at = key >> p.block_shift;
-            return table[at < last ? at : last];
-        };
-        if constexpr (BIG) {
-            ids[0] = id(kUnit * u + 16 * (lane & 1));
-        } else {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                ids[t] = id(kUnit * u + 16 * t + n);
-                ids[2 + t] = id(kUnit * u + 16 * t + 4 * kb);
-            }
-        }
-    };
-    auto inside = [&](int64_t id) { return (uint64_t)id < (uint64_t)p.num_blocks ? id : 0; };   // never out of the cache
-    auto load_scales = [&](const uint8_t* at) {
-        if (scales_together) return *reinterpret_cast<const uint32_t*>(at);
-        uint32_t w = 0;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) w |= (uint32_t)at[r * p.sss] << (8 * r);
-        return w;
-    };
     // K of a unit: rows 16 t + n; its scales, and V: rows 16 t + 4 kb + r.
-    uint32_t kw[2][KD], vw[2][4][VD], ksw[2], vsw[2];
-    int64_t v_row[2], s_row[2];
+    uint32_t kw[NT][KD], vw[NT][4][VD], ksw[NT], vsw[NT];
+    uint64_t v_row[NT], s_row[NT];
     auto load_k = [&](int u) {
+        uint32_t ids[NI];                       // none is followed out of the cache
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int64_t k_id = inside(BIG ? readlane64(ids[0], t) : ids[BIG ? 0 : t]);
-            const int64_t v_id = BIG ? k_id : inside(ids[BIG ? 0 : 2 + t]);
+        for (int i = 0; i < NI; ++i) ids[i] = (uint64_t)raw_ids[i] < (uint64_t)p.num_blocks ? (uint32_t)raw_ids[i] : 0u;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t k_id = BIG ? (uint32_t)__builtin_amdgcn_readlane((int)ids[0], t) : ids[BIG ? 0 : t];
+            const uint32_t v_id = BIG ? k_id : ids[BIG ? 0 : NT + t];
             const int k_at = (kUnit * u + 16 * t + (BIG ? 0 : n)) & in_block;
             const int v_at = (kUnit * u + 16 * t + (BIG ? 0 : 4 * kb)) & in_block;
-            const int64_t k_row = k_id * p.sb + k_at * p.ss;
-            v_row[t] = BIG ? k_row : v_id * p.sb + v_at * p.ss;
-            s_row[t] = v_id * p.ssb + v_at * p.sss;
-            load_dwords<KD>(kc + k_row + k_off, kw[t]);
-            ksw[t] = load_scales(ksb + s_row[t] + s_off);
+            // Strides of a block and offsets inside it fit 32 bits.
+            const uint64_t k_row = (uint64_t)k_id * (uint32_t)p.sb + (uint32_t)(k_at * (int)p.ss);
+            v_row[t] = BIG ? k_row : (uint64_t)v_id * (uint32_t)p.sb + (uint32_t)(v_at * (int)p.ss);
+            s_row[t] = (uint64_t)v_id * (uint32_t)p.ssb + (uint32_t)v_at;
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                uint32_t w[KW];
+                if constexpr (BIG) load_dwords<kNt<D>>(Uniform(kc + k_row), k_off, 64 * i, w);
+                else load_dwords<KW>(kc + k_row + k_off + 64 * i, w);
+#pragma unroll
+                for (int e = 0; e < KW; ++e) kw[t][KW * i + e] = w[e];
+            }
+            if constexpr (BIG) {
+                ksw[t] = __builtin_amdgcn_raw_buffer_load_b32(Uniform(ksb + s_row[t]).r, (int)s_off, 0, 0);
+            } else {
+                ksw[t] = *reinterpret_cast<const uint32_t*>(ksb + s_row[t]);
+            }
         }
     };
     auto load_v = [&]() {
+        constexpr int VL = D == 128 ? 1 : VD, VN = VD / VL;     // loads a row, dwords a load
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint8_t* vr = vc + v_row[t] + r * p.ss;
-                if constexpr (D == 128) {
-                    load_dwords<2>(vr + v_off[0], vw[t][r]);
-                } else {
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int c = 0; c < VD; ++c)
-                        vw[t][r][c] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vr + v_off[c]));
+                for (int c = 0; c < VL; ++c) {
+                    uint32_t w[VN];
+                    if constexpr (BIG) load_dwords<kNt<D>>(Uniform(vc + v_row[t]), v_off[c], r * (int)p.ss, w);
+                    else load_dwords<VN>(vc + v_row[t] + r * p.ss + v_off[c], w);
+#pragma unroll
+                    for (int i = 0; i < VN; ++i) vw[t][r][c + i] = w[i];
                 }
-            }
-            vsw[t] = load_scales(vsb + s_row[t] + s_off);
+            if constexpr (BIG) vsw[t] = __builtin_amdgcn_raw_buffer_load_b32(Uniform(vsb + s_row[t]).r, (int)s_off, 0, 0);
+            else vsw[t] = *reinterpret_cast<const uint32_t*>(vsb + s_row[t]);
         }
     };
 
-    // The first unit's ids, the queries, then its rows: in this order no load waits for one that it
-    // does not need.
     const bool any = ctx > 0 && x < b;
-    if (any) load_ids(x);
-    // Q^T: elements [kb D / 4, + D / 4) of the lane's row, 8 a step.
+    // Q^T: the lane's row, the dims that it has of K, 8 a step.
     constexpr int QW = D / 4 * (int)sizeof(T) / 8;
     uint2 qraw[QW];
     {
-        const T* q = reinterpret_cast<const T*>(p.q) + row_token(row) * p.q_st + row_head(row) * p.q_sh + kb * (D / 4);
+        const T* q = reinterpret_cast<const T*>(p.q) + row_token(row) * p.q_st + row_head(row) * p.q_sh + kb * (4 * KW);
 #pragma unroll
-        for (int i = 0; i < QW; ++i) qraw[i] = reinterpret_cast<const uint2*>(q)[i];
+        for (int i = 0; i < QW; ++i) qraw[i] = reinterpret_cast<const uint2*>(q + (i / (QW / KP)) * 64)[i % (QW / KP)];
     }
     if (any) {
         load_k(x);
         load_v();
-        load_ids(x + step);
+        load_ids(x + NW);
     }
     u32x4 qf[NQ][KS];
 #pragma unroll
@@ -387,10 +421,10 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
     while (any) {
         const int key0 = kUnit * x;
         const bool masked = key0 + kUnit - 1 > pos0;         // some row does not see some key
-        const bool more = x + step < b;
-        float s[8], vs[8];
+        const bool more = x + NW < b;
+        float s[4 * NT];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < NT; ++t) {
             f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
@@ -405,11 +439,11 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
         }
         // K's registers are free: the next unit's, under this one's softmax and second product. V's
         // follow below, under the next one's first product.
-        if (more) load_k(x + step);
+        if (more) load_k(x + NW);
         if (masked) {
             asm volatile("");                   // a branch, not selects in every unit
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4 * NT; ++e) {
                 const int key = key0 + 16 * (e >> 2) + 4 * kb + (e & 3);
                 if (key > limit) s[e] = kNegInf;
                 // Slots behind the context hold anything: 0 times a NaN would be NaN.
@@ -420,7 +454,7 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
         }
         float mt = s[0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) mt = fmaxf(mt, s[e]);
+        for (int e = 1; e < 4 * NT; ++e) mt = fmaxf(mt, s[e]);
         mt = max_across32(max_across16(mt));
         const bool raise = mt > m_run + kLazy;
         if (__builtin_amdgcn_ballot_w64(raise)) {
@@ -431,47 +465,57 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
             m_run = raise ? mt : m_run;
         }
         const float m_off = m_run == kNegInf ? 0.f : m_run;
-        scales8(vsw, vs);
-        float w[8];
+        float w[4 * NT];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float pe = fast_exp2(s[e] - m_off);
-            l_run += pe;
-            w[e] = pe * vs[e];
+        for (int t = 0; t < NT; ++t) {
+            float vs4[4];
+            scales4(vsw[t], vs4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float pe = fast_exp2(s[4 * t + r] - m_off);
+                l_run += pe;
+                w[4 * t + r] = pe * vs4[r];
+            }
         }
         if (masked) {
             asm volatile("");
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < 4 * NT; ++e)
                 if (key0 + 16 * (e >> 2) + 4 * kb + (e & 3) > limit) w[e] = 0.f;
         }
-        u32x4 pf[NP];
+        // 32 keys a step: tiles 2 h and 2 h + 1.
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            pf[i] = u32x4{pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3]), pack_bf16(w[4], w[5]), pack_bf16(w[6], w[7])};
-            if (i + 1 < NP)
+        for (int h = 0; h < NT / 2; ++h) {
+            float* wh = w + 8 * h;
+            u32x4 pf[NP];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] -= (float)(__bf16)w[e];
-        }
+            for (int i = 0; i < NP; ++i) {
+                pf[i] = u32x4{pack_bf16(wh[0], wh[1]), pack_bf16(wh[2], wh[3]), pack_bf16(wh[4], wh[5]),
+                              pack_bf16(wh[6], wh[7])};
+                if (i + 1 < NP)
 #pragma unroll
-        for (int c = 0; c < VD; ++c) {
-            uint32_t d0[4], d1[4];
-            const uint32_t r0[4] = {vw[0][0][c], vw[0][1][c], vw[0][2][c], vw[0][3][c]};
-            const uint32_t r1[4] = {vw[1][0][c], vw[1][1][c], vw[1][2][c], vw[1][3][c]};
-            transpose4(r0, d0);
-            transpose4(r1, d1);
+                    for (int e = 0; e < 8; ++e) wh[e] -= (float)(__bf16)wh[e];
+            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const u32x4 vf = u32x4{codes_bf16<false>(d0[j]), codes_bf16<true>(d0[j]), codes_bf16<false>(d1[j]),
-                                       codes_bf16<true>(d1[j])};
+            for (int c = 0; c < VD; ++c) {
+                uint32_t d0[4], d1[4];
+                const uint32_t r0[4] = {vw[2 * h][0][c], vw[2 * h][1][c], vw[2 * h][2][c], vw[2 * h][3][c]};
+                const uint32_t r1[4] = {vw[2 * h + 1][0][c], vw[2 * h + 1][1][c], vw[2 * h + 1][2][c], vw[2 * h + 1][3][c]};
+                transpose4(r0, d0);
+                transpose4(r1, d1);
 #pragma unroll
-                for (int i = 0; i < NP; ++i) o[4 * c + j] = mfma_bf16(vf, pf[i], o[4 * c + j]);
+                for (int j = 0; j < 4; ++j) {
+                    const u32x4 vf = u32x4{codes_bf16<false>(d0[j]), codes_bf16<true>(d0[j]), codes_bf16<false>(d1[j]),
+                                           codes_bf16<true>(d1[j])};
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) o[4 * c + j] = mfma_bf16(vf, pf[i], o[4 * c + j]);
+                }
             }
         }
         if (!more) break;
         load_v();
-        x += step;
-        load_ids(x + step);
+        x += NW;
+        load_ids(x + NW);
     }
 
     // ---- the waves' parts meet in LDS, row by row.
@@ -488,9 +532,9 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
             }
         if (kb == 0) lds.ml[wave][n] = make_float2(m_run, l_run);
     }
-    run_sync<COOP>();
-    constexpr int nthr = COOP ? 256 : 64;
-    const int thr = COOP ? (int)threadIdx.x : lane, wave0 = COOP ? 0 : wave;
+    run_sync<NW>();
+    constexpr int nthr = 64 * NW;
+    const int thr = NW > 1 ? (int)threadIdx.x : lane, wave0 = NW > 1 ? 0 : wave;
     const int items = rows * (D / 4);           // 4 elements of a row each
     auto out4 = [&](int e, const Part& x4) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
@@ -500,10 +544,23 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
     for (int e = thr; e < items; e += nthr) {
         const int r = e / (D / 4);
         Part acc = {kNegInf, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+        // All reads and exponentials side by side, as in Part::add.
+        float2 ml[NW];
+        float4 po[NW];
 #pragma unroll
-        for (int w = 0; w < (COOP ? 4 : 1); ++w) {
-            const float2 ml = lds.ml[wave0 + w][r];
-            acc.add(ml.x, ml.y, *reinterpret_cast<const float4*>(&lds.o[wave0 + w][e * 4]));
+        for (int w = 0; w < NW; ++w) {
+            ml[w] = lds.ml[wave0 + w][r];
+            po[w] = *reinterpret_cast<const float4*>(&lds.o[wave0 + w][e * 4]);
+            acc.m = fmaxf(acc.m, ml[w].x);
+        }
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float a = ml[w].y == 0.f ? 0.f : fast_exp2(ml[w].x - acc.m);
+            acc.l += a * ml[w].y;
+            acc.o.x += a * po[w].x;
+            acc.o.y += a * po[w].y;
+            acc.o.z += a * po[w].z;
+            acc.o.w += a * po[w].w;
         }
         if (whole) {
             out4(e, acc);
@@ -519,16 +576,16 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
         // The stores have reached the agent's coherence point before the counter moves (a
         // release fence would write back the XCD's whole L2 instead).
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        run_sync<COOP>();
+        run_sync<NW>();
         uint32_t* cnt = p.ws_cnt + ((int64_t)seq * heads + kvh);
         if (thr == 0) lds.arrived[wave0] = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        run_sync<COOP>();
+        run_sync<NW>();
         if (__builtin_amdgcn_readfirstlane(lds.arrived[wave0]) == (uint32_t)(parts - 1)) {
             if (thr == 0) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             // Threads beyond the items share the parts: group g takes g, g + groups, ...; group 0
             // then adds the groups up, in order.
             int groups = 1;
-            while (groups * 2 * items <= nthr) groups *= 2;
+            while (groups * 2 * items <= nthr && groups < parts) groups *= 2;
             const int g = groups > 1 ? thr / items : 0;
             float* so = lds.o[wave0];           // the parts are out: free (8 floats a thread)
             constexpr int CH = 4;               // partials whose loads are in flight together
@@ -558,7 +615,7 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
                         *reinterpret_cast<float4*>(to) = acc.o;
                         *reinterpret_cast<float2*>(to + 4) = make_float2(acc.m, acc.l);
                     }
-                    run_sync<COOP>();
+                    run_sync<NW>();
                     for (int k = 0; mine && g == 0 && k < groups - 1; ++k) {
                         const float* from = so + (k * items + e) * 8;
                         const float2 ml = *reinterpret_cast<const float2*>(from + 4);
@@ -573,9 +630,9 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, DecodeLds<D>&
 
 // (Slot, KV head) of a workgroup or wave: the heads of 8 slots take 8 * heads of them, one slot an
 // XCD (workgroup L runs on XCD L % 8).
-template <bool COOP>
+template <int NW>
 __device__ __forceinline__ void decode_place(const Kv8Params& p, int wave, int& slot, int& kvh) {
-    const int id = COOP ? (int)blockIdx.x : ((int)blockIdx.x >> 3) * 32 + (int)(blockIdx.x & 7) + 8 * wave;
+    const int id = NW > 1 ? (int)blockIdx.x : ((int)blockIdx.x >> 3) * 32 + (int)(blockIdx.x & 7) + 8 * wave;
     const int set = id / (8 * p.num_kv_heads), in = id - set * (8 * p.num_kv_heads);
     slot = set * 8 + (in & 7);
     kvh = in >> 3;
@@ -596,39 +653,45 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
-// Exclusive running sums of v over the workgroup's 256 threads, and their total.
+// Exclusive running sums of v over the workgroup's W waves, and their total.
+template <int W>
 __device__ __forceinline__ int block_scan(int v, int* s_wave, int& total) {
     const int lane = lane_id(), wave = (int)(threadIdx.x >> 6);
     int run = wave_scan(v);
     lds_barrier();                              // s_wave's last readers are done
     if (lane == 63) s_wave[wave] = run;
     lds_barrier();
-    total = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    total = 0;
+    for (int w = 0; w < W; ++w) total += s_wave[w];
     run -= v;
     for (int w = 0; w < wave; ++w) run += s_wave[w];
     return run;
 }
 // Waves a SIMD that registers are held to (128, 168 or 256 a lane): what fits without spills.
-template <typename T, int D>
-constexpr int kDecodeWaves = sizeof(T) == 2 ? (D <= 64 ? 4 : 3) : (D <= 80 ? 3 : 2);
+template <typename T, int D, bool LEAN>
+constexpr int kDecodeWaves = sizeof(T) == 2 ? (D <= 64 && LEAN ? 4 : 3) : (D <= 80 && (LEAN || D == 80) ? 3 : 2);
+// Waves of a workgroup that has one run: as many workgroups as registers have room for, so that
+// 8 waves only where two of them fit.
+template <typename T, int D, bool BIG>
+constexpr int kRunWaves = kDecodeWaves<T, D, BIG> == 4 ? 8 : 4;
 constexpr int kDecodePer = kDecodeMaxSeqs / 256;    // sequences per thread, at most
 
 // Even runs: the batch's units, sequence after sequence, cut into equal slots.
 template <typename T, int D, bool BIG>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWaves<T, D>))) void kv8_decode_even_kernel(const Kv8Params p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWaves<T, D, false>))) void kv8_decode_even_kernel(const Kv8Params p) {
     __shared__ int s_before[kDecodeMaxSeqs + 1];
     __shared__ int s_wave[4];
-    __shared__ DecodeLds<D> lds;
+    __shared__ DecodeLds<D, 4> lds;
     const int per = (p.num_seqs + 255) / 256, first = (int)threadIdx.x * per;
     int total;
     {
         int own = 0, u[kDecodePer];
 #pragma unroll
         for (int j = 0; j < kDecodePer; ++j) {
-            u[j] = j < per && first + j < p.num_seqs ? decode_units(p, first + j) : 0;
+            u[j] = j < per && first + j < p.num_seqs ? decode_units<D>(p, first + j) : 0;
             own += u[j];
         }
-        int run = block_scan(own, s_wave, total);
+        int run = block_scan<4>(own, s_wave, total);
 #pragma unroll
         for (int j = 0; j < kDecodePer; ++j)
             if (j < per && first + j < p.num_seqs) {
@@ -641,7 +704,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWave
     total = __builtin_amdgcn_readfirstlane(total);
     int slots = total / p.decode_min_units, slot, kvh;
     slots = slots < 1 ? 1 : slots < p.decode_slots ? slots : p.decode_slots;
-    decode_place<true>(p, 0, slot, kvh);
+    decode_place<4>(p, 0, slot, kvh);
     if (slot >= slots) return;
     // Slots [0, more) have len + 1 units, the others len.
     const int len = total / slots, more = total - len * slots;
@@ -660,40 +723,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWave
         if (before >= u1) break;
         if (after == before) continue;
         const int a = before < u0 ? u0 - before : 0, b = after > u1 ? u1 - before : after - before;
-        const bool whole = a == 0 && b == after - before;
         // A slot's partials: number 2 s of the sequence that it begins in, 2 s + 1 of the one that
         // it ends in.
         const int s0 = slot_of(before), s1 = slot_of(after - 1);
-        decode_segment<T, D, BIG, true>(
-            p, lds, seq, kvh, a, b, whole, s1 - s0 + 1, [&]() { return 2 * slot + (before <= u0 ? 0 : 1); },
+        decode_segment<T, D, BIG, 4>(
+            p, lds, seq, kvh, a, b, s1 - s0 + 1, [&]() { return 2 * slot + (before <= u0 ? 0 : 1); },
             [&](int k) { return 2 * (s0 + k) + (start_of(s0 + k) < before ? 1 : 0); });
         lds_barrier();                              // lds is free again
     }
 }
 
-// Runs that stay inside a sequence: the shortest runs, no less than decode_min_units, with which
-// all of them are at most decode_slots (twice the sequences if that is more); a sequence's are of
-// even lengths. A workgroup (COOP) or wave has one.
-template <typename T, int D, bool BIG, bool COOP>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWaves<T, D>))) void kv8_decode_runs_kernel(const Kv8Params p) {
-    __shared__ int s_wave[4];
-    __shared__ int s_found[4][5];                   // by run slot of the workgroup
-    __shared__ DecodeLds<D> lds;
+// Runs that stay inside a sequence: the shortest, no less than decode_min_units, with which all of
+// them are at most decode_slots (twice the sequences if that is more); a sequence's are of even
+// lengths. A workgroup of NW waves has one; NW = 1: each of four waves. decode_whole: no sequence
+// is cut, so that a run's sequence is its number and there is nothing to sum up.
+template <typename T, int D, bool BIG, int NW>
+__global__ __launch_bounds__(NW > 1 ? 64 * NW : 256) __attribute__((amdgpu_waves_per_eu(kDecodeWaves<T, D, BIG>)))
+void kv8_decode_runs_kernel(const Kv8Params p) {
+    constexpr int W = NW > 1 ? NW : 4;
+    __shared__ int s_wave[W];
+    __shared__ int s_found[4][4];                   // by run of the workgroup
+    __shared__ DecodeLds<D, W> lds;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     int slot, kvh;
-    decode_place<COOP>(p, wave, slot, kvh);
+    decode_place<NW>(p, wave, slot, kvh);
+    if (p.decode_whole) {
+        if (slot >= p.num_seqs || (p.qsl && p.qsl[slot + 1] <= p.qsl[slot])) return;
+        decode_segment<T, D, BIG, NW>(p, lds, slot, kvh, 0, 0, 1, [&]() { return 0; }, [&](int) { return 0; });
+        return;
+    }
     constexpr int kWhole = 1 << 30;                 // units: no sequence has more
     int seq, runs, number, units;                   // a sequence, its runs, this one's number, its units
     auto run_length = [&](int total) {
-        int len = p.ws_o ? p.decode_min_units : kWhole;     // no room for partials: sequences stay whole
         const int room = p.decode_slots > 2 * p.num_seqs ? p.decode_slots - p.num_seqs : p.num_seqs;
         const int even = (total + room - 1) / room;
-        return len > even ? len : even;
+        return p.decode_min_units > even ? p.decode_min_units : even;
     };
     if (p.num_seqs <= 64) {
         // Every wave for itself: lane i has sequence i.
         const int lane = lane_id();
-        const int u = lane < p.num_seqs ? decode_units(p, lane) : 0;
+        const int u = lane < p.num_seqs ? decode_units<D>(p, lane) : 0;
         int run = wave_scan(u);
         int len = run_length(__builtin_amdgcn_readlane(run, 63)), mine;
         while (true) {
@@ -709,32 +778,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWave
         number = slot - (__builtin_amdgcn_readlane(run, seq) - runs);
         units = __builtin_amdgcn_readlane(u, seq);
     } else {
-        const int per = (p.num_seqs + 255) / 256, first = (int)threadIdx.x * per;
+        const int per = (p.num_seqs + 255) / 256, first = (int)threadIdx.x * per;   // of the first 256 threads
         int own = 0, u[kDecodePer], total;
 #pragma unroll
         for (int j = 0; j < kDecodePer; ++j) {
-            u[j] = j < per && first + j < p.num_seqs ? decode_units(p, first + j) : 0;
+            u[j] = j < per && first + j < p.num_seqs ? decode_units<D>(p, first + j) : 0;
             own += u[j];
         }
-        block_scan(own, s_wave, total);
+        block_scan<W>(own, s_wave, total);
         int len = run_length(total), run;
         while (true) {
             own = 0;
 #pragma unroll
             for (int j = 0; j < kDecodePer; ++j) own += (u[j] + len - 1) / len;
-            run = block_scan(own, s_wave, total);
+            run = block_scan<W>(own, s_wave, total);
             if (total <= p.decode_grid || len == kWhole) break;
             len = kWhole;
         }
-        // The thread that has a run's sequence says so; a workgroup of wave runs has 4.
+        // The thread that has a run's sequence says so.
         if (threadIdx.x < 4) s_found[threadIdx.x][0] = -1;
         lds_barrier();
 #pragma unroll
         for (int j = 0; j < kDecodePer; ++j) {
             const int mine = (u[j] + len - 1) / len;
-            for (int w = 0; w < (COOP ? 1 : 4); ++w) {
+            for (int w = 0; w < (NW > 1 ? 1 : 4); ++w) {
                 int ws, head;
-                decode_place<COOP>(p, w, ws, head);
+                decode_place<NW>(p, w, ws, head);
                 if (mine && ws >= run && ws < run + mine) {
                     s_found[w][0] = first + j;
                     s_found[w][1] = mine;
@@ -745,7 +814,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWave
             run += mine;
         }
         lds_barrier();
-        const int w = COOP ? 0 : wave;
+        const int w = NW > 1 ? 0 : wave;
         seq = __builtin_amdgcn_readfirstlane(s_found[w][0]);
         if (seq < 0) return;
         runs = __builtin_amdgcn_readfirstlane(s_found[w][1]);
@@ -754,8 +823,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kDecodeWave
     }
     const int each = units / runs, more = units - each * runs;      // runs [0, more) have one more
     const int a = number * each + (number < more ? number : more), b = a + each + (number < more ? 1 : 0);
-    decode_segment<T, D, BIG, COOP>(p, lds, seq, kvh, a, b, runs == 1, runs, [&]() { return slot; },
-                                    [&](int k) { return slot - number + k; });
+    decode_segment<T, D, BIG, NW>(p, lds, seq, kvh, a, b, runs, [&]() { return slot; },
+                                  [&](int k) { return slot - number + k; });
 }
 
 template <typename T, int D, bool BIG>
@@ -765,8 +834,9 @@ int launch_kv8_decode_d(const Kv8Params& p, hipStream_t stream) {
     if (wgs > 0x7fffffff) return fail(PKV_EUNSUPPORTED, "kv8 decode attention: grid too large");
     const dim3 grid((unsigned)wgs);
     if (p.decode_mode == kKv8Even) kv8_decode_even_kernel<T, D, BIG><<<grid, 256, 0, stream>>>(p);
-    else if (p.decode_mode == kKv8Runs) kv8_decode_runs_kernel<T, D, BIG, true><<<grid, 256, 0, stream>>>(p);
-    else kv8_decode_runs_kernel<T, D, BIG, false><<<grid, 256, 0, stream>>>(p);
+    else if (p.decode_mode == kKv8Runs) 
+        kv8_decode_runs_kernel<T, D, BIG, kRunWaves<T, D, BIG>><<<grid, 64 * kRunWaves<T, D, BIG>, 0, stream>>>(p);
+    else kv8_decode_runs_kernel<T, D, BIG, 1><<<grid, 256, 0, stream>>>(p);
     return check_launch("kv8 decode attention");
 }
 
