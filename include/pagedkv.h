@@ -54,7 +54,8 @@ enum pkv_status {
     PKV_EINVAL = 1,        /* bad argument: null pointer, negative size, bad stride */
     PKV_EUNSUPPORTED = 2,  /* shape/dtype combination this build has no kernel for */
     PKV_EWORKSPACE = 3,    /* workspace smaller than pkv_*_workspace_bytes() says */
-    PKV_EHIP = 4           /* a HIP runtime call failed; message has hipGetErrorString */
+    PKV_EHIP = 4,          /* a HIP runtime call failed; message has hipGetErrorString */
+    PKV_ERANGE = 5         /* an index given in host memory is out of range */
 };
 
 /* ABI version of the loaded library; the host layer refuses a mismatch. */
@@ -457,7 +458,9 @@ int pkv_lm_head_argmax(
 /* Quantise row t of k_new / v_new ([num_tokens, num_kv_heads, head_dim], element strides
  * new_stride_t / new_stride_h, unit innermost stride) into flat slot slots[t] of the cache.
  * x * 2^(127 - b) is rounded once, to the nearest code, ties to even. Slots must be distinct;
- * those outside [0, num_blocks * block_size) are skipped. */
+ * those outside [0, num_blocks * block_size) are skipped. host_slots: the same values in HOST
+ * memory, or NULL; with them, such a slot is refused with PKV_ERANGE before anything is
+ * launched. */
 int pkv_kv8_append(
     void* k_codes, void* v_codes,
     int64_t code_stride_block, int64_t code_stride_slot, int64_t code_stride_head,
@@ -465,7 +468,7 @@ int pkv_kv8_append(
     int64_t scale_stride_block, int64_t scale_stride_slot, int64_t scale_stride_head,
     int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
     const void* k_new, const void* v_new, int64_t new_stride_t, int64_t new_stride_h,
-    const int64_t* slots, int64_t num_tokens, int dtype,
+    const int64_t* slots, const int64_t* host_slots, int64_t num_tokens, int dtype,
     hipStream_t stream);
 
 /* Attention over the 8-bit cache: pkv_paged_attention_prefill's contract (chunks of new

@@ -149,7 +149,7 @@ extern "C" int pkv_kv8_append(void* k_codes, void* v_codes, int64_t code_stride_
                               int64_t scale_stride_slot, int64_t scale_stride_head, int64_t num_blocks,
                               int64_t block_size, int64_t num_kv_heads, int64_t head_dim, const void* k_new,
                               const void* v_new, int64_t new_stride_t, int64_t new_stride_h, const int64_t* slots,
-                              int64_t num_tokens, int dtype, hipStream_t stream) {
+                              const int64_t* host_slots, int64_t num_tokens, int dtype, hipStream_t stream) {
     clear_error();
     if (dtype != PKV_FLOAT32 && dtype != PKV_FLOAT16 && dtype != PKV_BFLOAT16)
         return fail(PKV_EINVAL, "kv8_append: unknown dtype %d", dtype);
@@ -160,6 +160,12 @@ extern "C" int pkv_kv8_append(void* k_codes, void* v_codes, int64_t code_stride_
     if (num_tokens == 0) return PKV_OK;
     if (!k_codes || !v_codes || !k_scales || !v_scales || !k_new || !v_new || !slots)
         return fail(PKV_EINVAL, "kv8_append: null pointer");
+    if (host_slots) {
+        uint64_t high = 0;                      // a negative slot is above all others
+        for (int64_t i = 0; i < num_tokens; ++i) high = high > (uint64_t)host_slots[i] ? high : (uint64_t)host_slots[i];
+        if (high >= (uint64_t)(num_blocks * block_size))
+            return fail(PKV_ERANGE, "slot index outside [0, %lld)", (long long)(num_blocks * block_size));
+    }
     Kv8AppendArgs a = {};
     a.codes[0] = (uint8_t*)k_codes;
     a.codes[1] = (uint8_t*)v_codes;

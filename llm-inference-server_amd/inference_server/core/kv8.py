@@ -69,22 +69,29 @@ def _check_cache(name: str, cache: Kv8) -> None:
         raise ValueError(f"{name} codes are on {codes.device}, its scales on {scales.device}")
 
 
-def _check_pair(k: Kv8, v: Kv8) -> None:
+def _check_pair(k: Kv8, v: Kv8) -> torch.Size:
+    """The caches' shape, checked; messages for what is wrong are found only if something is."""
+    (kc, ks), (vc, vs) = k, v
+    shape = kc.shape
+    if (len(shape) == 4 and vc.shape == shape and kc.dtype is CODES and vc.dtype is CODES and ks.dtype is SCALES
+            and vs.dtype is SCALES and ks.shape == vs.shape == shape[:3]
+            and kc.get_device() == vc.get_device() == ks.get_device() == vs.get_device()):
+        return shape
     _check_cache("k_cache", k)
     _check_cache("v_cache", v)
-    if k.codes.shape != v.codes.shape:
-        raise ValueError(f"k_cache {tuple(k.codes.shape)} and v_cache {tuple(v.codes.shape)} differ")
-    if k.codes.device != v.codes.device:
-        raise ValueError(f"k_cache is on {k.codes.device}, v_cache on {v.codes.device}")
+    if vc.shape != shape:
+        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(vc.shape)} differ")
+    raise ValueError(f"k_cache is on {kc.device}, v_cache on {vc.device}")
 
 
 def _pointers(k: Kv8, v: Kv8) -> tuple | None:
     """The kernels' view of a cache: base pointers and strides, one set for K and V; None
     where it has no such view (codes' inner stride, or strides that differ)."""
-    c, s = k.codes.stride(), k.scales.stride()
-    if c[3] != 1 or v.codes.stride() != c or v.scales.stride() != s:
+    (kc, ks), (vc, vs) = k, v
+    c, s = kc.stride(), ks.stride()
+    if c[3] != 1 or vc.stride() != c or vs.stride() != s:
         return None
-    return (k.codes.data_ptr(), v.codes.data_ptr(), *c[:3], k.scales.data_ptr(), v.scales.data_ptr(), *s)
+    return (kc.data_ptr(), vc.data_ptr(), c[0], c[1], c[2], ks.data_ptr(), vs.data_ptr(), s[0], s[1], s[2])
 
 
 # ----------------------------------------------------------------------- append
@@ -96,39 +103,36 @@ def kv8_append(k_cache: Kv8, v_cache: Kv8, k: torch.Tensor, v: torch.Tensor, slo
     A slot outside the cache raises IndexError where the host knows the slots: `host_slots`,
     the same values on the CPU, or slots on the CPU themselves. On the device alone they are
     not read back: the kernel skips such rows (-1 is a padding row's slot)."""
-    k_cache, v_cache = Kv8(*k_cache), Kv8(*v_cache)
-    _check_pair(k_cache, v_cache)
-    n_blocks, bs, heads, dim = k_cache.codes.shape
-    if k.dim() != 3 or k.shape[1:] != (heads, dim) or v.shape != k.shape:
+    n_blocks, bs, heads, dim = _check_pair(k_cache, v_cache)
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape:
         raise ValueError(f"append rows {tuple(k.shape)} and {tuple(v.shape)} do not match cache rows [{heads}, {dim}]")
     if k.dtype not in _QUERY_DTYPES or v.dtype is not k.dtype:
         raise ValueError(f"append rows must both be float32, float16 or bfloat16, got {k.dtype} and {v.dtype}")
-    n_tok = k.shape[0]
-    if slots.shape != (n_tok,):
+    n_tok = shape[0]
+    if slots.dim() != 1 or slots.shape[0] != n_tok:
         raise ValueError(f"slots must be [{n_tok}], got {tuple(slots.shape)}")
-    dev = k_cache.codes.device
-    for name, t in (("k", k), ("v", v)):
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the cache on {dev}")
+    codes = k_cache[0]
+    if not k.get_device() == v.get_device() == codes.get_device():
+        raise ValueError(f"k is on {k.device}, v on {v.device}, the cache on {codes.device}")
     known = host_slots if host_slots is not None else slots if slots.device.type == "cpu" else None
     if known is not None:
         if known.shape != slots.shape:
             raise ValueError(f"host_slots must be [{n_tok}], got {tuple(known.shape)}")
-        if n_tok:
-            low, high = known.aminmax()
-            if int(low) < 0 or int(high) >= n_blocks * bs:
-                raise IndexError(f"slot index outside [0, {n_blocks * bs})")
+        if known.dtype is not torch.long or known.device.type != "cpu" or not known.is_contiguous():
+            known = known.to(device="cpu", dtype=torch.long).contiguous()
     if CONFIG.kv_backend != "hip":
-        _append_torch(k_cache, v_cache, k, v, slots, known is None)
+        _append_torch(Kv8(*k_cache), Kv8(*v_cache), k, v, slots, known)
         return
-    native.require_gpu(k_cache.codes, "kv8_append")
+    native.require_gpu(codes, "kv8_append")
     if n_tok == 0:
         return
     where = _pointers(k_cache, v_cache)
     if where is None:
         raise ValueError("kv8_append needs K and V caches of equal strides with unit head_dim stride; got "
-                         f"{k_cache.codes.stride()} / {v_cache.codes.stride()} and scales {k_cache.scales.stride()} / "
-                         f"{v_cache.scales.stride()}")
+                         f"{k_cache[0].stride()} / {v_cache[0].stride()} and scales {k_cache[1].stride()} / "
+                         f"{v_cache[1].stride()}")
+    dev = codes.device
     with native.on_device(dev):
         st = k.stride()
         if st[2] != 1 or v.stride() != st:
@@ -136,15 +140,20 @@ def kv8_append(k_cache: Kv8, v_cache: Kv8, k: torch.Tensor, v: torch.Tensor, slo
             st = k.stride()
         slots = _on_device(slots, dev).contiguous()
         rc = native.lib().pkv_kv8_append(
-            *where, n_blocks, bs, heads, dim, k.data_ptr(), v.data_ptr(), st[0], st[1], slots.data_ptr(), n_tok,
-            native.dtype_code(k.dtype), native.stream_handle(dev))
+            *where, n_blocks, bs, heads, dim, k.data_ptr(), v.data_ptr(), st[0], st[1], slots.data_ptr(),
+            None if known is None else known.data_ptr(), n_tok, native.DTYPE_CODES[k.dtype], native.stream_handle(dev))
+        if rc == native.PKV_ERANGE:
+            raise IndexError(native.lib().pkv_last_error().decode())
         native.check(rc, "pkv_kv8_append")
 
 
-def _append_torch(k_cache, v_cache, k, v, slots, unchecked: bool) -> None:
+def _append_torch(k_cache, v_cache, k, v, slots, known) -> None:
     n_blocks, bs = k_cache.codes.shape[:2]
     slots = slots.to(k_cache.codes.device, torch.long)
-    if unchecked:
+    if known is not None:
+        if known.numel() and (int(known.min()) < 0 or int(known.max()) >= n_blocks * bs):
+            raise IndexError(f"slot index outside [0, {n_blocks * bs})")
+    else:
         keep = (slots >= 0) & (slots < n_blocks * bs)
         k, v, slots = k[keep], v[keep], slots[keep]
     at = (slots // bs, slots % bs)
@@ -166,12 +175,11 @@ def paged_attention_kv8(query: torch.Tensor, k_cache: Kv8, v_cache: Kv8, block_t
     Softmax and sums are in fp32, the output is rounded once. A key that a query does not see
     does not reach it, whatever it holds. Lengths with host copies attached (attach_host) are
     checked without a device round trip."""
-    k_cache, v_cache = Kv8(*k_cache), Kv8(*v_cache)
     backend = CONFIG.attention
     if backend == "hip":
         return _attention_hip(query, k_cache, v_cache, block_tables, context_lens, query_lens, scale)
     if backend == "gather":
-        return _attention_gather(query, k_cache, v_cache, block_tables, context_lens, query_lens, scale)
+        return _attention_gather(query, Kv8(*k_cache), Kv8(*v_cache), block_tables, context_lens, query_lens, scale)
     if backend == "triton":
         raise NotImplementedError("ATTENTION=triton: this MI355X build ships no Triton kernel; use ATTENTION=hip "
                                   "(libpagedkv CDNA4 kernels) or ATTENTION=gather")
@@ -180,11 +188,11 @@ def paged_attention_kv8(query: torch.Tensor, k_cache: Kv8, v_cache: Kv8, block_t
 
 def _check_query(query: torch.Tensor, cache: Kv8) -> None:
     heads, dim = query.shape[1:]
-    kv, pool_dim = cache.codes.shape[2:]
+    kv, pool_dim = cache[0].shape[2:]
     if query.dtype not in _QUERY_DTYPES:
         raise ValueError(f"query must be float32, float16 or bfloat16, got {query.dtype}")
-    if query.device != cache.codes.device:
-        raise ValueError(f"the cache is on {cache.codes.device}, query is on {query.device}")
+    if query.get_device() != cache[0].get_device():
+        raise ValueError(f"the cache is on {cache[0].device}, query is on {query.device}")
     if dim != pool_dim:
         raise ValueError(f"query head_dim {dim} != cache head_dim {pool_dim}")
     if heads % kv:
@@ -193,6 +201,8 @@ def _check_query(query: torch.Tensor, cache: Kv8) -> None:
 
 def _attention_gather(query, k_cache, v_cache, tables, ctx, qlens, scale):
     _check_pair(k_cache, v_cache)
+    if tables.dim() != 2:
+        raise ValueError(f"block_tables must be [batch, width], got {tuple(tables.shape)}")
     check_contract(query.dim(), tuple(query.shape), 4, tuple(k_cache.codes.shape), tables.shape, ctx.shape, qlens.shape,
                    lambda: (int(qlens.sum()), bool((qlens > ctx).any()),
                             bool(((-(-ctx // k_cache.codes.shape[1])) > tables.shape[1]).any())))
@@ -213,38 +223,43 @@ def _attention_gather(query, k_cache, v_cache, tables, ctx, qlens, scale):
 
 def _attention_hip(query, k_cache, v_cache, tables, context_lens, query_lens, scale):
     native.require_gpu(query, "paged_attention_kv8")
-    _check_pair(k_cache, v_cache)
-    q_shape, c_shape, t_shape = query.shape, k_cache.codes.shape, tables.shape
+    c_shape = _check_pair(k_cache, v_cache)
+    q_shape, t_shape = query.shape, tables.shape
     n_blocks, block_size, n_kv, head_dim = c_shape
+    if len(t_shape) != 2:
+        raise ValueError(f"block_tables must be [batch, width], got {tuple(t_shape)}")
+    n_seqs, width = t_shape
     facts: dict | None = None
 
     def values():
         nonlocal facts
-        facts = _batch_facts(context_lens, query_lens, block_size, t_shape[1] if len(t_shape) == 2 else 0)
+        facts = _batch_facts(context_lens, query_lens, block_size, width)
+        if "negative" not in facts:
+            facts["negative"] = bool((facts["hql"] < 0).any())
         return facts["total"], facts["q_gt_c"], facts["too_few_blocks"]
 
     check_contract(len(q_shape), q_shape, 4, c_shape, t_shape, context_lens.shape, query_lens.shape, values)
     _check_query(query, k_cache)
-    if "negative" not in facts:
-        facts["negative"] = bool((facts["hql"] < 0).any())
     if facts["negative"]:
         raise ValueError("query_lens must not be negative")
-    dev, dt = query.device, native.dtype_code(query.dtype)
-    n_tok, n_heads = q_shape[:2]
-    n_seqs = t_shape[0]
+    dev, (n_tok, n_heads, _) = query.device, q_shape
     with native.on_device(dev):
         out = torch.empty(q_shape, dtype=query.dtype, device=dev)
         if n_tok == 0 or n_seqs == 0:
             return out
-        if query.stride(2) != 1:
+        q_st = query.stride()
+        if q_st[2] != 1:
             query = query.contiguous()
+            q_st = query.stride()
         where = _pointers(k_cache, v_cache)
         if where is None:
-            k_cache, v_cache = (Kv8(c.codes.contiguous(), c.scales.contiguous()) for c in (k_cache, v_cache))
+            k_cache, v_cache = (Kv8(*(t.contiguous() for t in c)) for c in (k_cache, v_cache))
             where = _pointers(k_cache, v_cache)
         tables = _on_device(tables, dev)
-        if tables.stride(1) != 1:
+        t_st = tables.stride()
+        if t_st[1] != 1:
             tables = tables.contiguous()
+            t_st = tables.stride()
         ctx_dev = _on_device(context_lens, dev).contiguous()
         stream = native.stream_handle(dev)
         qsl = None
@@ -252,23 +267,26 @@ def _attention_hip(query, k_cache, v_cache, tables, context_lens, query_lens, sc
             qsl = getattr(query_lens, _QSL_ATTR, None)
             if qsl is None:
                 qsl = _query_start(facts, context_lens, dev, stream)
+            qsl = qsl.data_ptr()
         lib = native.lib()
+        max_q, max_ctx = facts["max_q"], facts["max_ctx"]
         lens = (facts["hctx"].data_ptr(), facts["hql"].data_ptr())
-        sizes = (n_seqs, n_heads, n_kv, head_dim, n_tok, facts["max_q"], facts["max_ctx"], *lens)
-        shape = ("kv8", n_heads, n_kv, head_dim, n_tok)
-        ws_bytes = facts["split_ws"].get(shape)
+        # Workspace for contexts that are cut, sized by a step's first layer.
+        key = ("kv8", n_heads, n_kv, head_dim, n_tok)
+        ws_bytes = facts["split_ws"].get(key)
         if ws_bytes is None:
-            ws_bytes = facts["split_ws"][shape] = lib.pkv_kv8_attention_workspace_bytes(*sizes)
+            ws_bytes = facts["split_ws"][key] = lib.pkv_kv8_attention_workspace_bytes(
+                n_seqs, n_heads, n_kv, head_dim, n_tok, max_q, max_ctx, *lens)
         ws_ptr, ws_size = None, 0
         if ws_bytes:
             ws = _WORKSPACES.partials(dev, stream, ws_bytes)
             ws_ptr, ws_size = ws.data_ptr(), ws.numel()
         rc = lib.pkv_kv8_attention(
-            out.data_ptr(), out.stride(0), out.stride(1), query.data_ptr(), query.stride(0), query.stride(1),
+            out.data_ptr(), n_heads * head_dim, head_dim, query.data_ptr(), q_st[0], q_st[1],
             *where, n_blocks, block_size, n_kv, head_dim,
-            tables.data_ptr(), tables.stride(0), t_shape[1], ctx_dev.data_ptr(), None if qsl is None else qsl.data_ptr(),
-            n_seqs, n_heads, n_tok, facts["max_q"], facts["max_ctx"], *lens,
-            float(scale), dt, ws_ptr, ws_size, stream)
+            tables.data_ptr(), t_st[0], width, ctx_dev.data_ptr(), qsl,
+            n_seqs, n_heads, n_tok, max_q, max_ctx, *lens,
+            float(scale), native.DTYPE_CODES[query.dtype], ws_ptr, ws_size, stream)
         native.check(rc, "pkv_kv8_attention")
         return out
 

@@ -46,23 +46,24 @@ def step_layout(block_tables: torch.Tensor, held: torch.Tensor, context_lens: to
     context, a context wider than the table, held outside it, more new tokens than
     num_tokens), nothing is taken or written, every slot is -1 and query_start is all 0.
     `held` is not changed: the call can be repeated."""
+    inputs = (("block_tables", block_tables), ("held", held), ("context_lens", context_lens),
+              ("query_lens", query_lens), ("free_blocks", free_blocks))
     if block_tables.dim() != 2:
         raise ValueError(f"block_tables must be [batch, width], got {tuple(block_tables.shape)}")
     batch, width = block_tables.shape
-    for name, t in (("held", held), ("context_lens", context_lens), ("query_lens", query_lens)):
-        if t.shape != (batch,):
+    for name, t in inputs[1:4]:
+        if t.dim() != 1 or t.shape[0] != batch:
             raise ValueError(f"{name} must be [{batch}] to match block_tables, got {tuple(t.shape)}")
     if free_blocks.dim() != 1:
         raise ValueError(f"free_blocks must be one row of block ids, got {tuple(free_blocks.shape)}")
     if block_size < 1 or num_tokens < 0:
         raise ValueError(f"block_size must be positive and num_tokens not negative, got {block_size}, {num_tokens}")
-    dev = block_tables.device
-    for name, t in (("block_tables", block_tables), ("held", held), ("context_lens", context_lens),
-                    ("query_lens", query_lens), ("free_blocks", free_blocks)):
+    where = block_tables.get_device()
+    for name, t in inputs:
         if t.dtype is not torch.long:
             raise ValueError(f"{name} must be int64, got {t.dtype}")
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, block_tables on {dev}")
+        if t.get_device() != where:
+            raise ValueError(f"{name} is on {t.device}, block_tables on {block_tables.device}")
     if CONFIG.kv_backend != "hip":
         return _layout_torch(block_tables, held, context_lens, query_lens, free_blocks, block_size, num_tokens)
     native.require_gpu(block_tables, "step_layout")
@@ -70,13 +71,14 @@ def step_layout(block_tables: torch.Tensor, held: torch.Tensor, context_lens: to
     if batch and (width > 1 and stride[1] != 1 or batch > 1 and stride[0] < width):
         raise ValueError(f"block_tables are written in place: rows must be contiguous and distinct, "
                          f"got strides {stride}")
-    held, context_lens, query_lens, free_blocks = (
-        t.contiguous() for t in (held, context_lens, query_lens, free_blocks))
+    held, context_lens = held.contiguous(), context_lens.contiguous()
+    query_lens, free_blocks = query_lens.contiguous(), free_blocks.contiguous()
+    dev = block_tables.device
     with native.on_device(dev):
         # One allocation: held | query_start | counts | slots | positions.
         buf = torch.empty(2 * batch + 4 + 2 * num_tokens, dtype=torch.long, device=dev)
-        out = buf.split((batch, batch + 1, 3, num_tokens, num_tokens))
-        new_held, starts, counts, slots, positions = out
+        new_held, starts, counts, slots, positions = buf.split_with_sizes(
+            (batch, batch + 1, 3, num_tokens, num_tokens))
         rc = native.lib().pkv_step_layout(
             block_tables.data_ptr(), stride[0], width, held.data_ptr(), context_lens.data_ptr(),
             query_lens.data_ptr(), batch, free_blocks.data_ptr(), free_blocks.shape[0], block_size, num_tokens,

@@ -20,7 +20,7 @@ ABI_VERSION = 1
 PKV_FLOAT32, PKV_FLOAT16, PKV_BFLOAT16 = 0, 1, 2
 DTYPE_CODES = {torch.float32: PKV_FLOAT32, torch.float16: PKV_FLOAT16, torch.bfloat16: PKV_BFLOAT16}
 
-PKV_OK, PKV_EINVAL, PKV_EUNSUPPORTED, PKV_EWORKSPACE, PKV_EHIP = 0, 1, 2, 3, 4
+PKV_OK, PKV_EINVAL, PKV_EUNSUPPORTED, PKV_EWORKSPACE, PKV_EHIP, PKV_ERANGE = 0, 1, 2, 3, 4, 5
 #: include/pagedkv.h PKV_DECODE_SCRATCH_BYTES: the no-alloc decode entry's static scratch.
 DECODE_SCRATCH_BYTES = 96 * 1024 * 1024
 
@@ -154,7 +154,7 @@ SIGNATURES: dict[str, tuple] = {
          _ptr, _ptr, _i64, _i64, _i64,     # k_scales, v_scales, scale strides
          _i64, _i64, _i64, _i64,           # num_blocks, block_size, num_kv_heads, head_dim
          _ptr, _ptr, _i64, _i64,           # k_new, v_new, new strides (t, h)
-         _ptr, _i64, _int,                 # slots, num_tokens, dtype
+         _ptr, _ptr, _i64, _int,           # slots, host slots (or None), num_tokens, dtype
          _ptr],
     ),
     "pkv_kv8_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr]),
@@ -258,14 +258,13 @@ def stream_capture_id(stream: int) -> int:
 
 
 _HERE = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(device: torch.device):
-    """A context in which `device` is the current one: a stream takes launches and
-    allocations of its own device only."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)
+    """A context in which `device`, that of a tensor, is the current one: a stream takes
+    launches and allocations of its own device only."""
+    return _HERE if device.index == _current_device() else torch.cuda.device(device)
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

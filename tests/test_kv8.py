@@ -110,6 +110,8 @@ def test_refusals():
                                                       context_lens=ctx, query_lens=new, scale=0.1), **kw})
     with pytest.raises(ValueError, match="num_tokens, heads, dim"):
         call(query=s.q[0])
+    with pytest.raises(ValueError, match="batch, width"):
+        call(block_tables=tables[0])
     with pytest.raises(ValueError, match="sum to"):
         call(query=s.q[:2])
     with pytest.raises(ValueError, match="exceeds context_len"):
@@ -157,7 +159,7 @@ def test_library_refuses_bad_sizes():
 
     handle = native.load_library()
     append = lambda nb=1, d=64, t=1, dt=0: handle.pkv_kv8_append(  # noqa: E731
-        None, None, 1, 1, 1, None, None, 1, 1, 1, nb, 16, 1, d, None, None, 1, 1, None, t, dt, None)
+        None, None, 1, 1, 1, None, None, 1, 1, 1, nb, 16, 1, d, None, None, 1, 1, None, None, t, dt, None)
     assert append() == append(nb=0) == append(t=-1) == append(dt=3) == native.PKV_EINVAL
     assert append(d=513) == native.PKV_EUNSUPPORTED
     attend = lambda heads=2, kv=2, d=64, seqs=1, tok=1, dt=0, width=1: handle.pkv_kv8_attention(  # noqa: E731
