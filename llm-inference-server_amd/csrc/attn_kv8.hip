@@ -113,8 +113,7 @@ bool kv8_decode_applies(const Kv8Params& p, int dtype) {
     // Keys and units in 32 bits; so are the offsets of a lane inside 16 slots.
     const int64_t cap = p.table_width * p.block_size;
     if (cap > (1 << 30) || (cap / 32 + 1) * p.num_seqs > (1 << 30)) return false;
-    if (p.ss < 0 || p.ss > (1 << 26) || p.ss * p.block_size > (1 << 30)) return false;
-    if (p.sb < 0 || p.sb > 0x7fffffff || p.ssb < 0 || p.ssb > 0x7fffffff || p.num_blocks > 0x7fffffff) return false;
+    if (!kv8_offsets_fit(p)) return false;
     // 4 scale bytes are one load.
     const uint64_t scales = (uint64_t)(uintptr_t)p.ks | (uint64_t)(uintptr_t)p.vs | (uint64_t)p.ssb | (uint64_t)p.ssh;
     if (p.sss != 1 || scales % 4) return false;
@@ -166,7 +165,7 @@ int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* ho
 // ------------------------------------------------------------------ chunks
 bool kv8_chunk_applies(const Kv8Params& p, int dtype) {
     if (p.head_dim % 16 || p.head_dim < 32 || p.head_dim > 128 || p.block_shift < 0 || p.num_blocks < 1) return false;
-    if (!(p.scale > 0.f) || p.table_width * p.block_size > (1 << 30)) return false;
+    if (!(p.scale > 0.f) || p.table_width * p.block_size > (1 << 30) || p.num_blocks > 0x7fffffff) return false;
     const int64_t isz = dtype == PKV_FLOAT32 ? 4 : 2;
     const uint64_t probe = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * isz) |
                            (uint64_t)(p.q_sh * isz) | (uint64_t)(p.out_st * isz) | (uint64_t)(p.out_sh * isz) |

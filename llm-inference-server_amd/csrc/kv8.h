@@ -31,6 +31,14 @@ struct Kv8Params : AttnParams {
     int decode_mode, decode_slots, decode_grid, decode_min_units, decode_whole, decode_rows;
 };
 
+// Whether block strides, offsets inside a block and block numbers fit the 32-bit factors of the
+// kernels that compute uniform addresses from them.
+inline bool kv8_offsets_fit(const Kv8Params& p) {
+    auto small = [&](int64_t slot) { return slot >= 0 && slot <= (1 << 26) && slot * p.block_size <= (1 << 30); };
+    return small(p.ss) && small(p.sss) && p.sb >= 0 && p.sb <= 0x7fffffff && p.ssb >= 0 && p.ssb <= 0x7fffffff &&
+           p.num_blocks <= 0x7fffffff;
+}
+
 // 2^(b - 127), NaN for 255.
 __device__ __forceinline__ float scale_of(uint32_t b) {
     const uint32_t w = b << 23;

@@ -56,7 +56,10 @@ struct Stage<_Float16> {
     }
 };
 
-template <typename T, int D>
+// UNI: head_dim 64 or 128 and block sizes from 16 up: a wave's pieces of one load are 8 or 16
+// neighbouring rows of one block, so that addresses are uniform and loads cost no vector
+// arithmetic.
+template <typename T, int D, bool UNI>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void kv8_chunk_kernel(
     const Kv8Params p) {
     typedef typename Stage<T>::E E;
@@ -135,55 +138,85 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         lds0[j] = (uint32_t)(r * ROWB + (((2 * c) ^ lds_swizzle<D>(r)) << 4));
         lds1[j] = (uint32_t)(r * ROWB + (((2 * c + 1) ^ lds_swizzle<D>(r)) << 4));
     }
-    const int in_block = p.block_size - 1;
-    struct Raw {
-        Vec16 k[PIECES], v[PIECES];
-    };
-    // Bytes of a piece's scales: K's, V's in bits 8 to 15.
-    int64_t id[PIECES];
-    uint32_t sc[PIECES];
-    Raw raw;
-    // Keys past the last one of the workgroup repeat it: masked in S, finite in V.
-    auto key_of = [&](int kt, int j) {
-        const int key = kt * kKT + piece_row[j];
-        return key < kmax ? key : kmax - 1;
-    };
+    const int in_block = p.block_size - 1, last = kmax - 1;     // last: the workgroup's last key
+    // UNI: row of the wave's first piece of load j; a lane's offset from there.
+    auto wave_row = [&](int j) { return (256 * j + 64 * wave) / PPR; };
+    const uint32_t lane_off = (uint32_t)(lane / PPR * (int)p.ss + lane % PPR * 16);
+    const uint32_t lane_sc = (uint32_t)(lane / PPR * (int)p.sss);
+    constexpr int NI = UNI ? 1 : PIECES;
+    int64_t id[NI];                           // UNI: lane j holds that of load j
+    uint32_t ks_raw[PIECES], vs_raw[PIECES];
+    Vec16 k_raw[PIECES], v_raw[PIECES];
     auto load_ids = [&](int kt) {
+        if constexpr (UNI) {
+            const int key = kt * kKT + wave_row(lane % PIECES);
+            id[0] = table[(key < last ? key : last) >> p.block_shift];
+        } else {
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) id[j] = table[key_of(kt, j) >> p.block_shift];
-    };
-    auto load_tile = [&](int kt) {
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-            const int64_t b = (uint64_t)id[j] < (uint64_t)p.num_blocks ? id[j] : 0;   // never out of the cache
-            const int at = key_of(kt, j) & in_block;
-            const int64_t off = b * p.sb + at * p.ss + piece_at[j], so = b * p.ssb + at * p.sss;
-            raw.k[j] = load16(kc + off);
-            raw.v[j] = load16(vc + off);
-            sc[j] = (uint32_t)ksb[so] | (uint32_t)vsb[so] << 8;
+            for (int j = 0; j < PIECES; ++j) {
+                const int key = kt * kKT + piece_row[j];
+                id[j] = table[(key < last ? key : last) >> p.block_shift];
+            }
         }
     };
-    auto store_tile = [&](uint16_t* sk, uint16_t* sv) {
+    auto load_tile = [&](int kt) {
+        uint32_t blk[NI];                     // none is followed out of the cache
+#pragma unroll
+        for (int j = 0; j < NI; ++j) blk[j] = (uint64_t)id[j] < (uint64_t)p.num_blocks ? (uint32_t)id[j] : 0u;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            if constexpr (UNI) {
+                const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)blk[0], j);
+                const int at = (kt * kKT + wave_row(j)) & in_block;
+                const uint64_t off = (uint64_t)b * (uint32_t)p.sb + (uint32_t)(at * (int)p.ss);
+                const uint64_t so = (uint64_t)b * (uint32_t)p.ssb + (uint32_t)(at * (int)p.sss);
+                auto rsrc = [](const uint8_t* base) {
+                    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, -1, 0x00027000);
+                };
+                const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(rsrc(kc + off), (int)lane_off, 0, 0);
+                const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rsrc(vc + off), (int)lane_off, 0, 0);
+                k_raw[j] = Vec16{{k.x, k.y, k.z, k.w}};
+                v_raw[j] = Vec16{{v.x, v.y, v.z, v.w}};
+                ks_raw[j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(ksb + so), (int)lane_sc, 0, 0);
+                vs_raw[j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(vsb + so), (int)lane_sc, 0, 0);
+            } else {
+                const int key = kt * kKT + piece_row[j], at = (key < last ? key : last) & in_block;
+                const int64_t off = (int64_t)blk[j] * p.sb + at * p.ss + piece_at[j];
+                const int64_t so = (int64_t)blk[j] * p.ssb + at * p.sss;
+                k_raw[j] = load16(kc + off);
+                v_raw[j] = load16(vc + off);
+                ks_raw[j] = ksb[so];
+                vs_raw[j] = vsb[so];
+            }
+        }
+    };
+    // Rows past the last key are zeros (whatever was loaded there): masked in S, and V finite.
+    auto store_tile = [&](int kt, uint16_t* sk, uint16_t* sv) {
+        const bool ends = kt * kKT + kKT - 1 > last;
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
             if (!kWhole && 256 * j + tid >= kKT * PPR) continue;
-            const uint32_t kb = sc[j] & 255u, vb = sc[j] >> 8;
-            const bool bad = kb == (uint32_t)kScaleNan || vb == (uint32_t)kScaleNan;
-            const float ks = (bad ? 1.f : scale_of(kb)) * Stage<T>::kFactor;
-            const float vs = (bad ? 1.f : scale_of(vb)) * Stage<T>::kFactor;
+            auto scale = [&](uint32_t b) {    // 2^(b - 127), infinite for 255
+                const uint32_t e = b << 23;
+                return __builtin_bit_cast(float, e > 0x00400000u ? e : 0x00400000u) * Stage<T>::kFactor;
+            };
+            const float ks = scale(ks_raw[j]), vs = scale(vs_raw[j]);
             uint32_t a[8], b[8];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                a[2 * w] = Stage<T>::template cvt<false>(raw.k[j].w[w], ks);
-                a[2 * w + 1] = Stage<T>::template cvt<true>(raw.k[j].w[w], ks);
-                b[2 * w] = Stage<T>::template cvt<false>(raw.v[j].w[w], vs);
-                b[2 * w + 1] = Stage<T>::template cvt<true>(raw.v[j].w[w], vs);
+                a[2 * w] = Stage<T>::template cvt<false>(k_raw[j].w[w], ks);
+                a[2 * w + 1] = Stage<T>::template cvt<true>(k_raw[j].w[w], ks);
+                b[2 * w] = Stage<T>::template cvt<false>(v_raw[j].w[w], vs);
+                b[2 * w + 1] = Stage<T>::template cvt<true>(v_raw[j].w[w], vs);
             }
-            if (bad) {
+            const bool bad = ks_raw[j] == (uint32_t)kScaleNan || vs_raw[j] == (uint32_t)kScaleNan;
+            const bool none = ends && kt * kKT + piece_row[j] > last;
+            if (__builtin_amdgcn_ballot_w64(bad || none)) {
+                const uint32_t fill = none ? 0u : Stage<T>::kNan2;
 #pragma unroll
                 for (int w = 0; w < 8; ++w) {
-                    a[w] = Stage<T>::kNan2;
-                    b[w] = 0u;
+                    a[w] = bad || none ? fill : a[w];
+                    b[w] = bad || none ? 0u : b[w];
                 }
             }
             store16((char*)sk + lds0[j], Vec16{{a[0], a[1], a[2], a[3]}});
@@ -249,12 +282,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     auto tile = [&](int kt, const uint16_t* tile_k, const uint16_t* tile_v, uint16_t* nk, uint16_t* nv) {
         lds_barrier();                        // tile kt is staged, tile kt - 1 is done with
         const bool more = kt + 1 < t_end;
-        if (more) load_tile(kt + 1);
-        if (kt + 2 < t_end) load_ids(kt + 2);
         const bool sees = kt * kKT < wave_kmax;
+        f32x16 st[2];
         if (sees) {
             __builtin_amdgcn_s_setprio(1);
-            f32x16 st[2];
             st[0] = f32x16{};
             st[1] = f32x16{};
 #pragma unroll
@@ -267,6 +298,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
                     for (int i = 0; i < NP; ++i) st[half] = Mfma<E>::run(u32x4{a.x, a.y, a.z, a.w}, qf[i][s], st[half]);
                 }
             __builtin_amdgcn_s_setprio(0);
+        }
+        if (more) load_tile(kt + 1);          // behind the first product, which it would delay
+        if (kt + 2 < t_end) load_ids(kt + 2);
+        if (sees) {
             if (kt * kKT + kKT - 1 > first_pos) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
@@ -326,12 +361,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
                 }
             }
         }
-        if (more) store_tile(nk, nv);
+        if (more) store_tile(kt + 1, nk, nv);
     };
     if (t_begin < t_end) {
         load_tile(t_begin);
         if (t_begin + 1 < t_end) load_ids(t_begin + 1);
-        store_tile(s_k0, s_v0);
+        store_tile(t_begin, s_k0, s_v0);
     }
     for (int kt = t_begin; kt < t_end; kt += 2) {
         tile(kt, s_k0, s_v0, s_k1, s_v1);
@@ -389,7 +424,11 @@ inline int64_t kv8_chunk_workgroups(const Kv8Params& p) {
 
 template <typename T, int D>
 int launch_kv8_chunk_d(const Kv8Params& p, hipStream_t stream) {
-    kv8_chunk_kernel<T, D><<<dim3((unsigned)kv8_chunk_workgroups(p)), 256, 0, stream>>>(p);
+    const dim3 grid((unsigned)kv8_chunk_workgroups(p));
+    if ((D == 64 || D == 128) && p.block_size >= 16 && kv8_offsets_fit(p))
+        kv8_chunk_kernel<T, D, D == 64 || D == 128><<<grid, 256, 0, stream>>>(p);
+    else
+        kv8_chunk_kernel<T, D, false><<<grid, 256, 0, stream>>>(p);
     const int rc = check_launch("kv8 chunk attention");
     if (rc || p.splits == 1) return rc;
     const int64_t rows = p.num_tokens * p.num_heads;
