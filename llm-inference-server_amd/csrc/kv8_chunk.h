@@ -13,8 +13,8 @@
 //    v_cvt_scalef32_pk a pair, exact - and written to LDS as 16-bit rows. Converting once for the
 //    workgroup instead of in each of its four waves costs a quarter of the VALU time, of which
 //    the softmax leaves little; a tile's LDS traffic is the 16-bit kernel's.
-//  * Loads of the next tile are in flight under the current one's products, its block ids and
-//    scale bytes one tile further ahead.
+//  * A tile is loaded during the one before the one before it, and converted while the matrix unit
+//    is at the first product of the one before it; its block ids come a tile further ahead.
 //  * NaN: a row whose scale is NaN (its codes are 0) makes its key's scores NaN, also if it is
 //    V's, whose row is staged as zeros: the causal mask then hides it from rows that do not see
 //    it, which a weight of 0 times NaN would not.
@@ -212,6 +212,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
             const bool bad = ks_raw[j] == (uint32_t)kScaleNan || vs_raw[j] == (uint32_t)kScaleNan;
             const bool none = ends && kt * kKT + piece_row[j] > last;
             if (__builtin_amdgcn_ballot_w64(bad || none)) {
+                asm volatile("");             // a branch, not selects in every tile
                 const uint32_t fill = none ? 0u : Stage<T>::kNan2;
 #pragma unroll
                 for (int w = 0; w < 8; ++w) {
@@ -281,7 +282,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 
     auto tile = [&](int kt, const uint16_t* tile_k, const uint16_t* tile_v, uint16_t* nk, uint16_t* nv) {
         lds_barrier();                        // tile kt is staged, tile kt - 1 is done with
-        const bool more = kt + 1 < t_end;
         const bool sees = kt * kKT < wave_kmax;
         f32x16 st[2];
         if (sees) {
@@ -299,8 +299,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
                 }
             __builtin_amdgcn_s_setprio(0);
         }
-        if (more) load_tile(kt + 1);          // behind the first product, which it would delay
-        if (kt + 2 < t_end) load_ids(kt + 2);
+        // The next tile's rows, loaded a tile ago, go to LDS in the shadow of the first product; the
+        // loads of the one after it follow.
+        if (kt + 1 < t_end) store_tile(kt + 1, nk, nv);
+        if (kt + 2 < t_end) load_tile(kt + 2);
+        if (kt + 3 < t_end) load_ids(kt + 3);
         if (sees) {
             if (kt * kKT + kKT - 1 > first_pos) {
 #pragma unroll
@@ -322,6 +325,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
             const float m_new = raise ? mt : m_run;
             const float alpha = raise ? fast_exp2(m_run - mt) : 1.f;
             if (__builtin_amdgcn_ballot_w64(raise)) {
+                asm volatile("");             // likewise
 #pragma unroll
                 for (int t = 0; t < DTILES; ++t) o[t] *= alpha;
             }
@@ -361,12 +365,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
                 }
             }
         }
-        if (more) store_tile(kt + 1, nk, nv);
     };
     if (t_begin < t_end) {
         load_tile(t_begin);
         if (t_begin + 1 < t_end) load_ids(t_begin + 1);
         store_tile(t_begin, s_k0, s_v0);
+        if (t_begin + 1 < t_end) load_tile(t_begin + 1);
+        if (t_begin + 2 < t_end) load_ids(t_begin + 2);
     }
     for (int kt = t_begin; kt < t_end; kt += 2) {
         tile(kt, s_k0, s_v0, s_k1, s_v1);
