@@ -127,12 +127,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     const uint8_t* ksb = p.ks + kvh * p.ssh;
     const uint8_t* vsb = p.vs + kvh * p.ssh;
     const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
+    // UNI: the 8 lanes of one LDS write cycle have 4 pieces of each of two rows whose swizzles differ
+    // in parity (4 rows apart at head_dim 128, 8 at 64), so that they hit all 32 banks; a whole
+    // row's pieces, even chunks only, hit half of them twice.
+    const int lane_row = !UNI ? 0 : D == 128 ? (lane >> 4) + 4 * (lane >> 2 & 1) : (lane >> 3) + 8 * (lane >> 2 & 1);
+    const int lane_c = D == 128 ? (lane & 3) + 4 * (lane >> 3 & 1) : lane & 3;
     int piece_row[PIECES], piece_at[PIECES];
     uint32_t lds0[PIECES], lds1[PIECES];
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         const int i = 256 * j + tid;
-        const int r = i / PPR < kKT ? i / PPR : kKT - 1, c = i % PPR;
+        const int r = UNI ? (256 * j + 64 * wave) / PPR + lane_row : i / PPR < kKT ? i / PPR : kKT - 1;
+        const int c = UNI ? lane_c : i % PPR;
         piece_row[j] = r;
         piece_at[j] = 16 * c;
         lds0[j] = (uint32_t)(r * ROWB + (((2 * c) ^ lds_swizzle<D>(r)) << 4));
@@ -141,8 +147,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     const int in_block = p.block_size - 1, last = kmax - 1;     // last: the workgroup's last key
     // UNI: row of the wave's first piece of load j; a lane's offset from there.
     auto wave_row = [&](int j) { return (256 * j + 64 * wave) / PPR; };
-    const uint32_t lane_off = (uint32_t)(lane / PPR * (int)p.ss + lane % PPR * 16);
-    const uint32_t lane_sc = (uint32_t)(lane / PPR * (int)p.sss);
+    const uint32_t lane_off = (uint32_t)(lane_row * (int)p.ss + lane_c * 16);
+    const uint32_t lane_sc = (uint32_t)(lane_row * (int)p.sss);
     constexpr int NI = UNI ? 1 : PIECES;
     int64_t id[NI];                           // UNI: lane j holds that of load j
     uint32_t ks_raw[PIECES], vs_raw[PIECES];
