@@ -130,7 +130,15 @@ bool kv8_decode_applies(const Kv8Params& p, int dtype) {
 int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* host_qlen) {
     constexpr int64_t kWorkgroups = 256 * 3;    // that the GPU holds
     const int64_t keys = p.head_dim <= 64 ? 64 : 32;    // of a unit
-    constexpr int64_t kEvenKeys = 768;          // per workgroup of even runs, at least
+    // Even runs from this many keys a workgroup on: below, runs inside sequences are as good (us a
+    // call, 32/8 heads of 128: 16 sequences of 1-8k 34.1 even, 34.4 not; 64 of 1-16k 191 and 204;
+    // 128 of 0.5-8k 198 and 232). Not up to head_dim 64, where two heads share a line and the runs'
+    // heads, a workgroup each at the same place, find it in L2 (12 heads of 64: 64 sequences up to
+    // 8k 128 even, 106 not; 256 up to 1k 88 and 64).
+    constexpr int64_t kEvenKeys = 768;
+    // Two workgroups a CU read as fast as three, and leave fewer parts to merge (a lone sequence of
+    // 100k tokens 48.7 us with 768, 47.2 with 512).
+    constexpr int64_t kEvenWorkgroups = 256 * 2;
     const int64_t heads = p.num_kv_heads, seqs = p.num_seqs, pairs = seqs * heads;
     int64_t units = 0, runs = 0;
     auto each = [&](auto f) {
@@ -144,10 +152,10 @@ int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* ho
     p.decode_rows = (int)((int64_t)p.max_query_len * p.group);
     const bool cuts = pairs * 4 <= kMergeCounterBytes;
     auto bytes = [&](int64_t numbers) { return numbers * heads * p.decode_rows * (p.head_dim + 2) * 4; };
-    if (cuts && units * keys * heads >= kWorkgroups * kEvenKeys) {
+    if (cuts && p.head_dim > 64 && units * keys * heads >= kWorkgroups * kEvenKeys) {
         p.decode_mode = kKv8Even;
-        p.decode_min_units = (int)(256 / keys);
-        const int64_t most = kWorkgroups / heads;
+        p.decode_min_units = 8;
+        const int64_t most = kEvenWorkgroups / heads;
         p.decode_slots = p.decode_grid = (int)(most < 1 ? 1 : most);
         return bytes(2 * p.decode_slots);
     }
