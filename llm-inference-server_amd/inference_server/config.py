@@ -18,6 +18,7 @@ import torch
 SEED = 1337                      # config.py:16
 DEFAULT_NUM_BLOCKS = 2048        # config.py:20: max_running * max_seq_len / block_size
 ATTENTION_BACKENDS = ("gather", "triton", "hip")
+KV_CACHES = ("model", "fp8")
 
 
 def seed_everything(seed: int = SEED) -> None:
@@ -44,6 +45,9 @@ class Config:
     block_size: int = int(os.environ.get("BLOCK_SIZE", 16))
     num_blocks: int = int(os.environ.get("NUM_BLOCKS", DEFAULT_NUM_BLOCKS))
     attention: str = os.environ.get("ATTENTION", "gather")
+    # What the KV pool holds: "model" (the model's dtype, the reference's), or "fp8" (e4m3 with a
+    # power-of-two scale a row, core/kv8.py: half the bytes of fp16 a token).
+    kv_cache: str = os.environ.get("KV_CACHE", "model")
     prefix_caching: bool = os.environ.get("PREFIX_CACHING", "1") == "1"
     preemption: str = os.environ.get("PREEMPTION", "recompute")
     # ATTENTION=hip on a GPU: replay decode steps as captured HIP graphs (one per batch size),

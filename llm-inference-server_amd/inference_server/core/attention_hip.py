@@ -89,6 +89,7 @@ class _Workspaces:
         self._kept: list[torch.Tensor] = []
         # (capture id, buffer) of the capture under way on a stream.
         self._captured: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
+        self._own: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
 
     def partials(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -112,12 +113,26 @@ class _Workspaces:
                 self._bufs[key] = buf
             return buf
 
+    def of_capture(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+        """A buffer of the capture under way alone, whatever the stream has: shared by its calls
+        that ask here, cleared by every replay at the first of them."""
+        idx = device.index if device.index is not None else torch.cuda.current_device()
+        capture = native.stream_capture_id(stream)
+        with self._lock:
+            held = self._own.get((idx, stream))
+            if held is None or held[0] != capture or held[1].numel() < nbytes:
+                buf = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+                buf[:_COUNTER_BYTES].zero_()
+                held = self._own[(idx, stream)] = (capture, buf)
+            return held[1]
+
     def reset(self) -> None:
         """Forget every buffer (the next call on each stream allocates a zeroed one)."""
         with self._lock:
             self._bufs.clear()
             self._kept.clear()
             self._captured.clear()
+            self._own.clear()
 
 
 _WORKSPACES = _Workspaces()

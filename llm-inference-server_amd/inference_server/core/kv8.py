@@ -279,7 +279,10 @@ def _attention_hip(query, k_cache, v_cache, tables, context_lens, query_lens, sc
                 n_seqs, n_heads, n_kv, head_dim, n_tok, max_q, max_ctx, *lens)
         ws_ptr, ws_size = None, 0
         if ws_bytes:
-            ws = _WORKSPACES.partials(dev, stream, ws_bytes)
+            # A capture's calls have one of their own: replays of graphs that were captured on one
+            # stream may overlap.
+            capturing = torch.cuda.is_current_stream_capturing()
+            ws = (_WORKSPACES.of_capture if capturing else _WORKSPACES.partials)(dev, stream, ws_bytes)
             ws_ptr, ws_size = ws.data_ptr(), ws.numel()
         rc = lib.pkv_kv8_attention(
             out.data_ptr(), n_heads * head_dim, head_dim, query.data_ptr(), q_st[0], q_st[1],

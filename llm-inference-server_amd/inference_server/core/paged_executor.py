@@ -42,6 +42,7 @@ from inference_server.config import CONFIG
 from inference_server.core.attention import paged_attention
 from inference_server.core.attention_hip import attach_host, paged_attention_hip_launch
 from inference_server.core.decode_graphs import DecodeGraphs, PrefillGraphs
+from inference_server.core.kv8 import Kv8Pool, paged_attention_kv8
 from inference_server.core.kv_pool import PagedKVPool
 from inference_server.core.qkv_epilogue import QkvEpilogue
 from inference_server.core.sampling import fused_greedy_supported, fused_max_rows, lm_head_argmax, lm_head_weight
@@ -117,6 +118,9 @@ def _paged_attention_forward(module, query, key, value, attention_mask, scaling=
         new = (key[0].transpose(0, 1), value[0].transpose(0, 1), ctx.write_slots)
         out = paged_attention_hip_launch(q, ctx.pool.k[module.layer_idx], ctx.pool.v[module.layer_idx],
                                          ctx.block_tables, ctx.context_lens, ctx.query_lens, scaling, append=new)
+    elif isinstance(ctx.pool, Kv8Pool):
+        out = paged_attention_kv8(q, *ctx.pool.layer(module.layer_idx), ctx.block_tables, ctx.context_lens,
+                                  ctx.query_lens, scaling)
     else:
         out = paged_attention(q, ctx.pool.k[module.layer_idx], ctx.pool.v[module.layer_idx], ctx.block_tables,
                               ctx.context_lens, ctx.query_lens, scaling)

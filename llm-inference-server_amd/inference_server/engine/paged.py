@@ -16,8 +16,9 @@ from dataclasses import dataclass
 
 import torch
 
-from inference_server.config import CONFIG
+from inference_server.config import CONFIG, KV_CACHES
 from inference_server.core.block_allocator import BlockAllocator
+from inference_server.core.kv8 import Kv8Pool
 from inference_server.core.kv_pool import ModelDims, PagedKVPool
 from inference_server.core.paged_executor import PagedExecutor
 from inference_server.core.prefix_cache import PrefixCache
@@ -54,9 +55,12 @@ class PagedEngine:
         self.tokenizer = tokenizer
         self.device = device or str(next(model.parameters()).device)
         # The pool stores K/V in the model's own dtype (the reference takes it from the
-        # DTYPE setting, which must then match the loaded model).
+        # DTYPE setting, which must then match the loaded model), or quantised from it.
         dims = ModelDims.from_model(model, dtype=next(model.parameters()).dtype)
-        self.pool = PagedKVPool(dims, num_blocks=num_blocks, block_size=block_size, device=self.device)
+        if CONFIG.kv_cache not in KV_CACHES:
+            raise ValueError(f"unknown KV_CACHE={CONFIG.kv_cache!r}; expected one of {KV_CACHES}")
+        pool_type = Kv8Pool if CONFIG.kv_cache == "fp8" else PagedKVPool
+        self.pool = pool_type(dims, num_blocks=num_blocks, block_size=block_size, device=self.device)
         self.allocator = BlockAllocator(self.pool.num_blocks)
         use_prefix = CONFIG.prefix_caching if prefix_caching is None else prefix_caching
         self.prefix_cache = PrefixCache(self.allocator, block_size) if use_prefix else None

@@ -402,3 +402,34 @@ def test_pool_moves_codes_and_scales_together():
         want[[9, 0]] = b[[1, 4]]
         want[[3, 5, 6]] = b[[4, 2, 7]]
         assert torch.equal(t, want)
+
+
+def test_graphs_of_one_stream_replayed_side_by_side():
+    """Two graphs captured on one stream, each with contexts that are cut, replayed at the same
+    time on two others: each capture has its own workspace."""
+    batches = [batch([(6000, 1), (3000, 1)], heads=8, kv=2, d=128, bs=16, dtype=BF16, device="cuda", seed=k)
+               for k in range(2)]
+    for s in batches:
+        attach_host(s.args[1], torch.from_numpy(s.ctx))
+        attach_host(s.args[2], torch.from_numpy(s.new))
+    stream, want, graphs = torch.cuda.Stream(), [], []
+    for s in batches:
+        with torch.cuda.stream(stream):
+            want.append(call(s))
+        torch.cuda.synchronize()
+        check(s, want[-1])
+    for s in batches:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs = [call(s) for _ in range(8)]
+        graphs.append((graph, outs))
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for (graph, outs), side in zip(graphs, sides):
+            with torch.cuda.stream(side):
+                for o in outs:
+                    o.fill_(float("nan"))
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, outs), w in zip(graphs, want):
+            assert all(torch.equal(o, w) for o in outs)
