@@ -28,8 +28,6 @@
 //    several heads.
 #pragma once
 
-#include <type_traits>
-
 #include "kv8.h"
 
 namespace pkv {
@@ -662,21 +660,6 @@ __device__ __forceinline__ void decode_place(const Kv8Params& p, int wave, int& 
     const int set = id / (8 * p.num_kv_heads), in = id - set * (8 * p.num_kv_heads);
     slot = set * 8 + (in & 7);
     kvh = in >> 3;
-}
-
-// Inclusive running sums over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-    auto add = [&](auto ctrl, auto rows) {
-        v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
-    };
-    using std::integral_constant;
-    add(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());    // row_shr 1, 2, 4, 8
-    add(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
-    add(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
-    add(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
-    add(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());    // row_bcast 15, to rows 1 and 3
-    add(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());    // row_bcast 31, to rows 2 and 3
-    return v;
 }
 
 // Exclusive running sums of v over the workgroup's W waves, and their total.

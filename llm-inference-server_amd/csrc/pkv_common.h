@@ -220,6 +220,16 @@ __device__ __forceinline__ float fold_lanes(float x) {
     return x;
 }
 
+// Inclusive running sums over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);     // row_bcast 15, to rows 1 and 3
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast 31, to rows 2 and 3
+}
+
 // Workgroup barrier that orders LDS only. __syncthreads() also fences global memory,
 // which makes every wave wait for ALL of its outstanding global loads at the barrier;
 // this one lets prefetched loads stay in flight across it.

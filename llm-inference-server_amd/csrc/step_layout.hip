@@ -33,27 +33,28 @@ struct LayoutArgs {
     int64_t* counts;                 // blocks taken, blocks needed, impossible lengths
 };
 
-__device__ __forceinline__ int64_t shfl_up64(int64_t v, int by) {
-    const int lo = __shfl_up((int)(uint32_t)(uint64_t)v, by), hi = __shfl_up((int)(v >> 32), by);
-    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+// Inclusive running sums over the wave's lanes of values below 2^40, in 20-bit halves (DPP moves
+// 32 bits).
+__device__ __forceinline__ int64_t wave_scan64(int64_t v) {
+    const int lo = wave_scan((int)(v & 0xfffff)), hi = wave_scan((int)(v >> 20));
+    return ((int64_t)hi << 20) + lo;
 }
 
 struct Sums {
     int64_t tokens, blocks, bad;
-    __device__ __forceinline__ Sums operator+(const Sums& o) const {
-        return Sums{tokens + o.tokens, blocks + o.blocks, bad + o.bad};
-    }
 };
 
 // N threads: one sequence each, N sequences a pass.
 template <int N>
 __global__ __launch_bounds__(N) void step_layout_kernel(const LayoutArgs a) {
     constexpr int W = N / 64;
-    __shared__ Sums s_wave[W];
+    __shared__ int64_t s_tokens[W], s_blocks[W];
+    __shared__ int s_bad[W];
     __shared__ int64_t s_token0[N], s_block0[N];   // running sums before each sequence of the pass
     __shared__ int64_t s_shift[N];                 // token number -> position
     __shared__ int64_t s_held[N];
-    const int tid = (int)threadIdx.x, lane = lane_id(), wave = tid >> 6;
+    const int tid = (int)threadIdx.x, lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     auto div = [&](int64_t x) { return a.block_shift >= 0 ? x >> a.block_shift : x / a.block_size; };
 
     int64_t ctx = 0, q = 0, held = 0;              // this thread's sequence of the pass
@@ -67,28 +68,28 @@ __global__ __launch_bounds__(N) void step_layout_kernel(const LayoutArgs a) {
         }
         const int64_t need = ctx > 0 ? div(ctx - 1) + 1 : 0;
         const bool bad = q < 0 || q > ctx || held < 0 || held > a.width || need > a.width;
-        // An impossible sequence counts for nothing else.
-        return Sums{bad ? 0 : q, bad || need <= held ? 0 : need - held, bad ? 1 : 0};
+        // An impossible sequence counts for nothing else. Sums stay below 2^40: of blocks because the
+        // tables hold them, of tokens because none is counted past what the step has room for.
+        const int64_t most = a.num_tokens + 1;
+        return Sums{bad ? 0 : q < most ? q : most, bad || need <= held ? 0 : need - held, bad ? 1 : 0};
     };
     // Sums over the threads below this one; all of them in `total`.
-    auto scan = [&](Sums own, Sums& total) {
-        Sums run = own;
-#pragma unroll
-        for (int by = 1; by < 64; by *= 2) {
-            const Sums up{shfl_up64(run.tokens, by), shfl_up64(run.blocks, by), shfl_up64(run.bad, by)};
-            if (lane >= by) run = run + up;
-        }
+    auto scan = [&](const Sums& own, Sums& total) {
+        Sums run{wave_scan64(own.tokens), wave_scan64(own.blocks), 0};
+        const int bad = wave_scan((int)own.bad);
         __syncthreads();                           // the last pass's readers are done
-        if (lane == 63) s_wave[wave] = run;
-        __syncthreads();
-        Sums before{run.tokens - own.tokens, run.blocks - own.blocks, run.bad - own.bad};
-        total = Sums{0, 0, 0};
-        for (int w = 0; w < W; ++w) {
-            const Sums s = s_wave[w];
-            if (w < wave) before = before + s;
-            total = total + s;
+        if (lane == 63) {
+            s_tokens[wave] = run.tokens;
+            s_blocks[wave] = run.blocks;
+            s_bad[wave] = bad;
         }
-        return before;
+        __syncthreads();
+        // Every wave sums up the waves: lane w has wave w.
+        const int64_t tw = lane < W ? s_tokens[lane] : 0, bw = lane < W ? s_blocks[lane] : 0;
+        const int64_t ts = wave_scan64(tw), bs = wave_scan64(bw);
+        total = Sums{readlane64(ts, W - 1), readlane64(bs, W - 1),
+                     __builtin_amdgcn_readlane(wave_scan(lane < W ? s_bad[lane] : 0), W - 1)};
+        return Sums{run.tokens - own.tokens + readlane64(ts - tw, wave), run.blocks - own.blocks + readlane64(bs - bw, wave), 0};
     };
 
     // The verdict, over all sequences.
@@ -97,7 +98,11 @@ __global__ __launch_bounds__(N) void step_layout_kernel(const LayoutArgs a) {
     const bool one_pass = a.num_seqs <= N;
     if (!one_pass) {
         Sums part = own;
-        for (int first = N; first < a.num_seqs; first += N) part = part + load(first);
+        for (int first = N; first < a.num_seqs; first += N) {
+            const Sums next = load(first);
+            const int64_t t = part.tokens + next.tokens, most = a.num_tokens + 1;
+            part = Sums{t < most ? t : most, part.blocks + next.blocks, part.bad + next.bad};
+        }
         scan(part, all);
     }
     if (all.tokens > a.num_tokens) ++all.bad;
@@ -157,7 +162,7 @@ __global__ __launch_bounds__(N) void step_layout_kernel(const LayoutArgs a) {
                 a.tables[(int64_t)(first + s) * a.table_stride + s_held[s] + (e - s_block0[s])] = a.free_blocks[e];
             }
         }
-        base = base + sum;
+        base = Sums{base.tokens + sum.tokens, base.blocks + sum.blocks, 0};
     }
     // Rows of no sequence.
     const int64_t real = ok ? all.tokens : 0;
