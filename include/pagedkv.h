@@ -479,12 +479,17 @@ int pkv_kv8_append(
  * query lengths (0: num_tokens) and max_context_len the contexts: they size the grid.
  * Block ids outside the pool are never dereferenced.
  *
- * host_context_lens / host_query_lens (HOST memory, int64 [num_seqs], or NULL) decide whether
- * and how contexts are cut into runs of separate workgroups, as in
+ * Float16 queries expect cached values of float16's range, up to 2^17 (rows appended in float16
+ * always are): chunks of more than 16 (token, query head) pairs hold them as float16, to
+ * 2^-24.
+ *
+ * host_context_lens / host_query_lens (HOST memory, int64 [num_seqs], or NULL) only decide
+ * whether and how contexts are cut into runs of separate workgroups, as in
  * pkv_paged_attention_prefill_split, and so does workspace: at least
  * pkv_kv8_attention_workspace_bytes() bytes for the same sizes and lengths, its first 256 KiB
  * zero when a call starts (every completed call leaves them zero; it can be the decode calls'
- * workspace). With a smaller one, or NULL, no context is cut. */
+ * workspace). Calls that may run at the same time, graph replays included, need one each. With
+ * a smaller one, or NULL, no context is cut. */
 int64_t pkv_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
                                           int64_t head_dim, int64_t num_tokens, int64_t max_query_len,
                                           int64_t max_context_len, const int64_t* host_context_lens,
@@ -513,7 +518,7 @@ int pkv_kv8_attention(
  * query_lens[i] of them new, held[i] blocks in row i of block_tables
  * (int64 [num_seqs, table_width], row stride table_stride). The blocks that it lacks
  * (ceil(context / block_size) - held) come from the front of free_blocks [num_free], in
- * sequence order, and are written behind its held ones, in place.
+ * sequence order, and are written behind its held ones, in place (rows must not overlap).
  *
  * Out, int64: held_out [num_seqs] blocks held now (not `held` itself); slots and positions
  * [num_tokens] of the packed new tokens (the context's last query_lens[i] positions), -1 and 0

@@ -157,6 +157,8 @@ extern "C" int pkv_kv8_append(void* k_codes, void* v_codes, int64_t code_stride_
         return fail(PKV_EINVAL, "kv8_append: bad sizes");
     if (num_tokens > 0x7fffffff || num_kv_heads > 0x7fffffff || head_dim > 512 || block_size > 0x7fffffff)
         return fail(PKV_EUNSUPPORTED, "kv8_append: head_dim %lld > 512, or sizes beyond int32", (long long)head_dim);
+    if (num_blocks > 0x7fffffffffffffff / block_size || num_tokens > ((int64_t)1 << 48) / num_kv_heads)
+        return fail(PKV_EUNSUPPORTED, "kv8_append: slots or rows beyond what the kernel counts");
     if (num_tokens == 0) return PKV_OK;
     if (!k_codes || !v_codes || !k_scales || !v_scales || !k_new || !v_new || !slots)
         return fail(PKV_EINVAL, "kv8_append: null pointer");

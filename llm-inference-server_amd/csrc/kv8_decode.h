@@ -293,7 +293,7 @@ __device__ __forceinline__ void decode_segment(const Kv8Params& p, Lds& lds, int
     const int ctx = __builtin_amdgcn_readfirstlane(decode_ctx(p, seq));
     const int64_t q_first = p.qsl ? p.qsl[seq] : seq;
     const int q_len = __builtin_amdgcn_readfirstlane(p.qsl ? (int)(p.qsl[seq + 1] - q_first) : 1);
-    const int rows = q_len * G < kDecodeRows ? q_len * G : kDecodeRows;
+    const int rows = q_len * G < p.decode_rows ? q_len * G : p.decode_rows;
     const int pos0 = ctx - q_len;               // of the first token
     const int row = n < rows ? n : rows - 1;
     const int limit = pos0 + row / G;           // last key that the row sees

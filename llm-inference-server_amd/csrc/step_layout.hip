@@ -187,6 +187,9 @@ extern "C" int pkv_step_layout(int64_t* block_tables, int64_t table_stride, int6
         return fail(PKV_EINVAL, "step_layout: bad sizes");
     if (num_seqs > 0x7fffffff - 1024 || num_tokens > 0x7fffffff || block_size > 0x7fffffff || table_width > 0x7fffffff)
         return fail(PKV_EUNSUPPORTED, "step_layout: sizes beyond int32");
+    if (num_seqs > 1 && table_stride < table_width)
+        return fail(PKV_EINVAL, "step_layout: rows of %lld blocks overlap at a stride of %lld", (long long)table_width,
+                    (long long)table_stride);
     if (!query_start_loc || !counts ||
         (num_seqs > 0 && (!held || !context_lens || !query_lens || !held_out || (!block_tables && table_width > 0))) ||
         (num_tokens > 0 && (!slots || !positions)) || (num_free > 0 && !free_blocks))

@@ -173,7 +173,8 @@ def paged_attention_kv8(query: torch.Tensor, k_cache: Kv8, v_cache: Kv8, block_t
     query's dtype.
 
     Softmax and sums are in fp32, the output is rounded once. A key that a query does not see
-    does not reach it, whatever it holds. Lengths with host copies attached (attach_host) are
+    does not reach it, whatever it holds. fp16 queries expect cached values of fp16's range (up to
+    2^17, as rows that were appended in fp16 always are). Lengths with host copies attached (attach_host) are
     checked without a device round trip."""
     backend = CONFIG.attention
     if backend == "hip":
@@ -339,6 +340,9 @@ class Kv8Pool(PagedKVPool):
         if slots.device.type != "cpu":
             self.check_slots(slots, host_slots)
         kv8_append(*self._layers[layer], k, v, slots)
+
+    def describe(self) -> str:
+        return super().describe()[:-1] + " as e4m3)"
 
     def release(self) -> None:
         super().release()

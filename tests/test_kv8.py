@@ -168,4 +168,9 @@ def test_library_refuses_bad_sizes():
     assert attend(tok=0, seqs=0) == native.PKV_OK
     assert attend() == attend(heads=3) == attend(tok=2) == attend(dt=9) == attend(seqs=-1) == native.PKV_EINVAL
     assert attend(d=513) == attend(width=1 << 40) == native.PKV_EUNSUPPORTED
+    assert append(nb=1 << 60) == native.PKV_EUNSUPPORTED
+    layout = lambda seqs=2, stride=4, width=4, bs=16: handle.pkv_step_layout(  # noqa: E731
+        None, stride, width, None, None, None, seqs, None, 0, bs, 0, None, None, None, None, None, None)
+    assert layout() == layout(stride=3) == layout(bs=0) == layout(seqs=-1) == native.PKV_EINVAL
+    assert layout(width=1 << 31, stride=1 << 31) == native.PKV_EUNSUPPORTED
     assert append(t=0) == native.PKV_OK and handle.pkv_last_error() == b""

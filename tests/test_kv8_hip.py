@@ -433,3 +433,33 @@ def test_graphs_of_one_stream_replayed_side_by_side():
         torch.cuda.synchronize()
         for (_, outs), w in zip(graphs, want):
             assert all(torch.equal(o, w) for o in outs)
+
+
+@pytest.mark.parametrize("d,told", [(64, (1, 0)), (128, (0, 0)), (64, (900, 1)), (128, (100000, 1))])
+def test_host_lengths_only_decide_the_cut(d, told):
+    """The library's call with host lengths that are not the device's: shorter and longer
+    contexts, sequences without queries that have some."""
+    from inference_server import native
+
+    s = batch([(3000, 1), (70, 2), (0, 1), (2000, 2)] * 5, heads=4, kv=2, d=d, bs=16, dtype=BF16, device="cuda")
+    (kc, ks), (vc, vs) = s.k, s.v
+    out, n = torch.full_like(s.q, 7.0), len(s.ctx)
+    tables, ctx, new = s.args
+    start = torch.cat([new.new_zeros(1), new.cumsum(0)])
+    for last in (0, 1):                         # all of them told wrongly; the last one rightly
+        hctx, hnew = torch.full((n,), told[0]), torch.full((n,), told[1])
+        if last:
+            hctx[-1], hnew[-1] = int(s.ctx[-1]), int(s.new[-1])
+        sizes = (n, 4, 2, d, s.q.shape[0], 2, 100000, hctx.data_ptr(), hnew.data_ptr())
+        lib = native.lib()
+        ws = torch.zeros(max(1, lib.pkv_kv8_attention_workspace_bytes(*sizes)), dtype=torch.uint8, device="cuda")
+        rc = lib.pkv_kv8_attention(
+            out.data_ptr(), 4 * d, d, s.q.data_ptr(), 4 * d, d, kc.data_ptr(), vc.data_ptr(), *kc.stride()[:3],
+            ks.data_ptr(), vs.data_ptr(), *ks.stride(), kc.shape[0], 16, 2, d, tables.data_ptr(), tables.stride(0),
+            tables.shape[1], ctx.data_ptr(), start.data_ptr(), n, 4, s.q.shape[0], 2, 100000, hctx.data_ptr(),
+            hnew.data_ptr(), s.scale, native.DTYPE_CODES[BF16], ws.data_ptr(), ws.numel(),
+            torch.cuda.current_stream().cuda_stream)
+        native.check(rc, "pkv_kv8_attention")
+        check(s, out)
+        assert not ws[:1 << 18].any()
+        out.fill_(7.0)
