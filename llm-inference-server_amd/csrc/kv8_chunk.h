@@ -8,8 +8,8 @@
 // for one swap, and P^T feeds the second product from the accumulator; contexts of few rows cut
 // into runs (prefill_split_plan) and merged. What differs is the staging:
 //
-//  * 64 keys of K and V a tile are loaded as codes (16 bytes, 16 dims, a piece; a thread has
-//    head_dim / 64 pieces of each), converted to the cached values - code * 2^(b - 127) in one
+//  * 64 keys of K and V a tile are loaded as codes (16 bytes, 16 dims, a piece; a thread has one or
+//    two pieces of each), converted to the cached values - code * 2^(b - 127) in one
 //    v_cvt_scalef32_pk a pair, exact - and written to LDS as 16-bit rows. Converting once for the
 //    workgroup instead of in each of its four waves costs a quarter of the VALU time, of which
 //    the softmax leaves little; a tile's LDS traffic is the 16-bit kernel's.
@@ -56,11 +56,16 @@ struct Stage<_Float16> {
     }
 };
 
-// UNI: head_dim 64 or 128 and block sizes from 16 up: a wave's pieces of one load are 8 or 16
-// neighbouring rows of one block, so that addresses are uniform and loads cost no vector
-// arithmetic.
+// Waves a SIMD that registers are held to. Three up to head_dim 80 (which then keeps 11 registers in
+// scratch: 12 sequences of 1-200 new tokens behind 0-1,500 44.4 -> 42.4 us, 4 of 256-512 behind
+// 0-3,000 101.7 -> 96.5); at 96 three gained nothing (94.2 and 94.0).
+template <typename T, int D>
+constexpr int kChunkWaves = sizeof(T) == 4 ? 1 : D <= 80 ? 3 : 2;
+
+// UNI: block sizes from 16 up: a wave's pieces of one load are 8 or 16 neighbouring rows of one
+// block, so that addresses are uniform and loads cost no vector arithmetic.
 template <typename T, int D, bool UNI>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 1 : 2))) void kv8_chunk_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves<T, D>))) void kv8_chunk_kernel(
     const Kv8Params p) {
     typedef typename Stage<T>::E E;
     constexpr int DSTEPS = D / 16;            // S^T contraction steps
@@ -68,8 +73,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     constexpr int ROWB = D * 2;               // bytes of a staged row
     constexpr int CPR = ROWB / 16;            // its 16-byte chunks
     constexpr int PPR = D / 16;               // its pieces of 16 codes
-    constexpr int PIECES = (kKT * PPR + 255) / 256;   // per thread and tile, of K and of V
-    constexpr bool kWhole = kKT * PPR % 256 == 0;
+    constexpr int PIECES = (PPR + 3) / 4;     // per thread and tile, of K and of V
+    constexpr bool kWhole = PPR % 4 == 0;     // all threads have as many
+    constexpr bool LINES = D == 128 && UNI;   // a thread's pieces are of PIECES rows, else of one
+    constexpr int NR = LINES ? PIECES : 1;
     constexpr int NP = sizeof(T) == 4 ? 3 : 1;
 
     __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kKT * D];
@@ -104,7 +111,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
 
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int tid = (int)threadIdx.x;
     const int h = lane >> 5, col = lane & 31;
     const int wrow = wave * kQT + col;
     const bool my_live = wrow < rows;         // rows past the last one repeat it, not stored
@@ -127,73 +133,67 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
     const uint8_t* ksb = p.ks + kvh * p.ssh;
     const uint8_t* vsb = p.vs + kvh * p.ssh;
     const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
-    // UNI: the 8 lanes of one LDS write cycle have 4 pieces of each of two rows whose swizzles differ
-    // in parity (4 rows apart at head_dim 128, 8 at 64), so that they hit all 32 banks; a whole
-    // row's pieces, even chunks only, hit half of them twice.
-    const int lane_row = !UNI ? 0 : D == 128 ? (lane >> 4) + 4 * (lane >> 2 & 1) : (lane >> 3) + 8 * (lane >> 2 & 1);
-    const int lane_c = D == 128 ? (lane & 3) + 4 * (lane >> 3 & 1) : lane & 3;
-    int piece_row[PIECES], piece_at[PIECES];
-    uint32_t lds0[PIECES], lds1[PIECES];
+    // A wave's load is 16 rows of 64 bytes, or at head_dim 128 (LINES) 8 whole ones. The 8 lanes of
+    // one LDS write cycle have 4 pieces of each of two rows whose swizzles differ in parity (4 or 8
+    // rows apart, as the width has it), so that they hit all 32 banks; a whole row's pieces, even
+    // chunks only, hit half of them twice.
+    constexpr bool FOUR = D % 32 == 0 && D != 64;
+    const int pair = lane >> 2 & 1;
+    const int lane_row = LINES ? (lane >> 4) + 4 * pair
+                               : FOUR ? (lane >> 3 & 3) + 4 * pair + 8 * (lane >> 5) : (lane >> 3) + 8 * pair;
+    const int lane_c = LINES ? (lane & 3) + 4 * (lane >> 3 & 1) : lane & 3;
+    auto wave_row = [&](int j) { return LINES ? 32 * j + 8 * wave : 16 * wave; };   // of the wave's first piece
+    auto row_of = [&](int j) { return wave_row(j) + lane_row; };
+    auto live = [&](int j) { return kWhole || lane_c + 4 * j < PPR; };
+    uint32_t lds0[PIECES], lds1[PIECES], at_row[PIECES];        // at_row: dims, inside the row for all
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
-        const int i = 256 * j + tid;
-        const int r = UNI ? (256 * j + 64 * wave) / PPR + lane_row : i / PPR < kKT ? i / PPR : kKT - 1;
-        const int c = UNI ? lane_c : i % PPR;
-        piece_row[j] = r;
-        piece_at[j] = 16 * c;
+        const int r = row_of(j), c = LINES ? lane_c : live(j) ? lane_c + 4 * j : 0;
+        at_row[j] = (uint32_t)(16 * c);
         lds0[j] = (uint32_t)(r * ROWB + (((2 * c) ^ lds_swizzle<D>(r)) << 4));
         lds1[j] = (uint32_t)(r * ROWB + (((2 * c + 1) ^ lds_swizzle<D>(r)) << 4));
     }
     const int in_block = p.block_size - 1, last = kmax - 1;     // last: the workgroup's last key
-    // UNI: row of the wave's first piece of load j; a lane's offset from there.
-    auto wave_row = [&](int j) { return (256 * j + 64 * wave) / PPR; };
-    const uint32_t lane_off = (uint32_t)(lane_row * (int)p.ss + lane_c * 16);
-    const uint32_t lane_sc = (uint32_t)(lane_row * (int)p.sss);
-    constexpr int NI = UNI ? 1 : PIECES;
-    int64_t id[NI];                           // UNI: lane j holds that of load j
-    uint32_t ks_raw[PIECES], vs_raw[PIECES];
+    // UNI: a lane's offset from the wave's first row.
+    const uint32_t lane_off = (uint32_t)(lane_row * (int)p.ss), lane_sc = (uint32_t)(lane_row * (int)p.sss);
+    int64_t id;                               // LINES: lane j holds that of load j
+    uint32_t ks_raw[NR], vs_raw[NR];
     Vec16 k_raw[PIECES], v_raw[PIECES];
     auto load_ids = [&](int kt) {
-        if constexpr (UNI) {
-            const int key = kt * kKT + wave_row(lane % PIECES);
-            id[0] = table[(key < last ? key : last) >> p.block_shift];
-        } else {
-#pragma unroll
-            for (int j = 0; j < PIECES; ++j) {
-                const int key = kt * kKT + piece_row[j];
-                id[j] = table[(key < last ? key : last) >> p.block_shift];
-            }
-        }
+        const int key = kt * kKT + (LINES ? wave_row(lane % PIECES) : UNI ? wave_row(0) : row_of(0));
+        id = table[(key < last ? key : last) >> p.block_shift];
     };
     auto load_tile = [&](int kt) {
-        uint32_t blk[NI];                     // none is followed out of the cache
+        const uint32_t blk = (uint64_t)id < (uint64_t)p.num_blocks ? (uint32_t)id : 0u;   // none is followed out of the cache
+        if constexpr (UNI) {
+            auto rsrc = [](const uint8_t* base) {
+                return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, -1, 0x00027000);
+            };
 #pragma unroll
-        for (int j = 0; j < NI; ++j) blk[j] = (uint64_t)id[j] < (uint64_t)p.num_blocks ? (uint32_t)id[j] : 0u;
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-            if constexpr (UNI) {
-                const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)blk[0], j);
+            for (int j = 0; j < PIECES; ++j) {
+                const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)blk, LINES ? j : 0);
                 const int at = (kt * kKT + wave_row(j)) & in_block;
                 const uint64_t off = (uint64_t)b * (uint32_t)p.sb + (uint32_t)(at * (int)p.ss);
-                const uint64_t so = (uint64_t)b * (uint32_t)p.ssb + (uint32_t)(at * (int)p.sss);
-                auto rsrc = [](const uint8_t* base) {
-                    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, -1, 0x00027000);
-                };
-                const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(rsrc(kc + off), (int)lane_off, 0, 0);
-                const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rsrc(vc + off), (int)lane_off, 0, 0);
+                const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(rsrc(kc + off), (int)(lane_off + at_row[j]), 0, 0);
+                const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rsrc(vc + off), (int)(lane_off + at_row[j]), 0, 0);
                 k_raw[j] = Vec16{{k.x, k.y, k.z, k.w}};
                 v_raw[j] = Vec16{{v.x, v.y, v.z, v.w}};
-                ks_raw[j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(ksb + so), (int)lane_sc, 0, 0);
-                vs_raw[j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(vsb + so), (int)lane_sc, 0, 0);
-            } else {
-                const int key = kt * kKT + piece_row[j], at = (key < last ? key : last) & in_block;
-                const int64_t off = (int64_t)blk[j] * p.sb + at * p.ss + piece_at[j];
-                const int64_t so = (int64_t)blk[j] * p.ssb + at * p.sss;
-                k_raw[j] = load16(kc + off);
-                v_raw[j] = load16(vc + off);
-                ks_raw[j] = ksb[so];
-                vs_raw[j] = vsb[so];
+                if (j < NR) {
+                    const uint64_t so = (uint64_t)b * (uint32_t)p.ssb + (uint32_t)(at * (int)p.sss);
+                    ks_raw[j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(ksb + so), (int)lane_sc, 0, 0);
+                    vs_raw[j] = __builtin_amdgcn_raw_buffer_load_b8(rsrc(vsb + so), (int)lane_sc, 0, 0);
+                }
             }
+        } else {
+            const int key = kt * kKT + row_of(0), at = (key < last ? key : last) & in_block;
+            const int64_t off = (int64_t)blk * p.sb + at * p.ss, so = (int64_t)blk * p.ssb + at * p.sss;
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                k_raw[j] = load16(kc + off + at_row[j]);
+                v_raw[j] = load16(vc + off + at_row[j]);
+            }
+            ks_raw[0] = ksb[so];
+            vs_raw[0] = vsb[so];
         }
     };
     // Rows past the last key are zeros (whatever was loaded there): masked in S, and V finite.
@@ -201,12 +201,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
         const bool ends = kt * kKT + kKT - 1 > last;
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            if (!kWhole && 256 * j + tid >= kKT * PPR) continue;
+            const int jr = LINES ? j : 0;
             auto scale = [&](uint32_t b) {    // 2^(b - 127), infinite for 255
                 const uint32_t e = b << 23;
                 return __builtin_bit_cast(float, e > 0x00400000u ? e : 0x00400000u) * Stage<T>::kFactor;
             };
-            const float ks = scale(ks_raw[j]), vs = scale(vs_raw[j]);
+            const float ks = scale(ks_raw[jr]), vs = scale(vs_raw[jr]);
             uint32_t a[8], b[8];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
@@ -215,8 +215,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
                 b[2 * w] = Stage<T>::template cvt<false>(v_raw[j].w[w], vs);
                 b[2 * w + 1] = Stage<T>::template cvt<true>(v_raw[j].w[w], vs);
             }
-            const bool bad = ks_raw[j] == (uint32_t)kScaleNan || vs_raw[j] == (uint32_t)kScaleNan;
-            const bool none = ends && kt * kKT + piece_row[j] > last;
+            const bool bad = ks_raw[jr] == (uint32_t)kScaleNan || vs_raw[jr] == (uint32_t)kScaleNan;
+            const bool none = ends && kt * kKT + row_of(j) > last;
             if (__builtin_amdgcn_ballot_w64(bad || none)) {
                 asm volatile("");             // a branch, not selects in every tile
                 const uint32_t fill = none ? 0u : Stage<T>::kNan2;
@@ -226,6 +226,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(sizeof(T) =
                     b[w] = bad || none ? 0u : b[w];
                 }
             }
+            if (!live(j)) continue;
             store16((char*)sk + lds0[j], Vec16{{a[0], a[1], a[2], a[3]}});
             store16((char*)sk + lds1[j], Vec16{{a[4], a[5], a[6], a[7]}});
             store16((char*)sv + lds0[j], Vec16{{b[0], b[1], b[2], b[3]}});
@@ -436,10 +437,8 @@ inline int64_t kv8_chunk_workgroups(const Kv8Params& p) {
 template <typename T, int D>
 int launch_kv8_chunk_d(const Kv8Params& p, hipStream_t stream) {
     const dim3 grid((unsigned)kv8_chunk_workgroups(p));
-    if ((D == 64 || D == 128) && p.block_size >= 16 && kv8_offsets_fit(p))
-        kv8_chunk_kernel<T, D, D == 64 || D == 128><<<grid, 256, 0, stream>>>(p);
-    else
-        kv8_chunk_kernel<T, D, false><<<grid, 256, 0, stream>>>(p);
+    if (p.block_size >= 16 && kv8_offsets_fit(p)) kv8_chunk_kernel<T, D, true><<<grid, 256, 0, stream>>>(p);
+    else kv8_chunk_kernel<T, D, false><<<grid, 256, 0, stream>>>(p);
     const int rc = check_launch("kv8 chunk attention");
     if (rc || p.splits == 1) return rc;
     const int64_t rows = p.num_tokens * p.num_heads;
