@@ -1,20 +1,47 @@
 // Attention over the 8-bit paged cache: the generic kernel and the extern "C" entry points.
 //
-// Generic kernel: any block size, head_dim <= 512, GQA group, stride and softmax scale. One
-// wave per (token, query head), lanes split head_dim, one key a step, online softmax in fp32.
-// It takes the shapes that the matrix kernels decline.
+// Generic kernel: any block size, head_dim <= 512, GQA group, stride and softmax scale; it takes
+// the shapes that the matrix kernels decline. A workgroup has one (token, query head). A lane holds
+// 16 dims of a key, LPK lanes a key, so that a wave has 64 / LPK keys side by side; each such group
+// of lanes runs an online softmax of its own, in fp32, over every so-manieth key, and the groups
+// meet at the end. Bound: vector instructions (a code is converted and multiplied by itself), and
+// in small batches the latency of a step's loads, block ids and then rows: they go out for several
+// keys together, the next ids with them, and small batches get 16 waves a workgroup instead of 4.
+// Measured at 16/4 heads of 256, us a call: 8 sequences of 4k keys 66 (67 MB: 1.0 TB/s; one wave a
+// head, a key a step, took 8,332), 64 of them 262 (2.0 TB/s), one of 60,000 789, 2 of 200 new tokens
+// behind 2,000 635; 64 sequences of 500, 8 heads of 40, 19.6.
 #include "kv8.h"
 
 namespace pkv {
 namespace {
 
-// Elements [lane * EPL, +EPL) would need aligned rows; lane, lane + 64, ... needs nothing.
-template <typename T, int EPL>
-__global__ __launch_bounds__(256) void kv8_generic_kernel(const Kv8Params p) {
-    const int lane = lane_id();
-    const int64_t tok = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// (Token, head) pairs that get 16 waves each: 8 sequences of 4k at 16 heads took 179 us with 16 and 482
+// with 4 before lanes held 16 dims, 64 of them the same with both; 1,024 tokens of prompts 422 and 194.
+constexpr int kGenericFew = 1024;
+
+template <int L>
+__device__ __forceinline__ float group_sum(float x) {
+    x = quad_sum(x);
+    if constexpr (L >= 8) x += dpp_f32<kDppRowHalfMirror>(x);
+    if constexpr (L >= 16) x += dpp_f32<kDppRowMirror>(x);
+    if constexpr (L >= 32) {
+        const SwapPair s = swap16(x);
+        x = s.a + s.b;
+    }
+    return x;
+}
+
+// ALIGN: of codes, 1, 4 or 16; head_dim is a multiple of it.
+template <typename T, int LPK, int ALIGN>
+__global__ __launch_bounds__(1024) void kv8_generic_kernel(const Kv8Params p) {
+    constexpr int U = ALIGN == 16 ? 4 : ALIGN == 4 ? 2 : 1;   // keys of a group in a step: what registers have room for
+    constexpr int DP = 16 * LPK;              // dims that the lanes have room for
+    __shared__ float s_m[16], s_l[16];
+    __shared__ __attribute__((aligned(16))) float s_o[16 * DP];
+    const int lane = lane_id(), sub = lane % LPK, d0 = 16 * sub;
+    const int groups = (int)blockDim.x / LPK, group = (int)threadIdx.x / LPK;
+    const int64_t tok = blockIdx.x;
     const int head = (int)blockIdx.y;
-    if (tok >= p.num_tokens) return;
     int seq = (int)tok;
     int64_t q_start = tok, q_len = 1;
     if (p.qsl) {
@@ -30,69 +57,171 @@ __global__ __launch_bounds__(256) void kv8_generic_kernel(const Kv8Params p) {
         q_start = p.qsl[seq];
         q_len = p.qsl[seq + 1] - q_start;
     }
-    const int64_t cap = p.table_width * p.block_size;
-    int64_t n_keys = p.ctx_lens[seq] - q_len + (tok - q_start) + 1;
-    n_keys = n_keys < cap ? n_keys : cap;
+    const int64_t cap = p.table_width * p.block_size;           // fits 31 bits
+    const int64_t sees = p.ctx_lens[seq] - q_len + (tok - q_start) + 1;
+    // (Without blocks all ids are bad: zeros, as without keys.)
+    const int n_keys = (int)(sees < 0 || p.num_blocks < 1 ? 0 : sees < cap ? sees : cap);
     const int kvh = head / p.group;
     const T* qrow = reinterpret_cast<const T*>(p.q) + tok * p.q_st + (int64_t)head * p.q_sh;
-    float q[EPL], acc[EPL];
+    float q[16], acc[16];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        const int d = lane + 64 * e;
-        q[e] = d < p.head_dim ? to_f32(qrow[d]) : 0.f;
+    for (int e = 0; e < 16; ++e) {
+        q[e] = d0 + e < p.head_dim ? to_f32(qrow[d0 + e]) : 0.f;
         acc[e] = 0.f;
     }
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.k) + kvh * p.sh;
     const uint8_t* vc = reinterpret_cast<const uint8_t*>(p.v) + kvh * p.sh;
+    const uint8_t* ksb = p.ks + kvh * p.ssh;
+    const uint8_t* vsb = p.vs + kvh * p.ssh;
     const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
-    float m = kNegInf, l = 0.f;
-    for (int64_t j = 0; j < n_keys; ++j) {
-        int64_t blk = table[j / p.block_size];
-        const bool ok = (uint64_t)blk < (uint64_t)p.num_blocks;   // a bad id reads as zeros
-        blk = ok ? blk : 0;
-        const int64_t at = j % p.block_size;
-        const int64_t row = blk * p.sb + at * p.ss, sc = blk * p.ssb + at * p.sss + kvh * p.ssh;
-        const float ks = ok ? scale_of(p.ks[sc]) : 0.f, vs = ok ? scale_of(p.vs[sc]) : 0.f;
-        float s = 0.f;
+    // The lane's codes of a row. No load stands in a branch, where it would be waited for by itself:
+    // dims past head_dim read the row's first ones (against queries of 0, into outputs that are not
+    // stored).
+    auto codes = [&](const uint8_t* row) {
+        auto from = [&](int d) { return row + (d < p.head_dim ? d : 0); };
+        if constexpr (ALIGN == 16) return load16(from(d0));
+        Vec16 x;
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int d = lane + 64 * e;
-            if (d < p.head_dim && ok) s += q[e] * __builtin_amdgcn_cvt_f32_fp8(kc[row + d], 0);
+        for (int w = 0; w < 4; ++w) {
+            if constexpr (ALIGN == 4) {
+                x.w[w] = *reinterpret_cast<const uint32_t*>(from(d0 + 4 * w));
+            } else {
+                x.w[w] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x.w[w] |= (uint32_t)*from(d0 + 4 * w + e) << (8 * e);
+            }
         }
-        s = wave_sum(s) * ks * p.scale_log2;
-        const float m_new = fmaxf(m, s);
-        const float m_off = m_new == kNegInf ? 0.f : m_new;
-        const float alpha = fast_exp2(m - m_off);   // 0 on the first key (m = -inf)
-        const float pj = fast_exp2(s - m_off), w = pj * vs;
-        l = l * alpha + pj;
+        return x;
+    };
+    // Key u of a group's step from `first`; past the last key, that one again, of weight 0.
+    auto key_of = [&](int64_t first, int u) {
+        const int64_t key = first + u * groups + group;
+        return (uint32_t)(key < n_keys ? key : n_keys - 1);
+    };
+    auto block_of = [&](uint32_t key) {
+        return p.block_shift >= 0 ? key >> p.block_shift : key / (uint32_t)p.block_size;
+    };
+    float m = kNegInf, l = 0.f;
+    int64_t ids[U];
+    if (n_keys > 0)
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-            const int d = lane + 64 * e;
-            const float vd = d < p.head_dim && ok ? __builtin_amdgcn_cvt_f32_fp8(vc[row + d], 0) : 0.f;
-            acc[e] = acc[e] * alpha + w * vd;
+        for (int u = 0; u < U; ++u) ids[u] = table[block_of(key_of(0, u))];
+    for (int64_t first = 0; first < n_keys; first += U * groups) {
+        Vec16 k[U], v[U];
+        uint32_t ks[U], vs[U], good = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t key = key_of(first, u);
+            const bool ok = (uint64_t)ids[u] < (uint64_t)p.num_blocks;  // a bad id reads as zeros
+            good |= ok ? 1u << u : 0u;
+            const int64_t id = ok ? ids[u] : 0;
+            const int64_t at = key - block_of(key) * (uint32_t)p.block_size;
+            const int64_t row = id * p.sb + at * p.ss, sc = id * p.ssb + at * p.sss;
+            ks[u] = ksb[sc];
+            vs[u] = vsb[sc];
+            k[u] = codes(kc + row);
+            v[u] = codes(vc + row);
+        }
+        if (first + U * groups < n_keys)
+#pragma unroll
+            for (int u = 0; u < U; ++u) ids[u] = table[block_of(key_of(first + U * groups, u))];
+        float s[U], m_new = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)k[u].w[w], false);
+                const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)k[u].w[w], true);
+                x += q[4 * w] * lo[0];
+                x += q[4 * w + 1] * lo[1];
+                x += q[4 * w + 2] * hi[0];
+                x += q[4 * w + 3] * hi[1];
+            }
+            x = group_sum<LPK>(x) * scale_of(ks[u]) * p.scale_log2;
+            x = good >> u & 1 ? x : 0.f;
+            s[u] = first + u * groups + group < n_keys ? x : kNegInf;
+            m_new = fmaxf(m_new, s[u]);
+        }
+        const float m_off = m_new == kNegInf ? 0.f : m_new;
+        const float alpha = fast_exp2(m - m_off);               // 0 on the first keys (m = -inf)
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] *= alpha;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool live = first + u * groups + group < n_keys, ok = good >> u & 1;
+            const float pj = fast_exp2(s[u] - m_off), x = live && ok ? pj * scale_of(vs[u]) : 0.f;
+            l += pj;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int c = (int)(ok ? v[u].w[w] : 0u);
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+                acc[4 * w] += x * lo[0];
+                acc[4 * w + 1] += x * lo[1];
+                acc[4 * w + 2] += x * hi[0];
+                acc[4 * w + 3] += x * hi[1];
+            }
         }
         m = m_new;
     }
-    T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)head * p.out_sh;
-    const float inv = n_keys > 0 ? 1.f / l : 0.f;   // a row without keys is zero
+    // The wave's groups, then the waves.
+    float M = m;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-        const int d = lane + 64 * e;
-        if (d < p.head_dim) orow[d] = from_f32<T>(acc[e] * inv);
+    for (int off = LPK; off < 64; off *= 2) M = fmaxf(M, __shfl_xor(M, off));
+    const float a = fast_exp2(m - (M == kNegInf ? 0.f : M));
+    l *= a;
+#pragma unroll
+    for (int off = LPK; off < 64; off *= 2) l += __shfl_xor(l, off);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        acc[e] *= a;
+#pragma unroll
+        for (int off = LPK; off < 64; off *= 2) acc[e] += __shfl_xor(acc[e], off);
     }
+    const int wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
+    if (lane < LPK)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s_o[wave * DP + d0 + e] = acc[e];
+    if (lane == 0) {
+        s_m[wave] = M;
+        s_l[wave] = l;
+    }
+    __syncthreads();
+    T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)head * p.out_sh;
+    for (int d = (int)threadIdx.x; d < p.head_dim; d += (int)blockDim.x) {
+        float top = kNegInf, L = 0.f, o = 0.f;
+        for (int w = 0; w < waves; ++w) top = fmaxf(top, s_m[w]);
+        if (top == kNegInf) top = 0.f;
+        for (int w = 0; w < waves; ++w) {
+            const float b = fast_exp2(s_m[w] - top);
+            L += b * s_l[w];
+            o += b * s_o[w * DP + d];
+        }
+        orow[d] = from_f32<T>(n_keys > 0 ? o / L : 0.f);        // a row without keys is zero
+    }
+}
+
+template <typename T, int LPK>
+int launch_generic_l(const Kv8Params& p, hipStream_t stream) {
+    if (p.num_tokens > 0x7fffffff) return fail(PKV_EUNSUPPORTED, "kv8_attention: grid too large");
+    const dim3 grid((unsigned)p.num_tokens, (unsigned)p.num_heads);
+    const int threads = p.num_tokens * p.num_heads <= kGenericFew ? 1024 : 256;
+    const uint64_t codes = (uint64_t)(uintptr_t)p.k | (uint64_t)(uintptr_t)p.v | (uint64_t)p.sb | (uint64_t)p.ss |
+                           (uint64_t)p.sh | (uint64_t)p.head_dim;
+    if (codes % 16 == 0) kv8_generic_kernel<T, LPK, 16><<<grid, threads, 0, stream>>>(p);
+    else if (codes % 4 == 0) kv8_generic_kernel<T, LPK, 4><<<grid, threads, 0, stream>>>(p);
+    else kv8_generic_kernel<T, LPK, 1><<<grid, threads, 0, stream>>>(p);
+    return check_launch("kv8 generic attention");
 }
 
 template <typename T>
 int launch_generic_t(const Kv8Params& p, hipStream_t stream) {
-    const int64_t gx = ceil_div(p.num_tokens, 4);
-    if (gx > 0x7fffffff) return fail(PKV_EUNSUPPORTED, "kv8_attention: grid too large");
-    const dim3 grid((unsigned)gx, (unsigned)p.num_heads);
-    if (p.head_dim <= 64) kv8_generic_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
-    else if (p.head_dim <= 128) kv8_generic_kernel<T, 2><<<grid, 256, 0, stream>>>(p);
-    else if (p.head_dim <= 256) kv8_generic_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
-    else if (p.head_dim <= 512) kv8_generic_kernel<T, 8><<<grid, 256, 0, stream>>>(p);
-    else return fail(PKV_EUNSUPPORTED, "kv8_attention: head_dim %d > 512", p.head_dim);
-    return check_launch("kv8 generic attention");
+    if (p.head_dim <= 64) return launch_generic_l<T, 4>(p, stream);
+    if (p.head_dim <= 128) return launch_generic_l<T, 8>(p, stream);
+    if (p.head_dim <= 256) return launch_generic_l<T, 16>(p, stream);
+    if (p.head_dim <= 512) return launch_generic_l<T, 32>(p, stream);
+    return fail(PKV_EUNSUPPORTED, "kv8_attention: head_dim %d > 512", p.head_dim);
 }
 
 }  // namespace

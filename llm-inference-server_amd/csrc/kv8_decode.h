@@ -4,26 +4,32 @@
 // 4 up, scale bytes of a block together (slot stride 1) and 4-byte aligned, codes in 4-byte
 // steps, queries and output in 8-byte ones.
 //
-// Bound: HBM for batches of tens of MB (head_dim + 1 bytes a cached row), latency below that.
+// Bound: HBM for batches of hundreds of MB (head_dim + 1 bytes a cached row: 64 sequences of
+// 1-16k tokens, 8 KV heads of 128, 1.10 GB in 179-190 us, 5.8-6.2 TB/s, of which the arithmetic
+// is 4 us); latency below that (32 sequences of 12 heads of 64, 23.5 MB, 13.9 us).
 //
-//  * Split: the batch's keys, in units of 32 (64 up to head_dim 64), sequence after sequence, are cut into `slots` even
-//    runs per KV head, whatever the lengths: a prefix sum over the sequences, which every
-//    workgroup takes by itself, tells it its own. A run is a workgroup's (its four waves take
-//    turns at the units) or, where sequences are short and many, a single wave's. A sequence
-//    that a run's end cuts leaves fp32 partials; the last workgroup to finish it merges them,
-//    in key order, so results do not depend on timing.
-//  * No LDS in the loop: S^T = K Q^T on 16x16x32 takes K rows as they lie in memory (a lane
-//    holds a quarter of a row; the order of a contraction is free as long as Q's is the
-//    same). Its result leaves a lane with 8 keys of one query row, which are the B operand of
-//    O^T += V^T P^T as they stand. V^T's operand is 8 keys of one dim a lane: the lane loads 4
-//    (or 8) neighbouring dims of those 8 keys, and byte permutes turn 4 x 4 blocks.
+//  * Split: a batch's keys are taken in units of 32 (64 up to head_dim 64), a wave a unit at a
+//    time, and cut into runs by one of three rules (attn_kv8.hip has the choice). Large batches:
+//    even runs, over the ends of sequences, one a workgroup. Others: runs inside a sequence, a
+//    workgroup each, or a wave each where there are more sequences than workgroups; a batch of
+//    which none is cut is not summed up at all. Every workgroup finds its run by running sums of
+//    its own over the lengths, so a graph's replays may change them.
+//  * A sequence in several runs leaves fp32 partials, which the last workgroup to finish it
+//    merges inside the launch, in key order, so results do not depend on timing.
+//  * Operands as they lie: S^T = K Q^T on 16x16x32 takes quarters of K rows (the order of a
+//    contraction is free as long as Q's is the same). Its result leaves a lane with 8 keys of one
+//    query row, which are the B operand of O^T += V^T P^T as they stand. V^T's operand is 8 keys
+//    of one dim a lane: the lane loads 4 (or 8) neighbouring dims of those 8 keys, and byte
+//    permutes turn 4 x 4 blocks. Only at head_dim 128 does K pass through LDS, so that loads take
+//    whole lines (below).
 //  * Codes are converted in pairs (v_cvt_scalef32_pk): exact. Key scales multiply the scores,
 //    value scales the weights, both in fp32.
 //  * Weights enter the second product as bf16 pieces (two for 16-bit types: 16 bits of them,
 //    three for fp32), fp32 queries the first one as three: the product is then as exact as its
 //    fp32 accumulation, and the matrix unit has time to spare (12-40 MFMAs a unit of 8 KiB).
-//  * Loads of the next unit are in flight while one is computed (16 KiB a wave at head_dim 128),
-//    nontemporal, block ids one unit further ahead.
+//  * A unit stays in registers; K of the next one is loaded when the first product has used
+//    this one's, V after the second, the other waves of the SIMD (2-4) being the cover. Two
+//    units in registers and half the waves were slower (64 sequences as above 203 us, 190 so).
 //  * Heads of one run share an XCD (workgroup L runs on XCD L % 8): a line of scale bytes holds
 //    several heads.
 #pragma once
@@ -843,7 +849,7 @@ int launch_kv8_decode_d(const Kv8Params& p, hipStream_t stream) {
     if (wgs > 0x7fffffff) return fail(PKV_EUNSUPPORTED, "kv8 decode attention: grid too large");
     const dim3 grid((unsigned)wgs);
     if (p.decode_mode == kKv8Even) kv8_decode_even_kernel<T, D, BIG><<<grid, 256, 0, stream>>>(p);
-    else if (p.decode_mode == kKv8Runs) 
+    else if (p.decode_mode == kKv8Runs)
         kv8_decode_runs_kernel<T, D, BIG, kRunWaves<T, D, BIG>><<<grid, 64 * kRunWaves<T, D, BIG>, 0, stream>>>(p);
     else kv8_decode_runs_kernel<T, D, BIG, 1><<<grid, 256, 0, stream>>>(p);
     return check_launch("kv8 decode attention");

@@ -6,7 +6,9 @@
 // table[position / bs] * bs + position % bs. All of it is two running sums over the sequences
 // (new blocks, new tokens) and gathers.
 //
-// Bound: latency (a decode step moves some hundred bytes). So there is one launch and no
+// Bound: latency (a decode step moves some hundred bytes): 8 sequences 3.4 us, 256 4.6, 1,024
+// 6.0, the last two loads behind one another (lengths, then table entries or free blocks) and an
+// empty launch 2. So there is one launch and no
 // workgroup waits for another: each sums over all sequences by itself (24 bytes a sequence,
 // from L2 but for the first reader) and writes its own share of the tokens and of the new
 // table entries. A token in a new block reads the free list, not the table entry that some

@@ -463,3 +463,24 @@ def test_host_lengths_only_decide_the_cut(d, told):
         check(s, out)
         assert not ws[:1 << 18].any()
         out.fill_(7.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens", [[(2999, 1), (0, 1), (1200, 1)], [(900, 300), (0, 3), (700, 30)]],
+                         ids=["few", "many"])
+@pytest.mark.parametrize("d,bs", [(40, 16), (101, 16), (256, 16), (512, 16), (64, 24)])
+def test_long_contexts_of_other_shapes(dtype, lens, d, bs):
+    """Shapes of no matrix kernel, few and many rows, a NaN row among the last keys."""
+    s = batch(lens, heads=8, kv=2, d=d, bs=bs, dtype=dtype, device="cuda")
+    for raw, cache, pos in ((s.k_raw, s.k, s.ctx[0] - 1), (s.v_raw, s.v, s.ctx[2] - 1)):
+        row = 0 if cache is s.k else 2
+        blk = s.tables[row, pos // bs]
+        raw[0][blk, pos % bs, 1] = 0
+        raw[1][blk, pos % bs, 1] = 255
+        put(cache, *raw)
+    check(s, call(s))
+
+
+def test_more_sequences_than_the_decode_kernel_takes():
+    s = batch([(n % 19, 1) for n in range(2500)], heads=4, kv=2, d=64, bs=16, dtype=BF16, device="cuda")
+    check(s, call(s))
