@@ -2,11 +2,12 @@
 //
 // Bound: HBM for prompts (a bf16 row of 128 is 256 bytes read, 129 written: 8,192 tokens of 8 KV
 // heads, 50.5 MB, in 12.0 us, 4.2 TB/s, where a large copy reaches 4.9), latency for decode steps
-// (32 tokens 2.8-3.8 us). One row a lane group: two or four, their loads in flight together, were
-// slower (12.8 and 13.2 us). A row is held by the fewest lanes that load it in 16-byte pieces (8 elements
-// a lane; fp32 two such pieces), so its largest magnitude is a reduction over 4 to 16
-// neighbouring lanes (DPP) for head_dims up to 128, with no LDS. The magnitude is taken on the
-// bit patterns as integers: above 0x7f7fffff is a value that is not finite.
+// (32 tokens 2.8-3.8 us). A row is held by the fewest lanes that load it in 16-byte pieces (8
+// elements a lane; fp32 two such pieces), so its largest magnitude is a reduction over 4 to 16
+// neighbouring lanes (DPP) for head_dims up to 128, with no LDS. Two or four rows a lane, their
+// loads in flight together, were slower (12.8 and 13.2 us), nontemporal loads too (14.1). The
+// magnitude is taken on the bit patterns as integers: above 0x7f7fffff is a value that is not
+// finite.
 #include <type_traits>
 
 #include "kv8.h"
