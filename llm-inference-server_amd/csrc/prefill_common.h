@@ -80,8 +80,8 @@ __device__ __forceinline__ int lds_swizzle(int r) {
 
 // Softmax maxima are only raised when a tile's max exceeds the running one by more
 // than 2^8: until then probabilities are exp2(s - m) <= 256 (exact enough in fp32 and
-// in the pool dtype), and the O accumulators need no rescale — FlashAttention-3's lazy
-// rescaling, which removes the per-tile multiply of every accumulator.
+// in the pool dtype), and the O accumulators need no rescale, which removes the per-tile
+// multiply of every accumulator.
 constexpr float kRescaleThreshold = 8.f;
 
 // Tiles per split of a workgroup with n_tiles key tiles: its splits are of even lengths.
