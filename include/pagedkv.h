@@ -473,15 +473,12 @@ int pkv_kv8_append(
 
 /* Attention over the 8-bit cache: pkv_paged_attention_prefill's contract (chunks of new
  * tokens, prompts, mixes with decode), or pkv_paged_attention_decode's where query_start_loc
- * is NULL (one token per sequence). Scores, softmax and sums are in float32, the output is
- * rounded once; a key that a row does not see never reaches it, whatever it holds (NaN rows
+ * is NULL (one token per sequence). Scores, softmax and sums are in float32, of a weight 16 bits
+ * at least (24 for float32 queries) meet the values, the output is rounded once; a key that a row
+ * does not see never reaches it, whatever it holds (NaN rows
  * included), and a row that sees no key (a context of 0) is zero. max_query_len bounds the
  * query lengths (0: num_tokens) and max_context_len the contexts: they size the grid.
  * Block ids outside the pool are never dereferenced.
- *
- * Float16 queries expect cached values of float16's range, up to 2^17 (rows appended in float16
- * always are): chunks of more than 16 (token, query head) pairs hold them as float16, to
- * 2^-24.
  *
  * host_context_lens / host_query_lens (HOST memory, int64 [num_seqs], or NULL) only decide
  * whether and how contexts are cut into runs of separate workgroups, as in

@@ -10,7 +10,7 @@
 //
 //  * 64 keys of K and V a tile are loaded as codes (16 bytes, 16 dims, a piece; a thread has one or
 //    two pieces of each), converted to the cached values - code * 2^(b - 127) in one
-//    v_cvt_scalef32_pk a pair, exact - and written to LDS as 16-bit rows. Converting once for the
+//    v_cvt_scalef32_pk a pair - and written to LDS as 16-bit rows. Converting once for the
 //    workgroup instead of in each of its four waves costs a quarter of the VALU time, of which
 //    the softmax leaves little; a tile's LDS traffic is the 16-bit kernel's.
 //  * A tile is loaded during the one before the one before it, and converted while the matrix unit
@@ -19,9 +19,11 @@
 //    V's, whose row is staged as zeros: the causal mask then hides it from rows that do not see
 //    it, which a weight of 0 times NaN would not.
 //
-// Values are bf16 for bf16 and fp32 queries (exact), fp16 for fp16 queries, halved: a row's
-// largest value may round up past fp16's. fp32 queries and weights enter as three bf16 pieces
-// each (24 bits); 16-bit types' weights are rounded to the type, as the 16-bit kernel does.
+// Values are bf16; for fp16 queries K is its codes as fp16, its scales multiply the scores. Weights
+// enter the second product as bf16 pieces, two for 16-bit types (16 bits of them: one of the type's
+// own width left up to 2^-9 of a weight in the output), three for fp32 (24 bits), fp32 queries the
+// first one as three. The second piece costs a third of the time of long chunks (16 chunks of
+// 512 behind 0-4,096, 32/8 heads of 128, bf16: 342 -> 442-460 us): half as many MFMAs again.
 #pragma once
 
 #include "kv8.h"
@@ -30,44 +32,49 @@
 namespace pkv {
 namespace {
 
-// The 16-bit type that values take in LDS, and what they are multiplied by; and the power of two
-// that weights are multiplied by. fp16 weights below 2^-14 would lose digits: with the running
-// maximum at 2^7, and raised past 2^8 only, they reach 2^15 and keep all of them down to 2^-21.
+// Two codes (the lower or upper half of w) times a power of two, as bf16.
+template <bool HI>
+__device__ __forceinline__ uint32_t scaled_bf16(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+
+// What keys are in LDS: their values as bf16, or for fp16 queries their codes as fp16, which has not
+// the range of the values; their scales are then multiplied to the scores (kAfter).
 template <typename T>
-struct Stage {
+struct Keys {
     typedef bf16_t E;
-    static constexpr float kFactor = 1.f;
-    static constexpr float kLift = 0.f;
+    static constexpr bool kAfter = false;
     static constexpr uint32_t kNan2 = 0x7fc07fc0u;
     template <bool HI>
     __device__ __forceinline__ static uint32_t cvt(uint32_t w, float scale) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+        return scaled_bf16<HI>(w, scale);
     }
 };
 template <>
-struct Stage<_Float16> {
+struct Keys<_Float16> {
     typedef _Float16 E;
-    static constexpr float kFactor = 0.5f;
-    static constexpr float kLift = 7.f;
+    static constexpr bool kAfter = true;
     static constexpr uint32_t kNan2 = 0x7e007e00u;
     template <bool HI>
-    __device__ __forceinline__ static uint32_t cvt(uint32_t w, float scale) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+    __device__ __forceinline__ static uint32_t cvt(uint32_t w, float) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
     }
 };
 
-// Waves a SIMD that registers are held to. Three up to head_dim 80 (which then keeps 11 registers in
-// scratch: 12 sequences of 1-200 new tokens behind 0-1,500 44.4 -> 42.4 us, 4 of 256-512 behind
-// 0-3,000 101.7 -> 96.5); at 96 three gained nothing (94.2 and 94.0).
-template <typename T, int D>
-constexpr int kChunkWaves = sizeof(T) == 4 ? 1 : D <= 80 ? 3 : 2;
+// Waves a SIMD that registers are held to. Three for 16-bit types gain nothing at head_dim 64 (92.5 us
+// and 92.3) and keep registers in scratch from 80 on (32 fp16 heads of 80: 12 sequences of 1-200 new
+// tokens behind 0-1,500 52.2 us, two 49.6; 4 of 256-512 behind 0-3,000 124.8 and 120.4, heads of 96
+// 165.5 and 131.2).
+template <typename T>
+constexpr int kChunkWaves = sizeof(T) == 4 ? 1 : 2;
 
 // UNI: block sizes from 16 up: a wave's pieces of one load are 8 or 16 neighbouring rows of one
 // block, so that addresses are uniform and loads cost no vector arithmetic.
 template <typename T, int D, bool UNI>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves<T, D>))) void kv8_chunk_kernel(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves<T>))) void kv8_chunk_kernel(
     const Kv8Params p) {
-    typedef typename Stage<T>::E E;
+    typedef typename Keys<T>::E E;
+    constexpr bool kAfter = Keys<T>::kAfter;
     constexpr int DSTEPS = D / 16;            // S^T contraction steps
     constexpr int DTILES = (D + 31) / 32;     // O^T tiles of 32 dims (the last may be half a tile)
     constexpr int ROWB = D * 2;               // bytes of a staged row
@@ -77,12 +84,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
     constexpr bool kWhole = PPR % 4 == 0;     // all threads have as many
     constexpr bool LINES = D == 128 && UNI;   // a thread's pieces are of PIECES rows, else of one
     constexpr int NR = LINES ? PIECES : 1;
-    constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+    constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;   // pieces of queries and weights
 
     __shared__ __attribute__((aligned(1024))) uint16_t s_k0[kKT * D];
     __shared__ __attribute__((aligned(1024))) uint16_t s_v0[kKT * D];
     __shared__ __attribute__((aligned(1024))) uint16_t s_k1[kKT * D];
     __shared__ __attribute__((aligned(1024))) uint16_t s_v1[kKT * D];
+    __shared__ __attribute__((aligned(16))) float s_ks[2][kAfter ? kKT : 4];    // key scales of either tile
 
     PrefillItem it;
     if (!prefill_item<kRows, kKT>(p, p.block_size, it)) return;
@@ -125,7 +133,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
 #pragma unroll
     for (int t = 0; t < DTILES; ++t) o[t] = f32x16{};
     float m_run = kNegInf, l_run = 0.f;
-    const float scale_log2 = p.scale_log2 * (1.f / Stage<T>::kFactor);
+    const float scale_log2 = p.scale_log2;
 
     // ---- staging: piece j of a thread is codes 16 c .. 16 c + 15 of key row r of the tile.
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(p.k) + kvh * p.sh;
@@ -197,35 +205,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
         }
     };
     // Rows past the last key are zeros (whatever was loaded there): masked in S, and V finite.
-    auto store_tile = [&](int kt, uint16_t* sk, uint16_t* sv) {
+    auto store_tile = [&](int kt, uint16_t* sk, uint16_t* sv, float* sks) {
         const bool ends = kt * kKT + kKT - 1 > last;
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
             const int jr = LINES ? j : 0;
             auto scale = [&](uint32_t b) {    // 2^(b - 127), infinite for 255
                 const uint32_t e = b << 23;
-                return __builtin_bit_cast(float, e > 0x00400000u ? e : 0x00400000u) * Stage<T>::kFactor;
+                return __builtin_bit_cast(float, e > 0x00400000u ? e : 0x00400000u);
             };
             const float ks = scale(ks_raw[jr]), vs = scale(vs_raw[jr]);
             uint32_t a[8], b[8];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                a[2 * w] = Stage<T>::template cvt<false>(k_raw[j].w[w], ks);
-                a[2 * w + 1] = Stage<T>::template cvt<true>(k_raw[j].w[w], ks);
-                b[2 * w] = Stage<T>::template cvt<false>(v_raw[j].w[w], vs);
-                b[2 * w + 1] = Stage<T>::template cvt<true>(v_raw[j].w[w], vs);
+                a[2 * w] = Keys<T>::template cvt<false>(k_raw[j].w[w], ks);
+                a[2 * w + 1] = Keys<T>::template cvt<true>(k_raw[j].w[w], ks);
+                b[2 * w] = scaled_bf16<false>(v_raw[j].w[w], vs);
+                b[2 * w + 1] = scaled_bf16<true>(v_raw[j].w[w], vs);
             }
             const bool bad = ks_raw[jr] == (uint32_t)kScaleNan || vs_raw[jr] == (uint32_t)kScaleNan;
             const bool none = ends && kt * kKT + row_of(j) > last;
             if (__builtin_amdgcn_ballot_w64(bad || none)) {
                 asm volatile("");             // a branch, not selects in every tile
-                const uint32_t fill = none ? 0u : Stage<T>::kNan2;
+                const uint32_t fill = none ? 0u : Keys<T>::kNan2;
 #pragma unroll
                 for (int w = 0; w < 8; ++w) {
                     a[w] = bad || none ? fill : a[w];
                     b[w] = bad || none ? 0u : b[w];
                 }
             }
+            if (kAfter && j < NR && lane_c == 0) sks[row_of(j)] = ks;
             if (!live(j)) continue;
             store16((char*)sk + lds0[j], Vec16{{a[0], a[1], a[2], a[3]}});
             store16((char*)sk + lds1[j], Vec16{{a[4], a[5], a[6], a[7]}});
@@ -259,8 +268,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
     }
 
     if (t_begin < t_end) load_ids(t_begin);
-    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7], in NP pieces.
-    u32x4 qf[NP][DSTEPS];
+    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7], in NQ pieces.
+    u32x4 qf[NQ][DSTEPS];
     {
         const T* q = reinterpret_cast<const T*>(p.q) + (q_first + my_q) * p.q_st + (int64_t)my_head * p.q_sh;
 #pragma unroll
@@ -277,7 +286,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
                     x[4 + i] = __builtin_bit_cast(float, b.w[i]);
                 }
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
+                for (int i = 0; i < NQ; ++i) {
                     qf[i][s] = u32x4{Mfma<E>::pack(x[0], x[1]), Mfma<E>::pack(x[2], x[3]), Mfma<E>::pack(x[4], x[5]),
                                      Mfma<E>::pack(x[6], x[7])};
 #pragma unroll
@@ -287,7 +296,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
         }
     }
 
-    auto tile = [&](int kt, const uint16_t* tile_k, const uint16_t* tile_v, uint16_t* nk, uint16_t* nv) {
+    auto tile = [&](int kt, const uint16_t* tile_k, const uint16_t* tile_v, const float* tile_ks, uint16_t* nk,
+                    uint16_t* nv, float* nks) {
         lds_barrier();                        // tile kt is staged, tile kt - 1 is done with
         const bool sees = kt * kKT < wave_kmax;
         f32x16 st[2];
@@ -302,16 +312,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
                     const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tile_k) +
                                                                     half * 32 * ROWB + koff[s]);
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) st[half] = Mfma<E>::run(u32x4{a.x, a.y, a.z, a.w}, qf[i][s], st[half]);
+                    for (int i = 0; i < NQ; ++i) st[half] = Mfma<E>::run(u32x4{a.x, a.y, a.z, a.w}, qf[i][s], st[half]);
                 }
             __builtin_amdgcn_s_setprio(0);
         }
         // The next tile's rows, loaded a tile ago, go to LDS in the shadow of the first product; the
         // loads of the one after it follow.
-        if (kt + 1 < t_end) store_tile(kt + 1, nk, nv);
+        if (kt + 1 < t_end) store_tile(kt + 1, nk, nv, nks);
         if (kt + 2 < t_end) load_tile(kt + 2);
         if (kt + 3 < t_end) load_ids(kt + 3);
         if (sees) {
+            if constexpr (kAfter) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 ks = *reinterpret_cast<const float4*>(tile_ks + half * 32 + 8 * i + 4 * h);
+                        st[half][4 * i] *= ks.x;
+                        st[half][4 * i + 1] *= ks.y;
+                        st[half][4 * i + 2] *= ks.z;
+                        st[half][4 * i + 3] *= ks.w;
+                    }
+            }
             if (kt * kKT + kKT - 1 > first_pos) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
@@ -337,7 +359,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
                 for (int t = 0; t < DTILES; ++t) o[t] *= alpha;
             }
             m_run = m_new;
-            const float m_off = m_new == kNegInf ? 0.f : m_new - Stage<T>::kLift;
+            const float m_off = m_new == kNegInf ? 0.f : m_new;
             float psum = 0.f;
 #pragma unroll
             for (int half = 0; half < 2; ++half)
@@ -356,8 +378,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
                 u32x4 pb[NP];
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
-                    pb[i] = u32x4{Mfma<E>::pack(sv[r0 + 0], sv[r0 + 1]), Mfma<E>::pack(sv[r0 + 2], sv[r0 + 3]),
-                                  Mfma<E>::pack(sv[r0 + 4], sv[r0 + 5]), Mfma<E>::pack(sv[r0 + 6], sv[r0 + 7])};
+                    pb[i] = u32x4{Mfma<bf16_t>::pack(sv[r0 + 0], sv[r0 + 1]), Mfma<bf16_t>::pack(sv[r0 + 2], sv[r0 + 3]),
+                                  Mfma<bf16_t>::pack(sv[r0 + 4], sv[r0 + 5]), Mfma<bf16_t>::pack(sv[r0 + 6], sv[r0 + 7])};
                     if (i + 1 < NP)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) sv[r0 + e] -= (float)(__bf16)sv[r0 + e];
@@ -368,7 +390,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
                     const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_lo[t]));
                     const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_hi[t]));
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) o[t] = Mfma<E>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
+                    for (int i = 0; i < NP; ++i) o[t] = Mfma<bf16_t>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
                 }
             }
         }
@@ -376,19 +398,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
     if (t_begin < t_end) {
         load_tile(t_begin);
         if (t_begin + 1 < t_end) load_ids(t_begin + 1);
-        store_tile(t_begin, s_k0, s_v0);
+        store_tile(t_begin, s_k0, s_v0, s_ks[0]);
         if (t_begin + 1 < t_end) load_tile(t_begin + 1);
         if (t_begin + 2 < t_end) load_ids(t_begin + 2);
     }
     for (int kt = t_begin; kt < t_end; kt += 2) {
-        tile(kt, s_k0, s_v0, s_k1, s_v1);
-        if (kt + 1 < t_end) tile(kt + 1, s_k1, s_v1, s_k0, s_v0);
+        tile(kt, s_k0, s_v0, s_ks[0], s_k1, s_v1, s_ks[1]);
+        if (kt + 1 < t_end) tile(kt + 1, s_k1, s_v1, s_ks[1], s_k0, s_v0, s_ks[0]);
     }
 
     // ---- store: the lane holds dims 32 t + 8 (r / 4) + 4 h + r % 4 of its row.
     if (!my_live) return;
     const int64_t tok = q_first + my_q;
-    constexpr float kBack = 1.f / Stage<T>::kFactor;
     if (run < n_tiles && my_pos >= 0) {
         const int64_t row = tok * p.num_heads + my_head;
         const int64_t slot = row * p.splits + split;
@@ -399,8 +420,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
             for (int i = 0; i < 4; ++i)
                 if (32 * t + 8 * i < D)
                     *reinterpret_cast<float4*>(po + 32 * t + 8 * i) =
-                        make_float4(o[t][4 * i] * kBack, o[t][4 * i + 1] * kBack, o[t][4 * i + 2] * kBack,
-                                    o[t][4 * i + 3] * kBack);
+                        make_float4(o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]);
         // The merge skips a part whose maximum is -inf; one whose scores were all NaN has to count.
         if (h == 0)
             *reinterpret_cast<float2*>(p.ws_ml + slot * 2) =
@@ -410,7 +430,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
     }
     if (split > 0) return;
     if (p.ws_rows && h == 0) p.ws_rows[tok * p.num_heads + my_head] = 0;   // finished here
-    const float inv = l_run == 0.f ? 0.f : kBack / l_run;                  // no key: zero
+    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;                    // no key: zero
     T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)my_head * p.out_sh;
 #pragma unroll
     for (int t = 0; t < DTILES; ++t)

@@ -172,10 +172,10 @@ def paged_attention_kv8(query: torch.Tensor, k_cache: Kv8, v_cache: Kv8, block_t
     query_lens [B] as there, same checks and messages. Returns [T, heads, head_dim] in the
     query's dtype.
 
-    Softmax and sums are in fp32, the output is rounded once. A key that a query does not see
-    does not reach it, whatever it holds. fp16 queries expect cached values of fp16's range (up to
-    2^17, as rows that were appended in fp16 always are). Lengths with host copies attached (attach_host) are
-    checked without a device round trip."""
+    Softmax and sums are in fp32; of a weight 16 bits at least (24 for fp32 queries) meet the
+    values; the output is rounded once. A key that a query does not see does not reach it, NaN
+    rows included. (A code that is NaN itself, which the append never writes, may.) Lengths with
+    host copies attached (attach_host) are checked without a device round trip."""
     backend = CONFIG.attention
     if backend == "hip":
         return _attention_hip(query, k_cache, v_cache, block_tables, context_lens, query_lens, scale)
