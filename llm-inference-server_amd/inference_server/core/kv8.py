@@ -210,8 +210,12 @@ def _attention_gather(query, k_cache, v_cache, tables, ctx, qlens, scale):
     _check_query(query, k_cache)
     if query.shape[0] == 0:
         return torch.empty_like(query)
-    # The blocks that the tables name, once each.
-    used, where = torch.unique(tables, return_inverse=True)
+    # The blocks that some query sees, once each. The other entries may hold anything.
+    blocks = torch.where(qlens > 0, -(-ctx // k_cache.codes.shape[1]), 0).to(tables.device)
+    seen = torch.arange(tables.shape[1], device=tables.device) < blocks[:, None]
+    used, number = torch.unique(tables[seen].to(query.device, torch.long), return_inverse=True)
+    where = torch.zeros(tables.shape, dtype=torch.long, device=query.device)
+    where[seen.to(query.device)] = number
     k, v = (Kv8(c.codes.view(torch.uint8)[used].view(CODES), c.scales.view(torch.uint8)[used].view(SCALES))
             for c in (k_cache, v_cache))
     keys, vals = kv8_dequantize(k), kv8_dequantize(v)
