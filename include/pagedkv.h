@@ -485,8 +485,10 @@ int pkv_kv8_append(
  * pkv_paged_attention_prefill_split, and so does workspace: at least
  * pkv_kv8_attention_workspace_bytes() bytes for the same sizes and lengths, its first 256 KiB
  * zero when a call starts (every completed call leaves them zero; it can be the decode calls'
- * workspace). Calls that may run at the same time, graph replays included, need one each. With
- * a smaller one, or NULL, no context is cut. */
+ * workspace). Calls that may run at the same time, graph replays included, need one each. A call
+ * may be two launches: host threads that share a stream and a workspace take turns, so that no
+ * other call with it gets between them. With a
+ * smaller one, or NULL, no context is cut. */
 int64_t pkv_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
                                           int64_t head_dim, int64_t num_tokens, int64_t max_query_len,
                                           int64_t max_context_len, const int64_t* host_context_lens,

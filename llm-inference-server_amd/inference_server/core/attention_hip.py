@@ -22,6 +22,7 @@ what runs afterwards:
 
 from __future__ import annotations
 
+import contextlib
 import threading
 
 import numpy as np
@@ -72,8 +73,8 @@ _COUNTER_BYTES = 256 * 1024
 
 class _Workspaces:
     """One attention workspace per (device, stream), grown on demand and reused across
-    calls (split-KV decode and split prefill; a stream runs one call at a time). It is
-    zero-filled when allocated: the decode merge counters at its front must read zero when
+    calls (split-KV decode and split prefill; a stream runs one call at a time, and host
+    threads that share one take turns, see `turn`). It is zero-filled when allocated: the decode merge counters at its front must read zero when
     a call starts, and every completed call leaves them zero again (the partials behind
     them need no initialisation). A different stream gets its own buffer. Sizes are powers
     of two and a buffer that had to grow is kept, not freed: a graph captured on that
@@ -90,6 +91,15 @@ class _Workspaces:
         # (capture id, buffer) of the capture under way on a stream.
         self._captured: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
         self._own: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
+        self._turns: dict[tuple[int, int], threading.Lock] = {}
+
+    def turn(self, device: torch.device, stream: int) -> threading.Lock:
+        """To be held from a call's look-up of its buffer until its last launch is queued. A
+        split call's merge kernel reads the partials that its first kernel left in the stream's
+        buffer, and the library runs without the interpreter's lock: another thread's call on
+        the stream must not get in between."""
+        idx = device.index if device.index is not None else torch.cuda.current_device()
+        return self._turns.setdefault((idx, stream), threading.Lock())
 
     def partials(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -136,6 +146,8 @@ class _Workspaces:
 
 
 _WORKSPACES = _Workspaces()
+#: In place of a turn where a call has no workspace.
+_ALONE = contextlib.nullcontext()
 
 
 def _on_device(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
@@ -302,33 +314,35 @@ def paged_attention_hip_launch(
     if facts["all_decode"] and append is not None:
         max_ctx = facts["max_ctx"]
         ws_bytes = L.pkv_paged_attention_decode_workspace_bytes(n_seqs, n_heads, n_kv, head_dim, max_ctx)
-        ws = _WORKSPACES.partials(dev, stream, ws_bytes)
-        rc = L.pkv_paged_attention_decode_append(
-            *rows,
-            *common_pool[:9],
-            k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), k_new.stride(1), slots.data_ptr(),
-            *common_pool[9:],
-            ctx_dev.data_ptr(),
-            n_seqs, n_heads, max_ctx,
-            float(scale), dt,
-            ws.data_ptr(), ws.numel(),
-            stream,
-        )
+        with _WORKSPACES.turn(dev, stream):
+            ws = _WORKSPACES.partials(dev, stream, ws_bytes)
+            rc = L.pkv_paged_attention_decode_append(
+                *rows,
+                *common_pool[:9],
+                k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), k_new.stride(1), slots.data_ptr(),
+                *common_pool[9:],
+                ctx_dev.data_ptr(),
+                n_seqs, n_heads, max_ctx,
+                float(scale), dt,
+                ws.data_ptr(), ws.numel(),
+                stream,
+            )
         native.check(rc, "pkv_paged_attention_decode_append")
         return out
     if facts["all_decode"]:
         max_ctx = facts["max_ctx"]
         ws_bytes = L.pkv_paged_attention_decode_workspace_bytes(n_seqs, n_heads, n_kv, head_dim, max_ctx)
-        ws = _WORKSPACES.partials(dev, stream, ws_bytes)
-        rc = L.pkv_paged_attention_decode(
-            *rows,
-            *common_pool,
-            ctx_dev.data_ptr(),
-            n_seqs, n_heads, max_ctx,
-            float(scale), dt,
-            ws.data_ptr(), ws.numel(),
-            stream,
-        )
+        with _WORKSPACES.turn(dev, stream):
+            ws = _WORKSPACES.partials(dev, stream, ws_bytes)
+            rc = L.pkv_paged_attention_decode(
+                *rows,
+                *common_pool,
+                ctx_dev.data_ptr(),
+                n_seqs, n_heads, max_ctx,
+                float(scale), dt,
+                ws.data_ptr(), ws.numel(),
+                stream,
+            )
         native.check(rc, "pkv_paged_attention_decode")
         return out
 
@@ -345,22 +359,23 @@ def paged_attention_hip_launch(
         if L.pkv_paged_attention_prefill_can_split(block_size, head_dim, dt):
             ws_bytes = L.pkv_paged_attention_prefill_workspace_bytes(n_seqs, n_heads, n_kv, head_dim, n_tok, *lens)
         facts["split_ws"][shape] = ws_bytes
-    ws_ptr, ws_size = None, 0
-    if ws_bytes:
-        ws = _WORKSPACES.partials(dev, stream, ws_bytes)
-        ws_ptr, ws_size = ws.data_ptr(), ws.numel()
     new = (None, None, 0, 0, None) if append is None else (
         k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0), k_new.stride(1), slots.data_ptr())
-    rc = L.pkv_paged_attention_prefill_split(
-        *rows,
-        *common_pool[:9],
-        *new,
-        *common_pool[9:],
-        ctx_dev.data_ptr(), qsl.data_ptr(),
-        n_seqs, n_heads, n_tok, facts["max_q"], *lens,
-        float(scale), dt,
-        ws_ptr, ws_size,
-        stream,
-    )
+    ws_ptr, ws_size = None, 0
+    with _WORKSPACES.turn(dev, stream) if ws_bytes else _ALONE:
+        if ws_bytes:
+            ws = _WORKSPACES.partials(dev, stream, ws_bytes)
+            ws_ptr, ws_size = ws.data_ptr(), ws.numel()
+        rc = L.pkv_paged_attention_prefill_split(
+            *rows,
+            *common_pool[:9],
+            *new,
+            *common_pool[9:],
+            ctx_dev.data_ptr(), qsl.data_ptr(),
+            n_seqs, n_heads, n_tok, facts["max_q"], *lens,
+            float(scale), dt,
+            ws_ptr, ws_size,
+            stream,
+        )
     native.check(rc, "pkv_paged_attention_prefill")
     return out

@@ -23,7 +23,8 @@ import torch
 from inference_server import native
 from inference_server.config import CONFIG
 from inference_server.core.attention import _gather_ragged, check_contract
-from inference_server.core.attention_hip import (_QSL_ATTR, _WORKSPACES, _batch_facts, _on_device, _query_start)
+from inference_server.core.attention_hip import (_ALONE, _QSL_ATTR, _WORKSPACES, _batch_facts, _on_device,
+                                                 _query_start)
 from inference_server.core.kv_pool import ModelDims, PagedKVPool
 
 CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -283,18 +284,19 @@ def _attention_hip(query, k_cache, v_cache, tables, context_lens, query_lens, sc
             ws_bytes = facts["split_ws"][key] = lib.pkv_kv8_attention_workspace_bytes(
                 n_seqs, n_heads, n_kv, head_dim, n_tok, max_q, max_ctx, *lens)
         ws_ptr, ws_size = None, 0
-        if ws_bytes:
-            # A capture's calls have one of their own: replays of graphs that were captured on one
-            # stream may overlap.
-            capturing = torch.cuda.is_current_stream_capturing()
-            ws = (_WORKSPACES.of_capture if capturing else _WORKSPACES.partials)(dev, stream, ws_bytes)
-            ws_ptr, ws_size = ws.data_ptr(), ws.numel()
-        rc = lib.pkv_kv8_attention(
-            out.data_ptr(), n_heads * head_dim, head_dim, query.data_ptr(), q_st[0], q_st[1],
-            *where, n_blocks, block_size, n_kv, head_dim,
-            tables.data_ptr(), t_st[0], width, ctx_dev.data_ptr(), qsl,
-            n_seqs, n_heads, n_tok, max_q, max_ctx, *lens,
-            float(scale), native.DTYPE_CODES[query.dtype], ws_ptr, ws_size, stream)
+        with _WORKSPACES.turn(dev, stream) if ws_bytes else _ALONE:
+            if ws_bytes:
+                # A capture's calls have one of their own: replays of graphs that were captured on
+                # one stream may overlap.
+                capturing = torch.cuda.is_current_stream_capturing()
+                ws = (_WORKSPACES.of_capture if capturing else _WORKSPACES.partials)(dev, stream, ws_bytes)
+                ws_ptr, ws_size = ws.data_ptr(), ws.numel()
+            rc = lib.pkv_kv8_attention(
+                out.data_ptr(), n_heads * head_dim, head_dim, query.data_ptr(), q_st[0], q_st[1],
+                *where, n_blocks, block_size, n_kv, head_dim,
+                tables.data_ptr(), t_st[0], width, ctx_dev.data_ptr(), qsl,
+                n_seqs, n_heads, n_tok, max_q, max_ctx, *lens,
+                float(scale), native.DTYPE_CODES[query.dtype], ws_ptr, ws_size, stream)
         native.check(rc, "pkv_kv8_attention")
         return out
 
