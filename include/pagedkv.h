@@ -526,8 +526,10 @@ int pkv_kv8_attention(
  * the table's width, held outside it, more new tokens than num_tokens).
  *
  * All or nothing: if blocks needed > num_free, or any length is impossible, no table changes,
- * held_out = held, every slot is -1 and query_start_loc is all 0, so that the appends and
- * attention calls queued behind it do nothing. A call repeated on the same inputs gives the
+ * held_out = held, every slot is -1 and query_start_loc is all 0, so that appends queued behind
+ * it with these slots do nothing, nor does attention that is given this query_start_loc. Attention
+ * without it (a decode call, or one with starts of other making) runs on tables that lack blocks:
+ * it reads nothing outside the cache, and its output means nothing. A call repeated on the same inputs gives the
  * same result (held is not advanced in place). */
 int pkv_step_layout(
     int64_t* block_tables, int64_t table_stride, int64_t table_width,

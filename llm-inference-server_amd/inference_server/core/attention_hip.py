@@ -35,8 +35,13 @@ _HOST_ATTR = "_pkv_host"
 
 
 def attach_host(device_tensor: torch.Tensor, host_tensor: torch.Tensor) -> torch.Tensor:
-    """Record a host (CPU) copy of `device_tensor`'s values for host-side checks.
-    The caller guarantees the two hold the same values. Returns device_tensor."""
+    """Record a host (CPU) copy of `device_tensor`'s values for host-side checks and for the
+    sizes of launches. The caller guarantees the two hold the same values, or, where the host
+    does not know a step's lengths, that the copies are bounds: no context longer than the
+    longest of context_lens' copy, no more query tokens in a sequence than the longest of
+    query_lens' copy, whose sum is the query's rows. The kernels then go by the device's
+    contexts, and by the query starts that are attached (attach_query_start; a query_lens copy
+    of ones says one token each). Returns device_tensor."""
     setattr(device_tensor, _HOST_ATTR, host_tensor)
     return device_tensor
 
