@@ -445,18 +445,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kChunkWaves
         }
 }
 
-// Workgroups of the flat grid, as the 16-bit kernel's.
-inline int64_t kv8_chunk_workgroups(const Kv8Params& p) {
-    const int64_t grid = ceil_div((int64_t)p.max_query_len * p.group, kRows) * p.num_seqs;
-    const int64_t fill = p.num_tokens * p.group / kRows + p.num_seqs;
-    int64_t items = (grid < fill || p.num_seqs > kPrefillSortSeqs ? grid : fill) * p.num_kv_heads;
-    if (p.splits > 1 && p.split_items > items) items = p.split_items;
-    return ceil_div(items, 8) * 8;
-}
-
 template <typename T, int D>
 int launch_kv8_chunk_d(const Kv8Params& p, hipStream_t stream) {
-    const dim3 grid((unsigned)kv8_chunk_workgroups(p));
+    const dim3 grid((unsigned)prefill_workgroups(p));
     if (p.block_size >= 16 && kv8_offsets_fit(p)) kv8_chunk_kernel<T, D, true><<<grid, 256, 0, stream>>>(p);
     else kv8_chunk_kernel<T, D, false><<<grid, 256, 0, stream>>>(p);
     const int rc = check_launch("kv8 chunk attention");
@@ -471,7 +462,7 @@ int launch_kv8_chunk_d(const Kv8Params& p, hipStream_t stream) {
 template <typename T>
 int launch_kv8_chunk(const Kv8Params& p, hipStream_t stream) {
     // One grid dimension; rows of a sequence in 32 bits.
-    if (kv8_chunk_workgroups(p) > 0x7fffffff) return PKV_EUNSUPPORTED;
+    if (prefill_workgroups(p) > 0x7fffffff) return PKV_EUNSUPPORTED;
     if (((int64_t)p.max_query_len + kRows) * p.group > 0x7fffffff) return PKV_EUNSUPPORTED;
     switch (p.head_dim) {
         case 32: return launch_kv8_chunk_d<T, 32>(p, stream);
