@@ -443,7 +443,8 @@ int pkv_lm_head_argmax(
  *
  * A row of one (token, KV head) is head_dim e4m3 codes (OCP: bias 7, largest magnitude 448,
  * no infinity) and one scale byte b (e8m0): value = code * 2^(b - 127), b the least with which
- * the row's largest magnitude is at most 448 (0 for a row of zeros). A row with a value that
+ * the row's largest magnitude is at most 448 (0 for a row of zeros); magnitudes from
+ * 1.9375 * 2^127 on round up to 2^128, float32's infinity. A row with a value that
  * is not finite is the NaN row: b = 255 and codes 0. Codes are finite (a code of NaN under
  * another scale is not a row that the append writes, and may reach rows that do not see it).
  *
@@ -476,7 +477,9 @@ int pkv_kv8_append(
  * is NULL (one token per sequence). Scores, softmax and sums are in float32, of a weight 16 bits
  * at least (24 for float32 queries) meet the values, the output is rounded once; a key that a row
  * does not see never reaches it, whatever it holds (NaN rows
- * included), and a row that sees no key (a context of 0) is zero. max_query_len bounds the
+ * included), and a row that sees no key (a context of 0) is zero. Cached values are expected
+ * between 2^-100 and 2^100 in magnitude, or zero: smaller ones lose digits below 2^-126, larger
+ * ones may overflow sums of weights that are not normalised yet. max_query_len bounds the
  * query lengths (0: num_tokens) and max_context_len the contexts: they size the grid.
  * Block ids outside the pool are never dereferenced.
  *

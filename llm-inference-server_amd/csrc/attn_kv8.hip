@@ -257,7 +257,9 @@ bool kv8_decode_applies(const Kv8Params& p, int dtype) {
 // How a decode batch is cut; the bytes of partials that it takes (0: none are wanted, or there are
 // more (sequence, KV head) pairs than merge counters).
 int64_t kv8_decode_plan(Kv8Params& p, const int64_t* host_ctx, const int64_t* host_qlen) {
-    constexpr int64_t kWorkgroups = 256 * 3;    // that the GPU holds
+    // Workgroups that the GPU holds, three of four waves a CU. (Of 8 waves, as 16-bit heads up to
+    // 64 have in runs of a workgroup, it holds 512, and what a plan has more starts late.)
+    constexpr int64_t kWorkgroups = 256 * 3;
     const int64_t keys = p.head_dim <= 64 ? 64 : 32;    // of a unit
     // Even runs from this many keys a workgroup on: below, runs inside sequences are as good (us a
     // call, 32/8 heads of 128: 16 sequences of 1-8k 34.1 even, 34.4 not; 64 of 1-16k 191 and 204;

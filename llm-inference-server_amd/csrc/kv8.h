@@ -6,8 +6,10 @@
 // is not finite is the NaN row: b = 255, codes 0.
 //
 // Why a power of two: e4m3 has an exponent of its own, so a finer scale would buy no relative
-// precision; code * 2^k is exact in bf16 and fp32 (8 exponent bits), so the matrix
-// instructions run on the cache's exact values; and quantising x * 2^(127 - b) rounds once.
+// precision; code * 2^k is exact in bf16 and fp32 (8 exponent bits) wherever it is a normal number
+// of theirs, so the matrix instructions run on the cache's exact values; and quantising
+// x * 2^(127 - b) rounds once. (Not 2^128, code 256 at b = 247, to which |x| of 1.9375 * 2^127 and
+// more round up, as they do in other conversions to few bits; nor what is below 2^-126.)
 // Why NaN in the scale: codes stay finite, so 0 * V is 0 where a key is masked.
 #pragma once
 

@@ -15,7 +15,8 @@
 //    which none is cut is not summed up at all. Every workgroup finds its run by running sums of
 //    its own over the lengths, so a graph's replays may change them.
 //  * A sequence in several runs leaves fp32 partials, which the last workgroup to finish it
-//    merges inside the launch, in key order, so results do not depend on timing.
+//    merges inside the launch, in an order that the number of parts fixes, so results do not depend
+//    on timing.
 //  * Operands as they lie: S^T = K Q^T on 16x16x32 takes quarters of K rows (the order of a
 //    contraction is free as long as Q's is the same). Its result leaves a lane with 8 keys of one
 //    query row, which are the B operand of O^T += V^T P^T as they stand. V^T's operand is 8 keys
@@ -26,7 +27,8 @@
 //    value scales the weights, both in fp32.
 //  * Weights enter the second product as bf16 pieces (two for 16-bit types: 16 bits of them,
 //    three for fp32), fp32 queries the first one as three: the product is then as exact as its
-//    fp32 accumulation, and the matrix unit has time to spare (12-40 MFMAs a unit of 8 KiB).
+//    fp32 accumulation, and the matrix unit has time to spare (20-24 MFMAs a unit of up to 8 KiB,
+//    36-48 for fp32).
 //  * A unit stays in registers; K of the next one is loaded when the first product has used
 //    this one's, V after the second, the other waves of the SIMD (2-4) being the cover. Two
 //    units in registers and half the waves were slower (64 sequences as above 203 us, 190 so).

@@ -6,7 +6,8 @@ Format. A cached row (one token, one KV head, K or V) is head_dim e4m3 codes and
 power-of-two scale, an exponent byte: torch.float8_e4m3fn and torch.float8_e8m0fnu, so a
 row's value is `codes.float() * scale.float()`. The scale is the least with which the row's
 largest magnitude is at most e4m3's 448. A power of two costs no relative precision (e4m3 has
-an exponent of its own) and makes code * scale exact in bf16 and fp32. A row with a value that
+an exponent of its own) and makes code * scale exact in bf16 and fp32, as far as their normal
+numbers go: magnitudes from 1.9375 * 2^127 on round up to 2^128, infinity there. A row with a value that
 is not finite is stored as the NaN row: scale NaN, codes 0.
 
 Backends follow CONFIG.attention, as for the 16- and 32-bit pools: "gather" runs tensor ops
