@@ -42,6 +42,9 @@ def attach_host(device_tensor: torch.Tensor, host_tensor: torch.Tensor) -> torch
     query_lens' copy, whose sum is the query's rows. The kernels then go by the device's
     contexts, and by the query starts that are attached (attach_query_start; a query_lens copy
     of ones says one token each). Returns device_tensor."""
+    if host_tensor.shape != device_tensor.shape:
+        raise ValueError(f"a host copy of {tuple(device_tensor.shape)} must have that shape, got "
+                         f"{tuple(host_tensor.shape)}")
     setattr(device_tensor, _HOST_ATTR, host_tensor)
     return device_tensor
 
@@ -54,6 +57,10 @@ def attach_query_start(query_lens: torch.Tensor, query_start: torch.Tensor) -> t
     that a prefill launch should use instead of building one from the host lengths
     (a caller that keeps its metadata in persistent device buffers, such as a captured
     graph, supplies it). The caller guarantees the values match. Returns query_lens."""
+    if (query_start.dtype is not torch.long or query_start.shape != (query_lens.numel() + 1,)
+            or not query_start.is_contiguous() or query_start.device != query_lens.device):
+        raise ValueError(f"query_start must be contiguous int64 [{query_lens.numel() + 1}] on {query_lens.device}, got "
+                         f"{query_start.dtype} {tuple(query_start.shape)} on {query_start.device}")
     setattr(query_lens, _QSL_ATTR, query_start)
     return query_lens
 
