@@ -210,6 +210,8 @@ def _attention_gather(query, k_cache, v_cache, tables, ctx, qlens, scale):
                    lambda: (int(qlens.sum()), bool((qlens > ctx).any()),
                             bool(((-(-ctx // k_cache.codes.shape[1])) > tables.shape[1]).any())))
     _check_query(query, k_cache)
+    if bool((qlens < 0).any()):
+        raise ValueError("query_lens must not be negative")
     if query.shape[0] == 0:
         return torch.empty_like(query)
     # The blocks that some query sees, once each. The other entries may hold anything.

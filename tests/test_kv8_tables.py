@@ -42,3 +42,10 @@ def test_entries_that_queries_read_are_followed_or_refused_on_the_cpu(monkeypatc
     tables[1, 1] = s.k.codes.shape[0]
     with pytest.raises(IndexError):
         paged_attention_kv8(s.q, s.k, s.v, tables, *s.args[1:], s.scale)
+
+@pytest.mark.parametrize("d", [32, 40])
+def test_negative_query_lengths_are_refused(device, d):
+    s = batch([(5, 1), (3, 1)], heads=4, kv=2, d=d, bs=8, dtype=torch.float16, device=device)
+    new = torch.tensor([-1, 3], device=s.q.device)
+    with pytest.raises(ValueError, match="must not be negative"):
+        paged_attention_kv8(s.q, s.k, s.v, *s.args[:2], new, s.scale)
