@@ -42,9 +42,6 @@ def attach_host(device_tensor: torch.Tensor, host_tensor: torch.Tensor) -> torch
     query_lens' copy, whose sum is the query's rows. The kernels then go by the device's
     contexts, and by the query starts that are attached (attach_query_start; a query_lens copy
     of ones says one token each). Returns device_tensor."""
-    if host_tensor.shape != device_tensor.shape:
-        raise ValueError(f"a host copy of {tuple(device_tensor.shape)} must have that shape, got "
-                         f"{tuple(host_tensor.shape)}")
     setattr(device_tensor, _HOST_ATTR, host_tensor)
     return device_tensor
 
@@ -110,8 +107,9 @@ class _Workspaces:
         split call's merge kernel reads the partials that its first kernel left in the stream's
         buffer, and the library runs without the interpreter's lock: another thread's call on
         the stream must not get in between."""
-        idx = device.index if device.index is not None else torch.cuda.current_device()
-        return self._turns.setdefault((idx, stream), threading.Lock())
+        key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+        lock = self._turns.get(key)
+        return lock if lock is not None else self._turns.setdefault(key, threading.Lock())
 
     def partials(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -191,8 +189,11 @@ def _batch_facts(context_lens: torch.Tensor, query_lens: torch.Tensor, block_siz
     # Copies: facts are kept past this call, and the caller's tensors may be written to. In
     # numpy: the same operations on small tensors took 58-73 us of a first call (16 so).
     hctx, hql = np.array(hc, dtype=np.int64), np.array(hq, dtype=np.int64)
+    if hctx.shape != hql.shape:
+        raise ValueError(f"host copies of context_lens and query_lens differ: {hctx.shape} and {hql.shape}")
     longest = int(hctx.max()) if hctx.size else 0
     facts = {
+        "seqs": hctx.size,
         "hctx": torch.from_numpy(hctx),
         "hql": torch.from_numpy(hql),
         "total": int(hql.sum()),
@@ -206,6 +207,14 @@ def _batch_facts(context_lens: torch.Tensor, query_lens: torch.Tensor, block_siz
     }
     if key is not None:
         setattr(context_lens, _META_ATTR, (key, facts))
+    return facts
+
+
+def _step_facts(context_lens: torch.Tensor, query_lens: torch.Tensor, block_size: int, width: int) -> dict:
+    """_batch_facts for a call: the library reads the host copies by address, one entry a sequence."""
+    facts = _batch_facts(context_lens, query_lens, block_size, width)
+    if facts["seqs"] != context_lens.shape[0]:
+        raise ValueError(f"host copies of {context_lens.shape[0]} lengths hold {facts['seqs']}")
     return facts
 
 
@@ -265,7 +274,7 @@ def paged_attention_hip_launch(
 
     def values():
         nonlocal facts
-        facts = _batch_facts(context_lens, query_lens, bs, width)
+        facts = _step_facts(context_lens, query_lens, bs, width)
         return facts["total"], facts["q_gt_c"], facts["too_few_blocks"]
 
     check_contract(len(q_shape), q_shape, len(p_shape), p_shape, t_shape, context_lens.shape, query_lens.shape, values)

@@ -24,8 +24,8 @@ import torch
 from inference_server import native
 from inference_server.config import CONFIG
 from inference_server.core.attention import _gather_ragged, check_contract
-from inference_server.core.attention_hip import (_ALONE, _QSL_ATTR, _WORKSPACES, _batch_facts, _on_device,
-                                                 _query_start)
+from inference_server.core.attention_hip import (_ALONE, _QSL_ATTR, _WORKSPACES, _on_device, _query_start,
+                                                 _step_facts)
 from inference_server.core.kv_pool import ModelDims, PagedKVPool
 
 CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -242,7 +242,7 @@ def _attention_hip(query, k_cache, v_cache, tables, context_lens, query_lens, sc
 
     def values():
         nonlocal facts
-        facts = _batch_facts(context_lens, query_lens, block_size, width)
+        facts = _step_facts(context_lens, query_lens, block_size, width)
         if "negative" not in facts:
             facts["negative"] = bool((facts["hql"] < 0).any())
         return facts["total"], facts["q_gt_c"], facts["too_few_blocks"]

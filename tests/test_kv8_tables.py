@@ -43,6 +43,7 @@ def test_entries_that_queries_read_are_followed_or_refused_on_the_cpu(monkeypatc
     with pytest.raises(IndexError):
         paged_attention_kv8(s.q, s.k, s.v, tables, *s.args[1:], s.scale)
 
+
 @pytest.mark.parametrize("d", [32, 40])
 def test_negative_query_lengths_are_refused(device, d):
     s = batch([(5, 1), (3, 1)], heads=4, kv=2, d=d, bs=8, dtype=torch.float16, device=device)
