@@ -357,12 +357,11 @@ extern "C" int64_t pkv_kv8_attention_workspace_bytes(int64_t num_seqs, int64_t n
         num_seqs > 0x7fffffff || num_tokens > 0x7fffffff || num_heads % num_kv_heads)
         return 0;
     Kv8Params p = sizes_of(num_seqs, num_heads, num_kv_heads, head_dim, num_tokens, max_query_len, max_context_len);
-    if (few_rows(p)) {
-        const int64_t parts = kv8_decode_plan(p, host_context_lens, host_query_lens);
-        if (parts) return kMergeCounterBytes + parts;
-    }
+    // Few rows: strides and addresses decide between the kernels.
+    const int64_t parts = few_rows(p) ? kv8_decode_plan(p, host_context_lens, host_query_lens) : 0;
     const SplitPlan plan = chunk_plan(p, host_context_lens, host_query_lens);
-    return plan.splits > 1 ? kMergeCounterBytes + plan.total() : 0;
+    const int64_t chunks = plan.splits > 1 ? plan.total() : 0, most = parts > chunks ? parts : chunks;
+    return most ? kMergeCounterBytes + most : 0;
 }
 
 extern "C" int pkv_kv8_attention(

@@ -293,7 +293,8 @@ def _attention_hip(query, k_cache, v_cache, tables, context_lens, query_lens, sc
                 # one stream may overlap.
                 capturing = torch.cuda.is_current_stream_capturing()
                 ws = (_WORKSPACES.of_capture if capturing else _WORKSPACES.partials)(dev, stream, ws_bytes)
-                ws_ptr, ws_size = ws.data_ptr(), ws.numel()
+                # Not what it has: the cut, and with it the output's bits, go by the call alone.
+                ws_ptr, ws_size = ws.data_ptr(), ws_bytes
             rc = lib.pkv_kv8_attention(
                 out.data_ptr(), n_heads * head_dim, head_dim, query.data_ptr(), q_st[0], q_st[1],
                 *where, n_blocks, block_size, n_kv, head_dim,

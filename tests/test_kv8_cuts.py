@@ -1,7 +1,7 @@
 """Decode and chunks over the 8-bit cache where contexts are cut and merged, one test for each way in
 which a batch is cut: runs of a workgroup and of a wave, inside a sequence, in batches of up to
-64 sequences and of more; and even runs over the ends of sequences. Which way a batch goes is
-read from the workspace that it asks for."""
+64 sequences and of more; and even runs over the ends of sequences. Which way a batch goes follows
+from the rules of the plan, restated below."""
 
 from __future__ import annotations
 
@@ -26,14 +26,28 @@ def hip_backend(monkeypatch):
     monkeypatch.setattr(CONFIG, "attention", "hip")
 
 
-def partials(s, heads, kv, d, bound=None):
-    """How many partials per KV head the batch's plan has room for; 0: it is not cut."""
+def workspace(s, heads, kv, d, bound=None):
     ctx = torch.from_numpy(s.ctx if bound is None else np.full_like(s.ctx, bound))
-    new = torch.from_numpy(s.new)
-    max_q = int(s.new.max())
-    size = native.lib().pkv_kv8_attention_workspace_bytes(
-        len(s.ctx), heads, kv, d, int(s.new.sum()), max_q, int(ctx.max()), ctx.data_ptr(), new.data_ptr())
-    return 0 if size == 0 else (size - COUNTERS) / (kv * max_q * (heads // kv) * (d + 2) * 4)
+    new = torch.from_numpy(s.new).contiguous()
+    return native.lib().pkv_kv8_attention_workspace_bytes(
+        len(s.ctx), heads, kv, d, int(s.new.sum()), int(s.new.max()), int(ctx.max()), ctx.data_ptr(), new.data_ptr())
+
+
+def partials(s, heads, kv, d, bound=None):
+    """How many partials per KV head the decode plan makes of a batch; 0: it is not cut. By the
+    plan's rules, and checked to have room in the workspace that the library asks for."""
+    ctx, n = s.ctx if bound is None else np.full_like(s.ctx, bound), len(s.ctx)
+    keys = 64 if d <= 64 else 32
+    units = np.maximum(-(-ctx // keys), 1)[s.new > 0]
+    if d > 64 and units.sum() * keys * kv >= 768 * 768:                  # even runs
+        numbers = 2 * (512 // kv)
+    else:
+        waves = n * kv >= 768                                            # a run is a wave's
+        runs = int((-(-units // (4 if waves else 8))).sum())
+        numbers = 0 if runs <= n else min(runs, max(768 * (4 if waves else 1) // kv, 2 * n))
+    room = numbers * kv * int(s.new.max()) * (heads // kv) * (d + 2) * 4
+    assert workspace(s, heads, kv, d, bound) >= (COUNTERS + room if numbers else 0)
+    return numbers
 
 
 def nan_rows(s, seq, k_at, v_at, bs):
@@ -134,7 +148,7 @@ def test_chunks_of_nan_rows(dtype, which, d):
     last tokens see."""
     heads, kv = 4, 2
     s = batch([(2500, 40), (10, 30)], heads=heads, kv=kv, d=d, bs=16, dtype=dtype, device="cuda")
-    assert partials(s, heads, kv, d) > 0
+    assert workspace(s, heads, kv, d) > 0
     none, some, every, last = np.arange(0), np.arange(500, 1800), np.arange(2540), np.arange(2530, 2540)
     nan_rows(s, 0, *{"k": (some, none), "v": (none, some), "all": (every, none), "hidden": (none, last)}[which], 16)
     out = twice(s)
