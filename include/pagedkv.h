@@ -541,6 +541,113 @@ int pkv_step_layout(
     int64_t* held_out, int64_t* slots, int64_t* positions, int64_t* query_start_loc, int64_t* counts,
     hipStream_t stream);
 
+/* ------------------------------------------------------------------ drafted token trees
+ * A step that verifies drafted tokens, without counterpart in the reference: every sequence's new tokens are
+ * the nodes of a tree of continuations, scored in one forward pass; the longest path that the
+ * model agrees with is kept. A sequence's nodes are its rows of the packed step
+ * (query_start_loc[i] .. query_start_loc[i + 1]) in an order in which parents come first, node 0
+ * the token that was sampled before; in the cache they are its last positions, in that order. */
+
+/* What each node sees and where it stands. parents int64 [num_tokens]: a node's parent as its
+ * number in the sequence, -1 for a root. Out: masks [num_tokens, ceil(max_nodes / 64)], 64 bits a
+ * word: bit j % 64 of word j / 64 says that the token sees node j of its sequence (its ancestors
+ * and itself); positions [num_tokens]: context_lens[i] minus the sequence's nodes (its cached
+ * tokens), plus the node's depth. max_nodes bounds the nodes of a sequence, at most 8192 (else
+ * PKV_EUNSUPPORTED).
+ *
+ * Rows past the last sequence get masks of 0 and position 0, and so do a node whose parent is
+ * impossible (not -1 and not before it), the nodes below it, and all nodes of a sequence with
+ * more of them than max_nodes or than its context. A proper node sees itself: its masks are not all 0. */
+int pkv_tree_layout(
+    const int64_t* parents, const int64_t* query_start_loc, const int64_t* context_lens,
+    int64_t num_seqs, int64_t num_tokens, int64_t max_nodes,
+    int64_t* masks, int64_t* positions,
+    hipStream_t stream);
+
+/* Attention of the nodes over the paged cache: pkv_paged_attention_prefill's contract, but that token
+ * t of a sequence with n new tokens sees the keys 0 .. context - n - 1, all of them, and of the n
+ * drafted ones those whose bits are set in row t of masks [num_tokens, mask_words] (row stride
+ * mask_stride, in words): any masks, those of pkv_tree_layout among them. Drafted keys from
+ * 64 * mask_words on are seen by none. A key that a row does not see does not reach it, whatever
+ * its K and V hold; a row that sees no key is zero. Scores, softmax and sums are in float32, the
+ * output is rounded once. query_start_loc is not NULL.
+ * Block ids outside the pool are never dereferenced. max_query_len bounds the query lengths (0:
+ * num_tokens).
+ *
+ * host_context_lens / host_query_lens (HOST memory, int64 [num_seqs], or NULL) only decide whether
+ * and how contexts are cut into runs of separate workgroups, as in
+ * pkv_paged_attention_prefill_split, and so does workspace: at least
+ * pkv_tree_attention_workspace_bytes() bytes for the same sizes and lengths, of which the first
+ * 256 KiB are not touched and the rest needs no initialisation. With a smaller one, or NULL, no
+ * context is cut. A call may be two launches: host threads that share a stream and a workspace
+ * take turns. Calls that may run at the same time, graph replays included, need one each. */
+int64_t pkv_tree_attention_workspace_bytes(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads,
+                                           int64_t head_dim, int64_t num_tokens, int64_t max_query_len, int dtype,
+                                           const int64_t* host_context_lens, const int64_t* host_query_lens);
+int pkv_tree_attention(
+    void* out, int64_t out_stride_t, int64_t out_stride_h,
+    const void* query, int64_t q_stride_t, int64_t q_stride_h,
+    const void* k_pool, const void* v_pool,
+    int64_t pool_stride_block, int64_t pool_stride_slot, int64_t pool_stride_head,
+    int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+    const int64_t* block_tables, int64_t table_stride, int64_t table_width,
+    const int64_t* context_lens, const int64_t* query_start_loc,
+    const int64_t* masks, int64_t mask_stride, int64_t mask_words,
+    int64_t num_seqs, int64_t num_heads, int64_t num_tokens, int64_t max_query_len,
+    const int64_t* host_context_lens, const int64_t* host_query_lens,
+    float scale, int dtype,
+    void* workspace, int64_t workspace_bytes,
+    hipStream_t stream);
+
+/* The path of each tree that the target model accepts: from node 0, on to the first child whose
+ * token (tokens int64 [num_tokens]) is the target's token at the node (targets int64 [num_tokens],
+ * greedy or sampled), until there is none. Out, int64: paths [num_seqs, max_depth] the
+ * accepted nodes' numbers, -1 past the last; counts [num_seqs]; next_tokens [num_seqs] the
+ * target's token at the last of them. At most max_depth nodes are accepted. A sequence without
+ * nodes (or with impossible bounds, or more than 8192 nodes) has count 0 and next token -1. Nodes
+ * whose parent is not before them have no parent here. */
+int pkv_tree_accept(
+    const int64_t* tokens, const int64_t* parents, const int64_t* targets, const int64_t* query_start_loc,
+    int64_t num_seqs, int64_t num_tokens, int64_t max_depth,
+    int64_t* paths, int64_t* counts, int64_t* next_tokens,
+    hipStream_t stream);
+
+/* The accepted paths' cached rows, moved behind the sequences' cached tokens in every pool
+ * tensor, in place: the row at position c + paths[i][d] goes to position c + d, c =
+ * context_lens[i] - (query_start_loc[i + 1] - query_start_loc[i]). Bits are copied. tensors:
+ * DEVICE array of num_tensors pool bases (16-byte aligned); a block is block_bytes, its rows
+ * (slots) row_bytes each from its start on, followed, in 8-bit pools, by `scales` bytes a slot,
+ * stored [scales][block_size] (0 elsewhere). paths int64 [num_seqs, max_depth]; a path ends at the
+ * first number that is not above the one before it or not below the sequence's nodes. Rows in blocks
+ * outside the pool or the table stay. Sequences must not share the blocks of their drafted rows. */
+int pkv_keep_paths(
+    void* const* tensors, int64_t num_tensors, int64_t num_blocks, int64_t block_size,
+    int64_t block_bytes, int64_t row_bytes, int64_t scales,
+    const int64_t* block_tables, int64_t table_stride, int64_t table_width,
+    const int64_t* context_lens, const int64_t* query_start_loc, int64_t num_seqs,
+    const int64_t* paths, int64_t max_depth,
+    hipStream_t stream);
+
+/* ------------------------------------------------------------------ log probabilities
+ * Of token ids[r] in the softmax of row r of logits [num_rows, vocab_size] (`dtype`, any row
+ * stride, logits_stride elements): logprobs [num_rows] its log probability and ranks int64 [num_rows] 1 +
+ * the number of larger logits; entropy [num_rows] that of the row, in nats; the `top` (0 .. 64) largest
+ * logits' log probabilities and ids, in order, equal ones by ascending id: top_logprobs
+ * [num_rows, top], top_ids int64 [num_rows, top]. Sums are in float32 (outputs too).
+ *
+ * Logits of -inf are tokens that cannot be: log probability -inf. A row with a NaN or +inf, or of
+ * -inf alone, has no distribution: NaN, rank 0, ids -1. An id outside the vocabulary (a padding row's -1): NaN
+ * and rank 0. workspace: at least pkv_token_logprobs_workspace_bytes() bytes, its first
+ * 256 KiB zero when a call starts; every completed call leaves them zero (it can be the attention
+ * calls' workspace). Calls that may run at the same time need one each. One launch. */
+int64_t pkv_token_logprobs_workspace_bytes(int64_t num_rows, int64_t vocab_size, int64_t top, int dtype);
+int pkv_token_logprobs(
+    const void* logits, int64_t logits_stride, int64_t num_rows, int64_t vocab_size, int dtype,
+    const int64_t* ids, int64_t top,
+    float* logprobs, int64_t* ranks, float* entropy, float* top_logprobs, int64_t* top_ids,
+    void* workspace, int64_t workspace_bytes,
+    hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

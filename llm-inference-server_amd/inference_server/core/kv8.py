@@ -341,6 +341,12 @@ class Kv8Pool(PagedKVPool):
     def block_bytes(self) -> int:
         return self._slab_bytes
 
+    def _slot_tensors(self) -> list[torch.Tensor]:
+        return [t.view(torch.uint8) for layer in self._layers for cache in layer for t in cache]
+
+    def _slot_bytes(self) -> tuple[int, int]:
+        return self.row_bytes // self.block_size, self.dims.num_kv_heads
+
     def _host_shape(self, n: int) -> tuple[tuple[int, ...], torch.dtype]:
         return (2 * self.dims.num_layers, n, self._slab_bytes), torch.uint8
 

@@ -270,6 +270,76 @@ class PagedKVPool:
         )
         native.check(rc, "pkv_copy_blocks")
 
+    # ------------------------------------------------------------ drafted tokens
+    def _slot_tensors(self) -> list[torch.Tensor]:
+        """Tensors [num_blocks, block_size, ...] that hold something of every slot."""
+        return self.k + self.v
+
+    def _slot_bytes(self) -> tuple[int, int]:
+        """Of one slot of one layer's K (or V): bytes of its row, and bytes that a block holds behind
+        its rows, as [..][block_size]."""
+        return self.block_bytes // self.block_size, 0
+
+    def keep_paths(self, block_tables: torch.Tensor, context_lens: torch.Tensor, query_start: torch.Tensor,
+                   paths: torch.Tensor) -> None:
+        """Move the accepted nodes' rows (core/token_tree.py) behind their sequences' cached tokens, in
+        every layer of K and V, in place: the row at position c + paths[i, d] goes to c + d, c =
+        context_lens[i] - (query_start[i + 1] - query_start[i]).
+
+        block_tables [B, W], context_lens [B] (of the step, all nodes among them), query_start
+        [B + 1], paths [B, P] (accept_tree's): int64, on the pool's device. A path ascends; it ends at the
+        first number that is not above the one before, or not of a node. Rows in blocks outside the
+        pool or the table stay. The blocks of a sequence's drafted rows are its own
+        (BlockTable.make_writable)."""
+        if block_tables.dim() != 2:
+            raise ValueError(f"block_tables must be [batch, width], got {tuple(block_tables.shape)}")
+        batch, width = block_tables.shape
+        if context_lens.shape != (batch,) or query_start.shape != (batch + 1,):
+            raise ValueError(f"context_lens and query_start must be [{batch}] and [{batch + 1}] to match block_tables, got "
+                             f"{tuple(context_lens.shape)} and {tuple(query_start.shape)}")
+        if paths.dim() != 2 or paths.shape[0] != batch:
+            raise ValueError(f"paths must be [{batch}, depth], got {tuple(paths.shape)}")
+        hip = self._use_hip()
+        pool = self.k[0] if self.k else None
+        for name, t in (("block_tables", block_tables), ("context_lens", context_lens), ("query_start", query_start),
+                        ("paths", paths)):
+            if t.dtype is not torch.long:
+                raise ValueError(f"{name} must be int64, got {t.dtype}")
+            if pool is not None and t.get_device() != pool.get_device():
+                raise ValueError(f"{name} is on {t.device}, the pool on {pool.device}")
+        if pool is None or batch == 0 or width == 0 or paths.shape[1] == 0 or self.num_blocks == 0:
+            return
+        if not hip:
+            self._keep_torch(block_tables, context_lens, query_start, paths)
+            return
+        with native.on_device(pool.device):
+            if block_tables.stride(1) != 1:
+                block_tables = block_tables.contiguous()
+            context_lens, query_start, paths = (t.contiguous() for t in (context_lens, query_start, paths))
+            rc = native.lib().pkv_keep_paths(
+                self.pointer_table().data_ptr(), 2 * self.dims.num_layers, self.num_blocks, self.block_size,
+                self.block_bytes, *self._slot_bytes(), block_tables.data_ptr(), block_tables.stride(0), width,
+                context_lens.data_ptr(), query_start.data_ptr(), batch, paths.data_ptr(), paths.shape[1],
+                native.stream_handle(pool.device))
+            native.check(rc, "pkv_keep_paths")
+
+    def _keep_torch(self, tables, ctx, starts, paths) -> None:
+        bs, width, depth = self.block_size, tables.shape[1], paths.shape[1]
+        nodes = starts[1:] - starts[:-1]
+        cached = ctx - nodes
+        left = torch.cat([paths.new_full((paths.shape[0], 1), -1), paths[:, :-1]], 1)
+        goes = ((paths > left) & (paths < nodes[:, None]) & (nodes > 0)[:, None] & (cached >= 0)[:, None]).long()
+        d = torch.arange(depth, device=tables.device)
+        source, to = cached[:, None] + paths, (cached[:, None] + d).expand_as(paths)
+        moves = (goes.cumprod(1) > 0) & (paths != d) & (source < width * bs)
+        seq, at = torch.nonzero(moves, as_tuple=True)
+        source, to = source[seq, at], to[seq, at]
+        from_block, to_block = tables[seq, source // bs], tables[seq, to // bs]
+        fine = (from_block >= 0) & (from_block < self.num_blocks) & (to_block >= 0) & (to_block < self.num_blocks)
+        where = [x[fine] for x in (from_block, source % bs, to_block, to % bs)]
+        for t in self._slot_tensors():
+            t[where[2], where[3]] = t[where[0], where[1]]
+
     # ------------------------------------------------------------ swap
     def swap_out(self, blocks: list[int]) -> HostBlocks:
         """Copy the named blocks to host memory; the caller frees them afterwards

@@ -1,4 +1,4 @@
-"""Greedy sampling fused into the LM head (HIP backend).
+"""Greedy sampling fused into the LM head (HIP backend), and log probabilities of tokens.
 
 The reference samples every step with `logits[0, ends - 1, :].argmax(-1)`
 (inference_server/core/paged_executor.py:194-203): the model's LM head writes
@@ -11,15 +11,22 @@ the logits are never materialised.
 fp16 and bf16 only; `fused_greedy_supported` says whether a model's LM head qualifies
 (bias-free Linear over the hidden size, a dtype with a kernel). Callers keep the
 matmul + argmax for everything else, and for more rows than `fused_max_rows` allows.
+
+`token_logprobs` is what a server answers a request for log probabilities with, and what scores
+the nodes of a drafted tree: of given tokens, with ranks, entropies and the likeliest alternatives. The
+reference returns token ids only.
 """
 
 from __future__ import annotations
 
 import threading
+from typing import NamedTuple
 
 import torch
 
 from inference_server import native
+from inference_server.config import CONFIG
+from inference_server.core import attention_hip
 
 _FUSED_DTYPES = (torch.float16, torch.bfloat16)
 
@@ -158,3 +165,94 @@ def lm_head_argmax(hidden: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
         _WORKSPACES.drop(hidden.device, stream)   # its merge state may be incomplete
     native.check(rc, "pkv_lm_head_argmax")
     return ids
+
+
+# ----------------------------------------------------------------------- log probabilities
+#: Most alternatives of a row that token_logprobs returns.
+MAX_TOP = 64
+
+
+class TokenLogprobs(NamedTuple):
+    """On the logits' device."""
+
+    logprobs: torch.Tensor       # fp32 [rows]: log probability of the row's token
+    ranks: torch.Tensor          # int64 [rows]: 1 + the number of larger logits
+    entropy: torch.Tensor        # fp32 [rows], in nats
+    top_logprobs: torch.Tensor   # fp32 [rows, top], largest first
+    top_ids: torch.Tensor        # int64 [rows, top]; equal logits by ascending id
+
+
+def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of token_ids (int64 [rows]) in the softmax of logits [rows, vocab] (fp32,
+    fp16 or bf16, any strides), with their ranks, the rows' entropies and the `top` (64 at most)
+    likeliest tokens of each row.
+
+    Sums are in fp32. A logit of -inf is a token that cannot be, of log probability -inf. A row that
+    holds a NaN or +inf, or nothing but -inf, has no distribution: NaN, rank 0 and ids -1. A token
+    outside the vocabulary (a padding row's -1) has NaN and rank 0. ATTENTION=hip: one launch of
+    libpagedkv (`pkv_token_logprobs`); else tensor ops, on any device."""
+    if logits.dim() != 2:
+        raise ValueError(f"token_logprobs: logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    if token_ids.dim() != 1 or token_ids.shape[0] != rows:
+        raise ValueError(f"token_logprobs: token_ids must be [{rows}], got {tuple(token_ids.shape)}")
+    if token_ids.dtype is not torch.long:
+        raise ValueError(f"token_logprobs: token_ids must be int64, got {token_ids.dtype}")
+    if logits.dtype not in native.DTYPE_CODES:
+        raise ValueError(f"token_logprobs: logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    if token_ids.get_device() != logits.get_device():
+        raise ValueError(f"token_logprobs: token_ids on {token_ids.device}, logits on {logits.device}")
+    if vocab < 1 or not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"token_logprobs: top must be between 0 and {MAX_TOP}, and no more than the vocabulary of "
+                         f"{vocab}; got {top}")
+    if CONFIG.kv_backend != "hip":
+        return _logprobs_torch(logits, token_ids, top)
+    native.require_gpu(logits, "token_logprobs")
+    dev = logits.device
+    with native.on_device(dev):
+        if logits.stride(1) != 1 and vocab > 1:
+            logits = logits.contiguous()
+        token_ids = token_ids.contiguous()
+        # One allocation each of the 8- and 4-byte outputs.
+        longs = torch.empty(rows * (1 + top), dtype=torch.long, device=dev)
+        floats = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev)
+        ranks, top_ids = longs.split_with_sizes((rows, rows * top))
+        logprobs, entropy, top_logprobs = floats.split_with_sizes((rows, rows, rows * top))
+        out = TokenLogprobs(logprobs, ranks, entropy, top_logprobs.view(rows, top), top_ids.view(rows, top))
+        if rows == 0:
+            return out
+        lib, dt, stream = native.lib(), native.DTYPE_CODES[logits.dtype], native.stream_handle(dev)
+        nbytes = lib.pkv_token_logprobs_workspace_bytes(rows, vocab, top, dt)
+        workspaces, ws_ptr = attention_hip._WORKSPACES, None
+        with workspaces.turn(dev, stream) if nbytes else attention_hip._ALONE:
+            if nbytes:
+                # A capture's calls have one of their own, as attention's over the 8-bit cache.
+                capturing = torch.cuda.is_current_stream_capturing()
+                ws_ptr = (workspaces.of_capture if capturing else workspaces.partials)(dev, stream, nbytes).data_ptr()
+            rc = lib.pkv_token_logprobs(
+                logits.data_ptr(), logits.stride(0), rows, vocab, dt, token_ids.data_ptr(), top,
+                logprobs.data_ptr(), ranks.data_ptr(), entropy.data_ptr(), top_logprobs.data_ptr(), top_ids.data_ptr(),
+                ws_ptr, nbytes, stream)
+        native.check(rc, "pkv_token_logprobs")
+    return out
+
+
+def _logprobs_torch(logits, ids, top) -> TokenLogprobs:
+    vocab = logits.shape[1]
+    x = logits.float()
+    asked = (ids >= 0) & (ids < vocab)
+    own = x.gather(1, ids.clamp(0, vocab - 1)[:, None])
+    m = x.amax(1, keepdim=True)                       # keeps NaN
+    proper = torch.isfinite(m)[:, 0]
+    d = x - torch.where(proper[:, None], m, 0.0)
+    e = torch.exp(d)
+    z = e.sum(1, keepdim=True)
+    log_z = torch.log(z)
+    entropy = (log_z - torch.where(e > 0, e * d, 0.0).sum(1, keepdim=True) / z)[:, 0].clamp(min=0)
+    ok = proper & asked
+    values, order = torch.sort(x, dim=1, descending=True, stable=True)
+    nan = float("nan")
+    return TokenLogprobs(
+        torch.where(ok, (own - m - log_z)[:, 0], nan), torch.where(ok, (x > own).sum(1) + 1, 0),
+        torch.where(proper, entropy, nan), torch.where(proper[:, None], values[:, :top] - m - log_z, nan),
+        torch.where(proper[:, None], order[:, :top], -1))

@@ -181,6 +181,54 @@ SIGNATURES: dict[str, tuple] = {
          _ptr, _ptr, _ptr, _ptr, _ptr,     # held_out, slots, positions, query_start_loc, counts
          _ptr],
     ),
+    "pkv_tree_layout": (
+        _int,
+        [_ptr, _ptr, _ptr,                 # parents, query_start_loc, context_lens
+         _i64, _i64, _i64,                 # num_seqs, num_tokens, max_nodes
+         _ptr, _ptr,                       # masks, positions
+         _ptr],
+    ),
+    "pkv_tree_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _int, _ptr, _ptr]),
+    "pkv_tree_attention": (
+        _int,
+        [_ptr, _i64, _i64,                 # out, strides
+         _ptr, _i64, _i64,                 # query, strides
+         _ptr, _ptr, _i64, _i64, _i64,     # k_pool, v_pool, pool strides
+         _i64, _i64, _i64, _i64,           # num_blocks, block_size, num_kv_heads, head_dim
+         _ptr, _i64, _i64,                 # block_tables, table_stride, table_width
+         _ptr, _ptr,                       # context_lens, query_start_loc
+         _ptr, _i64, _i64,                 # masks, mask_stride, mask_words
+         _i64, _i64, _i64, _i64,           # num_seqs, num_heads, num_tokens, max_query_len
+         _ptr, _ptr,                       # host context_lens, host query_lens
+         _f32, _int,                       # scale, dtype
+         _ptr, _i64,                       # workspace, workspace_bytes
+         _ptr],
+    ),
+    "pkv_tree_accept": (
+        _int,
+        [_ptr, _ptr, _ptr, _ptr,           # tokens, parents, targets, query_start_loc
+         _i64, _i64, _i64,                 # num_seqs, num_tokens, max_depth
+         _ptr, _ptr, _ptr,                 # paths, counts, next_tokens
+         _ptr],
+    ),
+    "pkv_keep_paths": (
+        _int,
+        [_ptr, _i64, _i64, _i64,           # tensors, num_tensors, num_blocks, block_size
+         _i64, _i64, _i64,                 # block_bytes, row_bytes, scales
+         _ptr, _i64, _i64,                 # block_tables, table_stride, table_width
+         _ptr, _ptr, _i64,                 # context_lens, query_start_loc, num_seqs
+         _ptr, _i64,                       # paths, max_depth
+         _ptr],
+    ),
+    "pkv_token_logprobs_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "pkv_token_logprobs": (
+        _int,
+        [_ptr, _i64, _i64, _i64, _int,     # logits, stride, num_rows, vocab_size, dtype
+         _ptr, _i64,                       # ids, top
+         _ptr, _ptr, _ptr, _ptr, _ptr,     # logprobs, ranks, entropy, top_logprobs, top_ids
+         _ptr, _i64,                       # workspace, workspace_bytes
+         _ptr],
+    ),
     "pkv_lm_head_argmax_workspace_bytes": (_i64, [_i64, _i64]),
     "pkv_lm_head_argmax": (
         _int,

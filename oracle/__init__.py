@@ -17,6 +17,9 @@ Modules (each function cites the reference file:line it restates):
   greedy.py  greedy sampling over the LM head's logits in the model dtype
              (core/paged_executor.py:194-203), in numpy
 
+  kv8.py     the 8-bit cache by its definition, in 64 bits (no counterpart in the reference)
+  tree.py    drafted token trees and log probabilities by their definitions, in 64 bits (likewise)
+
 How each function is pinned (tests/test_oracle.py): against the reference tests'
 closed forms and known answers — the textbook dense causal attention of
 tests/test_paged_attention.py:30-37 recomputed in float64, the token-map KAT of
