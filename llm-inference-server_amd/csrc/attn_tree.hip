@@ -192,6 +192,98 @@ int launch_generic_t(const TreeParams& p, hipStream_t stream) {
 
 }  // namespace
 
+// How the matrix kernels take a batch: rows a workgroup, and runs that contexts are cut into (splits = 1:
+// none), with the workspace that takes.
+struct TreePlan : SplitPlan {
+    int row_waves;
+};
+
+// The cheapest of a few run lengths in a model of the launch, in us: a workgroup takes kStart before and
+// after its tiles, a tile's time depends on how full the GPU is; once there are more workgroups than slots
+// the last ones start late, half a workgroup's time on average; a split launch adds the merge kernel and
+// its partials' way to memory and back.
+TreePlan tree_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_tokens,
+                   int64_t max_query_len, int dtype, const int64_t* ctx, const int64_t* qlen) {
+    constexpr float kStart = 6.f, kMerge = 4.f, kBytesPerUs = 4.5e6f, kWorth = 0.9f;
+    constexpr int64_t kMaxBytes = 128 << 20;     // of workspace
+    static const int kRuns[] = {2, 3, 4, 5, 6, 8, 10, 12, 14, 17, 20, 24, 28, 34, 40, 48, 56, 68, 80, 96, 112, 136, 160, 192};
+    TreePlan plan = {};
+    plan.splits = 1;
+    plan.split_tiles = 0x7fffffff;
+    const int64_t group = num_heads / num_kv_heads;
+    const int64_t most = (max_query_len && max_query_len < num_tokens ? max_query_len : num_tokens) * group;
+    plan.row_waves = most <= 32 ? 1 : most <= 64 ? 2 : 4;
+    if (!ctx || !qlen || num_seqs > kPrefillSortSeqs) return plan;
+    const int rows_of_wg = 32 * plan.row_waves, keys = plan.row_waves == 1 ? 128 : 64;
+    // Workgroups that the GPU holds, by LDS and by registers; us a tile, alone and in a full GPU.
+    const int64_t lds = 8 * keys * head_dim + 1024;
+    const int64_t slots = 256 * (160 * 1024 / lds < 2 ? 160 * 1024 / lds : 2);
+    const float alone = plan.row_waves == 4 ? 1.4f : 1.2f;
+    const float full = plan.row_waves == 4 ? 2.4f : (float)(slots * 4 * keys * head_dim) / 5.5e6f;
+    auto launch_us = [&](int64_t wgs, int64_t longest, int64_t work) {
+        const float fill = wgs < slots ? (float)wgs / slots : 1.f;
+        const float tile = full > alone ? alone + (full - alone) * fill : alone;
+        const float one = longest * tile + kStart;
+        if (wgs <= slots) return one;
+        const float all = (work * tile + wgs * kStart) / slots + 0.5f * one;
+        return all > one ? all : one;
+    };
+    int64_t wgs = 0, work = 0, longest = 0;
+    auto each = [&](auto f) {
+        for (int64_t i = 0; i < num_seqs; ++i) {
+            if (ctx[i] <= 0 || qlen[i] <= 0) continue;
+            const int64_t c = ctx[i] < (1ll << 36) ? ctx[i] : 1ll << 36;
+            f(ceil_div(c, keys), ceil_div(qlen[i] * group, rows_of_wg) * num_kv_heads, qlen[i] * num_heads);
+        }
+    };
+    each([&](int64_t tiles, int64_t w, int64_t) {
+        wgs += w;
+        work += w * tiles;
+        longest = longest > tiles ? longest : tiles;
+    });
+    const int64_t rows = num_tokens * num_heads;
+    float best = kWorth * launch_us(wgs, longest, work);
+    for (const int64_t run : kRuns) {
+        if (run >= longest) break;
+        const int64_t splits = ceil_div(longest, run);
+        if (kMergeCounterBytes + 3 * 256 + rows * 4 + rows * splits * (head_dim + 2) * 4 > kMaxBytes) continue;
+        int64_t items = 0, top = 0, parts = 0;
+        each([&](int64_t tiles, int64_t w, int64_t r) {
+            const int64_t n = ceil_div(tiles, run), even = ceil_div(tiles, n);
+            items += w * n;
+            top = top > even ? top : even;
+            parts += n > 1 ? r * n : 0;
+        });
+        const float us = launch_us(items, top, work) + kMerge + 2.f * parts * (head_dim + 2) * 4 / kBytesPerUs;
+        if (us >= best) continue;
+        best = us;
+        plan.splits = (int)splits;
+        plan.split_tiles = (int)run;
+        plan.items = items;
+    }
+    if (plan.splits == 1) return plan;
+    auto round256 = [](int64_t b) { return ceil_div(b, 256) * 256; };
+    plan.rows_bytes = round256(rows * 4);
+    plan.ml_bytes = round256(rows * plan.splits * 8);
+    plan.o_bytes = round256(rows * plan.splits * head_dim * 4);
+    return plan;
+}
+
+// Whether the matrix kernels take these parameters.
+bool tree_tiled(const TreeParams& p, int dtype) {
+    if (!prefill_shape(p.block_size, p.head_dim, dtype) || p.num_blocks < 1 || p.ss < 0) return false;
+    // They mask to -inf and take the maximum before they scale.
+    if (!(p.scale > 0.f)) return false;
+    // One grid dimension; keys and rows of a sequence in 32 bits.
+    if (tree_workgroups(p, 32 * p.row_waves) > 0x7fffffff || p.table_width * p.block_size > (1 << 30)) return false;
+    if (((int64_t)p.max_query_len + 128) * p.group > 0x7fffffff) return false;
+    const uint64_t probe = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.k | (uint64_t)(uintptr_t)p.v |
+                           (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * 2) | (uint64_t)(p.q_sh * 2) |
+                           (uint64_t)(p.sb * 2) | (uint64_t)(p.ss * 2) | (uint64_t)(p.sh * 2) |
+                           (uint64_t)(p.out_st * 2) | (uint64_t)(p.out_sh * 2);
+    return probe % 16 == 0;
+}
+
 int launch_tree_generic(const TreeParams& p, int dtype, hipStream_t stream) {
     switch (dtype) {
         case PKV_FLOAT32: return launch_generic_t<float>(p, stream);
@@ -208,7 +300,12 @@ extern "C" int64_t pkv_tree_attention_workspace_bytes(int64_t num_seqs, int64_t 
                                                       int64_t head_dim, int64_t num_tokens, int64_t max_query_len,
                                                       int dtype, const int64_t* host_context_lens,
                                                       const int64_t* host_query_lens) {
-    return 0;
+    if (num_seqs <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_tokens <= 0 ||
+        num_seqs > 0x7fffffff || num_tokens > 0x7fffffff || num_heads > 65535 || num_heads % num_kv_heads)
+        return 0;
+    const TreePlan plan = tree_plan(num_seqs, num_heads, num_kv_heads, head_dim, num_tokens, max_query_len, dtype,
+                                    host_context_lens, host_query_lens);
+    return plan.splits > 1 ? kMergeCounterBytes + plan.total() : 0;
 }
 
 extern "C" int pkv_tree_attention(
@@ -270,5 +367,19 @@ extern "C" int pkv_tree_attention(
     p.scale_log2 = scale * kLog2e;
     p.splits = 1;
     p.split_tiles = 0x7fffffff;
-    return launch_tree_generic(p, dtype, stream);
+    const TreePlan plan = tree_plan(num_seqs, num_heads, num_kv_heads, head_dim, num_tokens, p.max_query_len, dtype,
+                                    host_context_lens, host_query_lens);
+    p.row_waves = plan.row_waves;
+    if (!tree_tiled(p, dtype)) return launch_tree_generic(p, dtype, stream);
+    if (plan.splits > 1 && workspace && workspace_bytes >= kMergeCounterBytes + plan.total()) {
+        // Behind the decode calls' counters, which stay zero.
+        char* ws = reinterpret_cast<char*>(workspace) + kMergeCounterBytes;
+        p.splits = plan.splits;
+        p.split_tiles = plan.split_tiles;
+        p.split_items = plan.items;
+        p.ws_rows = reinterpret_cast<int*>(ws);
+        p.ws_ml = reinterpret_cast<float*>(ws + plan.rows_bytes);
+        p.ws_o = reinterpret_cast<float*>(ws + plan.rows_bytes + plan.ml_bytes);
+    }
+    return dtype == PKV_FLOAT16 ? launch_tree_mfma<_Float16>(p, stream) : launch_tree_mfma<bf16_t>(p, stream);
 }

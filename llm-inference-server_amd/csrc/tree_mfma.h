@@ -1,0 +1,542 @@
+// Attention of drafted token trees on MFMA (gfx950), fp16 / bf16: the kernel, instantiated by type in
+// attn_tree_*.hip. Head_dim a multiple of 16 from 32 to 128, any GQA group, block sizes that are powers
+// of two from 8 up, softmax scale > 0.
+//
+// The formulation is the prefill kernel's (attn_prefill.hip): rows are (token, query head) pairs of a
+// sequence and KV head; S^T = K Q^T and O^T += V^T P^T on 32x32x16, so that a lane owns one row, its
+// softmax is lane-local but for one swap, and P^T feeds the second product from the accumulator; K/V
+// tiles go HBM -> LDS by DMA, double buffered. What differs:
+//
+//  * Few rows. A tree has some dozens of rows at most a KV head, where a prompt fills the 128 of a
+//    workgroup, and the kernel is bound by the K/V stream. RW of the workgroup's four waves have 32 rows
+//    each, and 4 / RW waves share the keys of a tile: with RW = 1 each has 32 keys of 128, with
+//    RW = 2 32 of 64, with RW = 4 all 64. Waves of the same rows merge through LDS at the end.
+//  * Masks. All rows see all cached keys, so only the tiles that reach past them are masked, by a 32-bit
+//    window of the row's mask words.
+//  * What is not seen must not reach a row, and 0 * NaN would: in those tiles V's elements that are not finite
+//    are taken out of LDS (zeros), as are rows past the last key. A wave that took some out, or whose
+//    output turned NaN under finite weights (0 * infinity, or an infinity times two pieces of opposite
+//    signs), walks its keys once more at the end and puts into each row's dims what it sees of them.
+//
+// Weights enter the second product as two pieces of the type (16 bits of them at least: one alone is
+// off by up to 2^-9 of a weight in bf16, as much as the output's rounding).
+#pragma once
+
+#include <type_traits>
+
+#include "prefill_common.h"
+#include "tree.h"
+
+namespace pkv {
+namespace {
+
+__device__ __forceinline__ uint32_t lds_u32(const void* p) {
+    return (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) char*)p);
+}
+// 16 bytes per lane by LDS DMA to LDS address lds + 16 lane (M0 = lds), from the uniform base sbase plus
+// the lane's 32-bit offset, or from the lane's own 64-bit address; inline asm, hidden from the
+// compiler's wait counting, which would wait for it before every LDS read. M0 is reserved to the
+// compiler (a clobber of it is not honoured): all LDS DMAs of these kernels go through these helpers.
+__device__ __forceinline__ void dma16(const char* sbase, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(voff), "s"(sbase)
+                 : "memory");
+}
+__device__ __forceinline__ void dma16(const char* addr, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds), "v"(addr)
+                 : "memory");
+}
+
+template <typename T>
+struct Bits16;                       // exponent bits: all set in infinities and NaN
+template <>
+struct Bits16<_Float16> {
+    static constexpr uint32_t kExp = 0x7c00u;
+};
+template <>
+struct Bits16<bf16_t> {
+    static constexpr uint32_t kExp = 0x7f80u;
+};
+// The word's elements that are finite, the others as zeros.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_of(uint32_t w) {
+    constexpr uint32_t E = Bits16<T>::kExp;
+    const uint32_t lo = (w & E) == E ? 0u : 0xffffu, hi = (w >> 16 & E) == E ? 0u : 0xffff0000u;
+    return w & (lo | hi);
+}
+
+// Keys of a tile.
+template <int RW>
+constexpr int kTreeTile = RW == 1 ? 128 : 64;
+
+// Waves a SIMD: LDS leaves room for one workgroup a CU with long rows in tiles of 128 keys, else two.
+template <int D, int RW>
+constexpr int kTreeWaves = RW == 1 && D > 64 ? 1 : 2;
+
+template <typename T, int D, int RW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<D, RW>))) void tree_mfma_kernel(const TreeParams p) {
+    static_assert(D % 16 == 0 && D >= 32 && D <= 128, "head_dim");
+    constexpr int KW = 4 / RW;                // waves that share a tile's keys
+    constexpr int KT = kTreeTile<RW>;
+    constexpr int NH = KT / 32 / KW;          // 32-key halves of a wave and tile
+    constexpr int ROWS = 32 * RW;
+    constexpr int DSTEPS = D / 16;            // S^T contraction steps
+    constexpr int DTILES = (D + 31) / 32;     // O^T tiles of 32 dims (the last may be half a tile)
+    constexpr int ROWB = D * 2;               // bytes of a K/V row
+    constexpr int CPR = ROWB / 16;            // its 16-byte chunks
+    constexpr int G16 = KT / 64;              // groups of 16 keys that a wave stages
+    constexpr int IPB = (16 * CPR + 63) / 64; // DMA instructions of a group, of K or V
+    constexpr bool kWholeDma = 16 * CPR % 64 == 0;
+    constexpr bool kHalfDma = 64 % CPR == 0 && 64 / CPR <= 8;   // rows of one all in an 8-row half
+
+    __shared__ __attribute__((aligned(1024))) uint16_t s_all[4 * KT * D];     // K, V, K, V
+    __shared__ int s_taken;                   // whether V held what is not finite behind the cached keys
+    __shared__ float2 s_ml[4][32];
+
+    PrefillItem it;
+    if (!prefill_item<ROWS, KT>(p, p.block_size, it)) return;
+    const uint32_t G = (uint32_t)p.group;
+    const int kvh = it.kvh, split = it.split, seq = it.seq;
+    const int64_t q_first = it.q_first;
+    const int q_len = it.q_len;
+    const int kmax = it.ctx < 0 || p.num_blocks < 1 ? 0 : it.ctx;             // keys that there are
+    const int n_rows = q_len * (int)G;
+    const int row0 = it.row_tile * ROWS;
+    const int pos0 = it.ctx - q_len;          // first drafted key
+    const int rows = n_rows - row0 < ROWS ? n_rows - row0 : ROWS;
+    const int n_tiles = (kmax + KT - 1) / KT;
+    // A sequence without cached keys is not cut: a row of it may see nothing, which the merge cannot tell.
+    int t_begin = 0, t_end = n_tiles, run = n_tiles;
+    if (it.splits > 1 && n_tiles > 0 && pos0 > 0) {
+        run = split_run(n_tiles, it.splits, p.split_tiles);
+        t_begin = split * run;
+        t_end = n_tiles - t_begin < run ? n_tiles : t_begin + run;
+    }
+    // A later split of a sequence that ends before it; without keys the first one writes zeros.
+    if (split > 0 && (t_begin >= n_tiles || run == n_tiles)) return;
+
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int rw = wave / KW, kw = wave % KW;
+    const int h = lane >> 5, col = lane & 31;
+    const int wrow = rw * 32 + col;
+    const bool my_live = wrow < rows;         // rows past the last one repeat it, not stored
+    const uint32_t my_row = (uint32_t)(row0 + (my_live ? wrow : rows - 1));
+    const int my_q = (int)(my_row / G);
+    const int my_head = kvh * (int)G + (int)(my_row - (uint32_t)my_q * G);
+    const bool has_rows = rw * 32 < rows;     // else the wave only stages
+
+    f32x16 o[DTILES];
+#pragma unroll
+    for (int t = 0; t < DTILES; ++t) o[t] = f32x16{};
+    float m_run = kNegInf, l_run = 0.f;
+
+    const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
+    const char* kbase = reinterpret_cast<const char*>(p.k) + (int64_t)kvh * p.sh * (int64_t)sizeof(T);
+    const char* vbase = reinterpret_cast<const char*>(p.v) + (int64_t)kvh * p.sh * (int64_t)sizeof(T);
+    const int64_t block_bytes = p.sb * (int64_t)sizeof(T);
+    const int64_t slot_bytes = p.ss * (int64_t)sizeof(T);
+
+    // ---- staging, as in the prefill kernel: lane l holds the block id of the tile's 8-key group l %
+    // (KT / 8), the index clamped to the last block with a key.
+    const int nb_last = (kmax - 1) >> p.block_shift;
+    auto tile_ids = [&](int kt) -> int64_t {
+        const int b = (kt * KT + 8 * (lane & (KT / 8 - 1))) >> p.block_shift;
+        return table[b < nb_last ? b : nb_last];
+    };
+    auto dma_row = [&](int j) { return (64 * j + lane) / CPR; };
+    auto dma_chunk = [&](int j) { return (64 * j + lane) % CPR ^ lds_swizzle<D>((64 * j + lane) / CPR); };
+    uint32_t lane_off[IPB];
+#pragma unroll
+    for (int j = 0; j < IPB; ++j)
+        lane_off[j] = (uint32_t)((dma_row(j) & 7) * slot_bytes) + (uint32_t)(dma_chunk(j) * 16);
+    const bool offs_fit = 8 * slot_bytes + ROWB <= (int64_t)0xffffffff;
+    auto dma_tile = [&](int kt, int64_t ids, uint16_t* sk, uint16_t* sv) {
+#pragma unroll
+        for (int g = 0; g < G16; ++g) {
+            const int at = wave * G16 + g;                       // the group in the tile
+            const int first = kt * KT + 16 * at;                 // its first key
+            const int64_t id0 = readlane64(ids, 2 * at), id1 = readlane64(ids, 2 * at + 1);
+            const int64_t half0 = id0 * block_bytes + (first & (p.block_size - 1)) * slot_bytes;
+            const int64_t half1 = id1 * block_bytes + ((first + 8) & (p.block_size - 1)) * slot_bytes;
+            const bool ok = ((uint64_t)id0 < (uint64_t)p.num_blocks) & ((uint64_t)id1 < (uint64_t)p.num_blocks);
+            char* dk = reinterpret_cast<char*>(sk) + 16 * at * ROWB;
+            char* dv = reinterpret_cast<char*>(sv) + 16 * at * ROWB;
+            if (ok & offs_fit & (first + 16 <= kmax)) {
+#pragma unroll
+                for (int j = 0; j < IPB; ++j) {
+                    if constexpr (kHalfDma) {
+                        const int64_t half = 64 * j / CPR < 8 ? half0 : half1;
+                        dma16(kbase + half, lane_off[j], lds_u32(dk + j * 1024));
+                        dma16(vbase + half, lane_off[j], lds_u32(dv + j * 1024));
+                    } else if (kWholeDma || 64 * j + lane < 16 * CPR) {
+                        const int64_t off = (dma_row(j) < 8 ? half0 : half1) + lane_off[j];
+                        dma16(kbase + off, lds_u32(dk + j * 1024));
+                        dma16(vbase + off, lds_u32(dv + j * 1024));
+                    }
+                }
+                continue;
+            }
+            // Rows past the last key (masked, their V zeroed below) and those of blocks outside the pool are
+            // read from the pool's first row.
+#pragma unroll
+            for (int j = 0; j < IPB; ++j) {
+                const int r = dma_row(j);
+                const int64_t id = r < 8 ? id0 : id1;
+                int64_t off = (int64_t)(dma_chunk(j) * 16);
+                if ((uint64_t)id < (uint64_t)p.num_blocks && first + r < kmax)
+                    off += (r < 8 ? half0 : half1) + (int64_t)(r & 7) * slot_bytes;
+                if (kWholeDma || 64 * j + lane < 16 * CPR) {
+                    dma16(kbase + off, lds_u32(dk + j * 1024));
+                    dma16(vbase + off, lds_u32(dv + j * 1024));
+                }
+            }
+        }
+    };
+
+    // ---- LDS operands of this lane (as in the prefill kernel).
+    const int grp = lane >> 4;
+    const int tr_key = (lane & 15) >> 2;
+    const int tr_col = 16 * (grp & 1) + 4 * (lane & 3);
+    const int k_swz = lds_swizzle<D>(col);
+    const int v_cb = tr_col >> 3;
+    const int v_lo_swz = lds_swizzle<D>(4 * (grp >> 1) + tr_key);
+    const int v_hi_swz = lds_swizzle<D>(4 * (grp >> 1) + tr_key + 8);
+    const int v_byte = 8 * (lane & 1);
+    const uint32_t wave_off = (uint32_t)(kw * NH * 32 * ROWB);   // of the wave's keys
+    uint32_t koff[DSTEPS], voff_lo[DTILES], voff_hi[DTILES];
+#pragma unroll
+    for (int s = 0; s < DSTEPS; ++s) {
+        koff[s] = wave_off + (uint32_t)(col * ROWB + (((2 * s + h) ^ k_swz) << 4));
+        asm volatile("" : "+v"(koff[s]));
+    }
+#pragma unroll
+    for (int t = 0; t < DTILES; ++t) {
+        // Columns past head_dim re-read the tile's first chunks: output rows never stored.
+        const int c = 4 * t + v_cb < CPR ? 4 * t + v_cb : 4 * t + (v_cb & 1);
+        voff_lo[t] = wave_off + (uint32_t)((4 * (grp >> 1) + tr_key) * ROWB + v_byte + ((c ^ v_lo_swz) << 4));
+        voff_hi[t] = wave_off + (uint32_t)((4 * (grp >> 1) + tr_key + 8) * ROWB + v_byte + ((c ^ v_hi_swz) << 4));
+        asm volatile("" : "+v"(voff_lo[t]), "+v"(voff_hi[t]));
+    }
+
+    int64_t ids = 0;
+    if (t_begin < t_end) ids = tile_ids(t_begin);
+    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7].
+    u32x4 qfrag[DSTEPS];
+    {
+        const char* qrow = reinterpret_cast<const char*>(p.q) +
+                           ((q_first + my_q) * p.q_st + (int64_t)my_head * p.q_sh) * (int64_t)sizeof(T);
+#pragma unroll
+        for (int s = 0; s < DSTEPS; ++s) {
+            const Vec16 v = load16(qrow + (s * 16 + h * 8) * (int)sizeof(T));
+            qfrag[s] = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+        }
+    }
+    if (threadIdx.x == 0) s_taken = 0;
+
+    // Of the 32 keys from key0 on, those that the lane's row sees.
+    const uint64_t* mask = p.masks + (q_first + my_q) * p.mask_stride;
+    auto window = [&](int key0) -> uint32_t {
+        const int node = key0 - pos0, left = kmax - key0;
+        auto word = [&](int i) { return i < p.mask_words ? mask[i] : 0ull; };
+        uint32_t w = ~0u;
+        if (node >= 0) {
+            const int sh = node & 63;
+            const uint64_t lo = word(node >> 6) >> sh;
+            w = (uint32_t)(sh > 32 ? lo | word((node >> 6) + 1) << (64 - sh) : lo);
+        } else if (node > -32) {
+            w = (uint32_t)(word(0) << -node) | ((1u << -node) - 1);
+        }
+        return left >= 32 ? w : left <= 0 ? 0u : w & ((1u << left) - 1);
+    };
+
+    auto tile = [&](auto tail, int kt, uint16_t* tile_k, uint16_t* tile_v, uint16_t* nk, uint16_t* nv) {
+        constexpr bool drafted = decltype(tail)::value;          // keys past the cached ones among the tile's
+        __builtin_amdgcn_s_waitcnt(0);
+        lds_barrier();                        // tile kt is staged, tile kt - 1 is done with
+        f32x16 st[NH];
+        __builtin_amdgcn_s_setprio(1);
+        if (has_rows) {
+            u32x4 kf[NH][DSTEPS];
+#pragma unroll
+            for (int i = 0; i < NH; ++i)
+#pragma unroll
+                for (int s = 0; s < DSTEPS; ++s) {
+                    const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tile_k) + i * 32 * ROWB + koff[s]);
+                    kf[i][s] = u32x4{a.x, a.y, a.z, a.w};
+                }
+#pragma unroll
+            for (int i = 0; i < NH; ++i) st[i] = f32x16{};
+#pragma unroll
+            for (int s = 0; s < DSTEPS; ++s)
+#pragma unroll
+                for (int i = 0; i < NH; ++i) st[i] = Mfma<T>::run(kf[i][s], qfrag[s], st[i]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if (kt + 1 < t_end) {
+            dma_tile(kt + 1, ids, nk, nv);
+            ids = tile_ids(kt + 2);
+        }
+        if constexpr (drafted) {
+            // V of keys past the last one, and elements that are not finite: out. (Cached keys are seen
+            // by all rows.)
+            for (int c = (int)threadIdx.x; c < KT * CPR; c += 256) {
+                const int r = c / CPR, key = kt * KT + r;
+                if (key < pos0) continue;
+                uint4* at = reinterpret_cast<uint4*>(tile_v) + c;
+                const uint4 v = *at;
+                const uint4 f = key < kmax ? make_uint4(finite_of<T>(v.x), finite_of<T>(v.y), finite_of<T>(v.z), finite_of<T>(v.w))
+                                           : make_uint4(0, 0, 0, 0);
+                if (f.x == v.x && f.y == v.y && f.z == v.z && f.w == v.w) continue;
+                *at = f;
+                if (key < kmax) s_taken = 1;
+            }
+            lds_barrier();
+        }
+        if (!has_rows) return;
+        if constexpr (drafted) {
+#pragma unroll
+            for (int i = 0; i < NH; ++i) {
+                const uint32_t mine = window(kt * KT + (kw * NH + i) * 32) >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!(mine >> (8 * (r >> 2) + (r & 3)) & 1)) st[i][r] = kNegInf;
+            }
+        }
+        float mt = kNegInf;
+#pragma unroll
+        for (int i = 0; i < NH; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[i][r]);
+        mt = max_across32(mt) * p.scale_log2;   // scale > 0: max commutes with it
+        asm("" : "+v"(mt));                     // stays rounded: m_run - mt below is not contracted into an fma
+        const bool raise = mt > m_run + kRescaleThreshold;
+        const float m_new = raise ? mt : m_run;
+        const float alpha = raise ? fast_exp2(m_run - mt) : 1.f;
+        if (__builtin_amdgcn_ballot_w64(raise)) {
+#pragma unroll
+            for (int t = 0; t < DTILES; ++t) o[t] *= alpha;
+        }
+        m_run = m_new;
+        const float m_off = m_new == kNegInf ? 0.f : m_new;
+        float psum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NH; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = fast_exp2(fmaf(st[i][r], p.scale_log2, -m_off));
+                st[i][r] = e;
+                psum += e;
+            }
+        psum = sum_across32(psum);
+        l_run = l_run * alpha + psum;
+#pragma unroll
+        for (int s = 0; s < 2 * NH; ++s) {
+            f32x16& sv = st[s >> 1];
+            const int r0 = 8 * (s & 1);
+            u32x4 pb[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = sv[r0 + 2 * e], y = sv[r0 + 2 * e + 1];
+                const uint32_t w = Mfma<T>::pack(x, y);
+                pb[0][e] = w;
+                pb[1][e] = Mfma<T>::pack(x - Pair<T>::lo(w), y - Pair<T>::hi(w));
+            }
+            const char* vgrp = reinterpret_cast<const char*>(tile_v) + ((s >> 1) * 32 + 16 * (s & 1)) * ROWB;
+#pragma unroll
+            for (int t = 0; t < DTILES; ++t) {
+                const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_lo[t]));
+                const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_hi[t]));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) o[t] = Mfma<T>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
+            }
+        }
+    };
+
+    uint16_t* const k0 = s_all;
+    uint16_t* const v0 = s_all + KT * D;
+    uint16_t* const k1 = s_all + 2 * KT * D;
+    uint16_t* const v1 = s_all + 3 * KT * D;
+    if (t_begin < t_end) {
+        // (Tile t is in the buffers of t's parity.)
+        if (t_begin & 1) dma_tile(t_begin, ids, k1, v1);
+        else dma_tile(t_begin, ids, k0, v0);
+        ids = tile_ids(t_begin + 1);
+    }
+    const int t_cached = pos0 / KT < t_end ? pos0 / KT : t_end;  // tiles of cached keys alone (pos0 >= 0 if it is cut)
+    int kt = t_begin;
+    if (kt < t_cached && (kt & 1)) {
+        tile(std::false_type{}, kt, k1, v1, k0, v0);
+        ++kt;
+    }
+    for (; kt + 1 < t_cached; kt += 2) {
+        tile(std::false_type{}, kt, k0, v0, k1, v1);
+        tile(std::false_type{}, kt + 1, k1, v1, k0, v0);
+    }
+    for (; kt < t_end; ++kt) {
+        uint16_t* const k = kt & 1 ? k1 : k0;
+        uint16_t* const nk = kt & 1 ? k0 : k1;
+        tile(std::true_type{}, kt, k, k + KT * D, nk, nk + KT * D);
+    }
+
+    // ---- what is not finite in V, for the rows that see it.
+    constexpr int UNITS = D / 8;              // of the output: dims 8 u .. + 7, four of each half
+    if (has_rows && t_begin < t_end) {
+        float any = 0.f;                      // NaN if some output is
+#pragma unroll
+        for (int t = 0; t < DTILES; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (32 * t + 8 * (r >> 2) < D) any += o[t][r] * 0.f;
+        if (s_taken || __builtin_amdgcn_ballot_w64(any != any && l_run == l_run)) {
+            float4 extra[UNITS];
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) extra[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int at = t_begin; at < t_end; ++at)
+                for (int k = 0; k < 32 * NH; ++k) {
+                    const int first = at * KT + kw * NH * 32 + (k & ~31), key = first + (k & 31);
+                    if (key >= kmax) break;
+                    const int64_t id = table[key >> p.block_shift];
+                    const bool sees = key < pos0 || (window(first) >> (k & 31) & 1);
+                    if ((uint64_t)id >= (uint64_t)p.num_blocks || !sees) continue;
+                    const char* row = vbase + id * block_bytes + (key & (p.block_size - 1)) * slot_bytes + 8 * h;
+#pragma unroll
+                    for (int u = 0; u < UNITS; ++u) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(row + 16 * u);
+                        const uint2 rest = make_uint2(v.x ^ finite_of<T>(v.x), v.y ^ finite_of<T>(v.y));
+                        extra[u].x += Pair<T>::lo(rest.x);
+                        extra[u].y += Pair<T>::hi(rest.x);
+                        extra[u].z += Pair<T>::lo(rest.y);
+                        extra[u].w += Pair<T>::hi(rest.y);
+                    }
+                }
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                auto put = [&](int r, float x) {
+                    if (x != 0.f) o[u / 4][4 * (u % 4) + r] = x;
+                };
+                put(0, extra[u].x);
+                put(1, extra[u].y);
+                put(2, extra[u].z);
+                put(3, extra[u].w);
+            }
+        }
+    }
+
+    // ---- the waves of the same rows: unit u of the output is summed by wave u % KW of them.
+    float inv, m_all = m_run, l_all = l_run, f_own = 1.f;
+    if constexpr (KW > 1) {
+        if (h == 0) s_ml[wave][col] = make_float2(m_run, l_run);
+        lds_barrier();                        // the tiles are done with
+        float* so = reinterpret_cast<float*>(s_all);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+            if (u % KW != kw)
+                *reinterpret_cast<float4*>(so + ((wave * UNITS + u) * 64 + lane) * 4) =
+                    make_float4(o[u / 4][4 * (u % 4)], o[u / 4][4 * (u % 4) + 1], o[u / 4][4 * (u % 4) + 2], o[u / 4][4 * (u % 4) + 3]);
+        lds_barrier();
+        float2 ml[KW];
+        m_all = kNegInf;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            ml[w] = s_ml[rw * KW + w][col];
+            m_all = fmaxf(m_all, ml[w].x);
+        }
+        const float m_off = m_all == kNegInf ? 0.f : m_all;
+        float f[KW];
+        l_all = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            f[w] = fast_exp2(ml[w].x - m_off);
+            l_all += f[w] * ml[w].y;
+        }
+        f_own = fast_exp2(m_run - m_off);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            if (u % KW != kw) continue;
+            float4 x = make_float4(o[u / 4][4 * (u % 4)] * f_own, o[u / 4][4 * (u % 4) + 1] * f_own,
+                                   o[u / 4][4 * (u % 4) + 2] * f_own, o[u / 4][4 * (u % 4) + 3] * f_own);
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                if (w == kw) continue;
+                const float4 y = *reinterpret_cast<const float4*>(so + (((rw * KW + w) * UNITS + u) * 64 + lane) * 4);
+                x.x += y.x * f[w];
+                x.y += y.y * f[w];
+                x.z += y.z * f[w];
+                x.w += y.w * f[w];
+            }
+            o[u / 4][4 * (u % 4)] = x.x;
+            o[u / 4][4 * (u % 4) + 1] = x.y;
+            o[u / 4][4 * (u % 4) + 2] = x.z;
+            o[u / 4][4 * (u % 4) + 3] = x.w;
+        }
+    }
+    if (!my_live) return;
+    const int64_t tok = q_first + my_q;
+    if (run < n_tiles) {
+        // One of several splits: this row's partial, unnormalised. (The merge skips a part whose maximum
+        // is -inf; one whose scores were all NaN has to count.)
+        const int64_t row = tok * p.num_heads + my_head;
+        const int64_t slot = row * p.splits + split;
+        float* po = p.ws_o + slot * D + 4 * h;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+            if (u % KW == kw)
+                *reinterpret_cast<float4*>(po + 8 * u) =
+                    make_float4(o[u / 4][4 * (u % 4)], o[u / 4][4 * (u % 4) + 1], o[u / 4][4 * (u % 4) + 2], o[u / 4][4 * (u % 4) + 3]);
+        if (h == 0 && kw == 0) {
+            *reinterpret_cast<float2*>(p.ws_ml + slot * 2) =
+                make_float2(m_all == kNegInf && l_all != 0.f ? 0.f : m_all, l_all);
+            if (split == 0) p.ws_rows[row] = (n_tiles + run - 1) / run;
+        }
+        return;
+    }
+    if (p.ws_rows && h == 0 && kw == 0) p.ws_rows[tok * p.num_heads + my_head] = 0;    // finished here
+    inv = l_all == 0.f ? 0.f : 1.f / l_all;                                            // no key: zero
+    T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)my_head * p.out_sh + 4 * h;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u)
+        if (u % KW == kw)
+            *reinterpret_cast<uint2*>(orow + 8 * u) =
+                make_uint2(Mfma<T>::pack(o[u / 4][4 * (u % 4)] * inv, o[u / 4][4 * (u % 4) + 1] * inv),
+                           Mfma<T>::pack(o[u / 4][4 * (u % 4) + 2] * inv, o[u / 4][4 * (u % 4) + 3] * inv));
+}
+
+template <typename T, int D, int RW>
+int launch_tree_rows(const TreeParams& p, hipStream_t stream) {
+    tree_mfma_kernel<T, D, RW><<<dim3((unsigned)tree_workgroups(p, 32 * RW)), 256, 0, stream>>>(p);
+    const int rc = check_launch("tree attention");
+    if (rc || p.splits == 1) return rc;
+    const int64_t rows = p.num_tokens * p.num_heads;
+    prefill_merge_kernel<T, D><<<dim3((unsigned)ceil_div(rows, kMergeRows<D>)), 256, 0, stream>>>(p);
+    return check_launch("tree attention, merge");
+}
+
+template <typename T, int D>
+int launch_tree_d(const TreeParams& p, hipStream_t stream) {
+    switch (p.row_waves) {
+        case 1: return launch_tree_rows<T, D, 1>(p, stream);
+        case 2: return launch_tree_rows<T, D, 2>(p, stream);
+        default: return launch_tree_rows<T, D, 4>(p, stream);
+    }
+}
+
+}  // namespace
+
+template <typename T>
+int launch_tree_mfma(const TreeParams& p, hipStream_t stream) {
+    switch (p.head_dim) {
+        case 32: return launch_tree_d<T, 32>(p, stream);
+        case 48: return launch_tree_d<T, 48>(p, stream);
+        case 64: return launch_tree_d<T, 64>(p, stream);
+        case 80: return launch_tree_d<T, 80>(p, stream);
+        case 96: return launch_tree_d<T, 96>(p, stream);
+        case 112: return launch_tree_d<T, 112>(p, stream);
+        default: return launch_tree_d<T, 128>(p, stream);
+    }
+}
+
+}  // namespace pkv
