@@ -212,14 +212,20 @@ TreePlan tree_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, in
     plan.split_tiles = 0x7fffffff;
     const int64_t group = num_heads / num_kv_heads;
     const int64_t most = (max_query_len && max_query_len < num_tokens ? max_query_len : num_tokens) * group;
-    plan.row_waves = most <= 32 ? 1 : most <= 64 ? 2 : 4;
+    const bool f32 = dtype == PKV_FLOAT32;
+    // (fp32 rows above 64 dims: 128 keys do not fit LDS twice.)
+    plan.row_waves = most <= 32 && (!f32 || head_dim <= 64) ? 1 : most <= 64 ? 2 : 4;
     if (!ctx || !qlen || num_seqs > kPrefillSortSeqs) return plan;
     const int rows_of_wg = 32 * plan.row_waves, keys = plan.row_waves == 1 ? 128 : 64;
     // Workgroups that the GPU holds, by LDS and by registers; us a tile, alone and in a full GPU.
-    const int64_t lds = 8 * keys * head_dim + 1024;
-    const int64_t slots = 256 * (160 * 1024 / lds < 2 ? 160 * 1024 / lds : 2);
-    const float alone = plan.row_waves == 4 ? 1.4f : 1.2f;
-    const float full = plan.row_waves == 4 ? 2.4f : (float)(slots * 4 * keys * head_dim) / 5.5e6f;
+    const int64_t lds = (f32 ? 16 : 8) * keys * head_dim;
+    const int64_t slots = 256 * (lds <= 72 * 1024 ? 2 : 1);
+    float alone = plan.row_waves == 4 ? 1.4f : 1.2f;
+    float full = plan.row_waves == 4 ? 2.4f : (float)(slots * lds / 2) / 5.5e6f;
+    if (f32) {
+        alone = (plan.row_waves == 4 ? 0.055f : 0.028f) * head_dim;
+        full = full > 2 * alone ? full : alone * (slots / 256);
+    }
     auto launch_us = [&](int64_t wgs, int64_t longest, int64_t work) {
         const float fill = wgs < slots ? (float)wgs / slots : 1.f;
         const float tile = full > alone ? alone + (full - alone) * fill : alone;
@@ -271,16 +277,17 @@ TreePlan tree_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, in
 
 // Whether the matrix kernels take these parameters.
 bool tree_tiled(const TreeParams& p, int dtype) {
-    if (!prefill_shape(p.block_size, p.head_dim, dtype) || p.num_blocks < 1 || p.ss < 0) return false;
+    const int64_t isz = dtype == PKV_FLOAT32 ? 4 : 2;
+    if (!prefill_shape(p.block_size, p.head_dim, PKV_FLOAT16) || p.num_blocks < 1 || p.ss < 0) return false;
     // They mask to -inf and take the maximum before they scale.
     if (!(p.scale > 0.f)) return false;
     // One grid dimension; keys and rows of a sequence in 32 bits.
     if (tree_workgroups(p, 32 * p.row_waves) > 0x7fffffff || p.table_width * p.block_size > (1 << 30)) return false;
     if (((int64_t)p.max_query_len + 128) * p.group > 0x7fffffff) return false;
     const uint64_t probe = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.k | (uint64_t)(uintptr_t)p.v |
-                           (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * 2) | (uint64_t)(p.q_sh * 2) |
-                           (uint64_t)(p.sb * 2) | (uint64_t)(p.ss * 2) | (uint64_t)(p.sh * 2) |
-                           (uint64_t)(p.out_st * 2) | (uint64_t)(p.out_sh * 2);
+                           (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * isz) | (uint64_t)(p.q_sh * isz) |
+                           (uint64_t)(p.sb * isz) | (uint64_t)(p.ss * isz) | (uint64_t)(p.sh * isz) |
+                           (uint64_t)(p.out_st * isz) | (uint64_t)(p.out_sh * isz);
     return probe % 16 == 0;
 }
 
@@ -381,5 +388,9 @@ extern "C" int pkv_tree_attention(
         p.ws_ml = reinterpret_cast<float*>(ws + plan.rows_bytes);
         p.ws_o = reinterpret_cast<float*>(ws + plan.rows_bytes + plan.ml_bytes);
     }
-    return dtype == PKV_FLOAT16 ? launch_tree_mfma<_Float16>(p, stream) : launch_tree_mfma<bf16_t>(p, stream);
+    switch (dtype) {
+        case PKV_FLOAT32: return launch_tree_mfma<float>(p, stream);
+        case PKV_FLOAT16: return launch_tree_mfma<_Float16>(p, stream);
+        default: return launch_tree_mfma<bf16_t>(p, stream);
+    }
 }

@@ -25,7 +25,7 @@ inline int64_t tree_workgroups(const TreeParams& p, int rows) {
     return ceil_div(items, 8) * 8;
 }
 
-// fp16 / bf16 (tree_mfma.h), for the shapes of tree_mfma_applies.
+// The matrix kernels (tree_mfma.h).
 template <typename T>
 int launch_tree_mfma(const TreeParams& p, hipStream_t stream);
 

@@ -1,5 +1,5 @@
-// Attention of drafted token trees on MFMA (gfx950), fp16 / bf16: the kernel, instantiated by type in
-// attn_tree_*.hip. Head_dim a multiple of 16 from 32 to 128, any GQA group, block sizes that are powers
+// Attention of drafted token trees on MFMA (gfx950): the kernel, instantiated by type in
+// attn_tree_*.hip. fp16, bf16 and fp32 pools, head_dim a multiple of 16 from 32 to 128, any GQA group, block sizes that are powers
 // of two from 8 up, softmax scale > 0.
 //
 // The formulation is the prefill kernel's (attn_prefill.hip): rows are (token, query head) pairs of a
@@ -18,8 +18,11 @@
 //    output turned NaN under finite weights (0 * infinity, or an infinity times two pieces of opposite
 //    signs), walks its keys once more at the end and puts into each row's dims what it sees of them.
 //
-// Weights enter the second product as two pieces of the type (16 bits of them at least: one alone is
-// off by up to 2^-9 of a weight in bf16, as much as the output's rounding).
+// 16-bit pools: weights enter the second product as two pieces of the type (16 bits of them at least: one
+// alone is off by up to 2^-9 of a weight in bf16, as much as the output's rounding).
+// fp32 pools: both products on 32x32x2, nothing below fp32. A step of the first contracts element s (lanes
+// 0-31) and s + D / 2 (lanes 32-63), so that one 16-byte LDS read of a K row feeds four steps; register r of
+// its result is the operand of one step of the second, over keys 8 (r / 4) + r % 4 and that + 4, as it is.
 #pragma once
 
 #include <type_traits>
@@ -50,49 +53,96 @@ __device__ __forceinline__ void dma16(const char* addr, uint32_t lds) {
                  : "memory");
 }
 
-template <typename T>
-struct Bits16;                       // exponent bits: all set in infinities and NaN
-template <>
-struct Bits16<_Float16> {
-    static constexpr uint32_t kExp = 0x7c00u;
-};
-template <>
-struct Bits16<bf16_t> {
-    static constexpr uint32_t kExp = 0x7f80u;
-};
-// The word's elements that are finite, the others as zeros.
+// A 32-bit word of the pool (two elements of a 16-bit type) with those elements that are not finite, whose
+// exponent bits are all set, as zeros.
 template <typename T>
 __device__ __forceinline__ uint32_t finite_of(uint32_t w) {
-    constexpr uint32_t E = Bits16<T>::kExp;
-    const uint32_t lo = (w & E) == E ? 0u : 0xffffu, hi = (w >> 16 & E) == E ? 0u : 0xffff0000u;
-    return w & (lo | hi);
+    if constexpr (sizeof(T) == 4) {
+        return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+    } else {
+        constexpr uint32_t E = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+        const uint32_t lo = (w & E) == E ? 0u : 0xffffu, hi = (w >> 16 & E) == E ? 0u : 0xffff0000u;
+        return w & (lo | hi);
+    }
+}
+
+// Four elements of a pool row.
+template <typename T>
+struct Four {
+    uint32_t w[sizeof(T)];
+    __device__ __forceinline__ static Four load(const T* p) {
+        Four f;
+        if constexpr (sizeof(T) == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            f.w[0] = v.x; f.w[1] = v.y; f.w[2] = v.z; f.w[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            f.w[0] = v.x; f.w[1] = v.y;
+        }
+        return f;
+    }
+    // x + its elements that are not finite.
+    __device__ __forceinline__ float4 add_rest(float4 x) const {
+        uint32_t r[sizeof(T)];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i) r[i] = w[i] ^ finite_of<T>(w[i]);
+        if constexpr (sizeof(T) == 4) {
+            auto f = [](uint32_t b) { return __builtin_bit_cast(float, b); };
+            return make_float4(x.x + f(r[0]), x.y + f(r[1]), x.z + f(r[2]), x.w + f(r[3]));
+        } else {
+            return make_float4(x.x + Pair<T>::lo(r[0]), x.y + Pair<T>::hi(r[0]), x.z + Pair<T>::lo(r[1]),
+                               x.w + Pair<T>::hi(r[1]));
+        }
+    }
+};
+
+__device__ __forceinline__ f32x16 mfma_f32(float a, float b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+
+// XOR swizzles of a row's 16-byte chunks in LDS. 16 bits: lds_swizzle, for both. fp32: a K read takes one
+// chunk of 16 rows, which rows of whole bank sweeps (D = 64, 128) put into one bank but for this, others every
+// 2nd or 4th row; a V read takes 32 consecutive elements of two rows 4 apart (free of conflicts at 64 and 128).
+template <typename T, int D>
+__device__ __forceinline__ int k_swizzle(int r) {
+    if constexpr (sizeof(T) == 2) return lds_swizzle<D>(r);
+    else if constexpr (D % 64 == 0) return r & 15;
+    else if constexpr (D % 32 == 0) return (r >> 1) & 7;
+    else return (r >> 2) & 3;
+}
+template <typename T, int D>
+__device__ __forceinline__ int v_swizzle(int r) {
+    if constexpr (sizeof(T) == 2) return lds_swizzle<D>(r);
+    else if constexpr (D % 64 == 0) return 8 * ((r >> 2) & 1);
+    else return 0;
 }
 
 // Keys of a tile.
 template <int RW>
 constexpr int kTreeTile = RW == 1 ? 128 : 64;
 
-// Waves a SIMD: LDS leaves room for one workgroup a CU with long rows in tiles of 128 keys, else two.
-template <int D, int RW>
-constexpr int kTreeWaves = RW == 1 && D > 64 ? 1 : 2;
+// Waves a SIMD: LDS has room for two workgroups a CU, or for one.
+template <typename T, int D, int RW>
+constexpr int kTreeWaves = 4 * kTreeTile<RW> * D * (int)sizeof(T) <= 72 * 1024 ? 2 : 1;
 
 template <typename T, int D, int RW>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<D, RW>))) void tree_mfma_kernel(const TreeParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<T, D, RW>))) void tree_mfma_kernel(const TreeParams p) {
     static_assert(D % 16 == 0 && D >= 32 && D <= 128, "head_dim");
     constexpr int KW = 4 / RW;                // waves that share a tile's keys
     constexpr int KT = kTreeTile<RW>;
     constexpr int NH = KT / 32 / KW;          // 32-key halves of a wave and tile
     constexpr int ROWS = 32 * RW;
-    constexpr int DSTEPS = D / 16;            // S^T contraction steps
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int KREADS = F32 ? D / 8 : D / 16;   // 16-byte reads of a K row by a lane
     constexpr int DTILES = (D + 31) / 32;     // O^T tiles of 32 dims (the last may be half a tile)
-    constexpr int ROWB = D * 2;               // bytes of a K/V row
+    constexpr int ROWB = D * (int)sizeof(T);  // bytes of a K/V row
     constexpr int CPR = ROWB / 16;            // its 16-byte chunks
     constexpr int G16 = KT / 64;              // groups of 16 keys that a wave stages
     constexpr int IPB = (16 * CPR + 63) / 64; // DMA instructions of a group, of K or V
     constexpr bool kWholeDma = 16 * CPR % 64 == 0;
     constexpr bool kHalfDma = 64 % CPR == 0 && 64 / CPR <= 8;   // rows of one all in an 8-row half
 
-    __shared__ __attribute__((aligned(1024))) uint16_t s_all[4 * KT * D];     // K, V, K, V
+    __shared__ __attribute__((aligned(1024))) char s_all[4 * KT * ROWB];      // K, V, K, V
     __shared__ int s_taken;                   // whether V held what is not finite behind the cached keys
     __shared__ float2 s_ml[4][32];
 
@@ -148,13 +198,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
         return table[b < nb_last ? b : nb_last];
     };
     auto dma_row = [&](int j) { return (64 * j + lane) / CPR; };
-    auto dma_chunk = [&](int j) { return (64 * j + lane) % CPR ^ lds_swizzle<D>((64 * j + lane) / CPR); };
-    uint32_t lane_off[IPB];
+    auto k_chunk = [&](int j) { return 16 * ((64 * j + lane) % CPR ^ k_swizzle<T, D>(dma_row(j))); };
+    auto v_chunk = [&](int j) { return 16 * ((64 * j + lane) % CPR ^ v_swizzle<T, D>(dma_row(j))); };
+    uint32_t k_off[IPB], v_off[IPB];
 #pragma unroll
-    for (int j = 0; j < IPB; ++j)
-        lane_off[j] = (uint32_t)((dma_row(j) & 7) * slot_bytes) + (uint32_t)(dma_chunk(j) * 16);
+    for (int j = 0; j < IPB; ++j) {
+        k_off[j] = (uint32_t)((dma_row(j) & 7) * slot_bytes) + (uint32_t)k_chunk(j);
+        v_off[j] = (uint32_t)((dma_row(j) & 7) * slot_bytes) + (uint32_t)v_chunk(j);
+    }
     const bool offs_fit = 8 * slot_bytes + ROWB <= (int64_t)0xffffffff;
-    auto dma_tile = [&](int kt, int64_t ids, uint16_t* sk, uint16_t* sv) {
+    // (Inlined by force: as calls, lambdas get their captures through memory.)
+    auto dma_tile = [&](int kt, int64_t ids, uint32_t sk, uint32_t sv) __attribute__((always_inline)) {
 #pragma unroll
         for (int g = 0; g < G16; ++g) {
             const int at = wave * G16 + g;                       // the group in the tile
@@ -163,19 +217,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             const int64_t half0 = id0 * block_bytes + (first & (p.block_size - 1)) * slot_bytes;
             const int64_t half1 = id1 * block_bytes + ((first + 8) & (p.block_size - 1)) * slot_bytes;
             const bool ok = ((uint64_t)id0 < (uint64_t)p.num_blocks) & ((uint64_t)id1 < (uint64_t)p.num_blocks);
-            char* dk = reinterpret_cast<char*>(sk) + 16 * at * ROWB;
-            char* dv = reinterpret_cast<char*>(sv) + 16 * at * ROWB;
+            const uint32_t dk = sk + (uint32_t)(16 * at * ROWB), dv = sv + (uint32_t)(16 * at * ROWB);
             if (ok & offs_fit & (first + 16 <= kmax)) {
 #pragma unroll
                 for (int j = 0; j < IPB; ++j) {
                     if constexpr (kHalfDma) {
                         const int64_t half = 64 * j / CPR < 8 ? half0 : half1;
-                        dma16(kbase + half, lane_off[j], lds_u32(dk + j * 1024));
-                        dma16(vbase + half, lane_off[j], lds_u32(dv + j * 1024));
+                        dma16(kbase + half, k_off[j], dk + j * 1024);
+                        dma16(vbase + half, v_off[j], dv + j * 1024);
                     } else if (kWholeDma || 64 * j + lane < 16 * CPR) {
-                        const int64_t off = (dma_row(j) < 8 ? half0 : half1) + lane_off[j];
-                        dma16(kbase + off, lds_u32(dk + j * 1024));
-                        dma16(vbase + off, lds_u32(dv + j * 1024));
+                        const int64_t half = dma_row(j) < 8 ? half0 : half1;
+                        dma16(kbase + half + k_off[j], dk + j * 1024);
+                        dma16(vbase + half + v_off[j], dv + j * 1024);
                     }
                 }
                 continue;
@@ -186,12 +239,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             for (int j = 0; j < IPB; ++j) {
                 const int r = dma_row(j);
                 const int64_t id = r < 8 ? id0 : id1;
-                int64_t off = (int64_t)(dma_chunk(j) * 16);
+                int64_t off = 0;
                 if ((uint64_t)id < (uint64_t)p.num_blocks && first + r < kmax)
-                    off += (r < 8 ? half0 : half1) + (int64_t)(r & 7) * slot_bytes;
+                    off = (r < 8 ? half0 : half1) + (int64_t)(r & 7) * slot_bytes;
                 if (kWholeDma || 64 * j + lane < 16 * CPR) {
-                    dma16(kbase + off, lds_u32(dk + j * 1024));
-                    dma16(vbase + off, lds_u32(dv + j * 1024));
+                    dma16(kbase + off + k_chunk(j), dk + j * 1024);
+                    dma16(vbase + off + v_chunk(j), dv + j * 1024);
                 }
             }
         }
@@ -201,37 +254,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
     const int grp = lane >> 4;
     const int tr_key = (lane & 15) >> 2;
     const int tr_col = 16 * (grp & 1) + 4 * (lane & 3);
-    const int k_swz = lds_swizzle<D>(col);
+    const int k_swz = k_swizzle<T, D>(col);
     const int v_cb = tr_col >> 3;
-    const int v_lo_swz = lds_swizzle<D>(4 * (grp >> 1) + tr_key);
-    const int v_hi_swz = lds_swizzle<D>(4 * (grp >> 1) + tr_key + 8);
     const int v_byte = 8 * (lane & 1);
     const uint32_t wave_off = (uint32_t)(kw * NH * 32 * ROWB);   // of the wave's keys
-    uint32_t koff[DSTEPS], voff_lo[DTILES], voff_hi[DTILES];
+    uint32_t koff[KREADS], voff_lo[DTILES], voff_hi[DTILES];
 #pragma unroll
-    for (int s = 0; s < DSTEPS; ++s) {
-        koff[s] = wave_off + (uint32_t)(col * ROWB + (((2 * s + h) ^ k_swz) << 4));
+    for (int s = 0; s < KREADS; ++s) {
+        const int c = F32 ? s + h * (CPR / 2) : 2 * s + h;
+        koff[s] = wave_off + (uint32_t)(col * ROWB + ((c ^ k_swz) << 4));
         asm volatile("" : "+v"(koff[s]));
     }
 #pragma unroll
     for (int t = 0; t < DTILES; ++t) {
-        // Columns past head_dim re-read the tile's first chunks: output rows never stored.
-        const int c = 4 * t + v_cb < CPR ? 4 * t + v_cb : 4 * t + (v_cb & 1);
-        voff_lo[t] = wave_off + (uint32_t)((4 * (grp >> 1) + tr_key) * ROWB + v_byte + ((c ^ v_lo_swz) << 4));
-        voff_hi[t] = wave_off + (uint32_t)((4 * (grp >> 1) + tr_key + 8) * ROWB + v_byte + ((c ^ v_hi_swz) << 4));
-        asm volatile("" : "+v"(voff_lo[t]), "+v"(voff_hi[t]));
+        // Columns past head_dim re-read the tile's first ones: output rows never stored.
+        if constexpr (F32) {
+            // V[4 h (+ a key group's)][32 t + col], of even and odd groups of four keys: their swizzles differ.
+            const int d = 32 * t + col < D ? 32 * t + col : 32 * t + (col & 15);
+            auto at = [&](int r) { return wave_off + (uint32_t)(r * ROWB + (((d >> 2) ^ v_swizzle<T, D>(r)) << 4) + 4 * (d & 3)); };
+            voff_lo[t] = at(4 * h);
+            voff_hi[t] = 0;
+        } else {
+            const int c = 4 * t + v_cb < CPR ? 4 * t + v_cb : 4 * t + (v_cb & 1);
+            const int r = 4 * (grp >> 1) + tr_key;
+            voff_lo[t] = wave_off + (uint32_t)(r * ROWB + v_byte + ((c ^ v_swizzle<T, D>(r)) << 4));
+            voff_hi[t] = wave_off + (uint32_t)((r + 8) * ROWB + v_byte + ((c ^ v_swizzle<T, D>(r + 8)) << 4));
+            asm volatile("" : "+v"(voff_hi[t]));
+        }
+        asm volatile("" : "+v"(voff_lo[t]));
     }
 
     int64_t ids = 0;
     if (t_begin < t_end) ids = tile_ids(t_begin);
-    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7].
-    u32x4 qfrag[DSTEPS];
+    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7]; fp32: elements 4 s + (D / 2) h .. + 3.
+    u32x4 qfrag[KREADS];
     {
-        const char* qrow = reinterpret_cast<const char*>(p.q) +
-                           ((q_first + my_q) * p.q_st + (int64_t)my_head * p.q_sh) * (int64_t)sizeof(T);
+        const T* qrow = reinterpret_cast<const T*>(p.q) + (q_first + my_q) * p.q_st + (int64_t)my_head * p.q_sh;
 #pragma unroll
-        for (int s = 0; s < DSTEPS; ++s) {
-            const Vec16 v = load16(qrow + (s * 16 + h * 8) * (int)sizeof(T));
+        for (int s = 0; s < KREADS; ++s) {
+            const Vec16 v = load16(qrow + (F32 ? 4 * s + h * (D / 2) : 16 * s + 8 * h));
             qfrag[s] = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
         }
     }
@@ -253,31 +314,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
         return left >= 32 ? w : left <= 0 ? 0u : w & ((1u << left) - 1);
     };
 
-    auto tile = [&](auto tail, int kt, uint16_t* tile_k, uint16_t* tile_v, uint16_t* nk, uint16_t* nv) {
+    auto tile = [&](auto tail, int kt, const char* tile_k, char* tile_v, uint32_t nk) __attribute__((always_inline)) {
         constexpr bool drafted = decltype(tail)::value;          // keys past the cached ones among the tile's
         __builtin_amdgcn_s_waitcnt(0);
         lds_barrier();                        // tile kt is staged, tile kt - 1 is done with
         f32x16 st[NH];
         __builtin_amdgcn_s_setprio(1);
         if (has_rows) {
-            u32x4 kf[NH][DSTEPS];
-#pragma unroll
-            for (int i = 0; i < NH; ++i)
-#pragma unroll
-                for (int s = 0; s < DSTEPS; ++s) {
-                    const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(tile_k) + i * 32 * ROWB + koff[s]);
-                    kf[i][s] = u32x4{a.x, a.y, a.z, a.w};
-                }
 #pragma unroll
             for (int i = 0; i < NH; ++i) st[i] = f32x16{};
+            if constexpr (F32) {
 #pragma unroll
-            for (int s = 0; s < DSTEPS; ++s)
+                for (int s = 0; s < KREADS; ++s)
 #pragma unroll
-                for (int i = 0; i < NH; ++i) st[i] = Mfma<T>::run(kf[i][s], qfrag[s], st[i]);
+                    for (int i = 0; i < NH; ++i) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(tile_k + i * 32 * ROWB + koff[s]);
+                        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t qe = qfrag[s][e];
+                            st[i] = mfma_f32(__builtin_bit_cast(float, w[e]), __builtin_bit_cast(float, qe), st[i]);
+                        }
+                    }
+            } else {
+                u32x4 kf[NH][KREADS];
+#pragma unroll
+                for (int i = 0; i < NH; ++i)
+#pragma unroll
+                    for (int s = 0; s < KREADS; ++s) {
+                        const uint4 a = *reinterpret_cast<const uint4*>(tile_k + i * 32 * ROWB + koff[s]);
+                        kf[i][s] = u32x4{a.x, a.y, a.z, a.w};
+                    }
+#pragma unroll
+                for (int s = 0; s < KREADS; ++s)
+#pragma unroll
+                    for (int i = 0; i < NH; ++i) st[i] = Mfma<T>::run(kf[i][s], qfrag[s], st[i]);
+            }
         }
         __builtin_amdgcn_s_setprio(0);
         if (kt + 1 < t_end) {
-            dma_tile(kt + 1, ids, nk, nv);
+            dma_tile(kt + 1, ids, nk, nk + KT * ROWB);
             ids = tile_ids(kt + 2);
         }
         if constexpr (drafted) {
@@ -333,53 +409,62 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             }
         psum = sum_across32(psum);
         l_run = l_run * alpha + psum;
+        if constexpr (F32) {
 #pragma unroll
-        for (int s = 0; s < 2 * NH; ++s) {
-            f32x16& sv = st[s >> 1];
-            const int r0 = 8 * (s & 1);
-            u32x4 pb[2];
+            for (int i = 0; i < NH; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = sv[r0 + 2 * e], y = sv[r0 + 2 * e + 1];
-                const uint32_t w = Mfma<T>::pack(x, y);
-                pb[0][e] = w;
-                pb[1][e] = Mfma<T>::pack(x - Pair<T>::lo(w), y - Pair<T>::hi(w));
-            }
-            const char* vgrp = reinterpret_cast<const char*>(tile_v) + ((s >> 1) * 32 + 16 * (s & 1)) * ROWB;
+                for (int r = 0; r < 16; ++r) {
+                    // Rows of the group 8 (r / 4): its swizzle is that of row 4 h, as 8 rows on.
+                    const char* vrow = tile_v + (i * 32 + 8 * (r >> 2) + (r & 3)) * ROWB;
 #pragma unroll
-            for (int t = 0; t < DTILES; ++t) {
-                const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_lo[t]));
-                const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_hi[t]));
+                    for (int t = 0; t < DTILES; ++t)
+                        o[t] = mfma_f32(*reinterpret_cast<const float*>(vrow + voff_lo[t]), st[i][r], o[t]);
+                }
+        } else {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) o[t] = Mfma<T>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
+            for (int s = 0; s < 2 * NH; ++s) {
+                f32x16& sv = st[s >> 1];
+                const int r0 = 8 * (s & 1);
+                u32x4 pb[2];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = sv[r0 + 2 * e], y = sv[r0 + 2 * e + 1];
+                    const uint32_t w = Mfma<T>::pack(x, y);
+                    pb[0][e] = w;
+                    pb[1][e] = Mfma<T>::pack(x - Pair<T>::lo(w), y - Pair<T>::hi(w));
+                }
+                const char* vgrp = tile_v + ((s >> 1) * 32 + 16 * (s & 1)) * ROWB;
+#pragma unroll
+                for (int t = 0; t < DTILES; ++t) {
+                    const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_lo[t]));
+                    const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_hi[t]));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) o[t] = Mfma<T>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
+                }
             }
         }
     };
 
-    uint16_t* const k0 = s_all;
-    uint16_t* const v0 = s_all + KT * D;
-    uint16_t* const k1 = s_all + 2 * KT * D;
-    uint16_t* const v1 = s_all + 3 * KT * D;
+    // Tile t is in the buffers of t's parity: K, then V.
+    constexpr int BUF = 2 * KT * ROWB;
+    const uint32_t lds = lds_u32(s_all);
     if (t_begin < t_end) {
-        // (Tile t is in the buffers of t's parity.)
-        if (t_begin & 1) dma_tile(t_begin, ids, k1, v1);
-        else dma_tile(t_begin, ids, k0, v0);
+        dma_tile(t_begin, ids, lds + (t_begin & 1) * BUF, lds + (t_begin & 1) * BUF + KT * ROWB);
         ids = tile_ids(t_begin + 1);
     }
     const int t_cached = pos0 / KT < t_end ? pos0 / KT : t_end;  // tiles of cached keys alone (pos0 >= 0 if it is cut)
     int kt = t_begin;
     if (kt < t_cached && (kt & 1)) {
-        tile(std::false_type{}, kt, k1, v1, k0, v0);
+        tile(std::false_type{}, kt, s_all + BUF, s_all + BUF + KT * ROWB, lds);
         ++kt;
     }
     for (; kt + 1 < t_cached; kt += 2) {
-        tile(std::false_type{}, kt, k0, v0, k1, v1);
-        tile(std::false_type{}, kt + 1, k1, v1, k0, v0);
+        tile(std::false_type{}, kt, s_all, s_all + KT * ROWB, lds + BUF);
+        tile(std::false_type{}, kt + 1, s_all + BUF, s_all + BUF + KT * ROWB, lds);
     }
     for (; kt < t_end; ++kt) {
-        uint16_t* const k = kt & 1 ? k1 : k0;
-        uint16_t* const nk = kt & 1 ? k0 : k1;
-        tile(std::true_type{}, kt, k, k + KT * D, nk, nk + KT * D);
+        char* const k = s_all + (kt & 1) * BUF;
+        tile(std::true_type{}, kt, k, k + KT * ROWB, lds + (~kt & 1) * BUF);
     }
 
     // ---- what is not finite in V, for the rows that see it.
@@ -402,16 +487,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
                     const int64_t id = table[key >> p.block_shift];
                     const bool sees = key < pos0 || (window(first) >> (k & 31) & 1);
                     if ((uint64_t)id >= (uint64_t)p.num_blocks || !sees) continue;
-                    const char* row = vbase + id * block_bytes + (key & (p.block_size - 1)) * slot_bytes + 8 * h;
+                    const T* row = reinterpret_cast<const T*>(vbase + id * block_bytes + (key & (p.block_size - 1)) * slot_bytes) + 4 * h;
 #pragma unroll
-                    for (int u = 0; u < UNITS; ++u) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(row + 16 * u);
-                        const uint2 rest = make_uint2(v.x ^ finite_of<T>(v.x), v.y ^ finite_of<T>(v.y));
-                        extra[u].x += Pair<T>::lo(rest.x);
-                        extra[u].y += Pair<T>::hi(rest.x);
-                        extra[u].z += Pair<T>::lo(rest.y);
-                        extra[u].w += Pair<T>::hi(rest.y);
-                    }
+                    for (int u = 0; u < UNITS; ++u) extra[u] = Four<T>::load(row + 8 * u).add_rest(extra[u]);
                 }
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
@@ -498,11 +576,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
     inv = l_all == 0.f ? 0.f : 1.f / l_all;                                            // no key: zero
     T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)my_head * p.out_sh + 4 * h;
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u)
-        if (u % KW == kw)
-            *reinterpret_cast<uint2*>(orow + 8 * u) =
-                make_uint2(Mfma<T>::pack(o[u / 4][4 * (u % 4)] * inv, o[u / 4][4 * (u % 4) + 1] * inv),
-                           Mfma<T>::pack(o[u / 4][4 * (u % 4) + 2] * inv, o[u / 4][4 * (u % 4) + 3] * inv));
+    for (int u = 0; u < UNITS; ++u) {
+        if (u % KW != kw) continue;
+        const float4 x = make_float4(o[u / 4][4 * (u % 4)] * inv, o[u / 4][4 * (u % 4) + 1] * inv,
+                                     o[u / 4][4 * (u % 4) + 2] * inv, o[u / 4][4 * (u % 4) + 3] * inv);
+        if constexpr (F32) *reinterpret_cast<float4*>(orow + 8 * u) = x;
+        else *reinterpret_cast<uint2*>(orow + 8 * u) = make_uint2(Mfma<T>::pack(x.x, x.y), Mfma<T>::pack(x.z, x.w));
+    }
 }
 
 template <typename T, int D, int RW>
@@ -518,7 +598,9 @@ int launch_tree_rows(const TreeParams& p, hipStream_t stream) {
 template <typename T, int D>
 int launch_tree_d(const TreeParams& p, hipStream_t stream) {
     switch (p.row_waves) {
-        case 1: return launch_tree_rows<T, D, 1>(p, stream);
+        case 1:
+            // (fp32 rows above 64 dims: 128 keys do not fit LDS, tree_plan does not ask for it.)
+            if constexpr (sizeof(T) == 2 || D <= 64) return launch_tree_rows<T, D, 1>(p, stream);
         case 2: return launch_tree_rows<T, D, 2>(p, stream);
         default: return launch_tree_rows<T, D, 4>(p, stream);
     }
