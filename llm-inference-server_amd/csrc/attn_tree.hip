@@ -200,7 +200,7 @@ struct TreePlan : SplitPlan {
 
 // The cheapest of a few run lengths in a model of the launch, in us: a workgroup takes kStart before and
 // after its tiles, a tile's time depends on how full the GPU is; once there are more workgroups than slots
-// the last ones start late, half a workgroup's time on average; a split launch adds the merge kernel and
+// the last ones, the shortest, start late, a third of a workgroup's time on average; a split launch adds the merge kernel and
 // its partials' way to memory and back.
 TreePlan tree_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_tokens,
                    int64_t max_query_len, int dtype, const int64_t* ctx, const int64_t* qlen) {
@@ -231,7 +231,7 @@ TreePlan tree_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, in
         const float tile = full > alone ? alone + (full - alone) * fill : alone;
         const float one = longest * tile + kStart;
         if (wgs <= slots) return one;
-        const float all = (work * tile + wgs * kStart) / slots + 0.5f * one;
+        const float all = (work * tile + wgs * kStart) / slots + 0.35f * one;
         return all > one ? all : one;
     };
     int64_t wgs = 0, work = 0, longest = 0;

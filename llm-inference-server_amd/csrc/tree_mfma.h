@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
     __shared__ float2 s_ml[4][32];
 
     PrefillItem it;
-    if (!prefill_item<ROWS, KT>(p, p.block_size, it)) return;
+    if (!tree_item<ROWS, KT>(p, it)) return;
     const uint32_t G = (uint32_t)p.group;
     const int kvh = it.kvh, split = it.split, seq = it.seq;
     const int64_t q_first = it.q_first;
