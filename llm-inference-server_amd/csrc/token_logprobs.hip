@@ -1,21 +1,26 @@
 // Log probabilities of given tokens over rows of logits, their ranks, the rows' entropies and the
 // `top` likeliest tokens of each row, in one pass over the logits.
 //
-//   m = some logit of the row near its largest, s = sum e^(x - m), t = sum e^(x - m) (x - m)
-//   log p(i) = x_i - m - ln s,   entropy = ln s - t / s,   rank = 1 + #{x > x_i}
+//   y = x log2(e),  c = a whole number near the row's largest y,  s = sum 2^(y - c),  t = sum 2^(y - c) (y - c)
+//   log p(i) = ln2 (y_i - c - log2 s),   entropy = ln2 (log2 s - t / s),   rank = 1 + #{x > x_i}
 //
 // A workgroup has one row, or one of `parts` pieces of it where there are few rows; the last piece
-// of a row to finish merges them. A lane keeps (m, s, t) of its own in fp32 and raises m only when a
-// tile exceeds it by more than 4. Logits are read
-// once, 16 bytes a lane, whatever a row's alignment: its first and last 16 bytes are taken apart.
+// of a row to finish merges them. A lane keeps (c, s, t) of its own in fp32 and raises c only when a
+// tile exceeds it by more than 4; c is whole so that y - c is one fma, rounded once, in every lane. Logits
+// are read once, 16 bytes a lane, whatever a row's alignment: its first and last 16 bytes are taken apart.
 //
-// Top: the k-th largest of a wave's 64 lane maxima so far is a lower bound tau of the row's k-th largest
-// logit, found by 16 ballots on the maxima's bits. A tile that holds something above tau (most do
-// not, after a few) raises it and appends what reaches it to the wave's list in LDS. Logits equal to tau are
-// taken once only up to k: of equal ones the lowest indices count, and a wave's indices rise. At the
-// end the waves' lists, cut by the row's tau, hold little more than k entries, which rank themselves
-// by counting. Masked logits (-inf) never enter a list; if a row has fewer others than k, the lowest
-// masked ids follow.
+// Such references need |y| below 2^30. Logits far below it are nothing beside others; rows (pieces) that
+// have a larger one, or only smaller ones, are summed again, against their largest logit itself.
+//
+// Top: the k-th largest of 64 maxima, of each lane over the waves, is a lower bound tau of the row's k-th
+// largest logit so far, found by 16 ballots on the maxima's bits. A tile that holds something above it (most do
+// not, after a few) raises it and appends what reaches it to the wave's list in LDS. Of logits equal to tau a
+// wave takes k: of equal ones the lowest indices count, and a wave's indices rise. At the end the waves'
+// lists, cut by the last tau, hold little more than k entries, which rank themselves by counting. Masked
+// logits (-inf) never enter a list; if a row has fewer others than k, the lowest masked ids follow.
+//
+// Bound: HBM and, for 16-bit logits, the vector unit (an exponential takes four slots of the nine that a logit
+// costs).
 #include "pkv_common.h"
 
 #include "attention.h"
@@ -27,8 +32,10 @@ constexpr int kWaves = 4;
 constexpr int kMaxTop = 64;             // a list's entries are ranked against one another; one lane max each
 constexpr int kList = 640;              // a wave's: kMaxTop after a cut and a load of 512 logits
 constexpr int kMerged = 1024;
-constexpr float kRaise = 4.f;           // 32: weights off by up to 1.3e-6, through the rounding of their exponents
-constexpr float kLeast = -200.f;        // e^kLeast is 0 in fp32
+constexpr float kRaise = 4.f;           // weights of up to 2^5: larger ones lose digits in their exponents' rounding
+constexpr float kFar = 536870912.f;     // 2^29
+constexpr float kLeast = -300.f;        // 2^kLeast and e^kLeast are 0 in fp32
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct LogprobArgs {
     const void* logits;
@@ -69,23 +76,35 @@ __device__ __forceinline__ float kth_of_lanes(float x, int k) {
     return -wave_max(u >= t ? -x : kNegInf);
 }
 
+// Of a lane, wave, piece or row. c, and t, in units of ln 2 for kNear, else of 1. The rows' levels:
+enum { kBelow = 0, kNear = 1, kBeyond = 2, kNone = 3 };      // nothing above -2^29; the rule; above 2^29; NaN
 struct Stat {
-    float m, s, t;                      // s = 0: nothing above -inf yet
+    float c, s, t;                      // s = 0: nothing yet
 };
 
+// BASE2: weights are 2^(y - c), else e^(x - c).
+template <bool BASE2>
 __device__ __forceinline__ Stat merge(Stat a, Stat b) {
-    const float m = fmaxf(a.m, b.m);
-    // (Bounded: sums of 0, and logits of the type's lowest value, are nothing and not 0 * -inf.)
-    const float da = fmaxf(a.m - m, kLeast), db = fmaxf(b.m - m, kLeast);
-    const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
-    return Stat{m, a.s * fa + b.s * fb, fmaf(da, a.s, a.t) * fa + fmaf(db, b.s, b.t) * fb};
+    const float c = fmaxf(a.c, b.c);
+    // (Bounded: c of -inf, and logits of the type's lowest value, are nothing and not 0 * -inf.)
+    const float da = fmaxf(a.c - c, kLeast), db = fmaxf(b.c - c, kLeast);
+    const float fa = fast_exp2(BASE2 ? da : da * kLog2e), fb = fast_exp2(BASE2 ? db : db * kLog2e);
+    return Stat{c, a.s * fa + b.s * fb, fmaf(da, a.s, a.t) * fa + fmaf(db, b.s, b.t) * fb};
 }
 
+template <bool BASE2>
 __device__ __forceinline__ Stat wave_merge(Stat x) {
 #pragma unroll
     for (int off = 1; off < 64; off *= 2)
-        x = merge(x, Stat{__shfl_xor(x.m, off), __shfl_xor(x.s, off), __shfl_xor(x.t, off)});
+        x = merge<BASE2>(x, Stat{__shfl_xor(x.c, off), __shfl_xor(x.s, off), __shfl_xor(x.t, off)});
     return x;
+}
+
+// The largest float below x (-inf stays).
+__device__ __forceinline__ float below(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    if (x == kNegInf) return x;
+    return __builtin_bit_cast(float, x == 0.f ? 0x80000001u : u >> 31 ? u + 1 : u - 1);
 }
 
 // The k largest of list[0 .. n), in order, to list2[0 .. min(n, k)); threads `id` of `count`.
@@ -122,13 +141,13 @@ struct Vec {
 
 // U: 16-byte loads of a lane and tile.
 template <typename T, int U>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void token_logprobs_kernel(const LogprobArgs a) {
     constexpr int N = Vec<T>::N;
     __shared__ uint64_t s_list[kWaves][kList];
     __shared__ uint64_t s_merged[kMerged], s_top[kMaxTop];
     __shared__ float s_max[kWaves][64];
     __shared__ Stat s_stat[kWaves];
-    __shared__ int s_above[kWaves], s_n, s_entries[64];
+    __shared__ int s_above[kWaves], s_far[kWaves], s_n, s_entries[64];
     __shared__ uint32_t s_arrived;
     const int tid = (int)threadIdx.x, lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -150,12 +169,16 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
     const int q_end = pieces - q_begin < per_part ? pieces : q_begin + per_part;
 
     Stat st = {kNegInf, 0.f, 0.f};
-    float ref = 0.f;                    // st.m where it is above -inf
+    float ref = 0.f;                    // st.c where it is above -inf
+    bool far = false;                   // a logit above 2^29
     int above = 0;                      // of the wave
-    // The wave's list of the likeliest, their bound, the lanes' largest logits.
+    // The wave's list of the likeliest, their bound, how many equal to it are listed, what a tile has to
+    // exceed to be looked at, the lane's largest logit.
     uint64_t* list = s_list[wave];
-    int listed = 0;
-    float tau = kNegInf, lane_max = kNegInf;
+    int listed = 0, equal = 0;
+    float tau = kNegInf, limit_top = a.top > 0 ? kNegInf : __builtin_huge_valf(), lane_max = kNegInf;
+    s_max[wave][lane] = kNegInf;
+    if (a.top > 0) __syncthreads();
 
     auto load = [&](int q0, Vec16* raw) {
         // q0: the wave's first piece.
@@ -217,80 +240,133 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
     const int q_first = q_begin + wave * 64 * U;
     if (q_first < q_end) load(q_first, raw);
     for (int q0 = q_first; q0 < q_end; q0 += kTile) {
-        float x[U][N];
+        float x[U][N], um[U], tm = kNegInf;
 #pragma unroll
-        for (int u = 0; u < U; ++u) values(q0, u, raw[u], x[u]);
+        for (int u = 0; u < U; ++u) {
+            values(q0, u, raw[u], x[u]);
+            um[u] = x[u][0];
+#pragma unroll
+            for (int e = 1; e < N; ++e) um[u] = fmaxf(um[u], x[u][e]);
+            tm = fmaxf(tm, um[u]);
+        }
         if (q0 + kTile < q_end) load(q0 + kTile, raw);
-        float tm = kNegInf;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < N; ++e) tm = fmaxf(tm, x[u][e]);
-        if (__builtin_amdgcn_ballot_w64(tm > st.m + kRaise)) {
-            if (tm > st.m + kRaise) {
-                const float d = fmaxf(st.m - tm, kLeast), f = fast_exp2(d * kLog2e);
-                st = Stat{tm, st.s * f, fmaf(d, st.s, st.t) * f};
-                ref = tm;
+        const float ym = tm * kLog2e;
+        if (__builtin_amdgcn_ballot_w64(ym > st.c + kRaise)) {
+            far |= ym > kFar;
+            if (ym > st.c + kRaise && ym > -kFar) {
+                const float c = rintf(ym), d = fmaxf(st.c - c, kLeast), f = fast_exp2(d);
+                st = Stat{c, st.s * f, fmaf(d, st.s, st.t) * f};
+                ref = c;
             }
         }
+        float s = 0.f, t = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float d = x[u][e] - ref;
-                const float w = fast_exp2(d * kLog2e);      // NaN stays NaN; -inf: 0
-                st.s += w;
-                st.t = fmaf(w, fmaxf(d, kLeast), st.t);     // 0 * kLeast, not 0 * -inf
-                above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] > limit));
+                const float d = fmaf(x[u][e], kLog2e, -ref);
+                const float w = fast_exp2(d);               // NaN stays NaN; -inf: 0
+                s += w;
+                t = fmaf(w, fmaxf(d, kLeast), t);           // 0 * kLeast, not 0 * -inf
             }
-        if (a.top > 0 && __builtin_amdgcn_ballot_w64(tm > tau)) {
+        st.s += s;
+        st.t += t;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (__builtin_amdgcn_ballot_w64(um[u] > limit)) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] > limit));
+            }
+        if (__builtin_amdgcn_ballot_w64(tm > limit_top)) {
             lane_max = fmaxf(lane_max, tm);
-            const float raised = kth_of_lanes(lane_max, a.top);
-            bool equal = raised > tau;  // whether logits equal to tau still count
-            tau = raised;
-            int equals = 0;
+            // What the other waves have found by now: any of it bounds the row's k-th.
+            float both = lane_max;
+            __hip_atomic_store(&s_max[wave][lane], lane_max, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+                both = fmaxf(both, __hip_atomic_load(&s_max[w][lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+            const float raised = kth_of_lanes(both, a.top);
+            if (raised > tau) {
+                tau = raised;
+                equal = 0;
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                auto takes = [&](float v) { return v > tau || (equal && v == tau && v > kNegInf); };
+                const bool more_equal = equal < a.top;
+                auto takes = [&](float v) { return v > tau || (more_equal && v == tau && v > kNegInf); };
+                if (!__builtin_amdgcn_ballot_w64(takes(um[u]))) continue;
                 int more = 0;
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(takes(x[u][e])));
-                    equals += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] == tau));
-                }
-                if (more == 0) continue;
+                for (int e = 0; e < N; ++e) more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(takes(x[u][e])));
                 if (listed + more > kList) shorten(more);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const bool take = takes(x[u][e]);
-                    const uint64_t lanes = __builtin_amdgcn_ballot_w64(take);
-                    if (take)
+                    const uint64_t lanes = __builtin_amdgcn_ballot_w64(takes(x[u][e]));
+                    if (takes(x[u][e]))
                         list[listed + lanes_below(lanes)] = key_of(x[u][e], (q0 + lane + 64 * u) * N + e - head);
                     listed += __builtin_popcountll(lanes);
+                    equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] == tau));
                 }
-                if (equals >= a.top) equal = false;
             }
+            limit_top = equal < a.top ? below(tau) : tau;
         }
     }
 
     // ---- the workgroup's.
-    st = wave_merge(st);
+    st = wave_merge<true>(st);
+    const bool any_far = __builtin_amdgcn_ballot_w64(far) != 0;
     if (lane == 0) {
         s_stat[wave] = st;
         s_above[wave] = above;
+        s_far[wave] = any_far;
     }
     if (tid == 0) s_n = 0;
     s_max[wave][lane] = lane_max;
     __syncthreads();
     Stat all = s_stat[0];
-    int more = s_above[0];
+    int more = s_above[0], level = s_far[0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) {
-        all = merge(all, s_stat[w]);
+        all = merge<true>(all, s_stat[w]);
         more += s_above[w];
+        level |= s_far[w];
+    }
+    level = level ? kBeyond : all.s > 0.f ? kNear : all.s == 0.f ? kBelow : kNone;
+    if (level == kBeyond || level == kBelow) {
+        // Once more, against the piece's largest logit.
+        float m = kNegInf;
+        auto each = [&](auto f) {
+            for (int q = q_begin + tid; q < q_end; q += 256)
+                for (int e = 0; e < N; ++e) {
+                    const int i = q * N + e - head;
+                    if (i >= 0 && i < a.vocab) f(to_f32(x0[i]));
+                }
+        };
+        each([&](float v) { m = fmaxf(m, v); });
+        m = wave_max(m);
+        __syncthreads();                               // s_stat has been read
+        if (lane == 0) s_stat[wave].c = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_stat[w].c);
+        Stat x = {m, 0.f, 0.f};
+        if (m > kNegInf)
+            each([&](float v) {
+                const float d = v - m, w = fast_exp2(d * kLog2e);
+                x.s += w;
+                x.t = fmaf(w, fmaxf(d, kLeast), x.t);
+            });
+        x = wave_merge<false>(x);
+        __syncthreads();
+        if (lane == 0) s_stat[wave] = x;
+        __syncthreads();
+        all = s_stat[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) all = merge<false>(all, s_stat[w]);
+        if (all.s != all.s) level = kNone;
     }
     int n = 0;
-    // Joins the lists of what reaches `bound` into s_merged.
+    // The lists, cut by the row's bound, into one.
     if (a.top > 0) {
         float both = s_max[0][lane];
 #pragma unroll
@@ -315,9 +391,9 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
         auto put = [&](int i, uint64_t v) { __hip_atomic_store(mine + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
         auto two = [](float lo, uint32_t hi) { return (uint64_t)hi << 32 | __builtin_bit_cast(uint32_t, lo); };
         if (tid == 0) {
-            put(0, two(all.m, __builtin_bit_cast(uint32_t, all.s)));
+            put(0, two(all.c, __builtin_bit_cast(uint32_t, all.s)));
             put(1, two(all.t, (uint32_t)more));
-            put(2, (uint64_t)n);
+            put(2, (uint64_t)n | (uint64_t)level << 32);
         }
         if (tid < n) put(3 + tid, s_top[tid]);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -329,18 +405,24 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
         auto get = [&](int p, int i) {
             return __hip_atomic_load(a.partials + (row * a.parts + p) * words + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         };
-        // Parts in a fixed order: lane p of every wave has part p, merged across the wave.
+        // Parts in a fixed order: lane p of every wave has part p, merged across the wave. Those of the highest
+        // level are the row's; the others are nothing beside them.
         Stat x = {kNegInf, 0.f, 0.f};
-        int count = 0;
+        int count = 0, its = 0;
         uint64_t entries = 0;
         if (lane < a.parts) {
             const uint64_t ms = get(lane, 0), tn = get(lane, 1);
             entries = get(lane, 2);
+            its = (int)(entries >> 32);
             x = Stat{__builtin_bit_cast(float, (uint32_t)ms), __builtin_bit_cast(float, (uint32_t)(ms >> 32)),
                      __builtin_bit_cast(float, (uint32_t)tn)};
             count = (int)(tn >> 32);
         }
-        all = wave_merge(x);
+        level = kBelow;
+        for (int l = kNear; l <= kNone; ++l)
+            if (__builtin_amdgcn_ballot_w64(its == l)) level = l;
+        if (its != level) x = Stat{kNegInf, 0.f, 0.f};
+        all = level == kNear ? wave_merge<true>(x) : wave_merge<false>(x);
         for (int off = 1; off < 64; off *= 2) count += __shfl_xor(count, off);
         more = count;
         if (a.top > 0) {
@@ -350,7 +432,7 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
             uint64_t* joined = &s_list[0][0];      // parts * top <= 32 * 64 of kWaves * kList
             // A part's list holds its k largest, in order. The largest last entry of a full list bounds
             // the row's k-th from below.
-            uint64_t least = lane < a.parts && (int)entries == a.top ? get(lane, 2 + a.top) : 0;
+            uint64_t least = lane < a.parts && (int)(uint32_t)entries == a.top ? get(lane, 2 + a.top) : 0;
             for (int off = 1; off < 64; off *= 2) {
                 const uint64_t o = __shfl_xor((unsigned long long)least, off);
                 least = o > least ? o : least;
@@ -369,18 +451,25 @@ __global__ __launch_bounds__(256) void token_logprobs_kernel(const LogprobArgs a
     }
 
     // ---- out. A row whose sum is NaN, or 0, has no distribution.
-    const bool proper = all.s > 0.f;    // not of NaN
+    const bool proper = all.s > 0.f && level != kNone;
+    const bool near = level == kNear;
     const float nan = __builtin_nanf("");
-    const float log_s = logf(all.s);
+    const float log_s = near ? log2f(all.s) : logf(all.s);
+    auto log_p = [&](float v) {
+        if (!near) return v - all.c - log_s;
+        // (The product overflows at the type's lowest value.)
+        return v < -kFar ? v - kLn2 * (all.c + log_s) : kLn2 * (fmaf(v, kLog2e, -all.c) - log_s);
+    };
     if (tid == 0) {
-        a.logprobs[row] = proper && asked ? own - all.m - log_s : nan;
+        a.logprobs[row] = proper && asked ? log_p(own) : nan;
         a.ranks[row] = proper && asked ? more + 1 : 0;
-        a.entropy[row] = proper ? fmaxf(log_s - all.t / all.s, 0.f) : nan;
+        const float h = log_s - all.t / all.s;
+        a.entropy[row] = proper ? fmaxf(near ? kLn2 * h : h, 0.f) : nan;
     }
     float* out = a.top_logprobs + row * a.top;
     int64_t* out_ids = a.top_ids + row * a.top;
     if (tid < a.top && (tid < n || !proper)) {
-        out[tid] = proper ? logit_of(s_top[tid]) - all.m - log_s : nan;
+        out[tid] = proper ? log_p(logit_of(s_top[tid])) : nan;
         out_ids[tid] = proper ? id_of(s_top[tid]) : -1;
     }
     if (proper && n < a.top && tid == 0) {

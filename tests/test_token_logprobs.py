@@ -132,7 +132,9 @@ def test_rows_without_a_distribution_and_odd_ids(device, dtype, vocab):
     check(x, ids, got, 12)
     assert got.ranks.tolist()[:4] == [0] * 4 and got.ranks.tolist()[5:] == [0] * 3
     assert got.logprobs[4].item() == -math.inf and got.ranks[4].item() == 2
-    assert got.top_ids[4].tolist() == list(range(12)) and got.entropy[4].item() == 0.0
+    # One token is left: s = 2^r and t = r 2^r against a reference within half of it, |r| <= 1/2, and
+    # log2 s - t / s is two values near r, each off by two roundings of it.
+    assert got.top_ids[4].tolist() == list(range(12)) and 0.0 <= got.entropy[4].item() <= 4 * E * 0.5
 
 
 def test_fp32_logits_at_the_types_ends(device):
@@ -146,6 +148,38 @@ def test_fp32_logits_at_the_types_ends(device):
     got = token_logprobs(x.to(device), ids.to(device), 6)
     check(x, ids, got, 6)
     assert abs(got.logprobs[0].item() + math.log(3000)) < 1e-5 and abs(got.logprobs[2].item() + math.log(1500)) < 1e-5
+
+
+@pytest.mark.parametrize("n", [1, 3, 600])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_logits_of_any_size(device, dtype, n):
+    """Sizes at which fp32 products with log2(e) no longer tell neighbours apart, in one place of a row, all
+    over it, among others and among masked ones."""
+    vocab = 9000
+    x = torch.zeros(9, vocab)
+    g = torch.Generator().manual_seed(0)
+    x[0] = torch.randn(vocab, generator=g)
+    x[0, 8000] = 1e12
+    x[1, 5], x[1, 8500] = 6e8, 6e8 + 64
+    x[2] = -1e10
+    x[2, 100], x[2, 8999] = -2e9, -2e9
+    x[3] = -1e9
+    x[3, 4000:4010] = torch.arange(10.0)
+    x[4] = -math.inf
+    x[4, 7], x[4, 8000] = -3e38, -3e38
+    x[5] = torch.randn(vocab, generator=g) * 1e6
+    x[6] = 4e8 + 32 * torch.randint(0, 4, (vocab,), generator=g)
+    x[7, 8990] = math.nan
+    x[7, 3] = 1e30
+    x[8, 3000:] = -1e9
+    x = x.to(dtype)
+    ids = torch.tensor([8000, 8500, 100, 4003, 7, 11, 5, 2, 10])
+    every = x.repeat(-(-n // 9), 1)[:max(n, 9)].to(device)
+    got = token_logprobs(every, ids.repeat(-(-n // 9))[:max(n, 9)].to(device), 9)
+    check(x, ids, type(got)(*(t[:9] for t in got)), 9)
+    for r in range(9) if n == 1 else ():
+        one = token_logprobs(x[r:r + 1].to(device), ids[r:r + 1].to(device), 9)
+        check(x[r:r + 1], ids[r:r + 1], one, 9)
 
 
 def test_refusals(device):
