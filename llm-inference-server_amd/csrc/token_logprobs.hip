@@ -12,12 +12,15 @@
 // Such references need |y| below 2^30. Logits far below it are nothing beside others; rows (pieces) that
 // have a larger one, or only smaller ones, are summed again, against their largest logit itself.
 //
-// Top: the k-th largest of 64 maxima, of each lane over the waves, is a lower bound tau of the row's k-th
-// largest logit so far, found by 16 ballots on the maxima's bits. A tile that holds something above it (most do
-// not, after a few) raises it and appends what reaches it to the wave's list in LDS. Of logits equal to tau a
-// wave takes k: of equal ones the lowest indices count, and a wave's indices rise. At the end the waves'
-// lists, cut by the last tau, hold little more than k entries, which rank themselves by counting. Masked
-// logits (-inf) never enter a list; if a row has fewer others than k, the lowest masked ids follow.
+// Top: of a tile, lanes keep only whether it holds their largest logit so far, and the second largest of
+// their tiles' largest. The k-th largest of the 256 lanes' largest logits, found by ballots on their bits, is a lower bound tau
+// of the row's k-th largest. Lanes that reach it, hardly more than k, read that one tile's logits again (64 bytes of 16-bit
+// ones; all their tiles where the second reaches tau too) and list what reaches tau. The entries, hardly more
+// than k, rank themselves by counting. A wave with more to list than there is room for (rows of many equal logits)
+// walks all its tiles again instead, in the order of the ids, and takes of logits equal to tau only the first k.
+// Masked logits (-inf) never enter a list; if a row has fewer others than k, the lowest masked ids follow.
+// (Lists grown while the logits stream by, against a bound that rises, cost 66 of 192 us of 2048 rows of 128000
+// at k = 20.)
 //
 // Bound: HBM and, for 16-bit logits, the vector unit (an exponential takes four slots of the nine that a logit
 // costs).
@@ -30,7 +33,7 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kMaxTop = 64;             // a list's entries are ranked against one another; one lane max each
-constexpr int kList = 640;              // a wave's: kMaxTop after a cut and a load of 512 logits
+constexpr int kList = 640;              // of a wave: kMaxTop after a cut, and a load of 512 logits
 constexpr int kMerged = 1024;
 constexpr float kRaise = 4.f;           // weights of up to 2^5: larger ones lose digits in their exponents' rounding
 constexpr float kFar = 536870912.f;     // 2^29
@@ -67,13 +70,23 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
-// A lower bound of the k-th largest of the lanes' x (k <= 64), itself one of them.
-__device__ __forceinline__ float kth_of_lanes(float x, int k) {
-    const uint32_t u = order_of(x);
-    uint32_t t = 0;
-    for (uint32_t bit = 0x80000000u; bit > 0x8000u; bit >>= 1)
-        if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(u >= (t | bit))) >= k) t |= bit;
-    return -wave_max(u >= t ? -x : kNegInf);
+// A lower bound of the k-th largest of the lanes' W values x (k <= 64), itself one of them.
+template <int W>
+__device__ __forceinline__ float kth_of_lanes(const float* x, int k) {
+    uint32_t u[W], t = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) u[w] = order_of(x[w]);
+    for (uint32_t bit = 0x80000000u; bit > 0x8000u; bit >>= 1) {
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(u[w] >= (t | bit)));
+        if (n >= k) t |= bit;
+        if (n == k) break;                    // the k-th itself bounds them
+    }
+    float least = kNegInf;
+#pragma unroll
+    for (int w = 0; w < W; ++w) least = fmaxf(least, u[w] >= t ? -x[w] : kNegInf);
+    return -wave_max(least);
 }
 
 // Of a lane, wave, piece or row. c, and t, in units of ln 2 for kNear, else of 1. The rows' levels:
@@ -98,13 +111,6 @@ __device__ __forceinline__ Stat wave_merge(Stat x) {
     for (int off = 1; off < 64; off *= 2)
         x = merge<BASE2>(x, Stat{__shfl_xor(x.c, off), __shfl_xor(x.s, off), __shfl_xor(x.t, off)});
     return x;
-}
-
-// The largest float below x (-inf stays).
-__device__ __forceinline__ float below(float x) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    if (x == kNegInf) return x;
-    return __builtin_bit_cast(float, x == 0.f ? 0x80000001u : u >> 31 ? u + 1 : u - 1);
 }
 
 // The k largest of list[0 .. n), in order, to list2[0 .. min(n, k)); threads `id` of `count`.
@@ -146,6 +152,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
     __shared__ uint64_t s_list[kWaves][kList];
     __shared__ uint64_t s_merged[kMerged], s_top[kMaxTop];
     __shared__ float s_max[kWaves][64];
+    __shared__ int s_at[kWaves][64];
     __shared__ Stat s_stat[kWaves];
     __shared__ int s_above[kWaves], s_far[kWaves], s_n, s_entries[64];
     __shared__ uint32_t s_arrived;
@@ -172,13 +179,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
     float ref = 0.f;                    // st.c where it is above -inf
     bool far = false;                   // a logit above 2^29
     int above = 0;                      // of the wave
-    // The wave's list of the likeliest, their bound, how many equal to it are listed, what a tile has to
-    // exceed to be looked at, the lane's largest logit.
-    uint64_t* list = s_list[wave];
-    int listed = 0, equal = 0;
-    float tau = kNegInf, limit_top = a.top > 0 ? kNegInf : __builtin_huge_valf(), lane_max = kNegInf;
-    s_max[wave][lane] = kNegInf;
-    if (a.top > 0) __syncthreads();
+    // The lane's largest logit and its tile's first piece, the second largest of its tiles' largest.
+    float best = kNegInf, second = kNegInf, tau = kNegInf;
+    int best_at = 0;
+    uint64_t* list = s_list[wave];      // of the wave's likeliest
+    int listed = 0;
 
     auto load = [&](int q0, Vec16* raw) {
         // q0: the wave's first piece.
@@ -200,23 +205,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
             }
         }
     };
-    // Drops what is below tau from the list; if that leaves too much for `more`, all but the k largest.
-    auto shorten = [&](int more) {
-        int kept = 0;
-        const uint32_t least = order_of(tau);
-        for (int i = 0; i < listed; i += 64) {
-            const uint64_t key = i + lane < listed ? list[i + lane] : 0;
-            const uint64_t keep = __builtin_amdgcn_ballot_w64(i + lane < listed && (uint32_t)(key >> 32) >= least);
-            wave_lds_sync();
-            if (keep >> lane & 1) list[kept + lanes_below(keep)] = key;
-            wave_lds_sync();
-            kept += __builtin_popcountll(keep);
-        }
-        listed = kept;
-        if (listed + more <= kList) return;
-        // Ranks first, then the moves: lists of 64 entries a round.
+    // Leaves the k largest of the list.
+    auto shorten = [&]() {
         uint64_t mine[kList / 64];
         int rank[kList / 64];
+        wave_lds_sync();
 #pragma unroll
         for (int r = 0; r < kList / 64; ++r) {
             mine[r] = 64 * r + lane < listed ? list[64 * r + lane] : 0;
@@ -277,39 +270,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
 #pragma unroll
                 for (int e = 0; e < N; ++e) above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] > limit));
             }
-        if (__builtin_amdgcn_ballot_w64(tm > limit_top)) {
-            lane_max = fmaxf(lane_max, tm);
-            // What the other waves have found by now: any of it bounds the row's k-th.
-            float both = lane_max;
-            __hip_atomic_store(&s_max[wave][lane], lane_max, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w)
-                both = fmaxf(both, __hip_atomic_load(&s_max[w][lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-            const float raised = kth_of_lanes(both, a.top);
-            if (raised > tau) {
-                tau = raised;
-                equal = 0;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const bool more_equal = equal < a.top;
-                auto takes = [&](float v) { return v > tau || (more_equal && v == tau && v > kNegInf); };
-                if (!__builtin_amdgcn_ballot_w64(takes(um[u]))) continue;
-                int more = 0;
-#pragma unroll
-                for (int e = 0; e < N; ++e) more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(takes(x[u][e])));
-                if (listed + more > kList) shorten(more);
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const uint64_t lanes = __builtin_amdgcn_ballot_w64(takes(x[u][e]));
-                    if (takes(x[u][e]))
-                        list[listed + lanes_below(lanes)] = key_of(x[u][e], (q0 + lane + 64 * u) * N + e - head);
-                    listed += __builtin_popcountll(lanes);
-                    equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(x[u][e] == tau));
-                }
-            }
-            limit_top = equal < a.top ? below(tau) : tau;
-        }
+        second = fmaxf(second, fminf(best, tm));
+        best_at = tm > best ? q0 : best_at;
+        best = fmaxf(best, tm);
     }
 
     // ---- the workgroup's.
@@ -321,7 +284,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
         s_far[wave] = any_far;
     }
     if (tid == 0) s_n = 0;
-    s_max[wave][lane] = lane_max;
+    s_max[wave][lane] = best;
     __syncthreads();
     Stat all = s_stat[0];
     int more = s_above[0], level = s_far[0];
@@ -333,31 +296,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
     }
     level = level ? kBeyond : all.s > 0.f ? kNear : all.s == 0.f ? kBelow : kNone;
     if (level == kBeyond || level == kBelow) {
-        // Once more, against the piece's largest logit.
-        float m = kNegInf;
-        auto each = [&](auto f) {
-            for (int q = q_begin + tid; q < q_end; q += 256)
-                for (int e = 0; e < N; ++e) {
-                    const int i = q * N + e - head;
-                    if (i >= 0 && i < a.vocab) f(to_f32(x0[i]));
-                }
-        };
-        each([&](float v) { m = fmaxf(m, v); });
+        // Once more, against the piece's largest logit (without any: nothing).
+        float m = fmaxf(fmaxf(s_max[0][lane], s_max[1][lane]), fmaxf(s_max[2][lane], s_max[3][lane]));
         m = wave_max(m);
-        __syncthreads();                               // s_stat has been read
-        if (lane == 0) s_stat[wave].c = m;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, s_stat[w].c);
         Stat x = {m, 0.f, 0.f};
-        if (m > kNegInf)
-            each([&](float v) {
-                const float d = v - m, w = fast_exp2(d * kLog2e);
+        for (int q = q_begin + tid; q < q_end && m > kNegInf; q += 256)
+            for (int e = 0; e < N; ++e) {
+                const int i = q * N + e - head;
+                if (i < 0 || i >= a.vocab) continue;
+                const float d = to_f32(x0[i]) - m, w = fast_exp2(d * kLog2e);
                 x.s += w;
                 x.t = fmaf(w, fmaxf(d, kLeast), x.t);
-            });
+            }
         x = wave_merge<false>(x);
-        __syncthreads();
+        __syncthreads();                               // s_stat has been read
         if (lane == 0) s_stat[wave] = x;
         __syncthreads();
         all = s_stat[0];
@@ -366,13 +318,107 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
         if (all.s != all.s) level = kNone;
     }
     int n = 0;
-    // The lists, cut by the row's bound, into one.
     if (a.top > 0) {
-        float both = s_max[0][lane];
+        float max_of[kWaves];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) both = fmaxf(both, s_max[w][lane]);
-        tau = fmaxf(tau, kth_of_lanes(both, a.top));
-        shorten(kList - kMerged / kWaves);          // a wave's share of s_merged at most
+        for (int w = 0; w < kWaves; ++w) max_of[w] = s_max[w][lane];
+        tau = kth_of_lanes<kWaves>(max_of, a.top);
+        // Of one piece a lane, of q's values or raw's, those that reach tau; false where the list has no room.
+        auto inner = [&](int q, bool live) { return live && q > 0 && q < pieces - 1; };
+        auto push = [&](int q, bool live, const Vec16& raw) {
+            float v[N];
+            if (inner(q, live)) {
+                Vec<T>::get(raw, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int i = q * N + e - head;
+                    v[e] = live && i >= 0 && i < a.vocab ? to_f32(x0[i]) : kNegInf;
+                }
+            }
+            int more = 0;
+            auto takes = [&](int e) { return v[e] >= tau && v[e] > kNegInf; };
+#pragma unroll
+            for (int e = 0; e < N; ++e) more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(takes(e)));
+            if (listed + more > kList) return false;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const uint64_t lanes = __builtin_amdgcn_ballot_w64(takes(e));
+                if (takes(e)) list[listed + lanes_below(lanes)] = key_of(v[e], q * N + e - head);
+                listed += __builtin_popcountll(lanes);
+            }
+            return true;
+        };
+        const uint64_t wide = __builtin_amdgcn_ballot_w64(second >= tau && second > kNegInf);
+        const uint64_t narrow = __builtin_amdgcn_ballot_w64(best >= tau && best > kNegInf) & ~wide;
+        const int n_wide = __builtin_popcountll(wide), n_narrow = __builtin_popcountll(narrow);
+        const int tiles = q_first < q_end ? (q_end - q_first + kTile - 1) / kTile : 0;
+        bool fits = true;
+        if (narrow >> lane & 1) s_at[wave][lanes_below(narrow)] = best_at + lane;
+        if (wide >> lane & 1) s_at[wave][n_narrow + lanes_below(wide)] = q_first + lane;
+        wave_lds_sync();
+        // Lane's piece in round r: first one tile of each narrow lane, U pieces of it side by side, then all tiles
+        // of each wide one, 64 pieces a round. Rounds load kAhead at a time.
+        constexpr int kAhead = 4;
+        const int first_wide = (n_narrow * U + 63) / 64, per_wide = (tiles * U + 63) / 64;
+        const int rounds = first_wide + n_wide * per_wide;
+        auto piece = [&](int r, bool& live) {
+            if (r < first_wide) {
+                const int mine = (64 * r + lane) / U;
+                live = mine < n_narrow;
+                return s_at[wave][live ? mine : 0] + 64 * (lane % U);
+            }
+            const int j = (r - first_wide) % per_wide * 64 + lane;
+            live = j < tiles * U;
+            return s_at[wave][n_narrow + (r - first_wide) / per_wide] + j / U * kTile + 64 * (j % U);
+        };
+        // (Of a lone tile every lane still has its piece.)
+        const bool lone = U == 1 && tiles == 1;
+        if (lone) fits = push(q_first + lane, q_first + lane < q_end, raw[0]);
+        for (int r0 = 0; fits && !lone && r0 < rounds; r0 += kAhead) {
+            Vec16 ahead[kAhead];
+            int q[kAhead];
+            bool live[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                live[i] = false;
+                q[i] = r0 + i < rounds ? piece(r0 + i, live[i]) : 0;
+                live[i] = live[i] && q[i] < q_end;
+                if (inner(q[i], live[i])) ahead[i] = load16(base + (int64_t)q[i] * N);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (fits && r0 + i < rounds) fits = push(q[i], live[i], ahead[i]);
+        }
+        if (!fits) {
+            // Everything once more, of what equals tau the first k.
+            listed = 0;
+            int equal = 0;
+            for (int q0 = q_first; q0 < q_end; q0 += kTile) {
+                load(q0, raw);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float v[N];
+                    values(q0, u, raw[u], v);
+                    const bool more_equal = equal < a.top;
+                    auto takes = [&](int e) { return v[e] > tau || (more_equal && v[e] == tau && v[e] > kNegInf); };
+                    int more = 0;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(takes(e)));
+                    if (more == 0) continue;
+                    if (listed + more > kList) shorten();
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const uint64_t lanes = __builtin_amdgcn_ballot_w64(takes(e));
+                        if (takes(e)) list[listed + lanes_below(lanes)] = key_of(v[e], (q0 + lane + 64 * u) * N + e - head);
+                        listed += __builtin_popcountll(lanes);
+                        equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[e] == tau));
+                    }
+                }
+            }
+        }
+        // A wave's share of s_merged at most.
+        if (listed > kMerged / kWaves) shorten();
         wave_lds_sync();
         int at = 0;
         if (lane == 0) at = atomicAdd(&s_n, listed);
@@ -430,13 +476,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void t
             if (tid < 64) s_entries[tid] = (int)entries;
             __syncthreads();
             uint64_t* joined = &s_list[0][0];      // parts * top <= 32 * 64 of kWaves * kList
-            // A part's list holds its k largest, in order. The largest last entry of a full list bounds
-            // the row's k-th from below.
-            uint64_t least = lane < a.parts && (int)(uint32_t)entries == a.top ? get(lane, 2 + a.top) : 0;
-            for (int off = 1; off < 64; off *= 2) {
-                const uint64_t o = __shfl_xor((unsigned long long)least, off);
-                least = o > least ? o : least;
-            }
+            // A part's list holds its k largest, in order. Where the m-th entries of k / m lists reach a value, k
+            // logits do: with m for half of the lists that there are, a bound that lets hardly more than twice
+            // k pass.
+            const int its_n = (int)(uint32_t)entries, lists = __builtin_popcountll(__builtin_amdgcn_ballot_w64(its_n > 0));
+            const int half = lists > 0 ? (2 * a.top + lists - 1) / lists : 1, m = half < a.top ? half : a.top;
+            const float mth = lane < a.parts && its_n >= m ? logit_of(get(lane, 2 + m)) : kNegInf;
+            const float bound = kth_of_lanes<1>(&mth, (a.top + m - 1) / m);
+            const uint64_t least = bound > kNegInf ? (uint64_t)order_of(bound) << 32 : 0;
             for (int i = tid; i < a.parts * a.top; i += 256) {
                 const int p = i / a.top, e = i - p * a.top;
                 const uint64_t key = get(p, 3 + e);
