@@ -213,18 +213,21 @@ TreePlan tree_plan(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, in
     const int64_t group = num_heads / num_kv_heads;
     const int64_t most = (max_query_len && max_query_len < num_tokens ? max_query_len : num_tokens) * group;
     const bool f32 = dtype == PKV_FLOAT32;
-    // (fp32 rows above 64 dims: 128 keys do not fit LDS twice.)
+    const int64_t wave_rows = f32 ? 16 : 32;
+    // (fp32: its tiles of 32 keys have no 16 for each of four waves, and two workgroups of 16 rows beat one of 32.)
     plan.row_waves = most <= 32 && (!f32 || head_dim <= 64) ? 1 : most <= 64 ? 2 : 4;
     if (!ctx || !qlen || num_seqs > kPrefillSortSeqs) return plan;
-    const int rows_of_wg = 32 * plan.row_waves, keys = plan.row_waves == 1 ? 128 : 64;
+    const int64_t rows_of_wg = wave_rows * plan.row_waves;
+    const int64_t keys = f32 ? (head_dim <= 64 ? 64 : 32) : plan.row_waves == 1 ? 128 : 64;
     // Workgroups that the GPU holds, by LDS and by registers; us a tile, alone and in a full GPU.
     const int64_t lds = (f32 ? 16 : 8) * keys * head_dim;
     const int64_t slots = 256 * (lds <= 72 * 1024 ? 2 : 1);
     float alone = plan.row_waves == 4 ? 1.4f : 1.2f;
     float full = plan.row_waves == 4 ? 2.4f : (float)(slots * lds / 2) / 5.5e6f;
     if (f32) {
-        alone = (plan.row_waves == 4 ? 0.055f : 0.028f) * head_dim;
-        full = full > 2 * alone ? full : alone * (slots / 256);
+        // 64 keys of 16 rows: 2 * 64 * 16 * head_dim products at 64 a cycle, shared by the waves of the rows.
+        alone = 0.5f + (float)(keys * head_dim) * plan.row_waves / 4.f * 2.2e-4f;
+        full = 2.f * alone - 0.5f;
     }
     auto launch_us = [&](int64_t wgs, int64_t longest, int64_t work) {
         const float fill = wgs < slots ? (float)wgs / slots : 1.f;
@@ -282,7 +285,8 @@ bool tree_tiled(const TreeParams& p, int dtype) {
     // They mask to -inf and take the maximum before they scale.
     if (!(p.scale > 0.f)) return false;
     // One grid dimension; keys and rows of a sequence in 32 bits.
-    if (tree_workgroups(p, 32 * p.row_waves) > 0x7fffffff || p.table_width * p.block_size > (1 << 30)) return false;
+    const int rows_of_wg = (dtype == PKV_FLOAT32 ? 16 : 32) * p.row_waves;
+    if (tree_workgroups(p, rows_of_wg) > 0x7fffffff || p.table_width * p.block_size > (1 << 30)) return false;
     if (((int64_t)p.max_query_len + 128) * p.group > 0x7fffffff) return false;
     const uint64_t probe = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.k | (uint64_t)(uintptr_t)p.v |
                            (uint64_t)(uintptr_t)p.out | (uint64_t)(p.q_st * isz) | (uint64_t)(p.q_sh * isz) |
@@ -389,7 +393,7 @@ extern "C" int pkv_tree_attention(
         p.ws_o = reinterpret_cast<float*>(ws + plan.rows_bytes + plan.ml_bytes);
     }
     switch (dtype) {
-        case PKV_FLOAT32: return launch_tree_mfma<float>(p, stream);
+        case PKV_FLOAT32: return launch_tree_f32(p, stream);
         case PKV_FLOAT16: return launch_tree_mfma<_Float16>(p, stream);
         default: return launch_tree_mfma<bf16_t>(p, stream);
     }

@@ -152,9 +152,13 @@ __device__ __forceinline__ bool tree_item(const TreeParams& p, PrefillItem& r) {
     return true;
 }
 
-// The matrix kernels (tree_mfma.h).
+// The matrix kernels: 16-bit pools (tree_mfma.h), rows of 32 a wave, and fp32 pools (attn_tree_f32.hip), of 16.
 template <typename T>
 int launch_tree_mfma(const TreeParams& p, hipStream_t stream);
+int launch_tree_f32(const TreeParams& p, hipStream_t stream);
+// Keys of an fp32 tile: two workgroups a CU.
+template <int D>
+constexpr int kTreeKeysF32 = D <= 64 ? 64 : 32;
 
 // The kernel for any shape.
 int launch_tree_generic(const TreeParams& p, int dtype, hipStream_t stream);

@@ -1,5 +1,5 @@
 // Attention of drafted token trees on MFMA (gfx950): the kernel, instantiated by type in
-// attn_tree_*.hip. fp16, bf16 and fp32 pools, head_dim a multiple of 16 from 32 to 128, any GQA group, block sizes that are powers
+// attn_tree_*.hip. fp16 and bf16 pools, head_dim a multiple of 16 from 32 to 128, any GQA group, block sizes that are powers
 // of two from 8 up, softmax scale > 0.
 //
 // The formulation is the prefill kernel's (attn_prefill.hip): rows are (token, query head) pairs of a
@@ -18,124 +18,33 @@
 //    output turned NaN under finite weights (0 * infinity, or an infinity times two pieces of opposite
 //    signs), walks its keys once more at the end and puts into each row's dims what it sees of them.
 //
-// 16-bit pools: weights enter the second product as two pieces of the type (16 bits of them at least: one
+// Weights enter the second product as two pieces of the type (16 bits of them at least: one
 // alone is off by up to 2^-9 of a weight in bf16, as much as the output's rounding).
-// fp32 pools: both products on 32x32x2, nothing below fp32. A step of the first contracts element s (lanes
-// 0-31) and s + D / 2 (lanes 32-63), so that one 16-byte LDS read of a K row feeds four steps; register r of
-// its result is the operand of one step of the second, over keys 8 (r / 4) + r % 4 and that + 4, as it is.
 #pragma once
 
-#include <type_traits>
-
-#include "prefill_common.h"
-#include "tree.h"
+#include "tree_common.h"
 
 namespace pkv {
 namespace {
-
-__device__ __forceinline__ uint32_t lds_u32(const void* p) {
-    return (uint32_t)(uintptr_t)((const __attribute__((address_space(3))) char*)p);
-}
-// 16 bytes per lane by LDS DMA to LDS address lds + 16 lane (M0 = lds), from the uniform base sbase plus
-// the lane's 32-bit offset, or from the lane's own 64-bit address; inline asm, hidden from the
-// compiler's wait counting, which would wait for it before every LDS read. M0 is reserved to the
-// compiler (a clobber of it is not honoured): all LDS DMAs of these kernels go through these helpers.
-__device__ __forceinline__ void dma16(const char* sbase, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(lds), "v"(voff), "s"(sbase)
-                 : "memory");
-}
-__device__ __forceinline__ void dma16(const char* addr, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-                 :
-                 : "s"(lds), "v"(addr)
-                 : "memory");
-}
-
-// A 32-bit word of the pool (two elements of a 16-bit type) with those elements that are not finite, whose
-// exponent bits are all set, as zeros.
-template <typename T>
-__device__ __forceinline__ uint32_t finite_of(uint32_t w) {
-    if constexpr (sizeof(T) == 4) {
-        return (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
-    } else {
-        constexpr uint32_t E = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
-        const uint32_t lo = (w & E) == E ? 0u : 0xffffu, hi = (w >> 16 & E) == E ? 0u : 0xffff0000u;
-        return w & (lo | hi);
-    }
-}
-
-// Four elements of a pool row.
-template <typename T>
-struct Four {
-    uint32_t w[sizeof(T)];
-    __device__ __forceinline__ static Four load(const T* p) {
-        Four f;
-        if constexpr (sizeof(T) == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            f.w[0] = v.x; f.w[1] = v.y; f.w[2] = v.z; f.w[3] = v.w;
-        } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            f.w[0] = v.x; f.w[1] = v.y;
-        }
-        return f;
-    }
-    // x + its elements that are not finite.
-    __device__ __forceinline__ float4 add_rest(float4 x) const {
-        uint32_t r[sizeof(T)];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T); ++i) r[i] = w[i] ^ finite_of<T>(w[i]);
-        if constexpr (sizeof(T) == 4) {
-            auto f = [](uint32_t b) { return __builtin_bit_cast(float, b); };
-            return make_float4(x.x + f(r[0]), x.y + f(r[1]), x.z + f(r[2]), x.w + f(r[3]));
-        } else {
-            return make_float4(x.x + Pair<T>::lo(r[0]), x.y + Pair<T>::hi(r[0]), x.z + Pair<T>::lo(r[1]),
-                               x.w + Pair<T>::hi(r[1]));
-        }
-    }
-};
-
-__device__ __forceinline__ f32x16 mfma_f32(float a, float b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
-}
-
-// XOR swizzles of a row's 16-byte chunks in LDS. 16 bits: lds_swizzle, for both. fp32: a K read takes one
-// chunk of 16 rows, which rows of whole bank sweeps (D = 64, 128) put into one bank but for this, others every
-// 2nd or 4th row; a V read takes 32 consecutive elements of two rows 4 apart (free of conflicts at 64 and 128).
-template <typename T, int D>
-__device__ __forceinline__ int k_swizzle(int r) {
-    if constexpr (sizeof(T) == 2) return lds_swizzle<D>(r);
-    else if constexpr (D % 64 == 0) return r & 15;
-    else if constexpr (D % 32 == 0) return (r >> 1) & 7;
-    else return (r >> 2) & 3;
-}
-template <typename T, int D>
-__device__ __forceinline__ int v_swizzle(int r) {
-    if constexpr (sizeof(T) == 2) return lds_swizzle<D>(r);
-    else if constexpr (D % 64 == 0) return 8 * ((r >> 2) & 1);
-    else return 0;
-}
 
 // Keys of a tile.
 template <int RW>
 constexpr int kTreeTile = RW == 1 ? 128 : 64;
 
 // Waves a SIMD: LDS has room for two workgroups a CU, or for one.
-template <typename T, int D, int RW>
-constexpr int kTreeWaves = 4 * kTreeTile<RW> * D * (int)sizeof(T) <= 72 * 1024 ? 2 : 1;
+template <int D, int RW>
+constexpr int kTreeWaves = 8 * kTreeTile<RW> * D <= 72 * 1024 ? 2 : 1;
 
 template <typename T, int D, int RW>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<T, D, RW>))) void tree_mfma_kernel(const TreeParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<D, RW>))) void tree_mfma_kernel(const TreeParams p) {
     static_assert(D % 16 == 0 && D >= 32 && D <= 128, "head_dim");
     constexpr int KW = 4 / RW;                // waves that share a tile's keys
     constexpr int KT = kTreeTile<RW>;
     constexpr int NH = KT / 32 / KW;          // 32-key halves of a wave and tile
     constexpr int ROWS = 32 * RW;
-    constexpr bool F32 = sizeof(T) == 4;
-    constexpr int KREADS = F32 ? D / 8 : D / 16;   // 16-byte reads of a K row by a lane
+    constexpr int KREADS = D / 16;            // 16-byte reads of a K row by a lane: S^T contraction steps
     constexpr int DTILES = (D + 31) / 32;     // O^T tiles of 32 dims (the last may be half a tile)
-    constexpr int ROWB = D * (int)sizeof(T);  // bytes of a K/V row
+    constexpr int ROWB = D * 2;               // bytes of a K/V row
     constexpr int CPR = ROWB / 16;            // its 16-byte chunks
     constexpr int G16 = KT / 64;              // groups of 16 keys that a wave stages
     constexpr int IPB = (16 * CPR + 63) / 64; // DMA instructions of a group, of K or V
@@ -198,14 +107,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
         return table[b < nb_last ? b : nb_last];
     };
     auto dma_row = [&](int j) { return (64 * j + lane) / CPR; };
-    auto k_chunk = [&](int j) { return 16 * ((64 * j + lane) % CPR ^ k_swizzle<T, D>(dma_row(j))); };
-    auto v_chunk = [&](int j) { return 16 * ((64 * j + lane) % CPR ^ v_swizzle<T, D>(dma_row(j))); };
-    uint32_t k_off[IPB], v_off[IPB];
+    auto dma_chunk = [&](int j) { return 16 * ((64 * j + lane) % CPR ^ lds_swizzle<D>(dma_row(j))); };
+    uint32_t lane_off[IPB];
 #pragma unroll
-    for (int j = 0; j < IPB; ++j) {
-        k_off[j] = (uint32_t)((dma_row(j) & 7) * slot_bytes) + (uint32_t)k_chunk(j);
-        v_off[j] = (uint32_t)((dma_row(j) & 7) * slot_bytes) + (uint32_t)v_chunk(j);
-    }
+    for (int j = 0; j < IPB; ++j) lane_off[j] = (uint32_t)((dma_row(j) & 7) * slot_bytes) + (uint32_t)dma_chunk(j);
     const bool offs_fit = 8 * slot_bytes + ROWB <= (int64_t)0xffffffff;
     // (Inlined by force: as calls, lambdas get their captures through memory.)
     auto dma_tile = [&](int kt, int64_t ids, uint32_t sk, uint32_t sv) __attribute__((always_inline)) {
@@ -223,12 +128,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
                 for (int j = 0; j < IPB; ++j) {
                     if constexpr (kHalfDma) {
                         const int64_t half = 64 * j / CPR < 8 ? half0 : half1;
-                        dma16(kbase + half, k_off[j], dk + j * 1024);
-                        dma16(vbase + half, v_off[j], dv + j * 1024);
+                        dma16(kbase + half, lane_off[j], dk + j * 1024);
+                        dma16(vbase + half, lane_off[j], dv + j * 1024);
                     } else if (kWholeDma || 64 * j + lane < 16 * CPR) {
                         const int64_t half = dma_row(j) < 8 ? half0 : half1;
-                        dma16(kbase + half + k_off[j], dk + j * 1024);
-                        dma16(vbase + half + v_off[j], dv + j * 1024);
+                        dma16(kbase + half + lane_off[j], dk + j * 1024);
+                        dma16(vbase + half + lane_off[j], dv + j * 1024);
                     }
                 }
                 continue;
@@ -243,8 +148,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
                 if ((uint64_t)id < (uint64_t)p.num_blocks && first + r < kmax)
                     off = (r < 8 ? half0 : half1) + (int64_t)(r & 7) * slot_bytes;
                 if (kWholeDma || 64 * j + lane < 16 * CPR) {
-                    dma16(kbase + off + k_chunk(j), dk + j * 1024);
-                    dma16(vbase + off + v_chunk(j), dv + j * 1024);
+                    dma16(kbase + off + dma_chunk(j), dk + j * 1024);
+                    dma16(vbase + off + dma_chunk(j), dv + j * 1024);
                 }
             }
         }
@@ -254,122 +159,71 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
     const int grp = lane >> 4;
     const int tr_key = (lane & 15) >> 2;
     const int tr_col = 16 * (grp & 1) + 4 * (lane & 3);
-    const int k_swz = k_swizzle<T, D>(col);
+    const int k_swz = lds_swizzle<D>(col);
     const int v_cb = tr_col >> 3;
-    const int v_byte = 8 * (lane & 1);
+    const int v_row = 4 * (grp >> 1) + tr_key, v_byte = 8 * (lane & 1);
     const uint32_t wave_off = (uint32_t)(kw * NH * 32 * ROWB);   // of the wave's keys
     uint32_t koff[KREADS], voff_lo[DTILES], voff_hi[DTILES];
 #pragma unroll
     for (int s = 0; s < KREADS; ++s) {
-        const int c = F32 ? s + h * (CPR / 2) : 2 * s + h;
-        koff[s] = wave_off + (uint32_t)(col * ROWB + ((c ^ k_swz) << 4));
+        koff[s] = wave_off + (uint32_t)(col * ROWB + (((2 * s + h) ^ k_swz) << 4));
         asm volatile("" : "+v"(koff[s]));
     }
 #pragma unroll
     for (int t = 0; t < DTILES; ++t) {
-        // Columns past head_dim re-read the tile's first ones: output rows never stored.
-        if constexpr (F32) {
-            // V[4 h (+ a key group's)][32 t + col], of even and odd groups of four keys: their swizzles differ.
-            const int d = 32 * t + col < D ? 32 * t + col : 32 * t + (col & 15);
-            auto at = [&](int r) { return wave_off + (uint32_t)(r * ROWB + (((d >> 2) ^ v_swizzle<T, D>(r)) << 4) + 4 * (d & 3)); };
-            voff_lo[t] = at(4 * h);
-            voff_hi[t] = 0;
-        } else {
-            const int c = 4 * t + v_cb < CPR ? 4 * t + v_cb : 4 * t + (v_cb & 1);
-            const int r = 4 * (grp >> 1) + tr_key;
-            voff_lo[t] = wave_off + (uint32_t)(r * ROWB + v_byte + ((c ^ v_swizzle<T, D>(r)) << 4));
-            voff_hi[t] = wave_off + (uint32_t)((r + 8) * ROWB + v_byte + ((c ^ v_swizzle<T, D>(r + 8)) << 4));
-            asm volatile("" : "+v"(voff_hi[t]));
-        }
-        asm volatile("" : "+v"(voff_lo[t]));
+        // Columns past head_dim re-read the tile's first chunks: output rows never stored.
+        const int c = 4 * t + v_cb < CPR ? 4 * t + v_cb : 4 * t + (v_cb & 1);
+        voff_lo[t] = wave_off + (uint32_t)(v_row * ROWB + v_byte + ((c ^ lds_swizzle<D>(v_row)) << 4));
+        voff_hi[t] = wave_off + (uint32_t)((v_row + 8) * ROWB + v_byte + ((c ^ lds_swizzle<D>(v_row + 8)) << 4));
+        asm volatile("" : "+v"(voff_lo[t]), "+v"(voff_hi[t]));
     }
 
     int64_t ids = 0;
     if (t_begin < t_end) ids = tile_ids(t_begin);
-    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7]; fp32: elements 4 s + (D / 2) h .. + 3.
+    // Q^T: lane supplies Q[its row][16 s + 8 h .. + 7].
     u32x4 qfrag[KREADS];
     {
         const T* qrow = reinterpret_cast<const T*>(p.q) + (q_first + my_q) * p.q_st + (int64_t)my_head * p.q_sh;
 #pragma unroll
         for (int s = 0; s < KREADS; ++s) {
-            const Vec16 v = load16(qrow + (F32 ? 4 * s + h * (D / 2) : 16 * s + 8 * h));
+            const Vec16 v = load16(qrow + 16 * s + 8 * h);
             qfrag[s] = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
         }
     }
     if (threadIdx.x == 0) s_taken = 0;
 
-    // Of the 32 keys from key0 on, those that the lane's row sees.
     const uint64_t* mask = p.masks + (q_first + my_q) * p.mask_stride;
-    auto window = [&](int key0) -> uint32_t {
-        const int node = key0 - pos0, left = kmax - key0;
-        auto word = [&](int i) { return i < p.mask_words ? mask[i] : 0ull; };
-        uint32_t w = ~0u;
-        if (node >= 0) {
-            const int sh = node & 63;
-            const uint64_t lo = word(node >> 6) >> sh;
-            w = (uint32_t)(sh > 32 ? lo | word((node >> 6) + 1) << (64 - sh) : lo);
-        } else if (node > -32) {
-            w = (uint32_t)(word(0) << -node) | ((1u << -node) - 1);
-        }
-        return left >= 32 ? w : left <= 0 ? 0u : w & ((1u << left) - 1);
-    };
+    auto window = [&](int key0) __attribute__((always_inline)) { return tree_window(mask, p.mask_words, key0, pos0, kmax); };
 
     auto tile = [&](auto tail, int kt, const char* tile_k, char* tile_v, uint32_t nk) __attribute__((always_inline)) {
         constexpr bool drafted = decltype(tail)::value;          // keys past the cached ones among the tile's
         __builtin_amdgcn_s_waitcnt(0);
         lds_barrier();                        // tile kt is staged, tile kt - 1 is done with
+        if (kt + 1 < t_end) {
+            dma_tile(kt + 1, ids, nk, nk + KT * ROWB);
+            ids = tile_ids(kt + 2);
+        }
         f32x16 st[NH];
         __builtin_amdgcn_s_setprio(1);
         if (has_rows) {
 #pragma unroll
             for (int i = 0; i < NH; ++i) st[i] = f32x16{};
-            if constexpr (F32) {
+            u32x4 kf[NH][KREADS];
 #pragma unroll
-                for (int s = 0; s < KREADS; ++s)
+            for (int i = 0; i < NH; ++i)
 #pragma unroll
-                    for (int i = 0; i < NH; ++i) {
-                        const uint4 a = *reinterpret_cast<const uint4*>(tile_k + i * 32 * ROWB + koff[s]);
-                        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+                for (int s = 0; s < KREADS; ++s) {
+                    const uint4 a = *reinterpret_cast<const uint4*>(tile_k + i * 32 * ROWB + koff[s]);
+                    kf[i][s] = u32x4{a.x, a.y, a.z, a.w};
+                }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t qe = qfrag[s][e];
-                            st[i] = mfma_f32(__builtin_bit_cast(float, w[e]), __builtin_bit_cast(float, qe), st[i]);
-                        }
-                    }
-            } else {
-                u32x4 kf[NH][KREADS];
+            for (int s = 0; s < KREADS; ++s)
 #pragma unroll
-                for (int i = 0; i < NH; ++i)
-#pragma unroll
-                    for (int s = 0; s < KREADS; ++s) {
-                        const uint4 a = *reinterpret_cast<const uint4*>(tile_k + i * 32 * ROWB + koff[s]);
-                        kf[i][s] = u32x4{a.x, a.y, a.z, a.w};
-                    }
-#pragma unroll
-                for (int s = 0; s < KREADS; ++s)
-#pragma unroll
-                    for (int i = 0; i < NH; ++i) st[i] = Mfma<T>::run(kf[i][s], qfrag[s], st[i]);
-            }
+                for (int i = 0; i < NH; ++i) st[i] = Mfma<T>::run(kf[i][s], qfrag[s], st[i]);
         }
         __builtin_amdgcn_s_setprio(0);
-        if (kt + 1 < t_end) {
-            dma_tile(kt + 1, ids, nk, nk + KT * ROWB);
-            ids = tile_ids(kt + 2);
-        }
         if constexpr (drafted) {
-            // V of keys past the last one, and elements that are not finite: out. (Cached keys are seen
-            // by all rows.)
-            for (int c = (int)threadIdx.x; c < KT * CPR; c += 256) {
-                const int r = c / CPR, key = kt * KT + r;
-                if (key < pos0) continue;
-                uint4* at = reinterpret_cast<uint4*>(tile_v) + c;
-                const uint4 v = *at;
-                const uint4 f = key < kmax ? make_uint4(finite_of<T>(v.x), finite_of<T>(v.y), finite_of<T>(v.z), finite_of<T>(v.w))
-                                           : make_uint4(0, 0, 0, 0);
-                if (f.x == v.x && f.y == v.y && f.z == v.z && f.w == v.w) continue;
-                *at = f;
-                if (key < kmax) s_taken = 1;
-            }
+            tree_take_out<T, KT, CPR>(tile_v, kt * KT, pos0, kmax, s_taken);
             lds_barrier();
         }
         if (!has_rows) return;
@@ -409,38 +263,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             }
         psum = sum_across32(psum);
         l_run = l_run * alpha + psum;
-        if constexpr (F32) {
 #pragma unroll
-            for (int i = 0; i < NH; ++i)
+        for (int s = 0; s < 2 * NH; ++s) {
+            f32x16& sv = st[s >> 1];
+            const int r0 = 8 * (s & 1);
+            u32x4 pb[2];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    // Rows of the group 8 (r / 4): its swizzle is that of row 4 h, as 8 rows on.
-                    const char* vrow = tile_v + (i * 32 + 8 * (r >> 2) + (r & 3)) * ROWB;
+            for (int e = 0; e < 4; ++e) {
+                const float x = sv[r0 + 2 * e], y = sv[r0 + 2 * e + 1];
+                const uint32_t w = Mfma<T>::pack(x, y);
+                pb[0][e] = w;
+                pb[1][e] = Mfma<T>::pack(x - Pair<T>::lo(w), y - Pair<T>::hi(w));
+            }
+            const char* vgrp = tile_v + ((s >> 1) * 32 + 16 * (s & 1)) * ROWB;
 #pragma unroll
-                    for (int t = 0; t < DTILES; ++t)
-                        o[t] = mfma_f32(*reinterpret_cast<const float*>(vrow + voff_lo[t]), st[i][r], o[t]);
-                }
-        } else {
+            for (int t = 0; t < DTILES; ++t) {
+                const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_lo[t]));
+                const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_hi[t]));
 #pragma unroll
-            for (int s = 0; s < 2 * NH; ++s) {
-                f32x16& sv = st[s >> 1];
-                const int r0 = 8 * (s & 1);
-                u32x4 pb[2];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x = sv[r0 + 2 * e], y = sv[r0 + 2 * e + 1];
-                    const uint32_t w = Mfma<T>::pack(x, y);
-                    pb[0][e] = w;
-                    pb[1][e] = Mfma<T>::pack(x - Pair<T>::lo(w), y - Pair<T>::hi(w));
-                }
-                const char* vgrp = tile_v + ((s >> 1) * 32 + 16 * (s & 1)) * ROWB;
-#pragma unroll
-                for (int t = 0; t < DTILES; ++t) {
-                    const uint2 lo = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_lo[t]));
-                    const uint2 hi = lds_read_tr16(reinterpret_cast<const uint16_t*>(vgrp + voff_hi[t]));
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) o[t] = Mfma<T>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
-                }
+                for (int i = 0; i < 2; ++i) o[t] = Mfma<T>::run(u32x4{lo.x, lo.y, hi.x, hi.y}, pb[i], o[t]);
             }
         }
     };
@@ -580,8 +421,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
         if (u % KW != kw) continue;
         const float4 x = make_float4(o[u / 4][4 * (u % 4)] * inv, o[u / 4][4 * (u % 4) + 1] * inv,
                                      o[u / 4][4 * (u % 4) + 2] * inv, o[u / 4][4 * (u % 4) + 3] * inv);
-        if constexpr (F32) *reinterpret_cast<float4*>(orow + 8 * u) = x;
-        else *reinterpret_cast<uint2*>(orow + 8 * u) = make_uint2(Mfma<T>::pack(x.x, x.y), Mfma<T>::pack(x.z, x.w));
+        *reinterpret_cast<uint2*>(orow + 8 * u) = make_uint2(Mfma<T>::pack(x.x, x.y), Mfma<T>::pack(x.z, x.w));
     }
 }
 
@@ -598,9 +438,7 @@ int launch_tree_rows(const TreeParams& p, hipStream_t stream) {
 template <typename T, int D>
 int launch_tree_d(const TreeParams& p, hipStream_t stream) {
     switch (p.row_waves) {
-        case 1:
-            // (fp32 rows above 64 dims: 128 keys do not fit LDS, tree_plan does not ask for it.)
-            if constexpr (sizeof(T) == 2 || D <= 64) return launch_tree_rows<T, D, 1>(p, stream);
+        case 1: return launch_tree_rows<T, D, 1>(p, stream);
         case 2: return launch_tree_rows<T, D, 2>(p, stream);
         default: return launch_tree_rows<T, D, 4>(p, stream);
     }
