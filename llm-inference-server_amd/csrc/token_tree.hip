@@ -48,16 +48,22 @@ __global__ __launch_bounds__(256) void tree_layout_kernel(const int64_t* __restr
         positions[row] = 0;
     };
     if ((int)blockIdx.x >= num_seqs) {
-        // Rows of no sequence, and those of a sequence with more nodes than there is room for.
-        const int64_t end = num_seqs > 0 ? starts[num_seqs] : 0;
-        const int64_t from = end < 0 ? 0 : end;
+        // Rows of no sequence: before the first one and past the last.
+        auto in_step = [&](int64_t r) { return r < 0 ? 0 : r < num_tokens ? r : num_tokens; };
+        const int64_t before = num_seqs > 0 ? in_step(starts[0]) : 0, from = num_seqs > 0 ? in_step(starts[num_seqs]) : 0;
         const int64_t step = (int64_t)(gridDim.x - num_seqs) * n_threads;
-        for (int64_t r = from + (int64_t)(blockIdx.x - num_seqs) * n_threads + tid; r < num_tokens; r += step) none(r);
+        for (int64_t i = (int64_t)(blockIdx.x - num_seqs) * n_threads + tid; i < before + num_tokens - from; i += step)
+            none(i < before ? i : from + i - before);
         return;
     }
     const int seq = (int)blockIdx.x;
     const Nodes at = nodes_of(starts, seq, num_tokens, num_tokens);
-    if (at.count == 0) return;
+    if (at.count == 0) {
+        // (Bounds outside the step: what of its rows are inside.)
+        const int64_t a = starts[seq], b = starts[seq + 1];
+        for (int64_t r = (a < 0 ? 0 : a) + tid; r < (b < num_tokens ? b : num_tokens); r += n_threads) none(r);
+        return;
+    }
     const int64_t cached = ctx[seq] - at.count;
     if (at.count > max_nodes || cached < 0) {
         for (int i = tid; i < at.count; i += n_threads) none(at.first + i);

@@ -290,7 +290,8 @@ class PagedKVPool:
         [B + 1], paths [B, P] (accept_tree's): int64, on the pool's device. A path ascends; it ends at the
         first number that is not above the one before, or not of a node. Rows in blocks outside the
         pool or the table stay. The blocks of a sequence's drafted rows are its own
-        (BlockTable.make_writable)."""
+        (BlockTable.make_writable). Captured into a graph it has to have run before, or
+        pointer_table(), which copies from the host. ATTENTION=hip: 65,535 sequences at most."""
         if block_tables.dim() != 2:
             raise ValueError(f"block_tables must be [batch, width], got {tuple(block_tables.shape)}")
         batch, width = block_tables.shape
@@ -313,6 +314,8 @@ class PagedKVPool:
             self._keep_torch(block_tables, context_lens, query_start, paths)
             return
         with native.on_device(pool.device):
+            if self._ptr_table is None and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("keep_paths: the pool's pointer_table() has to be there before a capture")
             if block_tables.stride(1) != 1:
                 block_tables = block_tables.contiguous()
             context_lens, query_start, paths = (t.contiguous() for t in (context_lens, query_start, paths))

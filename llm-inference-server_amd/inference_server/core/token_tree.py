@@ -79,9 +79,9 @@ def tree_layout(parents: torch.Tensor, query_start: torch.Tensor, context_lens: 
     [B + 1]: the sequences' first rows (step_layout's); context_lens [B]: tokens cached after the
     step, the nodes among them. max_nodes: the most nodes of a sequence, 8,192 at most. All int64.
 
-    Masks of 0 and position 0 for rows past the last sequence, for a node whose parent is not
+    Masks of 0 and position 0 for rows of no sequence, for a node whose parent is not
     before it and the nodes below that one, and for sequences with more nodes than max_nodes or
-    than their context: the host does not read the lengths back to refuse them."""
+    than their context, or rows past the last token: the host does not read the lengths back to refuse them."""
     tokens, batch = _check_rows((("parents", parents),), query_start)
     if context_lens.dim() != 1 or context_lens.shape[0] != batch:
         raise ValueError(f"context_lens must be [{batch}] to match query_start, got {tuple(context_lens.shape)}")
@@ -148,7 +148,8 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
 
     tokens, parents, targets [T]: the nodes' tokens, their parents' numbers, and the target's token
     after each node (its argmax, or a sample); query_start [B + 1]; all int64. At most
-    max_depth nodes are accepted. A sequence without nodes has count 0 and next token -1."""
+    max_depth nodes are accepted. A sequence without nodes, or with more than 8,192, has count 0 and next
+    token -1."""
     n_tok, batch = _check_rows((("tokens", tokens), ("parents", parents), ("targets", targets)), query_start)
     if not 1 <= max_depth <= MAX_NODES:
         raise ValueError(f"max_depth must be between 1 and {MAX_NODES}, got {max_depth}")

@@ -4,6 +4,7 @@ the kernel."""
 from __future__ import annotations
 
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -180,6 +181,61 @@ def test_logits_of_any_size(device, dtype, n):
     for r in range(9) if n == 1 else ():
         one = token_logprobs(x[r:r + 1].to(device), ids[r:r + 1].to(device), 9)
         check(x[r:r + 1], ids[r:r + 1], one, 9)
+
+
+def test_many_short_rows(device):
+    x, ids = rows(70_000 if device == "cuda" else 3000, 5, BF16)
+    check(x, ids, token_logprobs(x.to(device), ids.to(device), 5), 5)
+
+
+def test_one_row_for_all(device):
+    """Rows of stride 0."""
+    x, ids = rows(1, 9000, F32)
+    ids = torch.arange(40) * 200
+    x = x.expand(40, -1)
+    check(x, ids, token_logprobs(x[:1].to(device).expand(40, -1), ids.to(device), 3), 3)
+
+
+@pytest.mark.gpu
+def test_logits_past_2_31_elements(monkeypatch):
+    monkeypatch.setattr(CONFIG, "attention", "hip")
+    vocab, n = 50257, 43_000
+    x, ids = rows(2, vocab, F16)
+    big = torch.zeros(n, vocab, dtype=F16, device="cuda")
+    big[n - 2:] = x.cuda()
+    at = torch.zeros(n, dtype=torch.long, device="cuda")
+    at[n - 2:] = ids.cuda()
+    got = token_logprobs(big, at, 7)
+    check(x, ids, type(got)(*(t[n - 2:] for t in got)), 7)
+    same = type(got)(*(t[:1] for t in got))
+    check(torch.zeros(1, vocab), ids[:1] * 0, same, 7)
+    for t, s in zip(got, same):
+        assert torch.equal(t[:n - 2], s.expand_as(t[:n - 2]))
+
+
+@pytest.mark.gpu
+def test_calls_of_two_threads(monkeypatch):
+    """Threads with streams of their own, rows in pieces."""
+    monkeypatch.setattr(CONFIG, "attention", "hip")
+    cases = [tuple(t.cuda() for t in rows(3 + i, 50257, F16, i)) for i in range(2)]
+    want = [token_logprobs(*c, 10) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] += [token_logprobs(*cases[i], 10) for _ in range(30)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs, w in zip(got, want):
+        assert len(outs) == 30
+        for o in outs:
+            assert all(torch.equal(a, b) for a, b in zip(o, w))
 
 
 def test_refusals(device):

@@ -89,6 +89,66 @@ def test_layout_gives_impossible_nodes_nothing(device):
     assert not got.masks.any() and not got.positions.any()
 
 
+def test_layout_of_rows_that_no_sequence_has(device):
+    # Starts that leave rows before the first sequence, and that end behind the step.
+    parents = [0, 3, -1, 0, 1, -1, 0, 0, 1]
+    for starts, real in (([2, 5, 7], range(2, 7)), ([2, 5, 12], range(2, 5)), ([9, 9, 9], ()), ([12, 13, 20], ()),
+                         ([-3, 2, 5], range(2, 5)), ([0, 0, 5], ())):
+        got = tree_layout(long(parents, device), long(starts, device), long([9, 9], device), 4)
+        assert [t for t in range(9) if got.masks[t, 0]] == list(real), starts
+        assert not got.positions[[t for t in range(9) if t not in real]].any()
+
+
+@pytest.mark.gpu
+def test_a_captured_walk_follows_its_inputs(monkeypatch):
+    """Layout, path and the rows' move in one graph, replayed over other trees."""
+    monkeypatch.setattr(CONFIG, "attention", "hip")
+    counts, bs, depth = [9, 0, 40, 17], 8, 12
+    pools = [PagedKVPool(ModelDims(2, 2, 16, F16), num_blocks=40, block_size=bs, device="cuda") for _ in range(2)]
+
+    def case(seed):
+        tokens, parents, targets, starts = drafted(counts, seed)
+        rng = np.random.default_rng(seed)
+        ctx = rng.integers(0, 20, 4) + counts
+        return tokens, parents, targets, starts, ctx, rng.permutation(40).reshape(4, 10)
+
+    at = [long(x, "cuda") for x in case(0)]
+
+    def step(pool):
+        tokens, parents, targets, starts, ctx, tables = at
+        tree = tree_layout(parents, starts, ctx, 64)
+        path = accept_tree(tokens, parents, targets, starts, depth)
+        pool.keep_paths(tables, ctx, starts, path.paths)
+        return (*tree, *path)
+
+    stream, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream):
+        with pytest.raises(RuntimeError, match="pointer_table"), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            at[0] + 1                                     # (a graph of something)
+            step(pools[0])
+    torch.cuda.synchronize()
+    for pool in pools:
+        pool.pointer_table()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=stream):
+        outs = step(pools[0])
+    for seed in range(1, 6):
+        for dst, x in zip(at, case(seed)):
+            dst.copy_(long(x, "cuda"))
+        for pool in pools:
+            fill(pool, seed)
+        torch.cuda.synchronize()
+        g.replay()
+        want = step(pools[1])
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+        for a, b in zip(pools[0].k + pools[0].v, pools[1].k + pools[1].v):
+            assert np.array_equal(bits(a), bits(b))
+        tokens, parents, targets, starts, ctx, tables = case(seed)
+        assert np.array_equal(want[2].cpu().numpy(), oracle.accept(tokens, parents, targets, starts, depth)[0])
+
+
 def test_layout_refusals(device):
     p, s, c = long([-1, 0], device), long([0, 2], device), long([4], device)
     for bad in ((p[None], s, c, 2), (p, s[None], c, 2), (p, s, c[None], 2), (p.int(), s, c, 2), (p, s.int(), c, 2),
@@ -231,3 +291,20 @@ def test_keep_refusals(device):
                 (t.int(), c, s, p), (t, c, s.int(), p)):
         with pytest.raises(ValueError):
             pool.keep_paths(*bad)
+
+
+@pytest.mark.gpu
+def test_keep_refuses_more_sequences_than_a_grid_has(monkeypatch):
+    monkeypatch.setattr(CONFIG, "attention", "hip")
+    pool = PagedKVPool(ModelDims(1, 1, 8, F32), num_blocks=2, block_size=4, device="cuda")
+    before = [bits(t) for t in pool.k + pool.v]
+    for n in (65535, 65536):
+        args = (torch.zeros(n, 1, dtype=torch.long, device="cuda"), torch.full((n,), 4, device="cuda"),
+                torch.zeros(n + 1, dtype=torch.long, device="cuda"), torch.zeros(n, 2, dtype=torch.long, device="cuda"))
+        if n > 65535:
+            with pytest.raises(RuntimeError, match="keep_paths"):
+                pool.keep_paths(*args)
+        else:
+            pool.keep_paths(*args)                        # no nodes: nothing moves
+    for t, b in zip(pool.k + pool.v, before):
+        assert np.array_equal(bits(t), b)

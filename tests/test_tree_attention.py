@@ -4,6 +4,7 @@ exact attention over the keys that each token sees (64 bits)."""
 from __future__ import annotations
 
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -307,3 +308,32 @@ def test_a_call_repeats_bit_for_bit_on_any_stream(monkeypatch):
         torch.cuda.synchronize()
         for o in outs:
             assert torch.equal(o, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_calls_of_two_threads(monkeypatch, dtype):
+    """Threads with streams of their own, calls that cut their contexts."""
+    monkeypatch.setattr(CONFIG, "attention", "hip")
+    cases = [batch([(3000 + 500 * i, 5 + i), (70, 9)], heads=4, kv=1, d=64, bs=16, dtype=dtype, device="cuda", seed=i)
+             for i in range(2)]
+    want = [call(s) for s in cases]
+    for s, w in zip(cases, want):
+        check(s, w)
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] += [call(cases[i]) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs, w in zip(got, want):
+        assert len(outs) == 20
+        for o in outs:
+            assert torch.equal(o, w)
