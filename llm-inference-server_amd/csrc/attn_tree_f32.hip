@@ -206,8 +206,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void t
     }
     if (threadIdx.x == 0) s_taken = 0;
 
-    const uint64_t* mask = p.masks + (q_first + my_q) * p.mask_stride;
-    auto window = [&](int key0) __attribute__((always_inline)) { return tree_window(mask, p.mask_words, key0, pos0, kmax); };
+    const TreeRow seen(p.masks + (q_first + my_q) * p.mask_stride, t_end * KT > pos0 ? p.mask_words : 0);
+    auto window = [&](int key0) __attribute__((always_inline)) { return seen.window(p.mask_words, key0, pos0, kmax); };
 
     auto tile = [&](auto tail, int kt, const char* tile_k, char* tile_v, uint32_t next) __attribute__((always_inline)) {
         constexpr bool drafted = decltype(tail)::value;          // keys past the cached ones among the tile's

@@ -73,21 +73,30 @@ struct Four {
     }
 };
 
-// Of the 32 keys from key0 on, those that the row with this mask sees: all before pos0, and nodes by their
-// bits, up to kmax.
-__device__ __forceinline__ uint32_t tree_window(const uint64_t* mask, int words, int key0, int pos0, int kmax) {
-    const int node = key0 - pos0, left = kmax - key0;
-    auto word = [&](int i) { return i < words ? mask[i] : 0ull; };
-    uint32_t w = ~0u;
-    if (node >= 0) {
-        const int sh = node & 63;
-        const uint64_t lo = word(node >> 6) >> sh;
-        w = (uint32_t)(sh > 32 ? lo | word((node >> 6) + 1) << (64 - sh) : lo);
-    } else if (node > -32) {
-        w = (uint32_t)(word(0) << -node) | ((1u << -node) - 1);
+// What a row sees. Its first two mask words, all there are up to 128 nodes, are in registers: read in the
+// tile that needs them they hold it up by a memory round trip, and with it by the next tile's loads.
+struct TreeRow {
+    const uint64_t* mask;
+    uint64_t first, second;
+    __device__ __forceinline__ TreeRow(const uint64_t* m, int words)
+        : mask(m), first(words > 0 ? m[0] : 0), second(words > 1 ? m[1] : 0) {}
+    __device__ __forceinline__ uint64_t word(int i, int words) const {
+        return i == 0 ? first : i == 1 ? second : i < words ? mask[i] : 0;
     }
-    return left >= 32 ? w : left <= 0 ? 0u : w & ((1u << left) - 1);
-}
+    // Of the 32 keys from key0 on, those that it sees: all before pos0, and nodes by their bits, up to kmax.
+    __device__ __forceinline__ uint32_t window(int words, int key0, int pos0, int kmax) const {
+        const int node = key0 - pos0, left = kmax - key0;
+        uint32_t w = ~0u;
+        if (node >= 0) {
+            const int sh = node & 63;
+            const uint64_t lo = word(node >> 6, words) >> sh;
+            w = (uint32_t)(sh > 32 ? lo | word((node >> 6) + 1, words) << (64 - sh) : lo);
+        } else if (node > -32) {
+            w = (uint32_t)(first << -node) | ((1u << -node) - 1);
+        }
+        return left >= 32 ? w : left <= 0 ? 0u : w & ((1u << left) - 1);
+    }
+};
 
 // From a staged V tile of KEYS keys, key0 the first, of CPR 16-byte chunks each (in any order inside their
 // row): keys past the last one and, of drafted keys, elements that are not finite, out (zeros; `taken` set).
