@@ -3,8 +3,9 @@
  *
  * The library holds the device half of a paged-KV serving path: paged attention
  * (decode and prefill / chunked prefill), the KV append scatter, block copy for
- * copy-on-write, the gather/scatter halves of swap-out/swap-in, and greedy sampling
- * fused into the LM head. Everything else
+ * copy-on-write, the gather/scatter halves of swap-out/swap-in, greedy sampling
+ * fused into the LM head, attention over an 8-bit cache, steps that verify drafted token trees (what nodes see, their
+ * attention, the accepted path and its rows' move), and log probabilities of tokens. Everything else
  * (validation with the reference's exception texts, allocation, host bookkeeping)
  * stays in the Python host layer that binds this header with ctypes.
  *
@@ -555,9 +556,9 @@ int pkv_step_layout(
  * tokens), plus the node's depth. max_nodes bounds the nodes of a sequence, at most 8192 (else
  * PKV_EUNSUPPORTED).
  *
- * Rows past the last sequence get masks of 0 and position 0, and so do a node whose parent is
+ * Rows of no sequence get masks of 0 and position 0, and so do a node whose parent is
  * impossible (not -1 and not before it), the nodes below it, and all nodes of a sequence with
- * more of them than max_nodes or than its context. A proper node sees itself: its masks are not all 0. */
+ * more of them than max_nodes or than its context, or with rows outside the step. A proper node sees itself: its masks are not all 0. */
 int pkv_tree_layout(
     const int64_t* parents, const int64_t* query_start_loc, const int64_t* context_lens,
     int64_t num_seqs, int64_t num_tokens, int64_t max_nodes,
@@ -569,8 +570,9 @@ int pkv_tree_layout(
  * drafted ones those whose bits are set in row t of masks [num_tokens, mask_words] (row stride
  * mask_stride, in words): any masks, those of pkv_tree_layout among them. Drafted keys from
  * 64 * mask_words on are seen by none. A key that a row does not see does not reach it, whatever
- * its K and V hold; a row that sees no key is zero. Scores, softmax and sums are in float32, the
- * output is rounded once. query_start_loc is not NULL.
+ * its K and V hold; a row that sees no key is zero. Scores, softmax and sums are in float32 (weights
+ * meet 16-bit V as two pieces of its type, 16 bits of each at least), the output is rounded once. query_start_loc is
+ * not NULL.
  * Block ids outside the pool are never dereferenced. max_query_len bounds the query lengths (0:
  * num_tokens).
  *
@@ -619,7 +621,8 @@ int pkv_tree_accept(
  * (slots) row_bytes each from its start on, followed, in 8-bit pools, by `scales` bytes a slot,
  * stored [scales][block_size] (0 elsewhere). paths int64 [num_seqs, max_depth]; a path ends at the
  * first number that is not above the one before it or not below the sequence's nodes. Rows in blocks
- * outside the pool or the table stay. Sequences must not share the blocks of their drafted rows. */
+ * outside the pool or the table stay. Sequences must not share the blocks of their drafted rows;
+ * 65,535 of them at most (else PKV_EUNSUPPORTED). */
 int pkv_keep_paths(
     void* const* tensors, int64_t num_tensors, int64_t num_blocks, int64_t block_size,
     int64_t block_bytes, int64_t row_bytes, int64_t scales,

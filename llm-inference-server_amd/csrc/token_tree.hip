@@ -13,8 +13,8 @@
 //    fit, the first goes on. All nodes find that out side by side (an LDS minimum at the parent),
 //    then one thread follows the links.
 //
-// Both are bound by latency: launch, the sequence's bounds, one load of each input. 8 and 256
-// sequences take the same few microseconds.
+// Both are bound by latency: launch, the sequence's bounds, one load of each input. 8 sequences of 8-32 nodes
+// take 2.8 (layout) and 2.9 us (walk), 256 of 16-256 nodes 3.6 both, calls back to back in a graph.
 #include "pkv_common.h"
 
 namespace pkv {

@@ -20,6 +20,13 @@
 //
 // Weights enter the second product as two pieces of the type (16 bits of them at least: one
 // alone is off by up to 2^-9 of a weight in bf16, as much as the output's rounding).
+//
+// Bound: by matrix and vector instructions in turn where rows are many (64 sequences of 16-64 nodes behind
+// 1,024-8,192 keys, 32/8 heads of 128, bf16: 412 us; one piece of the weights 321), by start, a round trip
+// a tile and the longest context where they are few (32 of 8-32 nodes behind 16-960 keys, 12 heads of 64, fp16:
+// 18.7 us; RW = 2 21.8, RW = 4 24.0), by HBM and by the partials' way to memory and back in a lone long context
+// (32 nodes behind 100,000 keys, 32/8 heads of 128: 121 us, of which the merge is 10). The next
+// tile's loads start ahead of a tile's products: behind them, 422 and 122.
 #pragma once
 
 #include "tree_common.h"
