@@ -302,11 +302,12 @@ class PagedKVPool:
             raise ValueError(f"paths must be [{batch}, depth], got {tuple(paths.shape)}")
         hip = self._use_hip()
         pool = self.k[0] if self.k else None
+        where = None if pool is None else pool.get_device()
         for name, t in (("block_tables", block_tables), ("context_lens", context_lens), ("query_start", query_start),
                         ("paths", paths)):
             if t.dtype is not torch.long:
                 raise ValueError(f"{name} must be int64, got {t.dtype}")
-            if pool is not None and t.get_device() != pool.get_device():
+            if where is not None and t.get_device() != where:
                 raise ValueError(f"{name} is on {t.device}, the pool on {pool.device}")
         if pool is None or batch == 0 or width == 0 or paths.shape[1] == 0 or self.num_blocks == 0:
             return

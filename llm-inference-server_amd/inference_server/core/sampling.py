@@ -213,12 +213,13 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top: int = 0) 
         if logits.stride(1) != 1 and vocab > 1:
             logits = logits.contiguous()
         token_ids = token_ids.contiguous()
-        # One allocation each of the 8- and 4-byte outputs.
+        # One allocation each of the 8- and 4-byte outputs, and the views that cost the host least.
         longs = torch.empty(rows * (1 + top), dtype=torch.long, device=dev)
         floats = torch.empty(rows * (2 + top), dtype=torch.float32, device=dev)
-        ranks, top_ids = longs.split_with_sizes((rows, rows * top))
-        logprobs, entropy, top_logprobs = floats.split_with_sizes((rows, rows, rows * top))
-        out = TokenLogprobs(logprobs, ranks, entropy, top_logprobs.view(rows, top), top_ids.view(rows, top))
+        ranks, top_ids = longs.as_strided((rows,), (1,)), longs.as_strided((rows, top), (top, 1), rows)
+        logprobs, entropy = floats.as_strided((rows,), (1,)), floats.as_strided((rows,), (1,), rows)
+        top_logprobs = floats.as_strided((rows, top), (top, 1), 2 * rows)
+        out = TokenLogprobs(logprobs, ranks, entropy, top_logprobs, top_ids)
         if rows == 0:
             return out
         lib, dt, stream = native.lib(), native.DTYPE_CODES[logits.dtype], native.stream_handle(dev)

@@ -56,18 +56,28 @@ class TreePath(NamedTuple):
 def _check_rows(inputs, query_start: torch.Tensor) -> tuple[int, int]:
     """(tokens, sequences) of int64 rows [T] and query starts [B + 1], on one device."""
     name0, first = inputs[0]
-    if first.dim() != 1:
-        raise ValueError(f"{name0} must be one row of tokens, got {tuple(first.shape)}")
-    if query_start.dim() != 1 or query_start.shape[0] < 1:
-        raise ValueError(f"query_start must be [batch + 1], got {tuple(query_start.shape)}")
-    for name, t in (*inputs, ("query_start", query_start)):
+    rows, starts, dev = first.shape, query_start.shape, first.get_device()
+    if len(rows) != 1:
+        raise ValueError(f"{name0} must be one row of tokens, got {tuple(rows)}")
+    if len(starts) != 1 or starts[0] < 1:
+        raise ValueError(f"query_start must be [batch + 1], got {tuple(starts)}")
+    for name, t in inputs:
         if t.dtype is not torch.long:
             raise ValueError(f"{name} must be int64, got {t.dtype}")
-        if t.get_device() != first.get_device():
-            raise ValueError(f"{name} is on {t.device}, {name0} on {first.device}")
-        if t is not query_start and t.shape != first.shape:
-            raise ValueError(f"{name} must be [{first.shape[0]}] to match {name0}, got {tuple(t.shape)}")
-    return first.shape[0], query_start.shape[0] - 1
+        if t is not first:
+            if t.get_device() != dev:
+                raise ValueError(f"{name} is on {t.device}, {name0} on {first.device}")
+            if t.shape != rows:
+                raise ValueError(f"{name} must be [{rows[0]}] to match {name0}, got {tuple(t.shape)}")
+    if query_start.dtype is not torch.long:
+        raise ValueError(f"query_start must be int64, got {query_start.dtype}")
+    if query_start.get_device() != dev:
+        raise ValueError(f"query_start is on {query_start.device}, {name0} on {first.device}")
+    return rows[0], starts[0] - 1
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
 
 
 # ----------------------------------------------------------------------- layout
@@ -97,9 +107,11 @@ def tree_layout(parents: torch.Tensor, query_start: torch.Tensor, context_lens: 
     native.require_gpu(parents, "tree_layout")
     dev = parents.device
     with native.on_device(dev):
-        parents, query_start, context_lens = (t.contiguous() for t in (parents, query_start, context_lens))
+        parents, query_start, context_lens = _dense(parents), _dense(query_start), _dense(context_lens)
+        # One allocation, and the views that cost least: the call is bound by its host time.
         buf = torch.empty(tokens * (words + 1), dtype=torch.long, device=dev)
-        masks, positions = buf[:tokens * words].view(tokens, words), buf[tokens * words:]
+        masks = buf.as_strided((tokens, words), (words, 1))
+        positions = buf.as_strided((tokens,), (1,), tokens * words)
         rc = native.lib().pkv_tree_layout(
             parents.data_ptr(), query_start.data_ptr(), context_lens.data_ptr(), batch, tokens, max_nodes,
             masks.data_ptr(), positions.data_ptr(), native.stream_handle(dev))
@@ -158,10 +170,11 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
     native.require_gpu(tokens, "accept_tree")
     dev = tokens.device
     with native.on_device(dev):
-        tokens, parents, targets, query_start = (t.contiguous() for t in (tokens, parents, targets, query_start))
+        tokens, parents, targets, query_start = _dense(tokens), _dense(parents), _dense(targets), _dense(query_start)
         buf = torch.empty(batch * (max_depth + 2), dtype=torch.long, device=dev)
-        paths, counts, following = buf.split_with_sizes((batch * max_depth, batch, batch))
-        paths = paths.view(batch, max_depth)
+        paths = buf.as_strided((batch, max_depth), (max_depth, 1))
+        counts = buf.as_strided((batch,), (1,), batch * max_depth)
+        following = buf.as_strided((batch,), (1,), batch * (max_depth + 1))
         rc = native.lib().pkv_tree_accept(
             tokens.data_ptr(), parents.data_ptr(), targets.data_ptr(), query_start.data_ptr(), batch, n_tok, max_depth,
             paths.data_ptr(), counts.data_ptr(), following.data_ptr(), native.stream_handle(dev))
