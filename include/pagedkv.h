@@ -570,9 +570,9 @@ int pkv_tree_layout(
  * drafted ones those whose bits are set in row t of masks [num_tokens, mask_words] (row stride
  * mask_stride, in words): any masks, those of pkv_tree_layout among them. Drafted keys from
  * 64 * mask_words on are seen by none. A key that a row does not see does not reach it, whatever
- * its K and V hold; a row that sees no key is zero. Scores, softmax and sums are in float32 (weights
- * meet 16-bit V as two pieces of its type, 16 bits of each at least), the output is rounded once. query_start_loc is
- * not NULL.
+ * its K and V hold; a row that sees no key is zero. Scores, softmax and sums are in float32, the output is rounded once. Weights
+ * meet 16-bit V as two pieces of its type: bf16 leaves at most 2^-16 of a weight, fp16 2^-22 of it or 2^-38 of the row's
+ * largest, whichever is more. query_start_loc is not NULL.
  * Block ids outside the pool are never dereferenced. max_query_len bounds the query lengths (0:
  * num_tokens).
  *

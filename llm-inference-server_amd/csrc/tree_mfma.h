@@ -18,8 +18,12 @@
 //    output turned NaN under finite weights (0 * infinity, or an infinity times two pieces of opposite
 //    signs), walks its keys once more at the end and puts into each row's dims what it sees of them.
 //
-// Weights enter the second product as two pieces of the type (16 bits of them at least: one
-// alone is off by up to 2^-9 of a weight in bf16, as much as the output's rounding).
+// Weights enter the second product as two pieces of the type: one alone is off by up to 2^-9 of a weight in
+// bf16, as much as the output's rounding. Two bf16 pieces have 16 bits of any weight. fp16 ends at 2^-24, so
+// its weights reach up to the type's other end: the reference m that scores are taken from is 13 to 15 bits below
+// the largest score so far, where bf16's is at most 8 below it. Two pieces are then off by 2^-22 of a weight, or by 2^-38 of
+// the row's largest where that is more. (With bf16's rule a tail of keys at 2^-24 of the largest weight came out 20% off, and
+// one at 2^-26 not at all.)
 //
 // Bound: by matrix and vector instructions in turn where rows are many (64 sequences of 16-64 nodes behind
 // 1,024-8,192 keys, 32/8 heads of 128, bf16: 412 us; one piece of the weights 321), by start, a round trip
@@ -37,6 +41,20 @@ namespace {
 // Keys of a tile.
 template <int RW>
 constexpr int kTreeTile = RW == 1 ? 128 : 64;
+
+// Whether a row's reference for its scores (in base 2) is raised in a tile whose largest is `top`, and to what. Weights are
+// 2^(score - reference); fp16 holds less than 2^16. `top` is rounded, the scores are not: those of 2^22 and more
+// can be well above it, which the last term makes room for (up to 2^27).
+template <typename T>
+__device__ __forceinline__ bool tree_raises(float top, float ref) {
+    if constexpr (__is_same(T, _Float16)) return fmaf(fabsf(top), 0x1p-23f, top - ref) > 15.f;
+    else return top > ref + kRescaleThreshold;
+}
+template <typename T>
+__device__ __forceinline__ float tree_reference(float top) {
+    if constexpr (__is_same(T, _Float16)) return fmaf(fabsf(top), 0x1p-23f, top - 13.f);
+    else return top;
+}
 
 // Waves a SIMD: LDS has room for two workgroups a CU, or for one.
 template <int D, int RW>
@@ -250,9 +268,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             for (int r = 0; r < 16; ++r) mt = fmaxf(mt, st[i][r]);
         mt = max_across32(mt) * p.scale_log2;   // scale > 0: max commutes with it
         asm("" : "+v"(mt));                     // stays rounded: m_run - mt below is not contracted into an fma
-        const bool raise = mt > m_run + kRescaleThreshold;
-        const float m_new = raise ? mt : m_run;
-        const float alpha = raise ? fast_exp2(m_run - mt) : 1.f;
+        const bool raise = tree_raises<T>(mt, m_run);
+        const float m_new = raise ? tree_reference<T>(mt) : m_run;
+        const float alpha = raise ? fast_exp2(m_run - m_new) : 1.f;
         if (__builtin_amdgcn_ballot_w64(raise)) {
 #pragma unroll
             for (int t = 0; t < DTILES; ++t) o[t] *= alpha;

@@ -217,8 +217,9 @@ def paged_tree_attention(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
     head_dim] in the pools' dtype (fp32, fp16, bf16), block_tables [B, W], context_lens and
     query_lens [B], the same checks and messages; returns [T, heads, head_dim].
 
-    Softmax and sums are in fp32 (ATTENTION=hip: weights meet 16-bit V as two pieces of its type, 16 bits
-    of each at least) and the output is rounded once. The 8-bit cache has no such attention. A key that a token does
+    Softmax and sums are in fp32 and the output is rounded once. (ATTENTION=hip: weights meet 16-bit V as two
+    pieces of its type, which leave at most 2^-16 of a bf16 weight, and of an fp16 one 2^-22, or 2^-38 of the row's
+    largest where that is more.) The 8-bit cache has no such attention. A key that a token does
     not see does not reach it, whatever its K and V hold (NaN and infinities among it); a token that
     sees none gets zeros. Lengths with host copies attached (attach_host) are checked without a
     device round trip."""
