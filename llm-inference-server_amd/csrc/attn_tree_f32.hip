@@ -23,6 +23,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mfma16(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 share_of(f32x4 x, float f) {
+    return f32x4{share_of(x[0], f), share_of(x[1], f), share_of(x[2], f), share_of(x[3], f)};
+}
 __device__ __forceinline__ float max_of_row(float x) {
     const SwapPair a = swap16(x);
     return max_across32(fmaxf(a.a, a.b));
@@ -73,6 +76,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void t
 
     __shared__ __attribute__((aligned(1024))) char s_all[4 * KT * ROWB];      // K, V, K, V
     __shared__ int s_taken;                   // whether V held what is not finite behind the cached keys
+    __shared__ int s_walked;                  // whether a wave has put such into its rows
     __shared__ float2 s_ml[4][16];
 
     PrefillItem it;
@@ -204,7 +208,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void t
             qf[4 * c + 3] = v.w;
         }
     }
-    if (threadIdx.x == 0) s_taken = 0;
+    if (threadIdx.x == 0) s_taken = s_walked = 0;
 
     const TreeRow seen(p.masks + (q_first + my_q) * p.mask_stride, t_end * KT > pos0 ? p.mask_words : 0);
     auto window = [&](int key0) __attribute__((always_inline)) { return seen.window(p.mask_words, key0, pos0, kmax); };
@@ -312,6 +316,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void t
 #pragma unroll
             for (int r = 0; r < 4; ++r) any += o[t][r] * 0.f;
         if (s_taken || __builtin_amdgcn_ballot_w64(any != any && l_run == l_run)) {
+            s_walked = 1;
             float4 extra[DT];
 #pragma unroll
             for (int t = 0; t < DT; ++t) extra[t] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -362,15 +367,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void t
             l_all += f[w] * ml[w].y;
         }
         const float f_own = fast_exp2(m_run - m_off);
+        auto join = [&](auto times) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            if (t % KW != kw) continue;
-            f32x4 x = o[t] * f_own;
+            for (int t = 0; t < DT; ++t) {
+                if (t % KW != kw) continue;
+                f32x4 x = times(o[t], f_own);
 #pragma unroll
-            for (int w = 0; w < KW; ++w)
-                if (w != kw) x += so[((rw * KW + w) * DT + t) * 64 + lane] * f[w];
-            o[t] = x;
-        }
+                for (int w = 0; w < KW; ++w)
+                    if (w != kw) x += times(so[((rw * KW + w) * DT + t) * 64 + lane], f[w]);
+                o[t] = x;
+            }
+        };
+        if (s_walked) join([](f32x4 x, float y) { return share_of(x, y); });
+        else join([](f32x4 x, float y) { return x * y; });
     }
     if (!my_live) return;
     const int64_t tok = q_first + my_q;
@@ -391,7 +400,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void t
         return;
     }
     if (p.ws_rows && g == 0 && kw == 0) p.ws_rows[tok * p.num_heads + my_head] = 0;    // finished here
-    const float inv = l_all == 0.f ? 0.f : 1.f / l_all;                                // no key: zero
+    const float inv = l_all == 0.f ? 1.f : 1.f / l_all;        // no key, or weights of 0 alone: o is 0 where it is finite
     float* orow = reinterpret_cast<float*>(p.out) + tok * p.out_st + (int64_t)my_head * p.out_sh + 4 * g;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -404,7 +413,7 @@ int launch_rows(const TreeParams& p, hipStream_t stream) {
     const int rc = check_launch("tree attention");
     if (rc || p.splits == 1) return rc;
     const int64_t rows = p.num_tokens * p.num_heads;
-    prefill_merge_kernel<float, D><<<dim3((unsigned)ceil_div(rows, kMergeRows<D>)), 256, 0, stream>>>(p);
+    prefill_merge_kernel<float, D, true><<<dim3((unsigned)ceil_div(rows, kMergeRows<D>)), 256, 0, stream>>>(p);
     return check_launch("tree attention, merge");
 }
 

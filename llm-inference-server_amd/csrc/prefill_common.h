@@ -90,16 +90,22 @@ __device__ __forceinline__ int split_run(int n_tiles, int splits, int split_tile
     return (n_tiles + n - 1) / n;
 }
 
+// x times f, a weight above 0 that fp32 may not hold: all of what is not finite, where the product would be NaN.
+__device__ __forceinline__ float share_of(float x, float f) {
+    return f == 0.f && !(fabsf(x) < __builtin_huge_valf()) ? x : x * f;
+}
+
 // Merge of the splits, launched after the kernel above on the same stream: D / 4 lanes per
 // query row (four head_dim elements each), log-sum-exp rule over the row's splits in key
 // order. Rows that one workgroup finished are marked 0 and skipped, as are tokens of no
 // sequence (rows the launch above never wrote: tokens past query_start_loc's end). Bound by
 // the latency of its two dependent loads and by workgroup launches, hence as many rows per
-// wave as fit.
+// wave as fit. REST: what is not finite in a split's part reaches the row whatever the split's weight, and a row whose
+// weights are all 0 is zero.
 template <int D>
 constexpr int kMergeRows = 4 * (64 / (D / 4));   // query rows per 256-thread workgroup
 
-template <typename T, int D>
+template <typename T, int D, bool REST = false>
 __global__ __launch_bounds__(256) void prefill_merge_kernel(const AttnParams p) {
     constexpr int LPR = D / 4, RPW = 64 / LPR;
     const int lane = lane_id();
@@ -140,29 +146,37 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(const AttnParams p) 
 #pragma unroll
         for (int j = 0; j < CH; ++j) Mc = fmaxf(Mc, mlv[j].x);
         const float rescale = M == kNegInf ? 0.f : fast_exp2(M - Mc);
-        L *= rescale;
-        acc.x *= rescale;
-        acc.y *= rescale;
-        acc.z *= rescale;
-        acc.w *= rescale;
+        float sc[CH];
+        bool none = REST && rescale == 0.f && M != kNegInf;      // a weight that fp32 does not hold
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-            const float sc = mlv[j].x == kNegInf ? 0.f : fast_exp2(mlv[j].x - Mc);
-            L += sc * mlv[j].y;
-            acc.x += sc * ov[j].x;
-            acc.y += sc * ov[j].y;
-            acc.z += sc * ov[j].z;
-            acc.w += sc * ov[j].w;
+            sc[j] = mlv[j].x == kNegInf ? 0.f : fast_exp2(mlv[j].x - Mc);
+            if (REST) none |= sc[j] == 0.f && s0 + j < n;
         }
+        auto join = [&](auto times) __attribute__((always_inline)) {
+            L *= rescale;
+            acc.x = times(acc.x, rescale);
+            acc.y = times(acc.y, rescale);
+            acc.z = times(acc.z, rescale);
+            acc.w = times(acc.w, rescale);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                L += sc[j] * mlv[j].y;
+                acc.x += times(ov[j].x, sc[j]);
+                acc.y += times(ov[j].y, sc[j]);
+                acc.z += times(ov[j].z, sc[j]);
+                acc.w += times(ov[j].w, sc[j]);
+            }
+        };
+        if (REST && __builtin_amdgcn_ballot_w64(none)) join(share_of);
+        else join([](float x, float f) { return x * f; });
         M = Mc;
     }
     T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (row - tok * p.num_heads) * p.out_sh + d;
-    const float inv = 1.f / L;
-    if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<float4*>(orow) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    else
-        *reinterpret_cast<uint2*>(orow) =
-            make_uint2(Mfma<T>::pack(acc.x * inv, acc.y * inv), Mfma<T>::pack(acc.z * inv, acc.w * inv));
+    const float inv = REST && L == 0.f ? 1.f : 1.f / L;         // all weights 0: what is there, if anything, is not finite
+    const float4 x = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(orow) = x;
+    else *reinterpret_cast<uint2*>(orow) = make_uint2(Mfma<T>::pack(x.x, x.y), Mfma<T>::pack(x.z, x.w));
 }
 
 // Workgroups of the flat grid, a multiple of 8: the splits' items, or room for every row

@@ -16,7 +16,8 @@
 //  * What is not seen must not reach a row, and 0 * NaN would: in those tiles V's elements that are not finite
 //    are taken out of LDS (zeros), as are rows past the last key. A wave that took some out, or whose
 //    output turned NaN under finite weights (0 * infinity, or an infinity times two pieces of opposite
-//    signs), walks its keys once more at the end and puts into each row's dims what it sees of them.
+//    signs), walks its keys once more at the end and puts into each row's dims what it sees of them; it stays
+//    there where waves and runs are joined, however little they weigh (share_of).
 //
 // Weights enter the second product as two pieces of the type: one alone is off by up to 2^-9 of a weight in
 // bf16, as much as the output's rounding. Two bf16 pieces have 16 bits of any weight. fp16 ends at 2^-24, so
@@ -78,6 +79,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
 
     __shared__ __attribute__((aligned(1024))) char s_all[4 * KT * ROWB];      // K, V, K, V
     __shared__ int s_taken;                   // whether V held what is not finite behind the cached keys
+    __shared__ int s_walked;                  // whether a wave has put such into its rows
     __shared__ float2 s_ml[4][32];
 
     PrefillItem it;
@@ -215,7 +217,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             qfrag[s] = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
         }
     }
-    if (threadIdx.x == 0) s_taken = 0;
+    if (threadIdx.x == 0) s_taken = s_walked = 0;
 
     const TreeRow seen(p.masks + (q_first + my_q) * p.mask_stride, t_end * KT > pos0 ? p.mask_words : 0);
     auto window = [&](int key0) __attribute__((always_inline)) { return seen.window(p.mask_words, key0, pos0, kmax); };
@@ -343,6 +345,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             for (int r = 0; r < 16; ++r)
                 if (32 * t + 8 * (r >> 2) < D) any += o[t][r] * 0.f;
         if (s_taken || __builtin_amdgcn_ballot_w64(any != any && l_run == l_run)) {
+            s_walked = 1;
             float4 extra[UNITS];
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) extra[u] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -398,25 +401,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
             l_all += f[w] * ml[w].y;
         }
         f_own = fast_exp2(m_run - m_off);
+        auto join = [&](auto times) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            if (u % KW != kw) continue;
-            float4 x = make_float4(o[u / 4][4 * (u % 4)] * f_own, o[u / 4][4 * (u % 4) + 1] * f_own,
-                                   o[u / 4][4 * (u % 4) + 2] * f_own, o[u / 4][4 * (u % 4) + 3] * f_own);
+            for (int u = 0; u < UNITS; ++u) {
+                if (u % KW != kw) continue;
+                float4 x = make_float4(times(o[u / 4][4 * (u % 4)], f_own), times(o[u / 4][4 * (u % 4) + 1], f_own),
+                                       times(o[u / 4][4 * (u % 4) + 2], f_own), times(o[u / 4][4 * (u % 4) + 3], f_own));
 #pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                if (w == kw) continue;
-                const float4 y = *reinterpret_cast<const float4*>(so + (((rw * KW + w) * UNITS + u) * 64 + lane) * 4);
-                x.x += y.x * f[w];
-                x.y += y.y * f[w];
-                x.z += y.z * f[w];
-                x.w += y.w * f[w];
+                for (int w = 0; w < KW; ++w) {
+                    if (w == kw) continue;
+                    const float4 y = *reinterpret_cast<const float4*>(so + (((rw * KW + w) * UNITS + u) * 64 + lane) * 4);
+                    x.x += times(y.x, f[w]);
+                    x.y += times(y.y, f[w]);
+                    x.z += times(y.z, f[w]);
+                    x.w += times(y.w, f[w]);
+                }
+                o[u / 4][4 * (u % 4)] = x.x;
+                o[u / 4][4 * (u % 4) + 1] = x.y;
+                o[u / 4][4 * (u % 4) + 2] = x.z;
+                o[u / 4][4 * (u % 4) + 3] = x.w;
             }
-            o[u / 4][4 * (u % 4)] = x.x;
-            o[u / 4][4 * (u % 4) + 1] = x.y;
-            o[u / 4][4 * (u % 4) + 2] = x.z;
-            o[u / 4][4 * (u % 4) + 3] = x.w;
-        }
+        };
+        if (s_walked) join(share_of);
+        else join([](float x, float y) { return x * y; });
     }
     if (!my_live) return;
     const int64_t tok = q_first + my_q;
@@ -439,7 +446,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kTreeWaves<
         return;
     }
     if (p.ws_rows && h == 0 && kw == 0) p.ws_rows[tok * p.num_heads + my_head] = 0;    // finished here
-    inv = l_all == 0.f ? 0.f : 1.f / l_all;                                            // no key: zero
+    inv = l_all == 0.f ? 1.f : 1.f / l_all;                    // no key, or weights of 0 alone: o is 0 where it is finite
     T* orow = reinterpret_cast<T*>(p.out) + tok * p.out_st + (int64_t)my_head * p.out_sh + 4 * h;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -456,7 +463,7 @@ int launch_tree_rows(const TreeParams& p, hipStream_t stream) {
     const int rc = check_launch("tree attention");
     if (rc || p.splits == 1) return rc;
     const int64_t rows = p.num_tokens * p.num_heads;
-    prefill_merge_kernel<T, D><<<dim3((unsigned)ceil_div(rows, kMergeRows<D>)), 256, 0, stream>>>(p);
+    prefill_merge_kernel<T, D, true><<<dim3((unsigned)ceil_div(rows, kMergeRows<D>)), 256, 0, stream>>>(p);
     return check_launch("tree attention, merge");
 }
 
