@@ -10,8 +10,10 @@
 // shapes that the matrix kernels decline. A workgroup has one (token, query head). A lane holds 16
 // dims of a key, LPK lanes a key, so that a wave has 64 / LPK keys side by side; each such group of
 // lanes runs an online softmax of its own, in fp32, over every so-manieth key, and the groups meet at
-// the end. Bound: vector instructions and the latency of a step's loads (8 sequences of 16 nodes behind 4,000
+// the end. A group whose sums are not finite walks its keys once more, takes what of V is not finite, and keeps that
+// however little the key weighs. Bound: vector instructions and the latency of a step's loads (8 sequences of 16 nodes behind 4,000
 // keys, 16/4 heads of 256, bf16: 468 us).
+#include "prefill_common.h"
 #include "tree.h"
 
 namespace pkv {
@@ -135,6 +137,29 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
         }
         m = m_new;
     }
+    // What is not finite in V, for rows that see it: the sums may have lost it (0 * infinity is NaN).
+    float any = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) any += acc[e] * 0.f;
+    if (any != any && l == l) {
+        float rest[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) rest[e] = 0.f;
+        for (int key = group; key < n_keys; key += groups) {
+            const int64_t node = (int64_t)key - cached;
+            if (node >= 0 && (node >= 64ll * p.mask_words || !(mask[node >> 6] >> (node & 63) & 1))) continue;
+            const uint32_t blk = p.block_shift >= 0 ? (uint32_t)key >> p.block_shift : (uint32_t)key / (uint32_t)p.block_size;
+            const int64_t id = table[blk];
+            if ((uint64_t)id >= (uint64_t)p.num_blocks) continue;
+            float v[16];
+            dims(vb + id * p.sb + (int64_t)((uint32_t)key - blk * (uint32_t)p.block_size) * p.ss, v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) rest[e] += fabsf(v[e]) < __builtin_huge_valf() ? 0.f : v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (rest[e] != 0.f) acc[e] = rest[e];
+    }
     // The wave's groups, then the waves.
     float M = m;
 #pragma unroll
@@ -145,7 +170,7 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
     for (int off = LPK; off < 64; off *= 2) l += __shfl_xor(l, off);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        acc[e] *= a;
+        acc[e] = share_of(acc[e], a);
 #pragma unroll
         for (int off = LPK; off < 64; off *= 2) acc[e] += __shfl_xor(acc[e], off);
     }
@@ -166,9 +191,10 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
         for (int w = 0; w < waves; ++w) {
             const float b = fast_exp2(s_m[w] - top);
             L += b * s_l[w];
-            o += b * s_o[w * DP + d];
+            o += share_of(s_o[w * DP + d], b);
         }
-        orow[d] = from_f32<T>(L == 0.f ? 0.f : o / L);          // a row that sees no key is zero
+        // (No key, or weights of 0 alone: o is 0 where it is finite.)
+        orow[d] = from_f32<T>(L == 0.f ? o : o / L);
     }
 }
 
