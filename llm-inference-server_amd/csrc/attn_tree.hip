@@ -97,7 +97,7 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
     };
     float m = kNegInf, l = 0.f;
     for (int first = 0; first < n_keys; first += U * groups) {
-        float k[U][16], v[U][16], s[U], m_new = m;
+        float k[U][16], v[U][16], dot[U], m_new = m;
         bool seen[U], good[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -118,9 +118,9 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
             float x = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) x += q[e] * k[u][e];
-            x = lanes_sum<LPK>(x) * p.scale_log2;
-            s[u] = seen[u] ? (good[u] ? x : 0.f) : kNegInf;
-            m_new = fmaxf(m_new, s[u]);
+            x = lanes_sum<LPK>(x);
+            dot[u] = good[u] ? x : 0.f;
+            if (seen[u]) m_new = fmaxf(m_new, dot[u] * p.scale_log2);
         }
         const float m_off = m_new == kNegInf ? 0.f : m_new;
         const float alpha = fast_exp2(m - m_off);               // 0 on the first keys (m = -inf)
@@ -129,7 +129,8 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
         for (int e = 0; e < 16; ++e) acc[e] *= alpha;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float pj = fast_exp2(s[u] - m_off);
+            // (One rounding: that of a large product would be the weight's.)
+            const float pj = seen[u] ? fast_exp2(fmaf(dot[u], p.scale_log2, -m_off)) : 0.f;
             l += pj;
             // A key that is not seen does not reach the row, whatever it holds.
 #pragma unroll

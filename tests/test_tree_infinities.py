@@ -22,9 +22,9 @@ LENS = [pytest.param([(300, 9), (130, 3)], id="one"), pytest.param([(300, 40)], 
 
 @pytest.mark.parametrize("backend", BACKENDS)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("d", [32, 64, 128, 40, 160, 256, 512])
+@pytest.mark.parametrize("d", [32, 64, 128, 40, 160])
 @pytest.mark.parametrize("lens", LENS)
-@pytest.mark.parametrize("largest", [0, 0.4, 0.9, 1])
+@pytest.mark.parametrize("largest", [0, 0.9, 1])
 def test_infinities_below_the_largest_weight(monkeypatch, backend, dtype, d, lens, largest):
     """One key 200 nats above all others (2^-288 of it is 0 in fp32), at the start, inside or at the end of the
     cached ones, or the first node."""

@@ -17,7 +17,7 @@ BACKENDS = [pytest.param("gather", id="gather"), pytest.param("hip", id="hip", m
 #: (cached, nodes): rows of one wave, of two, of four; a context that is cut; one that is not, since more than 256
 #: sequences never are.
 LENS = [pytest.param([(700, 9), (130, 3)], id="one"), pytest.param([(700, 40)], id="two"), pytest.param([(700, 90)], id="four"),
-        pytest.param([(9000, 90)], id="cut"), pytest.param([(5000, 90)] + [(0, 1)] * 256, id="uncut")]
+        pytest.param([(6000, 70)], id="cut"), pytest.param([(3000, 70)] + [(0, 1)] * 256, id="uncut")]
 
 
 def tailed(lens, below, spread, d, dtype, device):
@@ -69,8 +69,8 @@ def test_a_tail_far_below_the_largest_weight(monkeypatch, backend, dtype, d, len
 
 @pytest.mark.parametrize("backend", BACKENDS)
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("lens", LENS[1:4])
+@pytest.mark.parametrize("d", [64, 40])
+@pytest.mark.parametrize("lens", LENS[2:4])
 @pytest.mark.parametrize("scale,step", [(1.0, 4.0), (2.0 ** 11, 2.0 ** -9), (2.0 ** 13, 2.0 ** -11), (2.0 ** 15, 2.0 ** -12)])
 @pytest.mark.parametrize("sign", [1, -1])
 def test_scores_that_rise_from_far_off(monkeypatch, backend, dtype, d, lens, scale, step, sign):
