@@ -344,9 +344,11 @@ def _attention_hip(query, k_pool, v_pool, tables, context_lens, query_lens, mask
             tables = tables.contiguous()
             t_st = tables.stride()
         m_st, words = masks.stride(), masks.shape[1]
-        if (words > 1 and m_st[1] != 1) or m_st[0] < words:
+        if (words > 1 and m_st[1] != 1) or (n_tok > 1 and m_st[0] < words):
             masks = masks.contiguous()
             m_st = masks.stride()
+        # (A lone row is contiguous whatever its stride.)
+        mask_stride = m_st[0] if n_tok > 1 else words
         ctx_dev = _on_device(context_lens, dev).contiguous()
         stream = native.stream_handle(dev)
         qsl = getattr(query_lens, _QSL_ATTR, None)
@@ -373,7 +375,7 @@ def _attention_hip(query, k_pool, v_pool, tables, context_lens, query_lens, mask
                 out.data_ptr(), n_heads * head_dim, head_dim, query.data_ptr(), q_st[0], q_st[1],
                 k_pool.data_ptr(), v_pool.data_ptr(), k_st[0], k_st[1], k_st[2], n_blocks, block_size, n_kv, head_dim,
                 tables.data_ptr(), t_st[0], width, ctx_dev.data_ptr(), qsl.data_ptr(),
-                masks.data_ptr(), m_st[0], words, n_seqs, n_heads, n_tok, max_q, *lens,
+                masks.data_ptr(), mask_stride, words, n_seqs, n_heads, n_tok, max_q, *lens,
                 float(scale), dt, ws_ptr, ws_size, stream)
         native.check(rc, "pkv_tree_attention")
         return out

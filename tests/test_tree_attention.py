@@ -201,6 +201,18 @@ def test_refusals(device):
     assert empty.shape == (0, 4, 64)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [64, 40])
+def test_strides_of_one_row_of_masks(device, dtype, d):
+    """A lone row's stride means nothing, and may be anything."""
+    s = batch([(70, 1)], heads=4, kv=2, d=d, bs=16, dtype=dtype, device=device, words=3)
+    row = s.masks.reshape(3)
+    for masks in (s.masks, row[:, None].t(), row.as_strided((1, 3), (0, 1)), torch.stack([row, ~row], 1)[:, 0][None],
+                  row[:1].as_strided((1, 1), (0, 5)), row[:1].as_strided((1, 1), (0, 0))):
+        s.masks = masks
+        check(s, call(s))
+
+
 # ------------------------------------------------------------------ GPU only
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
