@@ -62,6 +62,13 @@ def attach_query_start(query_lens: torch.Tensor, query_start: torch.Tensor) -> t
     return query_lens
 
 
+def _attached_start(query_lens: torch.Tensor, dev: torch.device) -> torch.Tensor | None:
+    """The query starts attached to query_lens, on dev: lengths that the caller has on the host, or on
+    another device, have theirs there, and the kernels read them by address."""
+    qsl = getattr(query_lens, _QSL_ATTR, None)
+    return None if qsl is None else _on_device(qsl, dev)
+
+
 def host_copy(t: torch.Tensor) -> torch.Tensor | None:
     if t.device.type == "cpu":
         return t
@@ -367,7 +374,7 @@ def paged_attention_hip_launch(
         native.check(rc, "pkv_paged_attention_decode")
         return out
 
-    qsl = getattr(query_lens, _QSL_ATTR, None)
+    qsl = _attached_start(query_lens, dev)
     if qsl is None:
         qsl = _query_start(facts, context_lens, dev, stream)
     # Workspace for split contexts (0 bytes: a batch that is not split), planned by a step's

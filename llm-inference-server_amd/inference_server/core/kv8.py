@@ -24,7 +24,7 @@ import torch
 from inference_server import native
 from inference_server.config import CONFIG
 from inference_server.core.attention import _gather_ragged, check_contract
-from inference_server.core.attention_hip import (_ALONE, _QSL_ATTR, _WORKSPACES, _on_device, _query_start,
+from inference_server.core.attention_hip import (_ALONE, _WORKSPACES, _attached_start, _on_device, _query_start,
                                                  _step_facts)
 from inference_server.core.kv_pool import ModelDims, PagedKVPool
 
@@ -271,12 +271,12 @@ def _attention_hip(query, k_cache, v_cache, tables, context_lens, query_lens, sc
             t_st = tables.stride()
         ctx_dev = _on_device(context_lens, dev).contiguous()
         stream = native.stream_handle(dev)
-        qsl = None
+        qsl, starts = None, None
         if not facts["all_decode"]:
-            qsl = getattr(query_lens, _QSL_ATTR, None)
-            if qsl is None:
-                qsl = _query_start(facts, context_lens, dev, stream)
-            qsl = qsl.data_ptr()
+            starts = _attached_start(query_lens, dev)
+            if starts is None:
+                starts = _query_start(facts, context_lens, dev, stream)
+            qsl = starts.data_ptr()
         lib = native.lib()
         max_q, max_ctx = facts["max_q"], facts["max_ctx"]
         lens = (facts["hctx"].data_ptr(), facts["hql"].data_ptr())

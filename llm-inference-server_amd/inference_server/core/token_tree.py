@@ -31,7 +31,7 @@ import torch
 from inference_server import native
 from inference_server.config import CONFIG
 from inference_server.core.attention import check_contract
-from inference_server.core.attention_hip import (_ALONE, _QSL_ATTR, _WORKSPACES, _on_device, _query_start,
+from inference_server.core.attention_hip import (_ALONE, _WORKSPACES, _attached_start, _on_device, _query_start,
                                                  _step_facts)
 
 #: Most nodes of a sequence that the layout and the walk take.
@@ -351,7 +351,7 @@ def _attention_hip(query, k_pool, v_pool, tables, context_lens, query_lens, mask
         mask_stride = m_st[0] if n_tok > 1 else words
         ctx_dev = _on_device(context_lens, dev).contiguous()
         stream = native.stream_handle(dev)
-        qsl = getattr(query_lens, _QSL_ATTR, None)
+        qsl = _attached_start(query_lens, dev)
         if qsl is None:
             qsl = _query_start(facts, context_lens, dev, stream)
         lib = native.lib()

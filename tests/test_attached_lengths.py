@@ -8,8 +8,9 @@ import torch
 
 from inference_server.config import CONFIG
 from inference_server.core.attention import paged_attention
-from inference_server.core.attention_hip import _step_facts, attach_host, attach_query_start
+from inference_server.core.attention_hip import _attached_start, _step_facts, attach_host, attach_query_start
 from inference_server.core.kv8 import paged_attention_kv8
+from inference_server.core.token_tree import paged_tree_attention
 from kv8_cases import batch
 
 
@@ -60,3 +61,35 @@ def test_query_starts_that_the_kernels_cannot_read_are_refused():
                 starts.repeat_interleave(2)[::2], starts.to("meta")):
         with pytest.raises(ValueError, match="query_start"):
             attach_query_start(lens, bad)
+
+
+def test_query_starts_are_read_where_the_query_is():
+    lens = torch.tensor([3, 4, 5])
+    assert _attached_start(lens, torch.device("cpu")) is None
+    starts = torch.tensor([0, 3, 7, 12])
+    attach_query_start(lens, starts)
+    assert _attached_start(lens, torch.device("cpu")) is starts
+    assert _attached_start(lens, torch.device("meta")).device.type == "meta"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["8-bit", "16-bit", "tree"])
+def test_lengths_and_query_starts_on_the_host(monkeypatch, cache):
+    monkeypatch.setattr(CONFIG, "attention", "hip")
+    s = batch([(5, 4), (30, 0), (40, 17)], heads=4, kv=2, d=32, bs=8, dtype=torch.float16, device="cuda")
+    tables, *lens = s.args
+    pool = torch.randn(s.k.codes.shape, device="cuda").half()
+    masks = torch.full((21, 1), -1, device="cuda")
+
+    def call(ctx, new):
+        if cache == "8-bit":
+            return paged_attention_kv8(s.q, s.k, s.v, tables, ctx, new, s.scale)
+        if cache == "16-bit":
+            return paged_attention(s.q, pool, pool, tables, ctx, new, s.scale)
+        return paged_tree_attention(s.q, pool, pool, tables, ctx, new, masks, s.scale)
+
+    want = call(*lens)
+    ctx, new = (t.cpu() for t in lens)
+    attach_query_start(new, torch.tensor([0, 4, 4, 21]))
+    for _ in range(3):
+        assert torch.equal(call(ctx, new), want)
