@@ -544,8 +544,8 @@ int pkv_step_layout(
 
 /* ------------------------------------------------------------------ drafted token trees
  * A step that verifies drafted tokens, without counterpart in the reference: every sequence's new tokens are
- * the nodes of a tree of continuations, scored in one forward pass; the longest path that the
- * model agrees with is kept. A sequence's nodes are its rows of the packed step
+ * the nodes of a tree of continuations, scored in one forward pass; a path that the
+ * model agrees with (pkv_tree_accept) is kept. A sequence's nodes are its rows of the packed step
  * (query_start_loc[i] .. query_start_loc[i + 1]) in an order in which parents come first, node 0
  * the token that was sampled before; in the cache they are its last positions, in that order. */
 
@@ -603,7 +603,9 @@ int pkv_tree_attention(
 
 /* The path of each tree that the target model accepts: from node 0, on to the first child whose
  * token (tokens int64 [num_tokens]) is the target's token at the node (targets int64 [num_tokens],
- * greedy or sampled), until there is none. Out, int64: paths [num_seqs, max_depth] the
+ * greedy or sampled), until there is none: the longest path that the target agrees with where a node's
+ * children have tokens of their own. (Of children with one token the walk takes the first, also where only
+ * another goes on.) Out, int64: paths [num_seqs, max_depth] the
  * accepted nodes' numbers, -1 past the last; counts [num_seqs]; next_tokens [num_seqs] the
  * target's token at the last of them. At most max_depth nodes are accepted. A sequence without
  * nodes (or with impossible bounds, or more than 8192 nodes) has count 0 and next token -1. Nodes

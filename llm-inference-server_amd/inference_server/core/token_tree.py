@@ -156,7 +156,9 @@ def _layout_torch(parents, starts, ctx, max_nodes, words) -> TreeLayout:
 def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tensor, query_start: torch.Tensor,
                 max_depth: int) -> TreePath:
     """The path of each tree that the target model agrees with: from node 0, on to the first
-    child whose token is the target's token at the node, until there is none.
+    child whose token is the target's token at the node, until there is none. Where a node's children have
+    tokens of their own, as a draft's likeliest ones have, that is the longest such path; of children with one token
+    the walk takes the first, also where only another goes on.
 
     tokens, parents, targets [T]: the nodes' tokens, their parents' numbers, and the target's token
     after each node (its argmax, or a sample); query_start [B + 1]; all int64. At most
