@@ -7,6 +7,8 @@ sequence's last positions, in that order (step_layout's slots), while a node's p
 the model is the cached tokens plus its depth. A step is
 
     layout = step_layout(...)                                   # slots, query starts
+    attach_host(context_lens, bounds), attach_host(query_lens, more_bounds)
+    attach_query_start(query_lens, layout.query_start)
     tree = tree_layout(parents, layout.query_start, context_lens, max_nodes)
     # per layer: append K/V to layout.slots, then
     paged_tree_attention(q, k, v, layout.block_tables, context_lens, query_lens, tree.masks, scale)
@@ -15,8 +17,13 @@ the model is the cached tokens plus its depth. A step is
     pool.keep_paths(layout.block_tables, context_lens, layout.query_start, path.paths)
 
 after which a sequence has its cached tokens and path.counts more, and path.next_tokens is
-sampled. Everything stays on the device. The reference has no such steps; the contract of the
-attention is core/attention.py's.
+sampled. The reference has no such steps; the contract of the attention is core/attention.py's.
+
+These operators leave their results on the device and read nothing back but the lengths, which the
+attention checks on the host: without the attached copies it reads both from the device in every call, every
+layer's. path.counts, and so the next step's lengths, only the device knows: the copies may be bounds (attach_host says
+which), and the layout's query starts are then what the kernels go by. Outside these operators, PagedKVPool.append reads
+its slots back unless it is given host_slots.
 
 Who computes follows CONFIG, as for the operators beside these: tensor ops on any device, or,
 with ATTENTION=hip, libpagedkv's kernels, never falling back.

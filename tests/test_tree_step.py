@@ -9,6 +9,7 @@ import torch
 
 from inference_server.config import CONFIG
 from inference_server.core.attention import paged_attention
+from inference_server.core.attention_hip import attach_host, attach_query_start
 from inference_server.core.kv_pool import ModelDims, PagedKVPool
 from inference_server.core.sampling import token_logprobs
 from inference_server.core.step_layout import step_layout
@@ -136,3 +137,59 @@ def test_verified_trees_decode_what_single_tokens_do(device):
         n = min(len(g), len(w))
         assert g[:n] == w[:n]
     assert longest == DEPTH and steps < 39
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", ["layout", "host"])
+def test_a_step_reads_nothing_back(monkeypatch, starts):
+    """With bounds of the lengths on the host and the layout's query starts (or lengths that the host has), no operator waits for
+    the device, in its first call or later ones; results are those of a step that reads the lengths back."""
+    monkeypatch.setattr(CONFIG, "attention", "hip")
+    rng = np.random.default_rng(3)
+    dims, new, cached = ModelDims(2, 2, 64, torch.float16), [7, 20, 1, 12], [30, 5, 90, 500]
+    pool = PagedKVPool(dims, num_blocks=64, block_size=BS, device="cuda")
+    for t in pool.k + pool.v:
+        t.normal_()
+    tokens, parents = zip(*(drafts(rng, 1, [1] * 9, n + 1) for n in new))
+    new = [len(t) for t in tokens]
+    total = sum(new)
+    cuda = lambda x: torch.as_tensor(x, dtype=torch.long).cuda()  # noqa: E731
+    tokens, parents = cuda(sum(tokens, [])), cuda(sum(parents, []))
+    held = [-(-c // BS) for c in cached]
+    tables = torch.zeros(4, 40, dtype=torch.long)
+    for i, h in enumerate(held):
+        tables[i, :h] = torch.arange(sum(held[:i]), sum(held[:i]) + h)
+    tables, free = tables.cuda(), torch.arange(sum(held), 64).cuda()
+    q, logits = torch.randn(total, 8, 64, device="cuda").half(), torch.randn(total, 61, device="cuda")
+    lens = [c + n for c, n in zip(cached, new)]
+    bounds = ([640] * 4, [total - 3, 1, 1, 1]) if starts == "layout" else (lens, new)
+
+    def step(attached):
+        ctx, query_lens = cuda(lens), cuda(new)
+        held_d, targets = cuda(held), logits.argmax(-1)
+        if attached:
+            attach_host(ctx, torch.tensor(bounds[0])), attach_host(query_lens, torch.tensor(bounds[1]))
+            torch.cuda.synchronize()
+            torch.cuda.set_sync_debug_mode("error")
+        try:
+            lay = step_layout(tables.clone(), held_d, ctx, query_lens, free, BS, total)
+            if attached and starts == "layout":
+                attach_query_start(query_lens, lay.query_start)
+            tree = tree_layout(parents, lay.query_start, ctx, 32)
+            out = [paged_tree_attention(q, k, v, lay.block_tables, ctx, query_lens, tree.masks, 0.125)
+                   for k, v in zip(pool.k, pool.v)]
+            scores = token_logprobs(logits, tokens, 3)
+            path = accept_tree(tokens, parents, targets, lay.query_start, DEPTH)
+            pool.keep_paths(lay.block_tables, ctx, lay.query_start, path.paths * 0 - 1)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        return [*tree, *out, *scores, *path]
+
+    pool.pointer_table()
+    want = step(False)
+    for _ in range(2):
+        for a, b in zip(step(True), want):
+            if a.dtype is torch.float16:            # contexts may be cut otherwise: one rounding of the output
+                assert (a.float() - b.float()).abs().max() <= 2.0 ** -10 * b.float().abs().max()
+            else:
+                assert torch.equal(a, b)
