@@ -23,13 +23,13 @@
 // bf16, as much as the output's rounding. Two bf16 pieces have 16 bits of any weight. fp16 ends at 2^-24, so
 // its weights reach up to the type's other end: the reference m that scores are taken from is 13 to 15 bits below
 // the largest score so far, where bf16's is at most 8 below it. Two pieces are then off by 2^-22 of a weight, or by 2^-38 of
-// the row's largest where that is more. (With bf16's rule a tail of keys at 2^-24 of the largest weight came out 20% off, and
-// one at 2^-26 not at all.)
+// the row's largest where that is more. (With bf16's rule a tail of keys at 2^-24.9 of the largest weight came out 24% off,
+// and one below 2^-25 not at all.)
 //
 // Bound: by matrix and vector instructions in turn where rows are many (64 sequences of 16-64 nodes behind
 // 1,024-8,192 keys, 32/8 heads of 128, bf16: 412 us; one piece of the weights 321), by start, a round trip
 // a tile and the longest context where they are few (32 of 8-32 nodes behind 16-960 keys, 12 heads of 64, fp16:
-// 18.7 us; RW = 2 21.8, RW = 4 24.0), by HBM and by the partials' way to memory and back in a lone long context
+// 19.0 us; RW = 2 21.8, RW = 4 24.0 where it took 18.7), by HBM and by the partials' way to memory and back in a lone long context
 // (32 nodes behind 100,000 keys, 32/8 heads of 128: 121 us, of which the merge is 10). The next
 // tile's loads start ahead of a tile's products: behind them, 422 and 122.
 #pragma once
