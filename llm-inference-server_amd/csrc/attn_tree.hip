@@ -71,8 +71,8 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
     const T* kb = reinterpret_cast<const T*>(p.k) + kvh * p.sh;
     const T* vb = reinterpret_cast<const T*>(p.v) + kvh * p.sh;
     const int64_t* table = p.tables + (int64_t)seq * p.table_stride;
-    // The lane's 16 dims of a row; those past head_dim read the row's first ones (against queries of 0,
-    // into outputs that are not stored).
+    // The lane's 16 dims of a row. Those past head_dim read the row's first ones: whole lanes (WIDE), whose share of a
+    // score is left out and whose outputs are not stored, or elements, which are zeros.
     auto dims = [&](const T* row, float* x) {
         if constexpr (WIDE) {
             const T* at = row + (d0 < p.head_dim ? d0 : 0);
@@ -92,7 +92,10 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = to_f32(row[d0 + e < p.head_dim ? d0 + e : 0]);
+            for (int e = 0; e < 16; ++e) {
+                const float at = to_f32(row[d0 + e < p.head_dim ? d0 + e : 0]);
+                x[e] = d0 + e < p.head_dim ? at : 0.f;
+            }
         }
     };
     float m = kNegInf, l = 0.f;
@@ -118,6 +121,7 @@ __global__ __launch_bounds__(1024) void tree_generic_kernel(const TreeParams p) 
             float x = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) x += q[e] * k[u][e];
+            if (WIDE) x = d0 < p.head_dim ? x : 0.f;            // (0 * infinity)
             x = lanes_sum<LPK>(x);
             dot[u] = good[u] ? x : 0.f;
             if (seen[u]) m_new = fmaxf(m_new, dot[u] * p.scale_log2);

@@ -49,3 +49,28 @@ def test_infinities_below_the_largest_weight(monkeypatch, backend, dtype, d, len
     out = paged_tree_attention(s.q, s.k, s.v, *s.args, s.masks, s.scale)
     assert torch.isinf(out).any() and torch.isnan(out).any() and torch.isfinite(out).any()
     check(s, out)
+
+
+@pytest.mark.parametrize("backend", BACKENDS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d", [1, 7, 24, 40, 72, 160, 272, 48, 64, 128])
+@pytest.mark.parametrize("lens", LENS[:1] + LENS[3:4])
+def test_infinities_in_k_that_make_a_score_lowest(monkeypatch, backend, dtype, d, lens):
+    """K of -infinity in its first dim, against queries of 1 there: the key weighs nothing, as one 400 nats below the others
+    (e^-400 is 0 in fp32), to the bit."""
+    monkeypatch.setattr(CONFIG, "attention", backend)
+    device = "cuda" if backend == "hip" else "cpu"
+    s = batch(lens, heads=4, kv=2, d=d, bs=16, dtype=dtype, device="cpu", seed=d)
+    s.q[..., 0] = 1
+    low = s.k.clone()
+    for i, (c, m) in enumerate(lens):
+        for p in [0, 5, 16, 33, c // 2, c - 1, c, c + m - 1]:
+            at = (int(s.tables[i, p // 16]), p % 16)
+            low[at][:, 0] = -400 * d ** 0.5
+            s.k[at][:, 0] = -math.inf
+    s.q, s.v, s.masks = s.q.to(device), s.v.to(device), s.masks.to(device)
+    s.args = tuple(t.to(device) for t in s.args)
+    outs = [paged_tree_attention(s.q, k.to(device), s.v, *s.args, s.masks, s.scale) for k in (s.k, low)]
+    assert torch.isfinite(outs[1]).all() and torch.equal(*outs)
+    s.k = low
+    check(s, outs[1])
