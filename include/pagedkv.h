@@ -572,7 +572,8 @@ int pkv_tree_layout(
  * 64 * mask_words on are seen by none. A key that a row does not see does not reach it, whatever
  * its K and V hold; a row that sees no key is zero. Scores, softmax and sums are in float32, the output is rounded once. Weights
  * meet 16-bit V as two pieces of its type: bf16 leaves at most 2^-16 of a weight, fp16 2^-22 of it or 2^-38 of the row's
- * largest, whichever is more. query_start_loc is not NULL.
+ * largest, whichever is more. Sums are divided by the weights' at the end, and scores are taken in base 2: V of 2^100 and
+ * more in size, or scores of 2^126 (fp16: 2^26), may leave the range. query_start_loc is not NULL.
  * Block ids outside the pool are never dereferenced. max_query_len bounds the query lengths (0:
  * num_tokens).
  *

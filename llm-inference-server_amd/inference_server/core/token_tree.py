@@ -228,7 +228,8 @@ def paged_tree_attention(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
 
     Softmax and sums are in fp32 and the output is rounded once. (ATTENTION=hip: weights meet 16-bit V as two
     pieces of its type, which leave at most 2^-16 of a bf16 weight, and of an fp16 one 2^-22, or 2^-38 of the row's
-    largest where that is more.) The 8-bit cache has no such attention. A key that a token does
+    largest where that is more; values of 2^100 and more in size, or scores of 2^126, in fp16 2^26, may leave
+    the range.) The 8-bit cache has no such attention. A key that a token does
     not see does not reach it, whatever its K and V hold (NaN and infinities among it); a token that
     sees none gets zeros. Lengths with host copies attached (attach_host) are checked without a
     device round trip."""
